@@ -29,6 +29,8 @@ extern "C" {
 #define QNT_F16 1
 #define QNT_Q8_0 2
 #define QNT_Q4_0 3
+/* activations only (the qnt_kv_* entries); no .qnt tensor has this type */
+#define QNT_BF16 4
 
 const char* qnt_last_error(void);
 int qnt_version(void);          /* 100 * major + minor */
@@ -263,6 +265,85 @@ void qnt_sampler_free(qnt_sampler* s);
  *            its stream (cudaStreamSynchronize) and writes the id to *token. */
 int qnt_sampler_sample_noalloc(const qnt_sampler_params* sp, uint64_t* rng_state, float* logits, int n_valid,
                                const int* history, int n_history, int* token, void* stream);
+
+/* ---------------------------------------------------------------- paged 8-bit KV cache
+ *
+ * No counterpart in the reference (its cache is one dense f16 array per sequence, engine/src/model.h:58): a cache of many
+ * sequences in pages, int8 codes with one f32 scale for each block of 16 tokens, K or V, layer and kv head, in device
+ * memory that the caller owns.  value = code * scale.
+ *   codes   [n_pages][n_layers][2: K, V][n_kv_heads][page_tokens * head_dim], 16-byte aligned; within a page the K tile is
+ *           [head_dim / 16][page_tokens][16 dims] and the V tile [page_tokens / 16][head_dim][16 tokens]
+ *   scales  [n_pages][n_layers][2][n_kv_heads][page_tokens / 16]
+ *   refs    [n_pages]: how many sequences use the page (0: free)
+ *   table   [max_seqs][max_pages]: the page of positions k * page_tokens .. of a sequence, -1 past its pages
+ *   lens    [max_seqs]: positions of the sequence; it holds ceil(len / page_tokens) pages
+ *   status  one word of error bits that kernels set (qnt_kv_check reports and clears them)
+ * An empty cache: refs and lens 0, table -1, status 0; codes and scales need no initial values.
+ * Limits: head_dim 64 or 128; page_tokens 16, 32, 64 or 128; n_pages <= 1048576; max_seqs <= 8192.
+ *
+ * Every call queues its work on `stream` (a cudaStream_t, NULL = legacy default) and returns.  All pointers are device
+ * pointers, sequence lists included.  Calls that write a cache must be ordered against every other call on it (one stream,
+ * or events); workspaces belong to one call at a time.  Nothing is allocated, so the calls can be captured into a graph. */
+typedef struct qnt_kv_cache {
+    int n_layers, n_kv_heads, head_dim, page_tokens;
+    int n_pages, max_seqs, max_pages;
+    int8_t* codes;
+    float* scales;
+    int* refs;
+    int* table;
+    int* lens;
+    unsigned* status;
+} qnt_kv_cache;
+
+/* Page operations.  Free pages are taken from the lowest index up, in the order of the list.  A call whose list is not
+ * valid, or that needs more pages than are free, changes nothing and sets an error bit.
+ *   qnt_kv_reserve  lens[seqs[i]] += extra[i] and the pages for it (distinct sequences)
+ *   qnt_kv_fork     sequence dst[i] (empty) becomes a copy of src[i]: full pages are shared (refs + 1), a part-filled last
+ *                   page is copied in every layer, so that both can go on; distinct dst, none of them also a src
+ *   qnt_kv_free     the sequences give back their pages (refs - 1) and become empty (distinct sequences)
+ *   qnt_kv_compact  the n pages in use move to indices 0 .. n - 1 (only those at or past n move); table and refs follow
+ *   qnt_kv_copy     page src[i]'s codes and scales, all layers, over page dst[i]'s (no dst twice, none also a src)
+ * workspace: qnt_kv_page_workspace bytes, 16-byte aligned, contents irrelevant. */
+size_t qnt_kv_page_workspace(const qnt_kv_cache* cache);
+int qnt_kv_reserve(const qnt_kv_cache* cache, const int* seqs, const int* extra, int n, void* workspace, size_t workspace_bytes,
+                   void* stream);
+int qnt_kv_fork(const qnt_kv_cache* cache, const int* src, const int* dst, int n, void* workspace, size_t workspace_bytes,
+                void* stream);
+int qnt_kv_free(const qnt_kv_cache* cache, const int* seqs, int n, void* stream);
+int qnt_kv_compact(const qnt_kv_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+int qnt_kv_copy(const qnt_kv_cache* cache, const int* src, const int* dst, int n, void* stream);
+
+/* Rows of a call: n distinct sequences, tokens starts[j] .. starts[j + 1] - 1 (of n_tok) belong to sequence seqs[j]
+ * (starts: n + 1 ascending ints from 0 to n_tok).
+ *   qnt_kv_append     quantizes rows into one layer.  A sequence's m new tokens are its last m positions (reserve first;
+ *                     then append in every layer): token i goes to position lens[seq] - m + i.  k, v: token t, head h,
+ *                     dim d at t * stride + h * head_dim + d, of dtype QNT_F32, QNT_F16 or QNT_BF16; max_new bounds m.
+ *                     Per block of 16 tokens, K or V, and head: d = max(the block's scale if it holds earlier tokens,
+ *                     max |x| * (1 / 127), in f32); earlier codes are rounded to the new scale, new codes are round(x / d).  A
+ *                     non-finite value makes its block read as NaN.
+ *   qnt_kv_read       values of positions first[j] + i of sequence seqs[j] to rows starts[j] + i of k_out and v_out,
+ *                     [n_tok][n_kv_heads][head_dim] of dtype (16-byte aligned)
+ *   qnt_kv_attention  out[t][h] = softmax attention of query row t, head h over its sequence's cache in one layer: query i
+ *                     of a sequence's m sits at p = lens[seq] - m + i and sees positions max(0, p - window + 1) .. p
+ *                     (window 0: 0 .. p).  scores are scaled by `scale`; head h reads kv head h / (n_heads /
+ *                     n_kv_heads).  q: token t, head h, dim d at t * q_stride + h * head_dim + d; out [n_tok][n_heads]
+ *                     [head_dim] of the same dtype, 16-byte aligned; lse (may be NULL) [n_tok][n_heads] f32: log of the
+ *                     sum of exp(score).  A query that sees nothing gets out 0 and lse -inf.  max_q bounds m; max_len
+ *                     bounds lens (a longer sequence is still read whole, only less evenly spread).
+ *                     workspace: qnt_kv_attention_workspace bytes for the same counts, 16-byte aligned, contents
+ *                     irrelevant. */
+int qnt_kv_append(const qnt_kv_cache* cache, int layer, const void* k, const void* v, int dtype, long long k_stride,
+                  long long v_stride, const int* seqs, const int* starts, int n, int n_tok, int max_new, void* stream);
+int qnt_kv_read(const qnt_kv_cache* cache, int layer, const int* seqs, const int* first, const int* starts, int n, int n_tok,
+                void* k_out, void* v_out, int dtype, void* stream);
+size_t qnt_kv_attention_workspace(const qnt_kv_cache* cache, int n_heads, int n, int n_tok, int max_q, int max_len);
+int qnt_kv_attention(const qnt_kv_cache* cache, int layer, const void* q, int dtype, long long q_stride, int n_heads,
+                     const int* seqs, const int* starts, int n, int n_tok, int max_q, int max_len, float scale, int window,
+                     void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Waits for `stream`, then reports (and clears) the error bits of earlier calls on this cache: QNT_ERR_DEVICE with the
+ * reason in qnt_last_error(). */
+int qnt_kv_check(const qnt_kv_cache* cache, void* stream);
 
 /* Diagnostics (no reference counterpart): copies an internal buffer of the last forward as floats -- 0 roped q,
  * 1 attention output, 2 residual x (of the last layer, before the final norm), 3 quantized SwiGLU output, 4 its block

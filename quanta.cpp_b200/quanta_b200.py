@@ -4,6 +4,7 @@ The names follow the reference's C++ interface (engine/src/model.h, ops.h, sampl
     Model(path, ctx).forward(token, pos, hq) / forward_batch(tokens, pos0, hq) / head(hq) / last_head_rows
     quantize_q8(x) ; DeviceTensor(dtype, rows, cols, raw).matvec(q, d, r0, r1) / .matmul(...)
     Model.generate(prompt, SamplerParams(...), shortlist=True, batch_prefill=True, n_gen=64)
+    PagedKV.empty(...).reserve / append / attention / read / fork / free / compact  the paged 8-bit KV cache (torch tensors)
     synth_model(path, ...)  seeded random-init .qnt writer
 There is no CPU fallback: importing works anywhere, but every call needs libquanta_b200.so and a GPU, and fails
 loudly when either is missing.
@@ -21,6 +22,7 @@ PKG = Path(__file__).resolve().parent
 LIB_DIR = Path(os.environ["QNT_LIB_DIR"]) if os.environ.get("QNT_LIB_DIR") else PKG / "lib"  # timeline.py: lib_stamps
 
 F32, F16, Q8_0, Q4_0 = 0, 1, 2, 3
+BF16 = 4  # activations of the paged KV cache
 QK = 32
 GEN_SHORTLIST, GEN_BATCH_PREFILL = 1, 2
 
@@ -56,6 +58,11 @@ class SynthCfg(C.Structure):
         ("rope_theta", C.c_float), ("norm_eps", C.c_float)] + [(n, C.c_int) for n in "mlp_q4 q4_group shortlist n_tokens".split()] + [
         ("w_std", C.c_float), ("seed", C.c_uint64), ("n_threads", C.c_int), ("flags", C.c_uint32),
         ("tok_blob", C.c_char_p), ("tok_len", C.c_uint64)]
+
+
+class KVCacheC(C.Structure):
+    _fields_ = [(n, C.c_int) for n in "n_layers n_kv_heads head_dim page_tokens n_pages max_seqs max_pages".split()] + [
+        (n, C.c_void_p) for n in "codes scales refs table lens status".split()]
 
 
 @dataclass
@@ -142,6 +149,20 @@ def lib() -> C.CDLL:
         L.qnt_token_id.argtypes = [P, C.c_char_p]
         L.qnt_sampler_sample_noalloc.argtypes = [C.POINTER(SamplerParamsC), C.POINTER(C.c_uint64), P, I, P, I,
                                                  C.POINTER(I), P]
+        K, Z, LL = C.POINTER(KVCacheC), C.c_size_t, C.c_longlong
+        L.qnt_kv_page_workspace.argtypes = [K]
+        L.qnt_kv_page_workspace.restype = Z
+        L.qnt_kv_reserve.argtypes = [K, P, P, I, P, Z, P]
+        L.qnt_kv_fork.argtypes = [K, P, P, I, P, Z, P]
+        L.qnt_kv_free.argtypes = [K, P, I, P]
+        L.qnt_kv_compact.argtypes = [K, P, Z, P]
+        L.qnt_kv_copy.argtypes = [K, P, P, I, P]
+        L.qnt_kv_append.argtypes = [K, I, P, P, I, LL, LL, P, P, I, I, I, P]
+        L.qnt_kv_read.argtypes = [K, I, P, P, P, I, I, P, P, I, P]
+        L.qnt_kv_attention_workspace.argtypes = [K, I, I, I, I, I]
+        L.qnt_kv_attention_workspace.restype = Z
+        L.qnt_kv_attention.argtypes = [K, I, P, I, LL, I, P, P, I, I, I, I, F, I, P, P, P, Z, P]
+        L.qnt_kv_check.argtypes = [K, P]
         _lib = L
     return _lib
 
@@ -264,6 +285,176 @@ def sample_noalloc(sp: SamplerParams, rng_state: int, logits, n_valid: int | Non
     _check(lib().qnt_sampler_sample_noalloc(C.byref(spc), C.byref(state), C.c_void_p(logits.data_ptr()), n_valid,
                                             _ptr(hist) if hist.size else None, hist.size, C.byref(tok), st))
     return tok.value, state.value
+
+
+class PagedKV:
+    """The paged 8-bit KV cache (qnt_kv_*): many sequences in pages of one pool, int8 codes with a f32 scale for each block
+    of 16 tokens, K or V, layer and kv head.  The arrays are torch CUDA tensors that the caller may keep and look at:
+        codes  int8 [n_pages, n_layers, 2, n_kv_heads, page_tokens * head_dim]  (K tile [head_dim/16][page_tokens][16
+               dims], V tile [page_tokens/16][head_dim][16 tokens])
+        scales float32 [n_pages, n_layers, 2, n_kv_heads, page_tokens / 16]
+        refs int32 [n_pages], table int32 [max_seqs, max_pages], lens int32 [max_seqs]
+    Sequence lists (seqs, starts, extra, ...) are contiguous int32 CUDA tensors: tokens starts[j] .. starts[j + 1] - 1 of a
+    call belong to sequence seqs[j].  Work is queued on `stream` (default: torch's current stream), nothing waits; errors
+    that kernels find (no free pages, a sequence out of range) are raised by check().  Calls that write the cache must be
+    ordered against its other calls; the object's workspaces are one per stream."""
+
+    def __init__(self, codes, scales, refs, table, lens):
+        import torch
+        self._torch = torch
+        i32 = torch.int32
+        for name, t, dt, dim in (("codes", codes, torch.int8, 5), ("scales", scales, torch.float32, 5), ("refs", refs, i32, 1),
+                                 ("table", table, i32, 2), ("lens", lens, i32, 1)):
+            if not (t.is_cuda and t.dtype == dt and t.dim() == dim and t.is_contiguous() and t.device == codes.device):
+                raise TypeError(f"{name} must be a contiguous {dim}-dimensional {dt} CUDA tensor on the codes' device")
+        n_pages, n_layers, two, n_kv, tile = codes.shape
+        page_tokens = scales.shape[4] * 16
+        if two != 2 or scales.shape[:4] != codes.shape[:4] or refs.shape[0] != n_pages or lens.shape[0] != table.shape[0] \
+                or page_tokens == 0 or tile % page_tokens:
+            raise ValueError("codes, scales, refs, table and lens do not describe one cache")
+        self.codes, self.scales, self.refs, self.table, self.lens = codes, scales, refs, table, lens
+        self.n_layers, self.n_kv_heads, self.head_dim, self.page_tokens = n_layers, n_kv, tile // page_tokens, page_tokens
+        self.device = codes.device
+        self._status = torch.zeros(1, dtype=i32, device=self.device)
+        self._c = KVCacheC(n_layers, n_kv, self.head_dim, page_tokens, n_pages, table.shape[0], table.shape[1], codes.data_ptr(),
+                           scales.data_ptr(), refs.data_ptr(), table.data_ptr(), lens.data_ptr(), self._status.data_ptr())
+        self._p = C.byref(self._c)
+        self._types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        self._ws, self._need = {}, {}
+        self._page_ws = lib().qnt_kv_page_workspace(self._p)
+        if self._page_ws == 0:
+            raise QntError(-1, lib().qnt_last_error().decode(errors="replace"))
+
+    @classmethod
+    def empty(cls, n_layers: int, n_kv_heads: int, head_dim: int, n_pages: int, max_seqs: int, max_pages: int,
+              page_tokens: int = 64, device="cuda"):
+        """A cache without sequences."""
+        import torch
+        z = dict(dtype=torch.int32, device=device)
+        return cls(torch.zeros((n_pages, n_layers, 2, n_kv_heads, page_tokens * head_dim), dtype=torch.int8, device=device),
+                   torch.zeros((n_pages, n_layers, 2, n_kv_heads, page_tokens // 16), dtype=torch.float32, device=device),
+                   torch.zeros(n_pages, **z), torch.full((max_seqs, max_pages), -1, **z), torch.zeros(max_seqs, **z))
+
+    def _stream(self, stream):
+        if stream is None:
+            return self._torch.cuda.current_stream(self.device).cuda_stream
+        return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+    def _workspace(self, stream: int, need: int):
+        ws = self._ws.get(stream)
+        if ws is None or ws.numel() < need:
+            if ws is not None:  # kernels queued on `stream` may still use the old one
+                ws.record_stream(self._torch.cuda.ExternalStream(stream, device=self.device))
+            ws = self._ws[stream] = self._torch.empty(max(need, self._page_ws, 1 << 20), dtype=self._torch.uint8, device=self.device)
+        return ws.data_ptr(), ws.numel()
+
+    def _list(self, *lists):
+        n = lists[0].numel()
+        for t in lists:
+            if not (t.is_cuda and t.dtype == self._torch.int32 and t.is_contiguous()):
+                raise TypeError("sequence lists must be contiguous int32 CUDA tensors")
+        return n
+
+    def _rows(self, name, x, heads=None):
+        if not (x.is_cuda and x.dim() == 3 and x.dtype in self._types and x.stride(2) == 1 and x.shape[2] == self.head_dim and
+                x.stride(1) == self.head_dim and (heads is None or x.shape[1] == heads)):
+            raise TypeError(f"{name} must be a float32, float16 or bfloat16 CUDA tensor [tokens, heads, {self.head_dim}] whose "
+                            "heads are contiguous within a token")
+        return self._types[x.dtype]
+
+    def reserve(self, seqs, extra, stream=None):
+        """lens[seqs] += extra, with the pages for it."""
+        n = self._list(seqs, extra)
+        if extra.numel() != n:
+            raise ValueError("one extra per sequence")
+        s = self._stream(stream)
+        w, nb = self._workspace(s, self._page_ws)
+        _check(lib().qnt_kv_reserve(self._p, seqs.data_ptr(), extra.data_ptr(), n, w, nb, s))
+
+    def fork(self, src, dst, stream=None):
+        """Empty sequences dst become copies of src: full pages shared, a part-filled last page copied."""
+        n = self._list(src, dst)
+        if dst.numel() != n:
+            raise ValueError("one dst per src")
+        s = self._stream(stream)
+        w, nb = self._workspace(s, self._page_ws)
+        _check(lib().qnt_kv_fork(self._p, src.data_ptr(), dst.data_ptr(), n, w, nb, s))
+
+    def free(self, seqs, stream=None):
+        """The sequences give back their pages and become empty."""
+        _check(lib().qnt_kv_free(self._p, seqs.data_ptr(), self._list(seqs), self._stream(stream)))
+
+    def compact(self, stream=None):
+        """The pages in use move together to the lowest indices."""
+        s = self._stream(stream)
+        w, nb = self._workspace(s, self._page_ws)
+        _check(lib().qnt_kv_compact(self._p, w, nb, s))
+
+    def copy_pages(self, src, dst, stream=None):
+        """Codes and scales of pages src over those of pages dst, all layers."""
+        n = self._list(src, dst)
+        if dst.numel() != n:
+            raise ValueError("one dst per src")
+        _check(lib().qnt_kv_copy(self._p, src.data_ptr(), dst.data_ptr(), n, self._stream(stream)))
+
+    def append(self, layer: int, k, v, seqs, starts, max_new: int | None = None, stream=None):
+        """Quantizes rows k, v [tokens, n_kv_heads, head_dim] into a layer, as the last positions of their sequences
+        (reserve first); max_new bounds a sequence's new tokens."""
+        dt = self._rows("k", k, self.n_kv_heads)
+        if self._rows("v", v, self.n_kv_heads) != dt or v.shape[0] != k.shape[0]:
+            raise TypeError("k and v must have the same type and number of tokens")
+        n, m = self._list(seqs, starts), k.shape[0]
+        if starts.numel() != n + 1:
+            raise ValueError("starts must have one entry more than seqs")
+        _check(lib().qnt_kv_append(self._p, layer, k.data_ptr(), v.data_ptr(), dt, k.stride(0), v.stride(0), seqs.data_ptr(),
+                                   starts.data_ptr(), n, m, m if max_new is None else max_new, self._stream(stream)))
+
+    def read(self, layer: int, seqs, first, starts, n_tok: int, dtype=None, stream=None):
+        """Values of positions first[j] + i of sequence seqs[j] as rows starts[j] + i: (K, V) [n_tok, n_kv_heads, head_dim]
+        (float32 unless dtype says otherwise)."""
+        t = self._torch
+        dtype = dtype or t.float32
+        if dtype not in self._types:
+            raise TypeError("dtype must be float32, float16 or bfloat16")
+        n = self._list(seqs, first, starts)
+        if first.numel() != n or starts.numel() != n + 1:
+            raise ValueError("one first per sequence, and one entry more in starts")
+        k = t.empty((n_tok, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        v = t.empty_like(k)
+        _check(lib().qnt_kv_read(self._p, layer, seqs.data_ptr(), first.data_ptr(), starts.data_ptr(), n, n_tok, k.data_ptr(),
+                                 v.data_ptr(), self._types[dtype], self._stream(stream)))
+        return k, v
+
+    def attention(self, layer: int, q, seqs, starts, max_q: int, max_len: int, scale: float | None = None, window: int = 0,
+                  lse: bool = False, stream=None):
+        """Attention of q [tokens, n_heads, head_dim] over the cache of their sequences; query i of a sequence's m sits at
+        position lens - m + i and sees the positions up to its own (the last `window` of them, if window > 0).  max_q bounds
+        a sequence's queries, max_len its length.  Returns out (q's type), or (out, lse) with lse float32 [tokens, n_heads]."""
+        t = self._torch
+        dt = self._rows("q", q)
+        n_tok, heads = q.shape[0], q.shape[1]
+        n = self._list(seqs, starts)
+        if starts.numel() != n + 1:
+            raise ValueError("starts must have one entry more than seqs")
+        key = (heads, n, n_tok, max_q, max_len)
+        need = self._need.get(key)
+        if need is None:
+            if len(self._need) > 4096:
+                self._need.clear()
+            need = self._need[key] = lib().qnt_kv_attention_workspace(self._p, heads, n, n_tok, max_q, max_len)
+        s = self._stream(stream)
+        w, nb = self._workspace(s, need)
+        out = t.empty((n_tok, heads, self.head_dim), dtype=q.dtype, device=self.device)
+        ls = t.empty((n_tok, heads), dtype=t.float32, device=self.device) if lse else None
+        _check(lib().qnt_kv_attention(self._p, layer, q.data_ptr(), dt, q.stride(0), heads, seqs.data_ptr(), starts.data_ptr(), n,
+                                      n_tok, max_q, max_len, self.head_dim ** -0.5 if scale is None else scale, window,
+                                      out.data_ptr(), None if ls is None else ls.data_ptr(), w, nb, s))
+        return (out, ls) if lse else out
+
+    def check(self, stream=None):
+        """Waits for the stream and raises the error that earlier calls on this cache ran into, if any."""
+        _check(lib().qnt_kv_check(self._p, self._stream(stream)))
+
 
 def bench_mma_i8(iters: int = 4096) -> float:
     """Measured dense int8 tensor-core TOP/s of the current GPU (qnt_bench_mma_i8)."""
