@@ -35,6 +35,7 @@
 #include "head_kernels.h"
 #include "kernels.cuh"
 #include "qkv_pair.cuh"
+#include "tcgen05.cuh"
 
 namespace qb {
 
@@ -68,56 +69,6 @@ struct Tc {
     static constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(TOK >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
     static_assert(epi % 128 == 0 && (tmem_cols & (tmem_cols - 1)) == 0, "ring entries and TMEM allocation");
 };
-constexpr unsigned kWaitLimit = 1u << 22;
-constexpr unsigned kSuspendHintNs = 20000;  // a waiting thread sleeps (up to this long) instead of spinning
-
-__device__ __forceinline__ unsigned smem_u32(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* b, unsigned count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* b, unsigned parity) {
-    unsigned ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity), "r"(kSuspendHintNs)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait: false when it gave up after `limit` tries or another role aborted (then the caller unwinds).
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, unsigned parity, volatile int* abort_flag, unsigned* status,
-                                          unsigned limit = kWaitLimit) {
-    for (unsigned i = 0; i < limit; ++i) {
-        if (mbar_try(b, parity)) return true;
-        if (*abort_flag) return false;
-    }
-    *abort_flag = 1;
-    set_error(status, ERR_WAIT_TIMEOUT);
-    return false;
-}
-
-// The same bounded wait run by a whole warp: every lane polls and a vote makes the outcome warp-uniform (a lane that
-// saw the phase complete polls again until all have; a completed phase keeps reading as complete until the barrier
-// moves on, which needs this warp's own arrival).
-__device__ __forceinline__ bool warp_wait(uint64_t* b, unsigned parity, volatile int* abort_flag, unsigned* status) {
-    for (unsigned i = 0; i < kWaitLimit; ++i) {
-        if (__all_sync(0xffffffffu, mbar_try(b, parity))) return true;
-        if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
-    }
-    *abort_flag = 1;
-    set_error(status, ERR_WAIT_TIMEOUT);
-    return false;
-}
-
 // The timeout path of the waits above, on its own: one thread waits on an mbarrier that nothing arrives on, with the
 // given limit, so the wait runs out, sets ERR_WAIT_TIMEOUT and the kernel returns (no copies or MMAs in flight).
 __global__ void k_wait_probe(unsigned limit, unsigned* status) {
@@ -154,21 +105,6 @@ __device__ __forceinline__ uint64_t sw128_desc(const void* p) {
     d |= uint64_t(2) << 61;                 // layout: 128B swizzle
     return d;
 }
-
-__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1 : 0), "r"(0), "r"(0), "r"(0), "r"(0)
-        : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
 // registers -> TMEM: this warp's 32 lanes, NC columns at each of taddr + 4 NC b (b = 0..3), all set to x.
 template <int NC>

@@ -6,7 +6,10 @@
 // A query that sees no key gets out = 0 and lse = -inf.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "kv_cache.h"
+#include "tcgen05.cuh"
 
 namespace qb {
 
@@ -97,6 +100,869 @@ __global__ void __launch_bounds__(128) k_kv_attn(KvView c, KvAttnArgs a, KvCall 
     }
 }
 
+
+// ---------------------------------------------------------------- few query rows per kv head (decode)
+//
+//   S^T [128 keys][3 digits x RM rows] = K tile [128][HD] . Q digits     int8 tensor cores, K codes as they lie in the cache
+//   O^T [HD dims][pieces x RM rows]   += V tile [HD][128] . W pieces     bf16 tensor cores, W = exp(s - ref) vs
+// A query row is split into three balanced base-256 digits, x = 65536 x2 + 256 x1 + x0 with |x| <= 127 * 65536: its rounding
+// is 2^-24 of the row's largest value, and the int32 sums are exact.  A weight is the sum of three bf16 pieces (24 bits;
+// two, 16 bits, where the result is a 16-bit type): bf16 has f32's range, so a weight keeps its relative precision however
+// far it is below the largest, and V codes are exact in it.  (Weights in fixed point, on the int8 tensor cores like S, lost
+// the small ones beside a much larger one.)  V codes become bf16 on their way through registers.
+// The softmax reference `ref` of a row is the score of the last key that it sees in its first tile (so the largest weight is
+// at least 1), raised only when a score passes it by 2^32: f32 and bf16 have the range, most tiles need no maximum over the
+// CTA, and O stays in TMEM; every 16 tiles it joins f32 registers, which bounds the tensor cores' accumulation error.
+//
+// The work of all (sequence, kv head) units, in order, is dealt evenly to the CTAs (`even`), whatever the lengths; a
+// unit cut between CTAs leaves partial sums in the workspace and k_kv_join adds them up in CTA order.  Where the host's
+// bound on the lengths keeps a unit short, every CTA takes one unit and nothing is joined.
+//   warp 4     loads K (cp.async; bulk copies of the pages' pieces measured about 0.15 us each, whatever their size) and
+//              the tile's page list two tiles ahead, and issues the MMAs
+//   warps 0-3  thread = key: scores, weights; thread = dim: V codes (copied one tile ahead) to bf16, and O
+constexpr int kDecThreads = 160;
+constexpr int kTileKeys = 128;
+constexpr float kDigitMax = 8323072.0f;  // 127 * 256^2: three digits
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFlush = 16;               // tiles whose O stays in TMEM
+constexpr float kRaise = 32.f;           // log2: how far a score may pass the reference
+
+template <int HD, int RM, int NP>
+struct Dec {
+    static constexpr int NC = (3 * RM + 15) / 16 * 16;                 // columns of S
+    static constexpr int WC = (NP * RM + 15) / 16 * 16;                // columns of O
+    static constexpr int stages = 3;                                   // K tiles
+    static constexpr int ctas = HD == 64 && RM <= 8 ? 3 : 2;           // per SM: shared memory, registers
+    static constexpr int k_bytes = kTileKeys * HD;
+    static constexpr int v_bytes = kTileKeys * HD * 2;                 // bf16: [16 groups of 8 keys][HD][8 keys]
+    static constexpr int w_pitch = WC * 16 + 16;                       // [16 groups of 8 keys] at this pitch: 4 groups, 4 bank quads
+    static constexpr int w_bytes = 16 * w_pitch;
+    static constexpr int q_bytes = HD * NC;
+    static constexpr int smem = stages * k_bytes + k_bytes + v_bytes + q_bytes + w_bytes + 128;
+    static constexpr int s_cols = NC <= 16 ? 16 : NC <= 32 ? 32 : 64;  // TMEM column pitch of an S buffer
+    static constexpr int tmem_need = 2 * s_cols + WC;
+    static constexpr int tmem_cols = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : 256;
+    static constexpr int items = HD / 16;                              // V pieces (a dim's 16 tokens) of a thread
+    static constexpr uint32_t idesc_s = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NC >> 3) << 17) | (uint32_t(kTileKeys >> 4) << 24);
+    static constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(WC >> 3) << 17) | (uint32_t(HD >> 4) << 24);
+    static_assert(tmem_need <= 256, "TMEM allocation");
+};
+
+struct DecPlan {
+    int even;       // 1: tiles dealt evenly over the CTAs, 0: one unit per CTA
+    int4* info;     // [CTAs] of the cut unit that a CTA begins: its last CTA, first token, queries, kv head; x = -1: none
+    float* ml;      // [2 CTAs][RM][2] maximum (log2 units) and sum of a partial
+    float* o;       // [2 CTAs][RM][HD]
+};
+
+// A call's sequence j: its rows and the keys that they see together.
+struct SeqWork {
+    int seq, t0, m, len, lo, tiles;  // keys [lo, len), in tiles of 128 from lo & ~127; tiles >= 1 where m > 0
+};
+
+// (Not inlined: it is called where a unit starts, and code that is not there need not be fetched.)
+__device__ __noinline__ SeqWork seq_work(const KvView& c, const KvAttnArgs& a, const KvCall& call, int j) {
+    SeqWork w;
+    const int t0 = __ldg(call.starts + j), t1 = __ldg(call.starts + j + 1), seq = __ldg(call.seqs + j);
+    const bool known = seq >= 0 && seq < c.max_seqs;
+    const int len = min(max(__ldg(c.lens + (known ? seq : 0)), 0), c.max_pages << c.pt_shift);
+    w.t0 = t0;
+    w.m = t0 < 0 ? 0 : max(min(t1, call.n_tok) - t0, 0);
+    w.seq = seq;
+    if (w.m > 0 && (!known || w.m > a.max_q)) {
+        set_error(c.status, ERR_BAD_POS);
+        w.m = 0;
+    }
+    w.len = w.m > 0 ? len : 0;
+    w.lo = a.window ? max(0, w.len - w.m + 1 - a.window) : 0;
+    w.tiles = w.m == 0 ? 0 : w.len > 0 ? (w.len - 1) / kTileKeys - w.lo / kTileKeys + 1 : 1;
+    return w;
+}
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float warp_max_redux(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ float load_q(const void* q, KvType t, long long i) {
+    return t == KV_F32 ? __ldg(static_cast<const float*>(q) + i)
+         : t == KV_F16 ? __half2float(static_cast<const __half*>(q)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(q)[i]);
+}
+__device__ __forceinline__ void store_out(void* o, KvType t, size_t i, float x) {
+    if (t == KV_F32) static_cast<float*>(o)[i] = x;
+    else if (t == KV_F16) static_cast<__half*>(o)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(o)[i] = __float2bfloat16_rn(x);
+}
+
+// warp_wait with its loop kept a loop (these kernels are bound by instruction fetches where their code grows).
+__device__ __forceinline__ bool wait_warp(uint64_t* b, unsigned parity, volatile int* abort_flag, unsigned* status) {
+#pragma unroll 1
+    for (unsigned i = 0; i < kWaitLimit; ++i) {
+        if (__all_sync(0xffffffffu, mbar_try(b, parity))) return true;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    }
+    *abort_flag = 1;
+    set_error(status, ERR_WAIT_TIMEOUT);
+    return false;
+}
+
+// Barrier of the 128 softmax threads; true for all of them if `bad` holds for one, so that they leave a loop together.
+__device__ __forceinline__ bool bar_any(bool bad) {
+    unsigned r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(bad ? 1u : 0u)
+        : "memory");
+    return r != 0;
+}
+
+// The value whose digits' dots are (d2, d1, d0).  |d2 * 256 + d1| < 2^30.
+__device__ __forceinline__ float join_digits(int d2, int d1, int d0) { return fmaf(float(d2 * 256 + d1), 256.f, float(d0)); }
+
+// 4 int8 codes -> 4 bf16, exactly: 128 + the low 7 bits, less 128 (or 256 for a negative code).
+__device__ __forceinline__ uint2 codes_bf16(unsigned w) {
+    const unsigned low = w & 0x7F7F7F7Fu, sign = w & 0x80808080u;
+    const unsigned a0 = __byte_perm(low, 0x43434343u, 0x4140), b0 = __byte_perm(sign, 0x43434343u, 0x4140);
+    const unsigned a1 = __byte_perm(low, 0x43434343u, 0x4342), b1 = __byte_perm(sign, 0x43434343u, 0x4342);
+    const __nv_bfloat162 x = __hsub2(reinterpret_cast<const __nv_bfloat162&>(a0), reinterpret_cast<const __nv_bfloat162&>(b0));
+    const __nv_bfloat162 y = __hsub2(reinterpret_cast<const __nv_bfloat162&>(a1), reinterpret_cast<const __nv_bfloat162&>(b1));
+    return make_uint2(reinterpret_cast<const unsigned&>(x), reinterpret_cast<const unsigned&>(y));
+}
+
+// What the loading warp tells the others about a unit and about a tile.
+struct UnitRec {
+    int t0, m, len, lo, j, head, tiles;
+    int first;  // this CTA has the unit's first tile
+    int cut;    // and not all of them
+    int at;     // the unit's place in the call's cost
+};
+struct TileRec {
+    long long kt[8];  // of the tile's 8 blocks of 16 tokens: the K tile number (KvView::at), 0 where no key is seen
+    int key0, unit, head_of_unit, tail_of_unit;
+};
+
+// The call's work is dealt in units of a tile's time: a unit's first tile counts 1 + kUnitCost (its queries, its sums and its
+// outputs cost about as much as that many tiles), the others 1.  CTA x has [x base + min(x, rem), ...) of it, and the tiles
+// that start there.
+constexpr int kUnitCost = 2;
+struct Deal {
+    int base, rem;
+    __device__ __forceinline__ int begin(int x) const { return x * base + min(x, rem); }
+    __device__ __noinline__ int owner(int t) const {
+        return t < rem * (base + 1) ? t / (base + 1) : rem + (t - rem * (base + 1)) / base;
+    }
+};
+// Tiles of a unit that start in the first `part` of its cost.
+__device__ __forceinline__ int tiles_before(int part, int tiles) { return part <= 0 ? 0 : min(tiles, max(1, part - kUnitCost)); }
+
+template <int HD, int RM, int NP>
+__global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decode(KvView c, KvAttnArgs a, KvCall call, DecPlan plan) {
+    using C = Dec<HD, RM, NP>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+    unsigned char* vb = smem + C::stages * C::k_bytes;
+    unsigned char* qd = vb + C::v_bytes;
+    unsigned char* wb = qd + C::q_bytes;
+    unsigned char* vc = wb + C::w_bytes;  // V codes of the next tile, each thread's pieces in its own places
+    __shared__ uint64_t k_full[C::stages], listed[4], s_done[2], w_ready[2], o_done, q_ready, fin;
+    __shared__ TileRec tile_rec[4];
+    __shared__ __align__(16) float scales[4][16];  // of a tile's 8 blocks: K's, V's
+    __shared__ UnitRec unit_rec[4];
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag, fresh[2];
+    __shared__ __align__(16) float tile_max[4][RM];
+    __shared__ __align__(16) float fac[2][RM], first_ref[2][RM], last_ref[RM], sum_part[4][RM];
+    __shared__ int row_off[2][RM];  // a row's place in out and lse, from its unit's first
+    __shared__ int2 scan_part[4];
+    __shared__ int first_j, first_head, first_tile, first_at, tiles_from, tiles_to;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* ab = &abort_flag;
+
+    if (tid == 0) {
+        for (int s = 0; s < C::stages; ++s) mbar_init(&k_full[s], 32);
+        for (int s = 0; s < 4; ++s) mbar_init(&listed[s], 32);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&s_done[b], 1);
+            mbar_init(&w_ready[b], 128);
+        }
+        mbar_init(&o_done, 1);
+        mbar_init(&q_ready, 128);
+        mbar_init(&fin, 1);
+        abort_flag = 0;
+        tiles_from = tiles_to = 0;
+        if (plan.even) plan.info[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4) tmem_alloc(&tmem_base, C::tmem_cols);
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- this CTA's tiles of the call's (even), or the tiles of unit blockIdx.x
+    Deal deal = {0, 0};
+    if (plan.even) {
+        const int per = (call.n + 127) / 128, j0 = min(tid * per, call.n), j1 = warp < 4 ? min(j0 + per, call.n) : j0;
+        int2 mine = make_int2(0, 0);  // cost and tiles of this thread's sequences
+        SeqWork w = {};
+#pragma unroll 1
+        for (int j = j0; j < j1; ++j) {
+            w = seq_work(c, a, call, j);
+            if (w.tiles) mine.x += c.n_kv * (w.tiles + kUnitCost);
+            mine.y += c.n_kv * w.tiles;
+        }
+        int2 inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
+            if (lane >= o) {
+                inc.x += x;
+                inc.y += y;
+            }
+        }
+        if (warp < 4 && lane == 31) scan_part[warp] = inc;
+        __syncthreads();
+        int2 before = make_int2(inc.x - mine.x, inc.y - mine.y);
+        int total = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (x < warp) {
+                before.x += scan_part[x].x;
+                before.y += scan_part[x].y;
+            }
+            total += scan_part[x].x;
+        }
+        // a part is never so small that no tile starts in it
+        const int parts = max(1, min(int(gridDim.x), total / (kUnitCost + 1)));
+        deal.base = total / parts;
+        deal.rem = total - deal.base * parts;
+        const int begin = deal.begin(blockIdx.x), end = deal.begin(blockIdx.x + 1);
+        if (warp < 4 && int(blockIdx.x) < parts && begin < before.x + mine.x && end >= before.x) {  // a bound is in this thread's sequences
+#pragma unroll 1
+            for (int j = j0; j < j1; ++j) {
+                if (j1 - j0 > 1) w = seq_work(c, a, call, j);
+                if (w.tiles == 0) continue;
+                const int cost = w.tiles + kUnitCost, all = cost * c.n_kv;
+                if (begin >= before.x && begin < before.x + all) {
+                    const int h = (begin - before.x) / cost, t = tiles_before(begin - before.x - h * cost, w.tiles);
+                    first_j = j;  // t == tiles: the first tile is the next unit's
+                    first_head = h;
+                    first_tile = t;
+                    first_at = before.x + h * cost;
+                    tiles_from = before.y + h * w.tiles + t;
+                }
+                if (end > before.x && end <= before.x + all) {
+                    const int h = min((end - before.x) / cost, c.n_kv - 1);
+                    tiles_to = before.y + h * w.tiles + tiles_before(end - before.x - h * cost, w.tiles);
+                }
+                before.x += all;
+                before.y += w.tiles * c.n_kv;
+            }
+        }
+    } else if (tid == 0) {
+        first_j = blockIdx.x / c.n_kv;
+        first_head = blockIdx.x % c.n_kv;
+        first_tile = first_at = tiles_from = 0;
+        tiles_to = seq_work(c, a, call, first_j).tiles;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    const int n_my = tiles_to - tiles_from;
+
+    if (warp == 4) {
+        // ---- loads, two tiles ahead, and MMAs
+        constexpr int kLead = C::stages - 1;
+        SeqWork w = {};
+        int j = first_j, head = first_head, tile = first_tile, at = first_at, end = 0, unit = -1;  // of the next tile to load
+        int key0 = 0, page = -1;  // its first key; lane b < 8: the page of block b (-1: no key of it is seen)
+        bool ok = true, new_unit = true;
+        int s_next = 0, q_next = 0;  // next tile whose scores are to be issued, next unit whose queries are to be waited for
+        auto look = [&](int left) {  // the page-table entries of the tile, read an iteration before they are used
+            if (new_unit) {
+                w = seq_work(c, a, call, j);
+                end = min(w.tiles, tile + left);
+            }
+            key0 = (w.lo / kTileKeys + tile) * kTileKeys;
+            const int lo = max(w.lo, key0), hi = min(w.len, key0 + kTileKeys), b0 = key0 + lane * kKvBlock;
+            page = -1;
+            if (lane < 8 && b0 < hi && b0 + kKvBlock > lo) page = __ldg(c.table + size_t(w.seq) * c.max_pages + (b0 >> c.pt_shift)) & 0x7fffffff;
+        };
+        auto next_unit = [&]() {
+            tile = 0;
+            at += w.tiles + kUnitCost;
+            if (++head == c.n_kv) {
+                head = 0;
+                do ++j;
+                while (j < call.n - 1 && __ldg(call.starts + j + 1) <= __ldg(call.starts + j));
+            }
+        };
+        if (n_my > 0) {
+            look(n_my);
+            if (tile == w.tiles) {  // this CTA's part begins after the start of that unit's last tile
+                next_unit();
+                look(n_my);
+            }
+        }
+#pragma unroll 1
+        for (int it = 0; it < n_my + kLead && ok; ++it) {
+            const int t = it - kLead;  // the tile to finish
+#pragma unroll 1
+            for (; t >= 0 && s_next <= min(t + 1, n_my - 1) && ok; ++s_next) {  // scores of this tile and of the next one
+                if (tile_rec[s_next & 3].head_of_unit) {  // its query digits are in place
+                    ok = wait_warp(&q_ready, q_next & 1, ab, c.status);
+                    ++q_next;
+                }
+                ok = ok && wait_warp(&k_full[s_next % C::stages], (s_next / C::stages) & 1, ab, c.status);
+                if (!ok) break;
+                fence_async_smem();  // the copies were made by the generic proxy
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t kt = smem_u32(smem + (s_next % C::stages) * C::k_bytes), qt = smem_u32(qd);
+#pragma unroll
+                    for (int k = 0; k < HD / 32; ++k)
+                        mma_i8(tmem + (s_next & 1) * C::s_cols, plain_desc(kt + k * 2 * kTileKeys * 16, kTileKeys * 16, 128),
+                               plain_desc(qt + k * 2 * C::NC * 16, C::NC * 16, 128), C::idesc_s, k > 0);
+                    mma_commit(&s_done[s_next & 1]);
+                }
+                __syncwarp();
+            }
+            if (it < n_my && ok) {  // K of tile `it` into stage it % stages (its last user was tile it - stages), its record into it % 4
+                if (new_unit) {
+                    ++unit;
+                    if (lane == 0) {
+                        UnitRec& u = unit_rec[unit & 3];
+                        u.t0 = w.t0;
+                        u.m = w.m;
+                        u.len = w.len;
+                        u.lo = w.lo;
+                        u.j = j;
+                        u.head = head;
+                        u.tiles = w.tiles;
+                        u.first = tile == 0;
+                        u.cut = end - tile < w.tiles;
+                        u.at = at;
+                    }
+                }
+                if (page >= c.n_pages) {  // -1 in the table, or past the pool
+                    set_error(c.status, ERR_BAD_POS);
+                    page = 0;
+                }
+                const long long kt = page < 0 ? 0 : (long long)c.at(page, a.layer, 0, head);
+                const unsigned live = __ballot_sync(0xffffffffu, page >= 0);
+                TileRec& rec = tile_rec[it & 3];
+                if (lane < 8) rec.kt[lane] = kt;
+                if (lane == 0) {
+                    rec.key0 = key0;
+                    rec.unit = unit & 3;
+                    rec.head_of_unit = new_unit;
+                    rec.tail_of_unit = tile + 1 == end;
+                }
+                __syncwarp();
+                mbar_arrive(&listed[it & 3]);
+                const int s = it % C::stages;
+                const uint32_t dst = smem_u32(smem + s * C::k_bytes) + lane * 16;
+                const int step = c.pt * 16;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {  // lane's keys kk * 32 + lane
+                    const int key = kk * 32 + lane;
+                    const long long tl = __shfl_sync(0xffffffffu, kt, key / kKvBlock);
+                    const int8_t* src = c.codes + (size_t(tl) << (c.pt_shift + (HD == 64 ? 6 : 7))) + (key & (c.pt - 1)) * 16;
+                    if (live >> (key / kKvBlock) & 1)
+#pragma unroll
+                        for (int g = 0; g < HD / 16; ++g)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + g * (kTileKeys * 16) + kk * 512),
+                                         "l"(src + g * step)
+                                         : "memory");
+                }
+                {  // lanes 0-7: K's scales of the 8 blocks, lanes 8-15: V's
+                    const int b = lane & 7;
+                    const size_t tl = size_t(__shfl_sync(0xffffffffu, kt, b)) + (lane & 8 ? c.n_kv : 0);
+                    if (lane < 16)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[it & 3][lane])),
+                                     "l"(c.scales + (tl << (c.pt_shift - 4)) + ((b * kKvBlock) & (c.pt - 1)) / kKvBlock)
+                                     : "memory");
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&k_full[s])) : "memory");
+                new_unit = ++tile == end;
+                if (it + 1 < n_my) {
+                    if (new_unit) next_unit();
+                    look(n_my - it - 1);
+                }
+            }
+            if (t < 0) continue;
+            ok = ok && wait_warp(&w_ready[t & 1], (t >> 1) & 1, ab, c.status);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t vt = smem_u32(vb), wt = smem_u32(wb);
+                const bool keep = !fresh[t & 1];
+#pragma unroll
+                for (int k = 0; k < kTileKeys / 16; ++k)
+                    mma_f16(tmem + 2 * C::s_cols, plain_desc(vt + k * 2 * HD * 16, HD * 16, 128),
+                            plain_desc(wt + k * 2 * C::w_pitch, C::w_pitch, 128), C::idesc_o, keep || k > 0);
+                mma_commit(&o_done);
+            }
+            __syncwarp();
+        }
+        if (lane == 0) {
+            mma_commit(&fin);
+            for (unsigned i = 0; i < kWaitLimit && !mbar_try(&fin, 0); ++i) {
+            }
+        }
+        __syncwarp();
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        // ---- scores, softmax, outputs: thread = key of the tile, then dim of the head
+        constexpr int lanes = HD == 64 ? 16 : 32;  // rows of O^T of a warp (M = 64 leaves the upper half of each quadrant unused)
+        const int dim = warp * lanes + lane;
+        const uint32_t my_tmem = tmem + (uint32_t(warp * 32) << 16);
+        const int vd = tid % HD, vblk = tid / HD;  // V pieces: dim vd of blocks vblk + x * (128 / HD)
+        const int v_shift = c.pt_shift + (HD == 64 ? 6 : 7);  // log2 of a tile's codes
+        bool ok = true;   // a wait that gave up is acted on at the next barrier, by all threads together
+        int in_tmem = 0;  // tiles whose sum lies in TMEM
+        UnitRec u = {};
+        int rows = 0, p0 = 0, units = 0;  // rows of the unit, position of its first query, units so far
+        unsigned unset = 0;               // rows without a reference: they have seen no key
+        float ref[RM], sum[RM], acc[RM], fq[RM];  // ref and fq are the same in all threads
+#pragma unroll 1
+        for (int i = -1; i < n_my; ++i) {
+            // the next tile begins a unit: its query digits, 128 / RM threads per row (loaded here, written below, as soon as
+            // this tile's scores are done and qd is free)
+            constexpr int per_row = 128 / RM, E = HD / per_row;
+            const int qr = tid / per_row, d0 = tid % per_row * E;
+            bool prep = false;
+            int q_rows = 0;
+            float x[E];
+            if (i + 1 < n_my) {
+                ok = wait_warp(&listed[(i + 1) & 3], ((i + 1) >> 2) & 1, ab, c.status) && ok;
+                if (tile_rec[(i + 1) & 3].head_of_unit) {
+                    const UnitRec& nu = unit_rec[tile_rec[(i + 1) & 3].unit];
+                    prep = true;
+                    q_rows = nu.m * a.group;
+                    const long long q0 = (long long)(nu.t0 + qr / a.group) * a.q_stride + (nu.head * a.group + qr % a.group) * HD + d0;
+#pragma unroll
+                    for (int y = 0; y < E; ++y) x[y] = qr < q_rows ? load_q(a.q, a.type, q0 + y) : 0.f;
+                }
+            }
+            float s[RM], vs = 0.f;  // score less ref, log2
+            if (i >= 0) {
+                const TileRec& rec = tile_rec[i & 3];
+                if (rec.head_of_unit) {
+                    u = unit_rec[rec.unit];
+                    rows = u.m * a.group;
+                    p0 = u.len - u.m;
+                    unset = (1u << rows) - 1;  // rows <= 16
+                    const float* f = fac[units & 1];
+                    ++units;
+#pragma unroll
+                    for (int r = 0; r < RM; ++r) {
+                        ref[r] = sum[r] = acc[r] = 0.f;
+                        fq[r] = f[r];
+                    }
+                }
+                ok = wait_warp(&k_full[i % C::stages], (i / C::stages) & 1, ab, c.status) && ok;
+                const float ks0 = scales[i & 3][tid >> 4], vs0 = scales[i & 3][8 + (tid >> 4)];
+                // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
+                vs = fabsf(vs0) < INFINITY ? vs0 : 0.f;
+                const float ks = fabsf(vs0) < INFINITY ? ks0 : __int_as_float(0x7fffffff);
+                ok = wait_warp(&s_done[i & 1], (i >> 1) & 1, ab, c.status) && ok;
+                tc_fence_after();
+                int d2[RM], d1[RM], d0[RM];
+                const uint32_t at = my_tmem + (i & 1) * C::s_cols;
+                tmem_ld(at, d2);
+                tmem_ld(at + RM, d1);
+                tmem_ld(at + 2 * RM, d0);
+                tmem_ld_wait();
+                tmem_ready(d2);
+                tmem_ready(d1);
+                tmem_ready(d0);
+                tc_fence_before();
+#pragma unroll
+                for (int r = 0; r < RM; ++r) s[r] = fmaf(join_digits(d2[r], d1[r], d0[r]), ks * fq[r], -ref[r]);
+            }
+            if (prep) {
+                struct alignas(E < 4 ? E : 4) Bytes {
+                    unsigned char b[E];
+                } digit[3];
+                float amax = 0.f;
+#pragma unroll
+                for (int y = 0; y < E; ++y) amax = max_nan(amax, fabsf(x[y]));
+#pragma unroll
+                for (int o = per_row / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const bool fine = amax < INFINITY;  // else the row's scores, and with them its result, are NaN
+                // very small or large rows are brought near 1 first, exactly, so that the quotient is in range
+                const float pre = amax < 0x1p-60f ? 0x1p64f : amax > 0x1p60f ? 0x1p-64f : 1.f;
+                const float inv = fine && amax > 0.f ? __fdividef(kDigitMax, amax * pre) : 0.f;
+#pragma unroll
+                for (int y = 0; y < E; ++y) {
+                    const int x3 = fine ? __float2int_rn(x[y] * pre * inv) : 0;
+                    const unsigned z = (unsigned(x3) + 0x808080u) ^ 0x808080u;
+                    digit[0].b[y] = (unsigned char)(z >> 16);
+                    digit[1].b[y] = (unsigned char)(z >> 8);
+                    digit[2].b[y] = (unsigned char)z;
+                }
+#pragma unroll
+                for (int z = 0; z < 3; ++z)
+                    *reinterpret_cast<Bytes*>(qd + ((d0 / 16) * C::NC + z * RM + qr) * 16 + d0 % 16) = digit[z];
+                if (tid < q_rows) row_off[units & 1][tid] = tid / a.group * a.n_heads + tid % a.group;
+                if (tid % per_row == 0) fac[units & 1][qr] = fine ? (amax * a.scale) * (kLog2e / kDigitMax) : __int_as_float(0x7fffffff);
+                fence_async_smem();
+                mbar_arrive(&q_ready);
+                if (i < 0 && bar_any(!ok)) break;  // else: fac and row_off are read after the barrier below
+            }
+            if (i >= 0) {
+                const TileRec& rec = tile_rec[i & 3];
+                const int key0 = rec.key0, key = key0 + tid;
+                const bool tail = rec.tail_of_unit;
+                const bool seen = key >= u.lo && key < u.len;  // by some row
+                // do all rows see the whole tile?
+                const bool whole = key0 >= u.lo && key0 + kTileKeys <= u.len &&
+                                   (u.m == 1 || (key0 + kTileKeys - 1 <= p0 && (!a.window || key0 > u.len - 1 - a.window)));
+                if (!whole) {
+                    if (u.m == 1) {
+#pragma unroll
+                        for (int r = 0; r < RM; ++r) s[r] = seen ? s[r] : -INFINITY;
+                    } else {
+                        int p = p0, g = a.group;
+#pragma unroll
+                        for (int r = 0; r < RM; ++r) {
+                            if (!seen || key > p || (a.window && key <= p - a.window)) s[r] = -INFINITY;
+                            if (--g == 0) {
+                                g = a.group;
+                                ++p;
+                            }
+                        }
+                    }
+                }
+                bool high = in_tmem == kFlush;
+                const unsigned had = unset;
+                unsigned can = 0;  // rows without a reference that see a key of this tile: they take the last one's score
+                if (had) {
+                    int p = p0, g = a.group;
+#pragma unroll
+                    for (int r = 0; r < RM; ++r) {
+                        const int last = min(p, key0 + kTileKeys - 1), lo = a.window ? max(p - a.window + 1, key0) : key0;
+                        if ((had >> r & 1) && last >= lo) {
+                            can |= 1u << r;
+                            if (key == last) first_ref[i & 1][r] = s[r];
+                        }
+                        if (--g == 0) {
+                            g = a.group;
+                            ++p;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < RM; ++r) high = high || s[r] > kRaise;
+                }
+                bool any = bar_any(high || !ok);
+                if (had) {
+#pragma unroll
+                    for (int r = 0; r < RM; ++r) {
+                        if (can >> r & 1) {
+                            ref[r] = first_ref[i & 1][r];
+                            s[r] -= ref[r];
+                        }
+                        high = high || s[r] > kRaise;
+                    }
+                    unset &= ~can;
+                    any = bar_any(high) || any;
+                }
+                bool waited = false;  // for the product of the tile before, which reads vb and wb
+                if (any) {
+                    // O leaves TMEM, and the references that a score passed are raised to the tile's maxima
+#pragma unroll
+                    for (int r = 0; r < RM; ++r) {
+                        const float top = warp_max_redux(s[r]);
+                        if (lane == 0) tile_max[warp][r] = top;
+                    }
+                    if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab, c.status) && ok;
+                    tc_fence_after();
+                    waited = true;
+                    if (bar_any(!ok)) break;
+                    if (in_tmem) {
+                        int o0[RM], o1[RM], o2[RM];
+                        const uint32_t at = my_tmem + 2 * C::s_cols;
+                        tmem_ld(at, o0);
+                        tmem_ld(at + RM, o1);
+                        if constexpr (NP == 3) tmem_ld(at + 2 * RM, o2);
+                        tmem_ld_wait();
+                        tmem_ready(o0);
+                        tmem_ready(o1);
+                        if constexpr (NP == 3) tmem_ready(o2);
+                        tc_fence_before();
+#pragma unroll
+                        for (int r = 0; r < RM; ++r) {
+                            float o = __int_as_float(o1[r]);
+                            if constexpr (NP == 3) o += __int_as_float(o2[r]);
+                            acc[r] += o + __int_as_float(o0[r]);
+                        }
+                        in_tmem = 0;
+                    }
+#pragma unroll
+                    for (int r = 0; r < RM; ++r) {
+                        const float top = fmaxf(fmaxf(tile_max[0][r], tile_max[1][r]), fmaxf(tile_max[2][r], tile_max[3][r]));
+                        if (top > kRaise) {
+                            ref[r] += top;
+                            s[r] -= top;
+                            const float f = ex2(-top);
+                            acc[r] *= f;
+                            sum[r] *= f;
+                        }
+                    }
+                }
+                unsigned w[RM / 2][NP];  // pieces of rows 2 x, 2 x + 1
+#pragma unroll
+                for (int x = 0; x < RM / 2; ++x) {
+                    float p[2];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int r = 2 * x + y;
+                        const float e = ex2(s[r]);
+                        sum[r] += e;
+                        p[y] = e * vs;
+                    }
+#pragma unroll
+                    for (int z = 0; z < NP; ++z) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(p[0], p[1]);
+                        w[x][z] = reinterpret_cast<const unsigned&>(h);
+                        if (z + 1 < NP) {
+                            p[0] -= __uint_as_float(w[x][z] << 16);
+                            p[1] -= __uint_as_float(w[x][z] & 0xffff0000u);
+                        }
+                    }
+                }
+                if (!waited) {
+                    if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab, c.status) && ok;
+                    tc_fence_after();
+                }
+                unsigned char* wt = wb + (tid >> 3) * C::w_pitch + (tid & 7) * 2;
+#pragma unroll
+                for (int x = 0; x < RM / 2; ++x)
+#pragma unroll
+                    for (int z = 0; z < NP; ++z) {
+                        *reinterpret_cast<unsigned short*>(wt + (z * RM + 2 * x) * 16) = (unsigned short)w[x][z];
+                        *reinterpret_cast<unsigned short*>(wt + (z * RM + 2 * x + 1) * 16) = (unsigned short)(w[x][z] >> 16);
+                    }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+                for (int x = 0; x < C::items; ++x) {
+                    const int b = vblk + x * (128 / HD);
+                    const uint4 v = reinterpret_cast<const uint4*>(vc)[x * 128 + tid];
+                    const uint2 x0 = codes_bf16(v.x), x1 = codes_bf16(v.y), x2 = codes_bf16(v.z), x3 = codes_bf16(v.w);
+                    uint4* dst = reinterpret_cast<uint4*>(vb) + 2 * b * HD + vd;
+                    dst[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
+                    dst[HD] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+                }
+                if (tid == 0) fresh[i & 1] = in_tmem == 0;
+                ++in_tmem;
+                fence_async_smem();
+                mbar_arrive(&w_ready[i & 1]);
+                if (tail) {
+                    // ---- the unit's sums over this CTA's keys
+                    ok = wait_warp(&o_done, i & 1, ab, c.status) && ok;
+                    tc_fence_after();
+                    {
+                        int o0[RM], o1[RM], o2[RM];
+                        const uint32_t at = my_tmem + 2 * C::s_cols;
+                        tmem_ld(at, o0);
+                        tmem_ld(at + RM, o1);
+                        if constexpr (NP == 3) tmem_ld(at + 2 * RM, o2);
+                        // meanwhile the sums: at each step a lane keeps half of its rows
+#pragma unroll
+                        for (int h = RM / 2, o = 16; h >= 1; h >>= 1, o >>= 1)
+#pragma unroll
+                            for (int r = 0; r < h; ++r) {
+                                const bool up = lane & o;
+                                const float mine = up ? sum[r + h] : sum[r], other = up ? sum[r] : sum[r + h];
+                                sum[r] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+                            }
+#pragma unroll
+                        for (int o = 16 / RM; o > 0; o >>= 1) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+                        if (lane % (32 / RM) == 0) sum_part[warp][lane / (32 / RM)] = sum[0];
+                        tmem_ld_wait();
+                        tmem_ready(o0);
+                        tmem_ready(o1);
+                        if constexpr (NP == 3) tmem_ready(o2);
+                        tc_fence_before();
+                        in_tmem = 0;
+#pragma unroll
+                        for (int r = 0; r < RM; ++r) {
+                            float o = __int_as_float(o1[r]);
+                            if constexpr (NP == 3) o += __int_as_float(o2[r]);
+                            acc[r] += o + __int_as_float(o0[r]);
+                            if (tid == 0) last_ref[r] = ref[r];
+                        }
+                    }
+                    if (bar_any(!ok)) break;
+                    const int* off = row_off[(units - 1) & 1];
+                    const size_t row0 = size_t(u.t0) * a.n_heads + u.head * a.group;
+                    const size_t slot = size_t(2 * blockIdx.x + u.first) * RM;  // if cut
+                    const int rr = lane % RM;  // lane r of a warp looks after row r
+                    const float l = (sum_part[0][rr] + sum_part[1][rr]) + (sum_part[2][rr] + sum_part[3][rr]);
+                    const bool none = (unset >> rr & 1) && l == 0.f;
+                    const float inv = u.cut ? 1.f : none ? 0.f : __fdividef(1.f, l);
+                    if (tid < rows) {
+                        if (u.cut) reinterpret_cast<float2*>(plan.ml)[slot + tid] = make_float2(none ? -INFINITY : last_ref[tid], l);
+                        else if (a.lse) a.lse[row0 + off[tid]] = none ? -INFINITY : (last_ref[tid] + __log2f(l)) * (1.f / kLog2e);
+                    }
+                    auto put_rows = [&](auto* out, bool own_order) {
+#pragma unroll
+                        for (int r = 0; r < RM; ++r) {
+                            const float o = acc[r] * __shfl_sync(0xffffffffu, inv, r);
+                            if (r < rows && lane < lanes) put(out + size_t(own_order ? r : off[r]) * HD + dim, o);
+                        }
+                    };
+                    if (a.type == KV_F32 || u.cut) put_rows(u.cut ? plan.o + slot * HD : static_cast<float*>(a.out) + row0 * HD, u.cut);
+                    else if (a.type == KV_F16) put_rows(static_cast<__half*>(a.out) + row0 * HD, false);
+                    else put_rows(static_cast<__nv_bfloat16*>(a.out) + row0 * HD, false);
+                    if (tid == 0 && u.first && u.cut)  // the unit's first CTA says which CTAs share it
+                        plan.info[blockIdx.x] = make_int4(deal.owner(u.at + u.tiles - 1 + (u.tiles > 1 ? kUnitCost : 0)), u.t0, u.m, u.head);
+                    if (bar_any(!ok)) break;  // last_ref and sum_part are read before the next unit writes them
+                }
+            }
+            if (i + 1 < n_my) {  // V codes of the next tile (any codes where no key is seen: their weights are 0)
+                const uint32_t dst = smem_u32(vc) + tid * 16;
+#pragma unroll
+                for (int x = 0; x < C::items; ++x) {
+                    const int b = vblk + x * (128 / HD);
+                    const int8_t* src = c.codes + (size_t(tile_rec[(i + 1) & 3].kt[b] + c.n_kv) << v_shift) +
+                                        (((b * kKvBlock) & (c.pt - 1)) * HD + vd * 16);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * 2048), "l"(src) : "memory");
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_free(tmem, C::tmem_cols);
+    }
+}
+
+// Joins the partial sums of the units that k_kv_decode cut: CTA (x, r) row r of the one that its CTA x began, in CTA order.
+constexpr int kJoinThreads = 512;
+
+template <int HD, int RM>
+__global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan plan) {
+    constexpr int G = kJoinThreads / HD;
+    extern __shared__ float weight[];  // [n] of the partials
+    __shared__ float part[G][HD], red[2][16];
+    const int r = blockIdx.y, tid = threadIdx.x, d = tid % HD, g = tid / HD, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    const int4 in = __ldcg(plan.info + blockIdx.x);  // last CTA, first token, queries, kv head
+    if (in.x < 0 || r >= in.z * a.group) return;
+    const int first = blockIdx.x, n = in.x - first + 1;
+    auto slot = [&](int x) { return size_t(2 * (first + x) + (x == 0)) * RM + r; };
+    float top = -INFINITY;
+    float2 ml = make_float2(-INFINITY, 0.f);
+#pragma unroll 1
+    for (int x = tid; x < n; x += kJoinThreads) {  // one partial each, but for the largest grids
+        ml = __ldcg(reinterpret_cast<const float2*>(plan.ml) + slot(x));
+        weight[x] = ml.x;
+        top = fmaxf(top, ml.x);
+    }
+    top = warp_max_redux(top);
+    if (lane == 0) red[0][warp] = top;
+    __syncthreads();
+    top = warp_max_redux(red[0][lane & 15]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+#pragma unroll 1
+    for (int x = tid; x < n; x += kJoinThreads) {
+        const float w = ex2(weight[x] - ref);
+        weight[x] = w;
+        l += w * (n <= kJoinThreads ? ml.y : __ldcg(plan.ml + slot(x) * 2 + 1));
+    }
+    l = warp_sum(l);
+    if (lane == 0) red[1][warp] = l;
+    __syncthreads();
+    float o = 0.f;
+#pragma unroll 8
+    for (int x = g; x < n; x += G) o = fmaf(__ldcg(plan.o + slot(x) * HD + d), weight[x], o);
+    part[g][d] = o;
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll
+    for (int q = 1; q < G; ++q) o += part[q][d];
+    l = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) l += red[1][q];
+    const size_t row = size_t(in.y + r / a.group) * a.n_heads + in.w * a.group + r % a.group;
+    const bool none = top == -INFINITY && l == 0.f;
+    store_out(a.out, a.type, row * HD + d, none ? 0.f : o / l);
+    if (a.lse && d == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+}
+
+// ---------------------------------------------------------------- host side
+
+constexpr int kDecRows = 16;  // most query rows (queries x heads of a kv head) of k_kv_decode
+
+bool takes_decode(const KvAttnArgs& a) { return (long long)a.max_q * a.group <= kDecRows; }
+
+int dec_rm(const KvAttnArgs& a) {
+    const int rows = a.max_q * a.group;
+    return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+}
+
+struct DecLaunch {
+    int even, grid;
+    size_t units;
+};
+
+DecLaunch dec_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
+    DecLaunch l;
+    l.units = size_t(call.n) * c.n_kv;
+    // a unit's tiles, at most; a window ends anywhere in its first and last tile
+    const long long span = a.window && a.window < a.max_len ? (long long)a.window + a.max_q : a.max_len;
+    const long long tiles = std::max(1LL, (span + kTileKeys - 1) / kTileKeys + (a.window != 0));
+    l.even = tiles > 8;
+    const int ctas = c.hd == 64 && dec_rm(a) <= 8 ? 3 : 2;  // per SM, as the kernel's
+    l.grid = int(l.even ? std::min<long long>(148 * ctas, std::max<long long>(1, (long long)l.units * tiles / 2)) : (long long)l.units);
+    return l;
+}
+
+
+template <int HD, int RM, int NP>
+cudaError_t decode_n(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
+    using C = Dec<HD, RM, NP>;
+    const DecLaunch l = dec_launch(c, a, call);
+    DecPlan p{};
+    p.even = l.even;
+    if (l.even) {
+        unsigned char* b = static_cast<unsigned char*>(ws);
+        p.o = reinterpret_cast<float*>(b);
+        p.ml = p.o + size_t(l.grid) * 2 * RM * HD;
+        p.info = reinterpret_cast<int4*>(p.ml + size_t(l.grid) * 2 * RM * 2);
+    }
+    // with its static part the shared memory passes the default limit of 48 KB
+    cudaError_t e = cudaFuncSetAttribute(k_kv_decode<HD, RM, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(k_kv_decode<HD, RM, NP>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
+    if (e != cudaSuccess || !l.even) return e;
+    return launch_pdl(k_kv_join<HD, RM>, dim3(unsigned(l.grid), unsigned(a.max_q * a.group)), dim3(kJoinThreads), size_t(l.grid) * 4, st,
+                      true, a, p);
+}
+
+template <int HD, int RM>
+cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
+    return (a.type == KV_F32 ? decode_n<HD, RM, 3> : decode_n<HD, RM, 2>)(c, a, call, ws, st);
+}
+
 template <class T>
 cudaError_t attn_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, cudaStream_t st) {
     const dim3 grid(unsigned((a.max_q * a.n_heads + 3) / 4), unsigned(call.n));
@@ -105,10 +971,20 @@ cudaError_t attn_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, cud
 
 }  // namespace
 
-size_t kv_attn_ws_bytes(const KvView&, const KvAttnArgs&, const KvCall&) { return 0; }
+size_t kv_attn_ws_bytes(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
+    if (!takes_decode(a)) return 0;
+    const DecLaunch l = dec_launch(c, a, call);
+    return l.even ? size_t(l.grid) * (2 * dec_rm(a) * (c.hd + 2) * 4 + sizeof(int4)) : 0;
+}
 
-cudaError_t launch_kv_attention(const KvView& c, const KvAttnArgs& a, const KvCall& call, void*, cudaStream_t st) {
+cudaError_t launch_kv_attention(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
     if (call.n == 0 || call.n_tok == 0) return cudaSuccess;
+    if (takes_decode(a)) {
+        const int rm = dec_rm(a);
+        if (c.hd == 64)
+            return rm == 4 ? decode_t<64, 4>(c, a, call, ws, st) : rm == 8 ? decode_t<64, 8>(c, a, call, ws, st) : decode_t<64, 16>(c, a, call, ws, st);
+        return rm == 4 ? decode_t<128, 4>(c, a, call, ws, st) : rm == 8 ? decode_t<128, 8>(c, a, call, ws, st) : decode_t<128, 16>(c, a, call, ws, st);
+    }
     return a.type == KV_F32 ? attn_t<float>(c, a, call, st)
          : a.type == KV_F16 ? attn_t<__half>(c, a, call, st) : attn_t<__nv_bfloat16>(c, a, call, st);
 }

@@ -94,6 +94,8 @@ int attn_args(const qb::KvView& v, int layer, const void* q, int dtype, long lon
         return set_err(QNT_ERR_INVALID, "bad max_q, max_len or window");
     if (n_tok > 0 && q_stride < (long long)n_heads * v.hd && n_tok > 1)
         return set_err(QNT_ERR_INVALID, "q_stride is smaller than a token's heads");
+    if ((long long)n * v.n_kv * ((long long)v.max_pages * v.pt / 128 + 2) > 0x7fffffffLL)
+        return set_err(QNT_ERR_UNSUPPORTED, "sequences x heads x longest length is too large for one call");
     a->q = q;
     a->q_stride = q_stride;
     a->out = out;
