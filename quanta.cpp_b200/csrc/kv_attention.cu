@@ -22,85 +22,6 @@ __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// One warp per (token, head), 32 keys at a time: lane l scores key l, then lane l sums dims l, l + 32, ...
-template <class T, int HD>
-__global__ void __launch_bounds__(128) k_kv_attn(KvView c, KvAttnArgs a, KvCall call) {
-    __shared__ float sq[4][HD], sw[4][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int j = blockIdx.y;
-    const int t0 = __ldg(call.starts + j), m = min(__ldg(call.starts + j + 1), call.n_tok) - t0, seq = __ldg(call.seqs + j);
-    if (t0 < 0 || m <= 0) return;
-    if (seq < 0 || seq >= c.max_seqs || m > a.max_q) {
-        set_error(c.status, ERR_BAD_POS);
-        return;
-    }
-    const int len = min(__ldg(c.lens + seq), c.max_pages << c.pt_shift);
-    for (int row = blockIdx.x * 4 + warp; row < m * a.n_heads; row += gridDim.x * 4) {
-        const int i = row / a.n_heads, h = row % a.n_heads, head = h / a.group, pos = len - m + i;
-        const T* q = static_cast<const T*>(a.q) + (long long)(t0 + i) * a.q_stride + h * HD;
-        __syncwarp();
-        for (int d = lane; d < HD; d += 32) sq[warp][d] = to_f(q[d]);
-        __syncwarp();
-        float top = -INFINITY, sum = 0.f, o[HD / 32] = {};
-        const int j0 = a.window ? max(0, pos - a.window + 1) : 0;
-        for (int k0 = j0 & ~31; k0 <= pos; k0 += 32) {
-            const int k = k0 + lane;
-            float s = -INFINITY, vs = 0.f;
-            if (k >= j0 && k <= pos) {
-                int page = __ldg(c.table + size_t(seq) * c.max_pages + (k >> c.pt_shift));
-                if (page < 0 || page >= c.n_pages) {
-                    set_error(c.status, ERR_BAD_POS);
-                    page = 0;
-                }
-                const int t = k & (c.pt - 1);
-                const size_t ak = c.at(page, a.layer, 0, head), av = c.at(page, a.layer, 1, head);
-                float acc = 0.f;
-                for (int g = 0; g < HD / 16; ++g) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(c.codes + ak * c.tile() + (size_t(g) * c.pt + t) * 16);
-                    const int8_t* b = reinterpret_cast<const int8_t*>(&w);
-#pragma unroll
-                    for (int z = 0; z < 16; ++z) acc += sq[warp][16 * g + z] * float(b[z]);
-                }
-                s = acc * (a.scale * __ldg(c.scales + ak * (c.pt / 16) + t / 16));
-                vs = __ldg(c.scales + av * (c.pt / 16) + t / 16);
-            }
-            float now = s;
-#pragma unroll
-            for (int z = 16; z > 0; z >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, z));
-            now = fmaxf(now, top);
-            const float keep = top == -INFINITY ? 0.f : expf(top - now);
-            const float p = s == -INFINITY ? 0.f : expf(s - now);
-            top = now;
-            sum = sum * keep + p;
-            __syncwarp();
-            sw[warp][lane] = p * vs;
-            __syncwarp();
-#pragma unroll
-            for (int u = 0; u < HD / 32; ++u) o[u] *= keep;
-            for (int z = 0; z < 32; z += 16) {
-                if (k0 + z > pos || k0 + z + 16 <= j0) continue;
-                int page = __ldg(c.table + size_t(seq) * c.max_pages + ((k0 + z) >> c.pt_shift));
-                if (page < 0 || page >= c.n_pages) page = 0;
-                const int8_t* tile = c.codes + c.at(page, a.layer, 1, head) * c.tile() + size_t(((k0 + z) & (c.pt - 1)) / 16) * HD * 16;
-                for (int u = 0; u < HD / 32; ++u) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(tile + (lane + 32 * u) * 16);
-                    const int8_t* b = reinterpret_cast<const int8_t*>(&w);
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) o[u] += k0 + z + y <= pos && k0 + z + y >= j0 ? sw[warp][z + y] * float(b[y]) : 0.f;
-                }
-            }
-        }
-#pragma unroll
-        for (int z = 16; z > 0; z >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);
-        const bool none = pos < 0;
-        T* out = static_cast<T*>(a.out) + (size_t(t0 + i) * a.n_heads + h) * HD;
-#pragma unroll
-        for (int u = 0; u < HD / 32; ++u) put(out + lane + 32 * u, none ? 0.f : o[u] / sum);
-        if (a.lse && lane == 0) a.lse[size_t(t0 + i) * a.n_heads + h] = none ? -INFINITY : top + logf(sum);
-    }
-}
-
-
 // ---------------------------------------------------------------- few query rows per kv head (decode)
 //
 //   S^T [128 keys][3 digits x RM rows] = K tile [128][HD] . Q digits     int8 tensor cores, K codes as they lie in the cache
@@ -125,6 +46,7 @@ constexpr int kTileKeys = 128;
 constexpr float kDigitMax = 8323072.0f;  // 127 * 256^2: three digits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kFlush = 16;               // tiles whose O stays in TMEM
+constexpr float kShift = 32.f;           // log2: weights are exp(s - ref) 2^kShift, so that none that f32 can hold is flushed
 constexpr float kRaise = 32.f;           // log2: how far a score may pass the reference
 
 template <int HD, int RM, int NP>
@@ -188,6 +110,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float ex2_full(float x) {  // results below 2^-126 too
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float warp_max_redux(float x) {
@@ -591,7 +518,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 tmem_ready(d0);
                 tc_fence_before();
 #pragma unroll
-                for (int r = 0; r < RM; ++r) s[r] = fmaf(join_digits(d2[r], d1[r], d0[r]), ks * fq[r], -ref[r]);
+                for (int r = 0; r < RM; ++r) s[r] = fmaf(join_digits(d2[r], d1[r], d0[r]), ks * fq[r], -ref[r]);  // (ref less kShift)
             }
             if (prep) {
                 struct alignas(E < 4 ? E : 4) Bytes {
@@ -666,17 +593,17 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                     }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < RM; ++r) high = high || s[r] > kRaise;
+                    for (int r = 0; r < RM; ++r) high = high || s[r] > kRaise + kShift;
                 }
                 bool any = bar_any(high || !ok);
                 if (had) {
 #pragma unroll
                     for (int r = 0; r < RM; ++r) {
                         if (can >> r & 1) {
-                            ref[r] = first_ref[i & 1][r];
+                            ref[r] = first_ref[i & 1][r] - kShift;
                             s[r] -= ref[r];
                         }
-                        high = high || s[r] > kRaise;
+                        high = high || s[r] > kRaise + kShift;
                     }
                     unset &= ~can;
                     any = bar_any(high) || any;
@@ -715,12 +642,12 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
 #pragma unroll
                     for (int r = 0; r < RM; ++r) {
                         const float top = fmaxf(fmaxf(tile_max[0][r], tile_max[1][r]), fmaxf(tile_max[2][r], tile_max[3][r]));
-                        if (top > kRaise) {
-                            ref[r] += top;
-                            s[r] -= top;
-                            const float f = ex2(-top);
-                            acc[r] *= f;
-                            sum[r] *= f;
+                        if (top > kRaise + kShift) {
+                            ref[r] += top - kShift;
+                            s[r] -= top - kShift;
+                            const float f = ex2(0.5f * (kShift - top));  // by halves: the factor may be below 2^-126
+                            acc[r] = acc[r] * f * f;
+                            sum[r] = sum[r] * f * f;
                         }
                     }
                 }
@@ -884,7 +811,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan 
     float l = 0.f;
 #pragma unroll 1
     for (int x = tid; x < n; x += kJoinThreads) {
-        const float w = ex2(weight[x] - ref);
+        const float w = ex2_full(weight[x] - ref);
         weight[x] = w;
         l += w * (n <= kJoinThreads ? ml.y : __ldcg(plan.ml + slot(x) * 2 + 1));
     }
@@ -906,6 +833,530 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan 
     const bool none = top == -INFINITY && l == 0.f;
     store_out(a.out, a.type, row * HD + d, none ? 0.f : o / l);
     if (a.lse && d == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+}
+
+// ---------------------------------------------------------------- many query rows per kv head (chunks of a prompt, drafts)
+//
+// A CTA takes 128 WG query rows (token-major: row r is query r / group, head r % group of the kv head) and a stretch of keys,
+// 64 at a time.  S = Q K^T and O += W V run on the 16-bit tensor cores; K and V codes become 16-bit numbers, exactly, once per
+// tile for all rows.
+//   float32 queries: bf16 operands, a query and a weight W = exp(s - ref) vs as the sum of three bf16 pieces (24 bits each)
+//   16-bit queries: f16 operands, one piece.  Queries are exact (a row is first scaled by a power of two); a weight's 11 bits
+//     cost as much as the result's own rounding to f16.  vs is divided by a power of two near the first tile's largest, and
+//     W held below 2^15, so that f16's range serves.
+//   warps 0 .. 4 WG - 1  softmax, thread = row: S from TMEM, weights back to TMEM (the A operand of the second product); the
+//                        reference of a row is raised only when a score passes it by 2^4 (O is then scaled in TMEM)
+//   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
+//                        to 16-bit operands
+//   last warp            issues the MMAs: S of tile i + 1 runs beside the softmax of tile i
+template <int HD, bool F32>
+struct Chunk {
+    static constexpr int WG = F32 && HD == 128 ? 1 : 2;  // row groups of 128: what shared memory holds of the queries
+    static constexpr int NP = F32 ? 3 : 1;               // pieces of a query and of a weight
+    static constexpr int rows = 128 * WG;
+    static constexpr int threads = 128 * WG + 128 + 32;
+    static constexpr int keys = 64;
+    static constexpr int q_bytes = 128 * HD * 2;         // a piece of a row group: [HD / 8][128 rows][8]
+    static constexpr int kv_bytes = keys * HD * 2;       // K: [HD / 8][64 keys][8], V: [8 groups of 8 keys][HD][8]
+    static constexpr int smem = WG * NP * q_bytes + 4 * kv_bytes + 2 * keys * HD + 128;
+    static constexpr int p_cols = NP * keys / 2;
+    static constexpr int s_at = 0, p_at = 64 * WG, o_at = p_at + p_cols * WG;  // TMEM columns
+    static constexpr int tmem_cols = 512;
+    static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // bf16 or f16 operands
+    static constexpr uint32_t idesc_s = (1u << 4) | fmt | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    static constexpr float shift = F32 ? kShift : 7.f;   // log2: weights carry 2^shift
+    static_assert(o_at + HD * WG <= 512, "TMEM");
+};
+constexpr float kChunkRaise = 4.f;
+
+struct ChunkPlan {
+    int splits;  // stretches of keys per row tile
+    float* ml;   // [n_tok * n_heads][splits][2] maximum (log2) and sum, if splits > 1
+    float* o;    // [n_tok * n_heads][splits][HD]
+};
+
+// 4 int8 codes -> 4 f16, exactly: 1024 + (code + 128), less 1152.
+__device__ __forceinline__ uint2 codes_f16(unsigned w) {
+    w ^= 0x80808080u;
+    const unsigned a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const __half2 x = __hsub2(reinterpret_cast<const __half2&>(a), off), y = __hsub2(reinterpret_cast<const __half2&>(b), off);
+    return make_uint2(reinterpret_cast<const unsigned&>(x), reinterpret_cast<const unsigned&>(y));
+}
+
+// 8 consecutive elements of a query row as f32; vec: the row is 16-byte aligned.
+__device__ __forceinline__ void load_q8(const void* q, KvType t, long long i, bool vec, float (&x)[8]) {
+    if (vec && t == KV_F32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + i);
+        const float4 a = __ldg(p), b = __ldg(p + 1);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else if (vec) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(q) + i));
+        const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            if (t == KV_F16) {
+                const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[z]));
+                x[2 * z] = f.x;
+                x[2 * z + 1] = f.y;
+            } else {
+                x[2 * z] = __uint_as_float(w[z] << 16);
+                x[2 * z + 1] = __uint_as_float(w[z] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int z = 0; z < 8; ++z) x[z] = load_q(q, t, i + z);
+    }
+}
+
+template <int HD, bool F32>
+__global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView c, KvAttnArgs a, KvCall call, ChunkPlan plan) {
+    using C = Chunk<HD, F32>;
+    constexpr int WG = C::WG, NP = C::NP;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+    unsigned char* kb = smem + WG * NP * C::q_bytes;   // 2 buffers
+    unsigned char* vb = kb + 2 * C::kv_bytes;          // 2 buffers
+    unsigned char* codes = vb + 2 * C::kv_bytes;       // of the next tile: K's pieces, V's pieces, 16 bytes each, by thread
+    __shared__ uint64_t q_full[WG], k_full[2], v_full[2], k_free[2], v_free[2], s_full[WG], s_free[WG], p_full[WG], o_done[WG], fin;
+    __shared__ __align__(16) float scales[4][8];       // of a tile's 4 blocks: K's, V's
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* ab = &abort_flag;
+
+    // ---- this CTA's rows and keys
+    const int split = blockIdx.x % plan.splits, r0 = int(blockIdx.x / plan.splits) * C::rows, head = blockIdx.y;
+    const SeqWork w = seq_work(c, a, call, blockIdx.z);
+    const int rows = w.m * a.group;
+    if (r0 >= rows) return;
+    const int p0 = w.len - w.m;  // position of the sequence's first query
+    const int hi = p0 + (min(r0 + C::rows, rows) - 1) / a.group + 1;                    // keys [lo, hi) are seen by some row
+    const int lo = a.window ? max(0, p0 + r0 / a.group - a.window + 1) : 0;
+    const int all = hi > lo ? (hi - 1) / C::keys - lo / C::keys + 1 : 0;
+    const int from = int((long long)all * split / plan.splits), nt = int((long long)all * (split + 1) / plan.splits) - from;
+    const int key_base = (lo / C::keys + from) * C::keys;
+    const int wgs = min(WG, (rows - r0 + 127) / 128);  // row groups with rows
+
+    if (tid == 0) {
+        for (int g = 0; g < WG; ++g) {
+            mbar_init(&q_full[g], 128);
+            mbar_init(&s_full[g], 1);
+            mbar_init(&s_free[g], 128);
+            mbar_init(&p_full[g], 128);
+            mbar_init(&o_done[g], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&k_full[b], 128);
+            mbar_init(&v_full[b], 128);
+            mbar_init(&k_free[b], 1);
+            mbar_init(&v_free[b], 1);
+        }
+        mbar_init(&fin, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4 * WG + 4) tmem_alloc(&tmem_base, C::tmem_cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    pdl_launch_dependents();
+
+    if (warp == 4 * WG + 4) {
+        // ---- MMAs
+        bool ok = true;
+        for (int g = 0; g < wgs && nt > 0; ++g) ok = ok && wait_warp(&q_full[g], 0, ab, c.status);
+#pragma unroll 1
+        for (int i = 0; i <= nt && ok && nt > 0; ++i) {
+            if (i < nt) {
+                ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab, c.status);
+#pragma unroll 1
+                for (int g = 0; g < wgs && ok; ++g) {
+                    if (i > 0) ok = wait_warp(&s_free[g], (i - 1) & 1, ab, c.status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t qt = smem_u32(smem + g * NP * C::q_bytes), kt = smem_u32(kb + (i & 1) * C::kv_bytes);
+#pragma unroll
+                        for (int z = 0; z < NP; ++z)
+#pragma unroll
+                            for (int k = 0; k < HD / 16; ++k)
+                                mma_f16(tmem + C::s_at + g * 64, plain_desc(qt + z * C::q_bytes + k * 2 * 2048, 2048, 128),
+                                        plain_desc(kt + k * 2 * C::keys * 16, C::keys * 16, 128), C::idesc_s, z > 0 || k > 0);
+                        mma_commit(&s_full[g]);
+                        if (g == wgs - 1) mma_commit(&k_free[i & 1]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (i > 0 && ok) {
+                const int t = i - 1;
+                ok = wait_warp(&v_full[t & 1], (t >> 1) & 1, ab, c.status);
+#pragma unroll 1
+                for (int g = 0; g < wgs && ok; ++g) {
+                    ok = wait_warp(&p_full[g], t & 1, ab, c.status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t vt = smem_u32(vb + (t & 1) * C::kv_bytes);
+#pragma unroll
+                        for (int z = 0; z < NP; ++z)
+#pragma unroll
+                            for (int k = 0; k < C::keys / 16; ++k)
+                                mma_f16_ts(tmem + C::o_at + g * HD, tmem + C::p_at + g * C::p_cols + z * (C::keys / 2) + k * 8,
+                                           plain_desc(vt + k * 2 * HD * 16, HD * 16, 128), C::idesc_o, t > 0 || z > 0 || k > 0);
+                        mma_commit(&o_done[g]);
+                        if (g == wgs - 1) mma_commit(&v_free[t & 1]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) {
+            mma_commit(&fin);
+            for (unsigned i = 0; i < kWaitLimit && !mbar_try(&fin, 0); ++i) {
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4 * WG) {
+        // ---- codes to operands
+        constexpr int pieces = HD / 32;  // of K and of V, each thread
+        const int ct = tid - 128 * WG, k_shift = c.pt_shift + (HD == 64 ? 6 : 7);
+        const uint32_t mine = smem_u32(codes) + ct * 16;
+        auto page_of = [&](int i) {  // lane b < 4: page of block b of tile i; 0 where no key is seen
+            const int k = key_base + i * C::keys + (lane & 3) * kKvBlock;
+            int page = 0;
+            if (i < nt && k < hi && k + kKvBlock > lo) {
+                page = __ldg(c.table + size_t(w.seq) * c.max_pages + (k >> c.pt_shift));
+                if (page < 0 || page >= c.n_pages) {
+                    set_error(c.status, ERR_BAD_POS);
+                    page = 0;
+                }
+            }
+            return page;
+        };
+        int page = page_of(0);  // of the next tile to copy
+        float ks = 0.f, vs = 0.f;  // its scales, in lanes 0 .. 3
+        auto copy = [&](int i) {
+            const int key0 = key_base + i * C::keys;
+            const size_t kt = c.at(page, a.layer, 0, head);
+            const int in_page = ((key0 + (lane & 3) * kKvBlock) & (c.pt - 1)) / kKvBlock;
+            const int b0 = key0 + (lane & 3) * kKvBlock;
+            const bool seen = b0 < hi && b0 + kKvBlock > lo;  // (what lies in the cache beyond may be anything)
+            ks = seen ? __ldg(c.scales + (kt << (c.pt_shift - 4)) + in_page) : 0.f;
+            vs = seen ? __ldg(c.scales + ((kt + c.n_kv) << (c.pt_shift - 4)) + in_page) : 0.f;
+#pragma unroll
+            for (int x = 0; x < pieces; ++x) {
+                const int key = ct % 64, g = ct / 64 + 2 * x;  // K piece: 16 dims of a key
+                const size_t tl = __shfl_sync(0xffffffffu, (long long)kt, key / kKvBlock);
+                const int8_t* src = c.codes + (tl << k_shift) + (size_t(g) * c.pt + ((key0 + key) & (c.pt - 1))) * 16;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + x * 2048), "l"(src) : "memory");
+            }
+#pragma unroll
+            for (int x = 0; x < pieces; ++x) {
+                const int d = ct % HD, b = ct / HD + x * (128 / HD);  // V piece: 16 keys of a dim
+                const size_t tl = __shfl_sync(0xffffffffu, (long long)kt, b) + c.n_kv;
+                const int8_t* src = c.codes + (tl << k_shift) + (size_t((key0 + b * kKvBlock) & (c.pt - 1)) * HD + d * 16);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (pieces + x) * 2048), "l"(src) : "memory");
+            }
+        };
+        auto convert = [&](unsigned char* to, int pitch, const uint4& v) {  // 16 codes -> 8 + 8 elements, `pitch` bytes apart
+            uint2 x[4];
+            const unsigned w4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int z = 0; z < 4; ++z) x[z] = F32 ? codes_bf16(w4[z]) : codes_f16(w4[z]);
+            *reinterpret_cast<uint4*>(to) = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+            *reinterpret_cast<uint4*>(to + pitch) = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
+        };
+        bool ok = true;
+        if (nt > 0) copy(0);
+        page = page_of(1);
+#pragma unroll 1
+        for (int i = 0; i < nt && ok; ++i) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            uint4 kc[pieces], vc[pieces];
+#pragma unroll
+            for (int x = 0; x < pieces; ++x) {
+                kc[x] = reinterpret_cast<const uint4*>(codes)[x * 128 + ct];
+                vc[x] = reinterpret_cast<const uint4*>(codes)[(pieces + x) * 128 + ct];
+            }
+            if (ct < 4) {  // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
+                scales[i & 3][ct] = fabsf(vs) < INFINITY ? ks : __int_as_float(0x7fffffff);
+                scales[i & 3][4 + ct] = fabsf(vs) < INFINITY ? vs : 0.f;
+            }
+            if (i + 1 < nt) copy(i + 1);
+            page = page_of(i + 2);
+            if (i >= 2) ok = wait_warp(&k_free[i & 1], ((i >> 1) - 1) & 1, ab, c.status);
+            unsigned char* kt = kb + (i & 1) * C::kv_bytes;
+#pragma unroll
+            for (int x = 0; x < pieces; ++x) convert(kt + ((ct / 64 + 2 * x) * 2 * C::keys + ct % 64) * 16, C::keys * 16, kc[x]);
+            fence_async_smem();
+            mbar_arrive(&k_full[i & 1]);
+            if (i >= 2) ok = ok && wait_warp(&v_free[i & 1], ((i >> 1) - 1) & 1, ab, c.status);
+            unsigned char* vt = vb + (i & 1) * C::kv_bytes;
+#pragma unroll
+            for (int x = 0; x < pieces; ++x) convert(vt + ((ct / HD + x * (128 / HD)) * 2 * HD + ct % HD) * 16, HD * 16, vc[x]);
+            fence_async_smem();
+            mbar_arrive(&v_full[i & 1]);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp < 4 * wgs) {
+        // ---- softmax: thread = row
+        const int g = warp >> 2, rt = tid & 127, r = r0 + g * 128 + rt;
+        const bool valid = r < rows, busy = r0 + g * 128 + (warp & 3) * 32 < rows;  // busy: the warp has rows
+        const int qi = valid ? r / a.group : 0, qh = head * a.group + (valid ? r % a.group : 0), pos = p0 + qi;
+        const uint32_t my = tmem + (uint32_t((warp & 3) * 32) << 16);
+        float fac = a.scale * kLog2e;  // score = S * fac * ks, log2
+        if (nt > 0) {
+            unsigned char* qt = smem + g * NP * C::q_bytes + rt * 16;
+            const long long q0 = (long long)(w.t0 + qi) * a.q_stride + (long long)qh * HD;
+            const int size = a.type == KV_F32 ? 4 : 2;
+            const bool vec = !((reinterpret_cast<uintptr_t>(a.q) | uintptr_t(a.q_stride * size)) & 15);
+            float pre = 1.f;
+            if (!F32) {  // a power of two brings the row's largest value to [1, 2)
+                float amax = 0.f;
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 8) {
+                    float x[8];
+                    load_q8(a.q, a.type, q0 + d, vec, x);
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) amax = fmaxf(amax, fabsf(x[z]));
+                }
+                const int e = int(__float_as_uint(amax) >> 23);  // biased exponent
+                if (e > 0 && e < 254) {
+                    pre = __uint_as_float(unsigned(254 - e) << 23);
+                    fac *= __uint_as_float(unsigned(e) << 23);
+                }
+            }
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 8) {
+                float x[8];
+                load_q8(a.q, a.type, q0 + d, vec, x);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int z = 0; z < NP; ++z) {
+                        unsigned o[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * y], x[2 * y + 1]);
+                            o[y] = reinterpret_cast<const unsigned&>(h);
+                            x[2 * y] -= __uint_as_float(o[y] << 16);
+                            x[2 * y + 1] -= __uint_as_float(o[y] & 0xffff0000u);
+                        }
+                        *reinterpret_cast<uint4*>(qt + z * C::q_bytes + d / 8 * 2048) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                } else {
+                    unsigned o[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const __half2 h = __floats2half2_rn(x[2 * y] * pre, x[2 * y + 1] * pre);
+                        o[y] = reinterpret_cast<const unsigned&>(h);
+                    }
+                    *reinterpret_cast<uint4*>(qt + d / 8 * 2048) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&q_full[g]);
+        }
+        float ref = -INFINITY, sum = 0.f, v_ref = 0.f, v_inv = 0.f;  // v_ref: 16-bit weights carry vs / v_ref
+        bool ok = true;
+#pragma unroll 1
+        for (int i = 0; i < nt && ok; ++i) {
+            const int key0 = key_base + i * C::keys;
+            ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab, c.status) && wait_warp(&s_full[g], i & 1, ab, c.status);
+            if (!ok) break;
+            tc_fence_after();
+            const float4 ks = *reinterpret_cast<const float4*>(scales[i & 3]), vs = *reinterpret_cast<const float4*>(scales[i & 3] + 4);
+            int s0[32], s1[32];
+            tmem_ld(my + C::s_at + g * 64, s0);
+            tmem_ld(my + C::s_at + g * 64 + 32, s1);
+            tmem_ld_wait();
+            tmem_ready(s0);
+            tmem_ready(s1);
+            tc_fence_before();
+            mbar_arrive(&s_free[g]);
+            const float f[4] = {ks.x * fac, ks.y * fac, ks.z * fac, ks.w * fac};
+            float s[64];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                s[k] = __int_as_float(s0[k]) * f[k / 16];
+                s[k + 32] = __int_as_float(s1[k]) * f[2 + k / 16];
+            }
+            // do all of the warp's rows see the whole tile?  (rows past the end do as they like)
+            const bool whole = key0 + C::keys - 1 <= pos && (!a.window || key0 > pos - a.window);
+            if (!__all_sync(0xffffffffu, whole)) {
+                const int last = pos - key0, first = a.window ? last - a.window + 1 : -1;
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (k > last || k < first) s[k] = -INFINITY;
+            }
+            float top = s[0];
+#pragma unroll
+            for (int k = 1; k < 64; ++k) top = fmaxf(top, s[k]);
+            const bool up = top > ref + kChunkRaise;
+            const float now = up ? top : ref;
+            float factor = up ? ex2(0.5f * (ref - now)) : 1.f;  // the square root of O's: that may be below 2^-126
+            if (ref == -INFINITY) factor = 0.f;  // (an infinite score as the first reference)
+            float v_factor = 1.f;
+            bool change = up;
+            if (!F32) {  // the same in all threads
+                const float v_max = fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w));
+                if (v_max > 16.f * v_ref) {
+                    const int e = min(max(int(__float_as_uint(v_max) >> 23), 1), 253);
+                    const float next = __uint_as_float(unsigned(e) << 23);
+                    if (v_ref > 0.f) v_factor = v_ref / next;
+                    v_ref = next;
+                    v_inv = __uint_as_float(unsigned(254 - e) << 23);
+                    change = true;
+                }
+            }
+            ref = now;
+            sum = sum * factor * factor;
+            if (i > 0) {  // the product of the last tile has read the weights and written O
+                ok = wait_warp(&o_done[g], (i - 1) & 1, ab, c.status);
+                if (!ok) break;
+                tc_fence_after();
+                if (__any_sync(0xffffffffu, change) && busy) {
+#pragma unroll 1
+                    for (int x = 0; x < HD; x += 16) {
+                        int o[16];
+                        tmem_ld(my + C::o_at + g * HD + x, o);
+                        tmem_ld_wait();
+                        tmem_ready(o);
+                        unsigned n[16];
+#pragma unroll
+                        for (int z = 0; z < 16; ++z) n[z] = __float_as_uint(__int_as_float(o[z]) * v_factor * factor * factor);
+                        tmem_st(my + C::o_at + g * HD + x, n);
+                    }
+                }
+            }
+            if (busy) {
+                const float base = (ref == -INFINITY ? 0.f : ref) - C::shift;
+                const float vr[4] = {F32 ? vs.x : vs.x * v_inv, F32 ? vs.y : vs.y * v_inv, F32 ? vs.z : vs.z * v_inv, F32 ? vs.w : vs.w * v_inv};
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float p[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) p[k] = ex2(s[16 * b + k] - base);
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        part[k & 3] += p[k];
+                        p[k] *= vr[b];
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+                    for (int z = 0; z < NP; ++z) {
+                        unsigned o[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            if constexpr (F32) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * y], p[2 * y + 1]);
+                                o[y] = reinterpret_cast<const unsigned&>(h);
+                                if (z + 1 < NP) {
+                                    p[2 * y] -= __uint_as_float(o[y] << 16);
+                                    p[2 * y + 1] -= __uint_as_float(o[y] & 0xffff0000u);
+                                }
+                            } else {
+                                const __half2 h = __floats2half2_rn(p[2 * y], p[2 * y + 1]);
+                                o[y] = reinterpret_cast<const unsigned&>(h);
+                            }
+                        }
+                        tmem_st(my + C::p_at + g * C::p_cols + z * (C::keys / 2) + b * 8, o);
+                    }
+                }
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            mbar_arrive(&p_full[g]);
+        }
+        // ---- results
+        if (nt > 0) ok = ok && wait_warp(&o_done[g], (nt - 1) & 1, ab, c.status);
+        tc_fence_after();
+        const bool none = sum == 0.f && ref == -INFINITY;
+        const size_t row = size_t(w.t0 + qi) * a.n_heads + qh;
+        const bool direct = plan.splits == 1;
+        const float factor = (F32 ? 1.f : v_ref) * (direct ? none ? 0.f : 1.f / sum : 1.f);
+        if (ok && busy) {
+#pragma unroll 1
+            for (int x = 0; x < HD; x += 16) {
+                int o[16] = {};
+                __syncwarp();
+                if (nt > 0) {
+                    tmem_ld(my + C::o_at + g * HD + x, o);
+                    tmem_ld_wait();
+                    tmem_ready(o);
+                }
+                float y[16];
+#pragma unroll
+                for (int z = 0; z < 16; ++z) y[z] = none ? 0.f : __int_as_float(o[z]) * factor;
+                if (!valid || (!direct && none)) continue;
+                if (!direct || a.type == KV_F32) {
+                    float* to = direct ? static_cast<float*>(a.out) + row * HD + x : plan.o + (row * plan.splits + split) * HD + x;
+#pragma unroll
+                    for (int z = 0; z < 16; z += 4) *reinterpret_cast<float4*>(to + z) = make_float4(y[z], y[z + 1], y[z + 2], y[z + 3]);
+                } else {
+                    unsigned h[8];
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) {
+                        if (a.type == KV_F16) {
+                            const __half2 v = __floats2half2_rn(y[2 * z], y[2 * z + 1]);
+                            h[z] = reinterpret_cast<const unsigned&>(v);
+                        } else {
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(y[2 * z], y[2 * z + 1]);
+                            h[z] = reinterpret_cast<const unsigned&>(v);
+                        }
+                    }
+                    uint4* to = reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.out) + row * HD + x);
+                    to[0] = make_uint4(h[0], h[1], h[2], h[3]);
+                    to[1] = make_uint4(h[4], h[5], h[6], h[7]);
+                }
+            }
+            if (valid) {
+                if (!direct)
+                    reinterpret_cast<float2*>(plan.ml)[row * plan.splits + split] =
+                        make_float2(none ? -INFINITY : ref - C::shift, sum);
+                else if (a.lse)
+                    a.lse[row] = none ? -INFINITY : (ref - C::shift + log2f(sum)) * (1.f / kLog2e);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4 * WG + 4) {
+        tc_fence_after();
+        tmem_free(tmem, C::tmem_cols);
+    }
+}
+
+// Joins the stretches of k_kv_chunk: a warp per (token, head), in order.  Stretches without a key have sum 0 and no O.
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan plan, long long n_rows) {
+    pdl_wait();
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= n_rows) return;
+    const float2* ml = reinterpret_cast<const float2*>(plan.ml) + row * plan.splits;
+    float top = -INFINITY;
+    for (int x = 0; x < plan.splits; ++x) top = fmaxf(top, __ldcg(ml + x).x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o[HD / 32] = {};
+    for (int x = 0; x < plan.splits; ++x) {
+        const float2 p = __ldcg(ml + x);
+        if (p.x == -INFINITY && p.y == 0.f) continue;
+        const float w = ex2_full(p.x - ref);
+        l += p.y * w;
+        const float* src = plan.o + (row * plan.splits + x) * HD + lane;
+#pragma unroll
+        for (int y = 0; y < HD / 32; ++y) o[y] = fmaf(__ldcg(src + 32 * y), w, o[y]);
+    }
+    const bool none = top == -INFINITY && l == 0.f;
+#pragma unroll
+    for (int y = 0; y < HD / 32; ++y) store_out(a.out, a.type, size_t(row) * HD + 32 * y + lane, none ? 0.f : o[y] / l);
+    if (a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
 }
 
 // ---------------------------------------------------------------- host side
@@ -963,16 +1414,40 @@ cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, v
     return (a.type == KV_F32 ? decode_n<HD, RM, 3> : decode_n<HD, RM, 2>)(c, a, call, ws, st);
 }
 
-template <class T>
-cudaError_t attn_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, cudaStream_t st) {
-    const dim3 grid(unsigned((a.max_q * a.n_heads + 3) / 4), unsigned(call.n));
-    return launch_pdl(c.hd == 128 ? k_kv_attn<T, 128> : k_kv_attn<T, 64>, grid, dim3(128), 0, st, false, c, a, call);
+// Stretches of keys per row tile of k_kv_chunk: as many as fill the SMs, of at least 16 key tiles (what a CTA's start and the
+// join cost).
+int chunk_splits(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
+    const int rows = 128 * (a.type == KV_F32 && c.hd == 128 ? 1 : 2);
+    // row tiles: of n_tok queries, and a part-filled one per sequence
+    const long long units = c.n_kv * (((long long)call.n_tok * a.group + rows - 1) / rows + call.n - 1);
+    const long long span = a.window && a.window < a.max_len ? std::min<long long>(a.max_len, (long long)a.window + a.max_q) : a.max_len;
+    return int(std::max<long long>(1, std::min<long long>({(span / 64 + 15) / 16, (2 * 148 + units - 1) / units, 32})));
+}
+
+template <int HD, bool F32>
+cudaError_t chunk_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
+    using C = Chunk<HD, F32>;
+    ChunkPlan p{};
+    p.splits = chunk_splits(c, a, call);
+    const long long n_rows = (long long)call.n_tok * a.n_heads;
+    if (p.splits > 1) {
+        p.o = static_cast<float*>(ws);
+        p.ml = p.o + n_rows * p.splits * HD;
+    }
+    const long long tiles = ((long long)std::min(a.max_q, call.n_tok) * a.group + C::rows - 1) / C::rows;
+    cudaError_t e = launch_pdl(k_kv_chunk<HD, F32>, dim3(unsigned(tiles * p.splits), unsigned(c.n_kv), unsigned(call.n)), dim3(C::threads),
+                               C::smem, st, false, c, a, call, p);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    return launch_pdl(k_kv_chunk_join<HD>, dim3(unsigned((n_rows + 7) / 8)), dim3(256), 0, st, true, a, p, n_rows);
 }
 
 }  // namespace
 
 size_t kv_attn_ws_bytes(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
-    if (!takes_decode(a)) return 0;
+    if (!takes_decode(a)) {
+        const int splits = chunk_splits(c, a, call);
+        return splits > 1 ? size_t(call.n_tok) * a.n_heads * splits * (c.hd + 2) * 4 : 0;
+    }
     const DecLaunch l = dec_launch(c, a, call);
     return l.even ? size_t(l.grid) * (2 * dec_rm(a) * (c.hd + 2) * 4 + sizeof(int4)) : 0;
 }
@@ -985,8 +1460,8 @@ cudaError_t launch_kv_attention(const KvView& c, const KvAttnArgs& a, const KvCa
             return rm == 4 ? decode_t<64, 4>(c, a, call, ws, st) : rm == 8 ? decode_t<64, 8>(c, a, call, ws, st) : decode_t<64, 16>(c, a, call, ws, st);
         return rm == 4 ? decode_t<128, 4>(c, a, call, ws, st) : rm == 8 ? decode_t<128, 8>(c, a, call, ws, st) : decode_t<128, 16>(c, a, call, ws, st);
     }
-    return a.type == KV_F32 ? attn_t<float>(c, a, call, st)
-         : a.type == KV_F16 ? attn_t<__half>(c, a, call, st) : attn_t<__nv_bfloat16>(c, a, call, st);
+    if (c.hd == 64) return a.type == KV_F32 ? chunk_t<64, true>(c, a, call, ws, st) : chunk_t<64, false>(c, a, call, ws, st);
+    return a.type == KV_F32 ? chunk_t<128, true>(c, a, call, ws, st) : chunk_t<128, false>(c, a, call, ws, st);
 }
 
 }  // namespace qb

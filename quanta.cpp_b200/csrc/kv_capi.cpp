@@ -147,11 +147,17 @@ int qnt_kv_read(const qnt_kv_cache* cache, int layer, const int* seqs, const int
 
 size_t qnt_kv_attention_workspace(const qnt_kv_cache* cache, int n_heads, int n, int n_tok, int max_q, int max_len) {
     qb::KvView c;
-    qb::KvAttnArgs a;
-    if (make_view(cache, &c) || check_call(c, reinterpret_cast<const int*>(cache), reinterpret_cast<const int*>(cache), n, n_tok) ||
-        attn_args(c, 0, nullptr, QNT_F32, (long long)n_heads * c.hd, n_heads, n, n_tok, max_q, max_len, 1.f, 0, nullptr, nullptr, &a))
-        return 0;
-    return n == 0 || n_tok == 0 ? 0 : qb::kv_attn_ws_bytes(c, a, qb::KvCall{nullptr, nullptr, n, n_tok});
+    size_t need = 0;
+    if (make_view(cache, &c) || n < 0 || n_tok < 0 || n > c.max_seqs) return 0;
+    if (n == 0 || n_tok == 0) return 0;
+    for (int dtype : {QNT_F32, QNT_F16}) {  // whichever type and window the call will have: a window never needs more
+        qb::KvAttnArgs a;
+        if (attn_args(c, 0, nullptr, dtype, (long long)n_heads * c.hd, n_heads, n, n_tok, max_q, max_len, 1.f, 0, nullptr, nullptr, &a))
+            return 0;
+        const size_t b = qb::kv_attn_ws_bytes(c, a, qb::KvCall{nullptr, nullptr, n, n_tok});
+        if (b > need) need = b;
+    }
+    return need;
 }
 
 int qnt_kv_attention(const qnt_kv_cache* cache, int layer, const void* q, int dtype, long long q_stride, int n_heads,
