@@ -15,9 +15,6 @@ namespace qb {
 
 namespace {
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
@@ -56,11 +53,10 @@ struct Dec {
     static constexpr int stages = 3;                                   // K tiles
     static constexpr int ctas = HD == 64 && RM <= 8 ? 3 : 2;           // per SM: shared memory, registers
     static constexpr int k_bytes = kTileKeys * HD;
-    static constexpr int v_bytes = kTileKeys * HD * 2;                 // bf16: [16 groups of 8 keys][HD][8 keys]
-    static constexpr int w_pitch = WC * 16 + 16;                       // [16 groups of 8 keys] at this pitch: 4 groups, 4 bank quads
-    static constexpr int w_bytes = 16 * w_pitch;
-    static constexpr int q_bytes = HD * NC;
-    static constexpr int smem = stages * k_bytes + k_bytes + v_bytes + q_bytes + w_bytes + 128;
+    static constexpr int v_half = HD * 128;                            // bf16: two halves of 64 keys, [HD rows][128 bytes] swizzled
+    static constexpr int w_half = WC * 128;                            // the same of the weights, [WC rows][128 bytes]
+    static constexpr int q_bytes = (HD * NC + 1023) / 1024 * 1024;     // [NC rows][HD bytes] swizzled, as K's rows
+    static constexpr int smem = stages * k_bytes + k_bytes + 2 * v_half + q_bytes + 2 * w_half + 1024;
     static constexpr int s_cols = NC <= 16 ? 16 : NC <= 32 ? 32 : 64;  // TMEM column pitch of an S buffer
     static constexpr int tmem_need = 2 * s_cols + WC;
     static constexpr int tmem_cols = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : 256;
@@ -82,8 +78,7 @@ struct SeqWork {
     int seq, t0, m, len, lo, tiles;  // keys [lo, len), in tiles of 128 from lo & ~127; tiles >= 1 where m > 0
 };
 
-// (Not inlined: it is called where a unit starts, and code that is not there need not be fetched.)
-__device__ __noinline__ SeqWork seq_work(const KvView& c, const KvAttnArgs& a, const KvCall& call, int j) {
+__device__ __forceinline__ SeqWork seq_work(const KvView& c, const KvAttnArgs& a, const KvCall& call, int j) {
     SeqWork w;
     const int t0 = __ldg(call.starts + j), t1 = __ldg(call.starts + j + 1), seq = __ldg(call.seqs + j);
     const bool known = seq >= 0 && seq < c.max_seqs;
@@ -171,10 +166,10 @@ __device__ __forceinline__ uint2 codes_bf16(unsigned w) {
 
 // What the loading warp tells the others about a unit and about a tile.
 struct UnitRec {
-    int t0, m, len, lo, j, head, tiles;
+    int t0, m, len, lo, head;
     int first;  // this CTA has the unit's first tile
     int cut;    // and not all of them
-    int at;     // the unit's place in the call's cost
+    int owner;  // if cut: the CTA that has its last tile
 };
 struct TileRec {
     long long kt[8];  // of the tile's 8 blocks of 16 tokens: the K tile number (KvView::at), 0 where no key is seen
@@ -188,7 +183,7 @@ constexpr int kUnitCost = 2;
 struct Deal {
     int base, rem;
     __device__ __forceinline__ int begin(int x) const { return x * base + min(x, rem); }
-    __device__ __noinline__ int owner(int t) const {
+    __device__ __forceinline__ int owner(int t) const {
         return t < rem * (base + 1) ? t / (base + 1) : rem + (t - rem * (base + 1)) / base;
     }
 };
@@ -199,11 +194,11 @@ template <int HD, int RM, int NP>
 __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decode(KvView c, KvAttnArgs a, KvCall call, DecPlan plan) {
     using C = Dec<HD, RM, NP>;
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* vb = smem + C::stages * C::k_bytes;
-    unsigned char* qd = vb + C::v_bytes;
-    unsigned char* wb = qd + C::q_bytes;
-    unsigned char* vc = wb + C::w_bytes;  // V codes of the next tile, each thread's pieces in its own places
+    unsigned char* wb = vb + 2 * C::v_half;
+    unsigned char* qd = wb + 2 * C::w_half;
+    unsigned char* vc = qd + C::q_bytes;  // V codes of the next tile, each thread's pieces in its own places
     __shared__ uint64_t k_full[C::stages], listed[4], s_done[2], w_ready[2], o_done, q_ready, fin;
     __shared__ TileRec tile_rec[4];
     __shared__ __align__(16) float scales[4][16];  // of a tile's 8 blocks: K's, V's
@@ -337,10 +332,11 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
             }
         };
         if (n_my > 0) {
-            look(n_my);
-            if (tile == w.tiles) {  // this CTA's part begins after the start of that unit's last tile
-                next_unit();
+#pragma unroll 1
+            for (int again = 0; again < 2; ++again) {
                 look(n_my);
+                if (tile < w.tiles) break;
+                next_unit();  // this CTA's part begins after the start of that unit's last tile
             }
         }
 #pragma unroll 1
@@ -357,11 +353,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 fence_async_smem();  // the copies were made by the generic proxy
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint32_t kt = smem_u32(smem + (s_next % C::stages) * C::k_bytes), qt = smem_u32(qd);
+                    const uint32_t kt = sw_lo(smem_u32(smem + (s_next % C::stages) * C::k_bytes)), qt = sw_lo(smem_u32(qd));
 #pragma unroll
                     for (int k = 0; k < HD / 32; ++k)
-                        mma_i8(tmem + (s_next & 1) * C::s_cols, plain_desc(kt + k * 2 * kTileKeys * 16, kTileKeys * 16, 128),
-                               plain_desc(qt + k * 2 * C::NC * 16, C::NC * 16, 128), C::idesc_s, k > 0);
+                        mma_i8_sw<sw_hi<HD>, sw_hi<HD>, C::idesc_s>(tmem + (s_next & 1) * C::s_cols, kt + 2 * k, qt + 2 * k, k > 0);
                     mma_commit(&s_done[s_next & 1]);
                 }
                 __syncwarp();
@@ -375,12 +370,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                         u.m = w.m;
                         u.len = w.len;
                         u.lo = w.lo;
-                        u.j = j;
                         u.head = head;
-                        u.tiles = w.tiles;
                         u.first = tile == 0;
                         u.cut = end - tile < w.tiles;
-                        u.at = at;
+                        u.owner = u.cut ? deal.owner(at + w.tiles - 1 + (w.tiles > 1 ? kUnitCost : 0)) : 0;
                     }
                 }
                 if (page >= c.n_pages) {  // -1 in the table, or past the pool
@@ -400,7 +393,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 __syncwarp();
                 mbar_arrive(&listed[it & 3]);
                 const int s = it % C::stages;
-                const uint32_t dst = smem_u32(smem + s * C::k_bytes) + lane * 16;
+                const uint32_t dst = smem_u32(smem + s * C::k_bytes);
                 const int step = c.pt * 16;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {  // lane's keys kk * 32 + lane
@@ -410,7 +403,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                     if (live >> (key / kKvBlock) & 1)
 #pragma unroll
                         for (int g = 0; g < HD / 16; ++g)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + g * (kTileKeys * 16) + kk * 512),
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + sw_offset<HD>(key, g)),
                                          "l"(src + g * step)
                                          : "memory");
                 }
@@ -434,12 +427,12 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
-                const uint32_t vt = smem_u32(vb), wt = smem_u32(wb);
+                const uint32_t vt = sw_lo(smem_u32(vb)), wt = sw_lo(smem_u32(wb));
                 const bool keep = !fresh[t & 1];
 #pragma unroll
-                for (int k = 0; k < kTileKeys / 16; ++k)
-                    mma_f16(tmem + 2 * C::s_cols, plain_desc(vt + k * 2 * HD * 16, HD * 16, 128),
-                            plain_desc(wt + k * 2 * C::w_pitch, C::w_pitch, 128), C::idesc_o, keep || k > 0);
+                for (int k = 0; k < kTileKeys / 16; ++k)  // 4 steps of 32 bytes in each half
+                    mma_f16_sw<sw_hi<128>, sw_hi<128>, C::idesc_o>(tmem + 2 * C::s_cols, vt + (k / 4) * (C::v_half >> 4) + 2 * (k % 4),
+                                                                   wt + (k / 4) * (C::w_half >> 4) + 2 * (k % 4), keep || k > 0);
                 mma_commit(&o_done);
             }
             __syncwarp();
@@ -543,7 +536,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 }
 #pragma unroll
                 for (int z = 0; z < 3; ++z)
-                    *reinterpret_cast<Bytes*>(qd + ((d0 / 16) * C::NC + z * RM + qr) * 16 + d0 % 16) = digit[z];
+                    *reinterpret_cast<Bytes*>(qd + sw_offset<HD>(z * RM + qr, d0 / 16) + d0 % 16) = digit[z];
                 if (tid < q_rows) row_off[units & 1][tid] = tid / a.group * a.n_heads + tid % a.group;
                 if (tid % per_row == 0) fac[units & 1][qr] = fine ? (amax * a.scale) * (kLog2e / kDigitMax) : __int_as_float(0x7fffffff);
                 fence_async_smem();
@@ -676,13 +669,14 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                     if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab, c.status) && ok;
                     tc_fence_after();
                 }
-                unsigned char* wt = wb + (tid >> 3) * C::w_pitch + (tid & 7) * 2;
+                unsigned char* wt = wb + (tid >> 6) * C::w_half + (tid & 7) * 2;
+                const int wc = tid >> 3 & 7;  // 16-byte chunk of the half's rows
 #pragma unroll
                 for (int x = 0; x < RM / 2; ++x)
 #pragma unroll
                     for (int z = 0; z < NP; ++z) {
-                        *reinterpret_cast<unsigned short*>(wt + (z * RM + 2 * x) * 16) = (unsigned short)w[x][z];
-                        *reinterpret_cast<unsigned short*>(wt + (z * RM + 2 * x + 1) * 16) = (unsigned short)(w[x][z] >> 16);
+                        *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(z * RM + 2 * x, wc)) = (unsigned short)w[x][z];
+                        *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(z * RM + 2 * x + 1, wc)) = (unsigned short)(w[x][z] >> 16);
                     }
                 asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
@@ -690,9 +684,9 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                     const int b = vblk + x * (128 / HD);
                     const uint4 v = reinterpret_cast<const uint4*>(vc)[x * 128 + tid];
                     const uint2 x0 = codes_bf16(v.x), x1 = codes_bf16(v.y), x2 = codes_bf16(v.z), x3 = codes_bf16(v.w);
-                    uint4* dst = reinterpret_cast<uint4*>(vb) + 2 * b * HD + vd;
-                    dst[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
-                    dst[HD] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+                    unsigned char* dst = vb + (b >> 2) * C::v_half;
+                    *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3))) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+                    *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3) + 1)) = make_uint4(x2.x, x2.y, x3.x, x3.y);
                 }
                 if (tid == 0) fresh[i & 1] = in_tmem == 0;
                 ++in_tmem;
@@ -757,7 +751,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                     else if (a.type == KV_F16) put_rows(static_cast<__half*>(a.out) + row0 * HD, false);
                     else put_rows(static_cast<__nv_bfloat16*>(a.out) + row0 * HD, false);
                     if (tid == 0 && u.first && u.cut)  // the unit's first CTA says which CTAs share it
-                        plan.info[blockIdx.x] = make_int4(deal.owner(u.at + u.tiles - 1 + (u.tiles > 1 ? kUnitCost : 0)), u.t0, u.m, u.head);
+                        plan.info[blockIdx.x] = make_int4(u.owner, u.t0, u.m, u.head);
                     if (bar_any(!ok)) break;  // last_ref and sum_part are read before the next unit writes them
                 }
             }
@@ -840,10 +834,11 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan 
 // A CTA takes 128 WG query rows (token-major: row r is query r / group, head r % group of the kv head) and a stretch of keys,
 // 64 at a time.  S = Q K^T and O += W V run on the 16-bit tensor cores; K and V codes become 16-bit numbers, exactly, once per
 // tile for all rows.
-//   float32 queries: bf16 operands, a query and a weight W = exp(s - ref) vs as the sum of three bf16 pieces (24 bits each)
-//   16-bit queries: f16 operands, one piece.  Queries are exact (a row is first scaled by a power of two); a weight's 11 bits
-//     cost as much as the result's own rounding to f16.  vs is divided by a power of two near the first tile's largest, and
-//     W held below 2^15, so that f16's range serves.
+// A query row is scaled by a power of two and is the sum of f16 pieces: two for float32 (2^-23 of the row's largest value), one,
+// exactly, for 16-bit types.  A weight W = exp(s - ref) vs is
+//   float32 queries: the sum of three bf16 pieces (24 bits, f32's range); V in bf16
+//   16-bit queries: one f16 (11 bits cost as much as the result's own rounding to f16); V in f16.  vs is divided by a power
+//     of two near the first tile's largest, and W held below 2^15, so that f16's range serves.
 //   warps 0 .. 4 WG - 1  softmax, thread = row: S from TMEM, weights back to TMEM (the A operand of the second product); the
 //                        reference of a row is raised only when a score passes it by 2^4 (O is then scaled in TMEM)
 //   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
@@ -851,19 +846,20 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan 
 //   last warp            issues the MMAs: S of tile i + 1 runs beside the softmax of tile i
 template <int HD, bool F32>
 struct Chunk {
-    static constexpr int WG = F32 && HD == 128 ? 1 : 2;  // row groups of 128: what shared memory holds of the queries
-    static constexpr int NP = F32 ? 3 : 1;               // pieces of a query and of a weight
+    static constexpr int WG = F32 && HD == 128 ? 1 : 2;  // row groups of 128: what TMEM holds of them
+    static constexpr int QP = F32 ? 2 : 1;               // pieces of a query
+    static constexpr int NP = F32 ? 3 : 1;               // pieces of a weight
     static constexpr int rows = 128 * WG;
     static constexpr int threads = 128 * WG + 128 + 32;
     static constexpr int keys = 64;
-    static constexpr int q_bytes = 128 * HD * 2;         // a piece of a row group: [HD / 8][128 rows][8]
-    static constexpr int kv_bytes = keys * HD * 2;       // K: [HD / 8][64 keys][8], V: [8 groups of 8 keys][HD][8]
-    static constexpr int smem = WG * NP * q_bytes + 4 * kv_bytes + 2 * keys * HD + 128;
+    // operands in swizzled rows of 128 bytes: of a query piece and of K, HD / 64 slabs of 64 dims; of V, a row per dim
+    static constexpr int q_bytes = 128 * HD * 2, kv_bytes = keys * HD * 2;
+    static constexpr int smem = WG * QP * q_bytes + 4 * kv_bytes + 2 * keys * HD + 1024;
     static constexpr int p_cols = NP * keys / 2;
     static constexpr int s_at = 0, p_at = 64 * WG, o_at = p_at + p_cols * WG;  // TMEM columns
     static constexpr int tmem_cols = 512;
-    static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // bf16 or f16 operands
-    static constexpr uint32_t idesc_s = (1u << 4) | fmt | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // W and V: bf16 or f16
+    static constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     static constexpr float shift = F32 ? kShift : 7.f;   // log2: weights carry 2^shift
     static_assert(o_at + HD * WG <= 512, "TMEM");
@@ -914,10 +910,10 @@ __device__ __forceinline__ void load_q8(const void* q, KvType t, long long i, bo
 template <int HD, bool F32>
 __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView c, KvAttnArgs a, KvCall call, ChunkPlan plan) {
     using C = Chunk<HD, F32>;
-    constexpr int WG = C::WG, NP = C::NP;
+    constexpr int WG = C::WG, QP = C::QP, NP = C::NP;
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
-    unsigned char* kb = smem + WG * NP * C::q_bytes;   // 2 buffers
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* kb = smem + WG * QP * C::q_bytes;   // 2 buffers
     unsigned char* vb = kb + 2 * C::kv_bytes;          // 2 buffers
     unsigned char* codes = vb + 2 * C::kv_bytes;       // of the next tile: K's pieces, V's pieces, 16 bytes each, by thread
     __shared__ uint64_t q_full[WG], k_full[2], v_full[2], k_free[2], v_free[2], s_full[WG], s_free[WG], p_full[WG], o_done[WG], fin;
@@ -979,13 +975,14 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        const uint32_t qt = smem_u32(smem + g * NP * C::q_bytes), kt = smem_u32(kb + (i & 1) * C::kv_bytes);
+                        const uint32_t qt = sw_lo(smem_u32(smem + g * QP * C::q_bytes)), kt = sw_lo(smem_u32(kb + (i & 1) * C::kv_bytes));
 #pragma unroll
-                        for (int z = 0; z < NP; ++z)
+                        for (int z = 0; z < QP; ++z)
 #pragma unroll
-                            for (int k = 0; k < HD / 16; ++k)
-                                mma_f16(tmem + C::s_at + g * 64, plain_desc(qt + z * C::q_bytes + k * 2 * 2048, 2048, 128),
-                                        plain_desc(kt + k * 2 * C::keys * 16, C::keys * 16, 128), C::idesc_s, z > 0 || k > 0);
+                            for (int k = 0; k < HD / 16; ++k)  // 4 steps of 32 bytes in each slab
+                                mma_f16_sw<sw_hi<128>, sw_hi<128>, C::idesc_s>(
+                                    tmem + C::s_at + g * 64, qt + ((z * C::q_bytes + (k / 4) * 128 * 128) >> 4) + 2 * (k % 4),
+                                    kt + ((k / 4) * C::keys * 128 >> 4) + 2 * (k % 4), z > 0 || k > 0);
                         mma_commit(&s_full[g]);
                         if (g == wgs - 1) mma_commit(&k_free[i & 1]);
                     }
@@ -1001,13 +998,14 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        const uint32_t vt = smem_u32(vb + (t & 1) * C::kv_bytes);
+                        const uint32_t vt = sw_lo(smem_u32(vb + (t & 1) * C::kv_bytes));
 #pragma unroll
                         for (int z = 0; z < NP; ++z)
 #pragma unroll
                             for (int k = 0; k < C::keys / 16; ++k)
-                                mma_f16_ts(tmem + C::o_at + g * HD, tmem + C::p_at + g * C::p_cols + z * (C::keys / 2) + k * 8,
-                                           plain_desc(vt + k * 2 * HD * 16, HD * 16, 128), C::idesc_o, t > 0 || z > 0 || k > 0);
+                                mma_f16_ts<sw_hi<128>, C::idesc_o>(tmem + C::o_at + g * HD,
+                                                                   tmem + C::p_at + g * C::p_cols + z * (C::keys / 2) + k * 8, vt + 2 * k,
+                                                                   t > 0 || z > 0 || k > 0);
                         mma_commit(&o_done[g]);
                         if (g == wgs - 1) mma_commit(&v_free[t & 1]);
                     }
@@ -1063,13 +1061,13 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (pieces + x) * 2048), "l"(src) : "memory");
             }
         };
-        auto convert = [&](unsigned char* to, int pitch, const uint4& v) {  // 16 codes -> 8 + 8 elements, `pitch` bytes apart
+        auto convert = [&](unsigned char* to, int row, int chunk, const uint4& v, bool bf16) {  // 16 codes -> chunks `chunk`, + 1 of a row
             uint2 x[4];
             const unsigned w4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int z = 0; z < 4; ++z) x[z] = F32 ? codes_bf16(w4[z]) : codes_f16(w4[z]);
-            *reinterpret_cast<uint4*>(to) = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
-            *reinterpret_cast<uint4*>(to + pitch) = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
+            for (int z = 0; z < 4; ++z) x[z] = bf16 ? codes_bf16(w4[z]) : codes_f16(w4[z]);
+            *reinterpret_cast<uint4*>(to + sw_offset<128>(row, chunk)) = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+            *reinterpret_cast<uint4*>(to + sw_offset<128>(row, chunk + 1)) = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
         };
         bool ok = true;
         if (nt > 0) copy(0);
@@ -1092,13 +1090,16 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
             if (i >= 2) ok = wait_warp(&k_free[i & 1], ((i >> 1) - 1) & 1, ab, c.status);
             unsigned char* kt = kb + (i & 1) * C::kv_bytes;
 #pragma unroll
-            for (int x = 0; x < pieces; ++x) convert(kt + ((ct / 64 + 2 * x) * 2 * C::keys + ct % 64) * 16, C::keys * 16, kc[x]);
+            for (int x = 0; x < pieces; ++x) {  // dims 16 g .. of key ct % 64
+                const int g = ct / 64 + 2 * x;
+                convert(kt + (g / 4) * C::keys * 128, ct % 64, 2 * (g % 4), kc[x], false);
+            }
             fence_async_smem();
             mbar_arrive(&k_full[i & 1]);
             if (i >= 2) ok = ok && wait_warp(&v_free[i & 1], ((i >> 1) - 1) & 1, ab, c.status);
             unsigned char* vt = vb + (i & 1) * C::kv_bytes;
 #pragma unroll
-            for (int x = 0; x < pieces; ++x) convert(vt + ((ct / HD + x * (128 / HD)) * 2 * HD + ct % HD) * 16, HD * 16, vc[x]);
+            for (int x = 0; x < pieces; ++x) convert(vt, ct % HD, 2 * (ct / HD + x * (128 / HD)), vc[x], F32);
             fence_async_smem();
             mbar_arrive(&v_full[i & 1]);
         }
@@ -1111,51 +1112,47 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
         const uint32_t my = tmem + (uint32_t((warp & 3) * 32) << 16);
         float fac = a.scale * kLog2e;  // score = S * fac * ks, log2
         if (nt > 0) {
-            unsigned char* qt = smem + g * NP * C::q_bytes + rt * 16;
+            unsigned char* qt = smem + g * QP * C::q_bytes;
             const long long q0 = (long long)(w.t0 + qi) * a.q_stride + (long long)qh * HD;
             const int size = a.type == KV_F32 ? 4 : 2;
             const bool vec = !((reinterpret_cast<uintptr_t>(a.q) | uintptr_t(a.q_stride * size)) & 15);
-            float pre = 1.f;
-            if (!F32) {  // a power of two brings the row's largest value to [1, 2)
-                float amax = 0.f;
-#pragma unroll 1
-                for (int d = 0; d < HD; d += 8) {
-                    float x[8];
-                    load_q8(a.q, a.type, q0 + d, vec, x);
-#pragma unroll
-                    for (int z = 0; z < 8; ++z) amax = fmaxf(amax, fabsf(x[z]));
-                }
-                const int e = int(__float_as_uint(amax) >> 23);  // biased exponent
-                if (e > 0 && e < 254) {
-                    pre = __uint_as_float(unsigned(254 - e) << 23);
-                    fac *= __uint_as_float(unsigned(e) << 23);
-                }
-            }
-#pragma unroll 1
+            float pre = 1.f, amax = 0.f;  // a power of two brings the row's largest value to [1, 2)
+#pragma unroll 4
             for (int d = 0; d < HD; d += 8) {
                 float x[8];
                 load_q8(a.q, a.type, q0 + d, vec, x);
-                if constexpr (F32) {
 #pragma unroll
-                    for (int z = 0; z < NP; ++z) {
-                        unsigned o[4];
+                for (int z = 0; z < 8; ++z) amax = fmaxf(amax, fabsf(x[z]));
+            }
+            const int e = int(__float_as_uint(amax) >> 23);  // biased exponent
+            if (e > 0 && e < 254) {
+                pre = __uint_as_float(unsigned(254 - e) << 23);
+                fac *= __uint_as_float(unsigned(e) << 23);
+            } else if (e != 255) {  // subnormal numbers or zeros; the largest numbers
+                pre = e == 0 ? 0x1p126f : 0x1p-126f;
+                fac *= e == 0 ? 0x1p-126f : 0x1p126f;
+            }
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                float x[8];
+                load_q8(a.q, a.type, q0 + d, vec, x);
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * y], x[2 * y + 1]);
-                            o[y] = reinterpret_cast<const unsigned&>(h);
-                            x[2 * y] -= __uint_as_float(o[y] << 16);
-                            x[2 * y + 1] -= __uint_as_float(o[y] & 0xffff0000u);
-                        }
-                        *reinterpret_cast<uint4*>(qt + z * C::q_bytes + d / 8 * 2048) = make_uint4(o[0], o[1], o[2], o[3]);
-                    }
-                } else {
+                for (int z = 0; z < 8; ++z) x[z] *= pre;
+#pragma unroll
+                for (int z = 0; z < QP; ++z) {
                     unsigned o[4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        const __half2 h = __floats2half2_rn(x[2 * y] * pre, x[2 * y + 1] * pre);
+                        const __half2 h = __floats2half2_rn(x[2 * y], x[2 * y + 1]);
                         o[y] = reinterpret_cast<const unsigned&>(h);
+                        if (z + 1 < QP) {
+                            const float2 f = __half22float2(h);
+                            x[2 * y] -= f.x;
+                            x[2 * y + 1] -= f.y;
+                        }
                     }
-                    *reinterpret_cast<uint4*>(qt + d / 8 * 2048) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(qt + z * C::q_bytes + (d / 64) * 128 * 128 + sw_offset<128>(rt, d / 8 % 8)) =
+                        make_uint4(o[0], o[1], o[2], o[3]);
                 }
             }
             fence_async_smem();
@@ -1281,7 +1278,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
         const bool direct = plan.splits == 1;
         const float factor = (F32 ? 1.f : v_ref) * (direct ? none ? 0.f : 1.f / sum : 1.f);
         if (ok && busy) {
-#pragma unroll 1
+#pragma unroll 2
             for (int x = 0; x < HD; x += 16) {
                 int o[16] = {};
                 __syncwarp();

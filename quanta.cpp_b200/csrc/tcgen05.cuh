@@ -70,36 +70,43 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+// K-major operands in shared memory with rows of 128 or 64 bytes, swizzled (unswizzled ones were read several times slower):
+// 16-byte chunk c of row r lies at sw_offset<ROW>(r, c); atoms of 8 rows follow each other.  The descriptor of K offset
+// `bytes` (a multiple of 32) into the rows at addr (1024-byte aligned) is {sw_lo(addr + bytes), sw_hi<ROW>}.
+template <int ROW>
+__device__ __forceinline__ uint32_t sw_offset(int r, int c) {
+    static_assert(ROW == 128 || ROW == 64, "bytes of a row");
+    return uint32_t(r) * ROW + uint32_t(ROW == 128 ? c ^ (r & 7) : c ^ (r >> 1 & 3)) * 16;
+}
+__device__ __forceinline__ uint32_t sw_lo(uint32_t addr) { return (addr >> 4) & 0x3FFF | 1u << 16; }
+template <int ROW>
+constexpr uint32_t sw_hi = uint32_t(8 * ROW >> 4) | 1u << 14 | (ROW == 128 ? 2u : 4u) << 29;
+
+// The MMAs on such operands: descriptors as their low words, the high ones constant.
+template <uint32_t AHI, uint32_t BHI, uint32_t IDESC>
+__device__ __forceinline__ void mma_i8_sw(uint32_t tmem_d, uint32_t a, uint32_t b, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1 : 0), "r"(0), "r"(0), "r"(0), "r"(0)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %6, p;\n\t}" ::"r"(tmem_d), "r"(a), "r"(b), "r"(accumulate ? 1 : 0), "n"(AHI),
+        "n"(BHI), "r"(IDESC)
         : "memory");
 }
-
-// The same with A in TMEM: lane = row, a 32-bit column holds two consecutive elements of K.
-__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+template <uint32_t AHI, uint32_t BHI, uint32_t IDESC>
+__device__ __forceinline__ void mma_f16_sw(uint32_t tmem_d, uint32_t a, uint32_t b, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1 : 0), "r"(0), "r"(0), "r"(0), "r"(0)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %6, p;\n\t}" ::"r"(tmem_d), "r"(a), "r"(b), "r"(accumulate ? 1 : 0), "n"(AHI),
+        "n"(BHI), "r"(IDESC)
         : "memory");
 }
-
-// Shared-memory matrix descriptor of an unswizzled K-major operand: core matrices of 8 rows x 16 bytes (128 contiguous
-// bytes), the next 8 rows sbo bytes on, the next 16 bytes of K lbo bytes on.
-__device__ __forceinline__ uint64_t plain_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(lbo >> 4) << 16) | (uint64_t(sbo >> 4) << 32) | (uint64_t(1) << 46);
-}
-
-// Untiled bulk copy global -> shared (16-byte aligned addresses and size), counted in the barrier's bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
+// A in TMEM: lane = row, a 32-bit column holds two consecutive elements of K.
+template <uint32_t BHI, uint32_t IDESC>
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 db, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(accumulate ? 1 : 0),
+        "n"(BHI), "r"(IDESC)
+        : "memory");
 }
 
 // This thread's writes to shared memory become visible to the tensor cores and bulk copies.
