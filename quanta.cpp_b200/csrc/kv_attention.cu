@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
     __shared__ int row_off[2][RM];  // a row's place in out and lse, from its unit's first
     __shared__ int2 scan_part[4];
     __shared__ int first_j, first_head, first_tile, first_at, tiles_from, tiles_to;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
     volatile int* ab = &abort_flag;
 
     if (tid == 0) {
@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base;
-    const int n_my = tiles_to - tiles_from;
+    const uint32_t tmem = uint32_t(warp_same(int(tmem_base)));
+    const int n_my = warp_same(tiles_to - tiles_from);
 
     if (warp == 4) {
         // ---- loads, two tiles ahead, and MMAs
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
             const int t = it - kLead;  // the tile to finish
 #pragma unroll 1
             for (; t >= 0 && s_next <= min(t + 1, n_my - 1) && ok; ++s_next) {  // scores of this tile and of the next one
-                if (tile_rec[s_next & 3].head_of_unit) {  // its query digits are in place
+                if (warp_same(tile_rec[s_next & 3].head_of_unit)) {  // its query digits are in place
                     ok = wait_warp(&q_ready, q_next & 1, ab, c.status);
                     ++q_next;
                 }
@@ -352,13 +352,12 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 if (!ok) break;
                 fence_async_smem();  // the copies were made by the generic proxy
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t kt = sw_lo(smem_u32(smem + (s_next % C::stages) * C::k_bytes)), qt = sw_lo(smem_u32(qd));
+                const uint32_t kt = sw_lo(uint32_t(warp_same(int(smem_u32(smem + (s_next % C::stages) * C::k_bytes)))));
+                const uint32_t qt = sw_lo(uint32_t(warp_same(int(smem_u32(qd)))));
 #pragma unroll
-                    for (int k = 0; k < HD / 32; ++k)
-                        mma_i8_sw<sw_hi<HD>, sw_hi<HD>, C::idesc_s>(tmem + (s_next & 1) * C::s_cols, kt + 2 * k, qt + 2 * k, k > 0);
-                    mma_commit(&s_done[s_next & 1]);
-                }
+                for (int k = 0; k < HD / 32; ++k)
+                    mma_i8_sw<sw_hi<HD>, sw_hi<HD>, C::idesc_s>(tmem + (s_next & 1) * C::s_cols, kt + 2 * k, qt + 2 * k, k > 0);
+                mma_commit_elect(&s_done[s_next & 1]);
                 __syncwarp();
             }
             if (it < n_my && ok) {  // K of tile `it` into stage it % stages (its last user was tile it - stages), its record into it % 4
@@ -426,23 +425,20 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
             ok = ok && wait_warp(&w_ready[t & 1], (t >> 1) & 1, ab, c.status);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t vt = sw_lo(smem_u32(vb)), wt = sw_lo(smem_u32(wb));
-                const bool keep = !fresh[t & 1];
+            {
+                const uint32_t vt = sw_lo(uint32_t(warp_same(int(smem_u32(vb))))), wt = sw_lo(uint32_t(warp_same(int(smem_u32(wb)))));
+                const bool keep = !warp_same(fresh[t & 1]);
 #pragma unroll
                 for (int k = 0; k < kTileKeys / 16; ++k)  // 4 steps of 32 bytes in each half
                     mma_f16_sw<sw_hi<128>, sw_hi<128>, C::idesc_o>(tmem + 2 * C::s_cols, vt + (k / 4) * (C::v_half >> 4) + 2 * (k % 4),
                                                                    wt + (k / 4) * (C::w_half >> 4) + 2 * (k % 4), keep || k > 0);
-                mma_commit(&o_done);
+                mma_commit_elect(&o_done);
             }
             __syncwarp();
         }
-        if (lane == 0) {
-            mma_commit(&fin);
-            for (unsigned i = 0; i < kWaitLimit && !mbar_try(&fin, 0); ++i) {
-            }
+        mma_commit_elect(&fin);
+        for (unsigned i = 0; i < kWaitLimit && !__all_sync(0xffffffffu, mbar_try(&fin, 0)); ++i) {
         }
-        __syncwarp();
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ---- scores, softmax, outputs: thread = key of the tile, then dim of the head
@@ -920,7 +916,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
     __shared__ __align__(16) float scales[4][8];       // of a tile's 4 blocks: K's, V's
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
     volatile int* ab = &abort_flag;
 
     // ---- this CTA's rows and keys
@@ -932,9 +928,9 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
     const int hi = p0 + (min(r0 + C::rows, rows) - 1) / a.group + 1;                    // keys [lo, hi) are seen by some row
     const int lo = a.window ? max(0, p0 + r0 / a.group - a.window + 1) : 0;
     const int all = hi > lo ? (hi - 1) / C::keys - lo / C::keys + 1 : 0;
-    const int from = int((long long)all * split / plan.splits), nt = int((long long)all * (split + 1) / plan.splits) - from;
+    const int from = int((long long)all * split / plan.splits), nt = warp_same(int((long long)all * (split + 1) / plan.splits) - from);
     const int key_base = (lo / C::keys + from) * C::keys;
-    const int wgs = min(WG, (rows - r0 + 127) / 128);  // row groups with rows
+    const int wgs = warp_same(min(WG, (rows - r0 + 127) / 128));  // row groups with rows
 
     if (tid == 0) {
         for (int g = 0; g < WG; ++g) {
@@ -958,7 +954,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base;
+    const uint32_t tmem = uint32_t(warp_same(int(tmem_base)));
     pdl_launch_dependents();
 
     if (warp == 4 * WG + 4) {
@@ -974,19 +970,17 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
                     if (i > 0) ok = wait_warp(&s_free[g], (i - 1) & 1, ab, c.status);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t qt = sw_lo(smem_u32(smem + g * QP * C::q_bytes)), kt = sw_lo(smem_u32(kb + (i & 1) * C::kv_bytes));
+                    const uint32_t qt = sw_lo(uint32_t(warp_same(int(smem_u32(smem + g * QP * C::q_bytes)))));
+                    const uint32_t kt = sw_lo(uint32_t(warp_same(int(smem_u32(kb + (i & 1) * C::kv_bytes)))));
 #pragma unroll
-                        for (int z = 0; z < QP; ++z)
+                    for (int z = 0; z < QP; ++z)
 #pragma unroll
-                            for (int k = 0; k < HD / 16; ++k)  // 4 steps of 32 bytes in each slab
-                                mma_f16_sw<sw_hi<128>, sw_hi<128>, C::idesc_s>(
-                                    tmem + C::s_at + g * 64, qt + ((z * C::q_bytes + (k / 4) * 128 * 128) >> 4) + 2 * (k % 4),
-                                    kt + ((k / 4) * C::keys * 128 >> 4) + 2 * (k % 4), z > 0 || k > 0);
-                        mma_commit(&s_full[g]);
-                        if (g == wgs - 1) mma_commit(&k_free[i & 1]);
-                    }
-                    __syncwarp();
+                        for (int k = 0; k < HD / 16; ++k)  // 4 steps of 32 bytes in each slab
+                            mma_f16_sw<sw_hi<128>, sw_hi<128>, C::idesc_s>(
+                                tmem + C::s_at + g * 64, qt + ((z * C::q_bytes + (k / 4) * 128 * 128) >> 4) + 2 * (k % 4),
+                                kt + ((k / 4) * C::keys * 128 >> 4) + 2 * (k % 4), z > 0 || k > 0);
+                    mma_commit_elect(&s_full[g]);
+                    if (g == wgs - 1) mma_commit_elect(&k_free[i & 1]);
                 }
             }
             if (i > 0 && ok) {
@@ -997,28 +991,22 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
                     ok = wait_warp(&p_full[g], t & 1, ab, c.status);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t vt = sw_lo(smem_u32(vb + (t & 1) * C::kv_bytes));
+                    const uint32_t vt = sw_lo(uint32_t(warp_same(int(smem_u32(vb + (t & 1) * C::kv_bytes)))));
 #pragma unroll
-                        for (int z = 0; z < NP; ++z)
+                    for (int z = 0; z < NP; ++z)
 #pragma unroll
-                            for (int k = 0; k < C::keys / 16; ++k)
-                                mma_f16_ts<sw_hi<128>, C::idesc_o>(tmem + C::o_at + g * HD,
-                                                                   tmem + C::p_at + g * C::p_cols + z * (C::keys / 2) + k * 8, vt + 2 * k,
-                                                                   t > 0 || z > 0 || k > 0);
-                        mma_commit(&o_done[g]);
-                        if (g == wgs - 1) mma_commit(&v_free[t & 1]);
-                    }
-                    __syncwarp();
+                        for (int k = 0; k < C::keys / 16; ++k)
+                            mma_f16_ts<sw_hi<128>, C::idesc_o>(tmem + C::o_at + g * HD,
+                                                               tmem + C::p_at + g * C::p_cols + z * (C::keys / 2) + k * 8, vt + 2 * k,
+                                                               t > 0 || z > 0 || k > 0);
+                    mma_commit_elect(&o_done[g]);
+                    if (g == wgs - 1) mma_commit_elect(&v_free[t & 1]);
                 }
             }
         }
-        if (lane == 0) {
-            mma_commit(&fin);
-            for (unsigned i = 0; i < kWaitLimit && !mbar_try(&fin, 0); ++i) {
-            }
+        mma_commit_elect(&fin);
+        for (unsigned i = 0; i < kWaitLimit && !__all_sync(0xffffffffu, mbar_try(&fin, 0)); ++i) {
         }
-        __syncwarp();
     } else if (warp >= 4 * WG) {
         // ---- codes to operands
         constexpr int pieces = HD / 32;  // of K and of V, each thread

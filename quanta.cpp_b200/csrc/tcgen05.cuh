@@ -82,29 +82,40 @@ __device__ __forceinline__ uint32_t sw_lo(uint32_t addr) { return (addr >> 4) & 
 template <int ROW>
 constexpr uint32_t sw_hi = uint32_t(8 * ROW >> 4) | 1u << 14 | (ROW == 128 ? 2u : 4u) << 29;
 
-// The MMAs on such operands: descriptors as their low words, the high ones constant.
+// The MMAs on such operands: descriptors as their low words, the high ones constant.  The whole (converged) warp makes the
+// call and one elected lane issues: with operands that the compiler knows to be the same in all lanes (warp_same) they go
+// straight to uniform registers.  Issued by a branch on the lane, an MMA cost about 100 cycles of moving its operands.
 template <uint32_t AHI, uint32_t BHI, uint32_t IDESC>
 __device__ __forceinline__ void mma_i8_sw(uint32_t tmem_d, uint32_t a, uint32_t b, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %6, p;\n\t}" ::"r"(tmem_d), "r"(a), "r"(b), "r"(accumulate ? 1 : 0), "n"(AHI),
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t@e tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %6, p;\n\t}" ::"r"(tmem_d), "r"(a), "r"(b), "r"(accumulate ? 1 : 0), "n"(AHI),
         "n"(BHI), "r"(IDESC)
         : "memory");
 }
 template <uint32_t AHI, uint32_t BHI, uint32_t IDESC>
 __device__ __forceinline__ void mma_f16_sw(uint32_t tmem_d, uint32_t a, uint32_t b, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %6, p;\n\t}" ::"r"(tmem_d), "r"(a), "r"(b), "r"(accumulate ? 1 : 0), "n"(AHI),
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %6, p;\n\t}" ::"r"(tmem_d), "r"(a), "r"(b), "r"(accumulate ? 1 : 0), "n"(AHI),
         "n"(BHI), "r"(IDESC)
         : "memory");
 }
+// mma_commit by one elected lane of the warp: the lane that issued the MMAs (the election is the same each time).
+__device__ __forceinline__ void mma_commit_elect(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
+}
+// A value that all lanes hold alike, told to the compiler.
+__device__ __forceinline__ int warp_same(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 // A in TMEM: lane = row, a 32-bit column holds two consecutive elements of K.
 template <uint32_t BHI, uint32_t IDESC>
 __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 db, {%2, %4};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(accumulate ? 1 : 0),
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b64 db, {%2, %4};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(accumulate ? 1 : 0),
         "n"(BHI), "r"(IDESC)
         : "memory");
 }
