@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.h"
 #include "tcgen05.cuh"
@@ -46,8 +47,9 @@ constexpr int kFlush = 16;               // tiles whose O stays in TMEM
 constexpr float kShift = 32.f;           // log2: weights are exp(s - ref) 2^kShift, so that none that f32 can hold is flushed
 constexpr float kRaise = 32.f;           // log2: how far a score may pass the reference
 
-template <int HD, int RM, int NP>
+template <int HD, int RM, class T>
 struct Dec {
+    static constexpr int NP = sizeof(T) == 4 ? 3 : 2;                  // pieces of a weight
     static constexpr int NC = (3 * RM + 15) / 16 * 16;                 // columns of S
     static constexpr int WC = (NP * RM + 15) / 16 * 16;                // columns of O
     static constexpr int stages = 3;                                   // K tiles
@@ -118,26 +120,35 @@ __device__ __forceinline__ float warp_max_redux(float x) {
     return r;
 }
 
-__device__ __forceinline__ float load_q(const void* q, KvType t, long long i) {
-    return t == KV_F32 ? __ldg(static_cast<const float*>(q) + i)
-         : t == KV_F16 ? __half2float(static_cast<const __half*>(q)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(q)[i]);
-}
-__device__ __forceinline__ void store_out(void* o, KvType t, size_t i, float x) {
-    if (t == KV_F32) static_cast<float*>(o)[i] = x;
-    else if (t == KV_F16) static_cast<__half*>(o)[i] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16*>(o)[i] = __float2bfloat16_rn(x);
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+// E consecutive elements; VEC: they lie aligned (E at most 16 bytes).
+template <bool VEC, class T, int E>
+__device__ __forceinline__ void load_row(const T* p, T (&x)[E]) {
+    if constexpr (VEC) {
+        struct alignas(E * sizeof(T)) V {
+            T v[E];
+        };
+        const V w = *reinterpret_cast<const V*>(p);
+#pragma unroll
+        for (int z = 0; z < E; ++z) x[z] = w.v[z];
+    } else {
+#pragma unroll
+        for (int z = 0; z < E; ++z) x[z] = p[z];
+    }
 }
 
-// warp_wait with its loop kept a loop (these kernels are bound by instruction fetches where their code grows).
-__device__ __forceinline__ bool wait_warp(uint64_t* b, unsigned parity, volatile int* abort_flag, unsigned* status) {
+// warp_wait in little code (it stands in a dozen places): a wait that gives up only sets the abort flag, which the kernel turns
+// into its error bit when it ends.
+__device__ __forceinline__ bool wait_warp(uint64_t* b, unsigned parity, volatile int* abort_flag) {
 #pragma unroll 1
-    for (unsigned i = 0; i < kWaitLimit; ++i) {
-        if (__all_sync(0xffffffffu, mbar_try(b, parity))) return true;
-        if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
-    }
-    *abort_flag = 1;
-    set_error(status, ERR_WAIT_TIMEOUT);
-    return false;
+    for (unsigned i = 0; !__all_sync(0xffffffffu, mbar_try(b, parity)); ++i)
+        if (__any_sync(0xffffffffu, *abort_flag != 0) || i == kWaitLimit) {
+            *abort_flag = 1;
+            return false;
+        }
+    return true;
 }
 
 // Barrier of the 128 softmax threads; true for all of them if `bad` holds for one, so that they leave a loop together.
@@ -190,9 +201,10 @@ struct Deal {
 // Tiles of a unit that start in the first `part` of its cost.
 __device__ __forceinline__ int tiles_before(int part, int tiles) { return part <= 0 ? 0 : min(tiles, max(1, part - kUnitCost)); }
 
-template <int HD, int RM, int NP>
-__global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decode(KvView c, KvAttnArgs a, KvCall call, DecPlan plan) {
-    using C = Dec<HD, RM, NP>;
+template <int HD, int RM, class T>
+__global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode(KvView c, KvAttnArgs a, KvCall call, DecPlan plan) {
+    using C = Dec<HD, RM, T>;
+    constexpr int NP = C::NP;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* vb = smem + C::stages * C::k_bytes;
@@ -345,10 +357,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
 #pragma unroll 1
             for (; t >= 0 && s_next <= min(t + 1, n_my - 1) && ok; ++s_next) {  // scores of this tile and of the next one
                 if (warp_same(tile_rec[s_next & 3].head_of_unit)) {  // its query digits are in place
-                    ok = wait_warp(&q_ready, q_next & 1, ab, c.status);
+                    ok = wait_warp(&q_ready, q_next & 1, ab);
                     ++q_next;
                 }
-                ok = ok && wait_warp(&k_full[s_next % C::stages], (s_next / C::stages) & 1, ab, c.status);
+                ok = ok && wait_warp(&k_full[s_next % C::stages], (s_next / C::stages) & 1, ab);
                 if (!ok) break;
                 fence_async_smem();  // the copies were made by the generic proxy
                 tc_fence_after();
@@ -422,7 +434,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 }
             }
             if (t < 0) continue;
-            ok = ok && wait_warp(&w_ready[t & 1], (t >> 1) & 1, ab, c.status);
+            ok = ok && wait_warp(&w_ready[t & 1], (t >> 1) & 1, ab);
             if (!ok) break;
             tc_fence_after();
             {
@@ -461,16 +473,18 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
             const int qr = tid / per_row, d0 = tid % per_row * E;
             bool prep = false;
             int q_rows = 0;
-            float x[E];
+            T x[E];
             if (i + 1 < n_my) {
-                ok = wait_warp(&listed[(i + 1) & 3], ((i + 1) >> 2) & 1, ab, c.status) && ok;
+                ok = wait_warp(&listed[(i + 1) & 3], ((i + 1) >> 2) & 1, ab) && ok;
                 if (tile_rec[(i + 1) & 3].head_of_unit) {
                     const UnitRec& nu = unit_rec[tile_rec[(i + 1) & 3].unit];
                     prep = true;
                     q_rows = nu.m * a.group;
-                    const long long q0 = (long long)(nu.t0 + qr / a.group) * a.q_stride + (nu.head * a.group + qr % a.group) * HD + d0;
-#pragma unroll
-                    for (int y = 0; y < E; ++y) x[y] = qr < q_rows ? load_q(a.q, a.type, q0 + y) : 0.f;
+                    // (rows past the unit's read its first: a load under a condition would be waited for right here)
+                    const int row = qr < q_rows ? qr : 0;
+                    const T* q = static_cast<const T*>(a.q) + (long long)(nu.t0 + row / a.group) * a.q_stride +
+                                 (nu.head * a.group + row % a.group) * HD + d0;
+                    load_row<false>(q, x);
                 }
             }
             float s[RM], vs = 0.f;  // score less ref, log2
@@ -489,12 +503,12 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                         fq[r] = f[r];
                     }
                 }
-                ok = wait_warp(&k_full[i % C::stages], (i / C::stages) & 1, ab, c.status) && ok;
+                ok = wait_warp(&k_full[i % C::stages], (i / C::stages) & 1, ab) && ok;
                 const float ks0 = scales[i & 3][tid >> 4], vs0 = scales[i & 3][8 + (tid >> 4)];
                 // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
                 vs = fabsf(vs0) < INFINITY ? vs0 : 0.f;
                 const float ks = fabsf(vs0) < INFINITY ? ks0 : __int_as_float(0x7fffffff);
-                ok = wait_warp(&s_done[i & 1], (i >> 1) & 1, ab, c.status) && ok;
+                ok = wait_warp(&s_done[i & 1], (i >> 1) & 1, ab) && ok;
                 tc_fence_after();
                 int d2[RM], d1[RM], d0[RM];
                 const uint32_t at = my_tmem + (i & 1) * C::s_cols;
@@ -515,7 +529,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 } digit[3];
                 float amax = 0.f;
 #pragma unroll
-                for (int y = 0; y < E; ++y) amax = max_nan(amax, fabsf(x[y]));
+                for (int y = 0; y < E; ++y) amax = max_nan(amax, fabsf(to_f(x[y])));
 #pragma unroll
                 for (int o = per_row / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 const bool fine = amax < INFINITY;  // else the row's scores, and with them its result, are NaN
@@ -524,7 +538,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 const float inv = fine && amax > 0.f ? __fdividef(kDigitMax, amax * pre) : 0.f;
 #pragma unroll
                 for (int y = 0; y < E; ++y) {
-                    const int x3 = fine ? __float2int_rn(x[y] * pre * inv) : 0;
+                    const int x3 = fine ? __float2int_rn(to_f(x[y]) * pre * inv) : 0;
                     const unsigned z = (unsigned(x3) + 0x808080u) ^ 0x808080u;
                     digit[0].b[y] = (unsigned char)(z >> 16);
                     digit[1].b[y] = (unsigned char)(z >> 8);
@@ -605,7 +619,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                         const float top = warp_max_redux(s[r]);
                         if (lane == 0) tile_max[warp][r] = top;
                     }
-                    if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab, c.status) && ok;
+                    if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab) && ok;
                     tc_fence_after();
                     waited = true;
                     if (bar_any(!ok)) break;
@@ -662,7 +676,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                     }
                 }
                 if (!waited) {
-                    if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab, c.status) && ok;
+                    if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab) && ok;
                     tc_fence_after();
                 }
                 unsigned char* wt = wb + (tid >> 6) * C::w_half + (tid & 7) * 2;
@@ -690,7 +704,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                 mbar_arrive(&w_ready[i & 1]);
                 if (tail) {
                     // ---- the unit's sums over this CTA's keys
-                    ok = wait_warp(&o_done, i & 1, ab, c.status) && ok;
+                    ok = wait_warp(&o_done, i & 1, ab) && ok;
                     tc_fence_after();
                     {
                         int o0[RM], o1[RM], o2[RM];
@@ -743,9 +757,8 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
                             if (r < rows && lane < lanes) put(out + size_t(own_order ? r : off[r]) * HD + dim, o);
                         }
                     };
-                    if (a.type == KV_F32 || u.cut) put_rows(u.cut ? plan.o + slot * HD : static_cast<float*>(a.out) + row0 * HD, u.cut);
-                    else if (a.type == KV_F16) put_rows(static_cast<__half*>(a.out) + row0 * HD, false);
-                    else put_rows(static_cast<__nv_bfloat16*>(a.out) + row0 * HD, false);
+                    if (u.cut) put_rows(plan.o + slot * HD, true);
+                    else put_rows(static_cast<T*>(a.out) + row0 * HD, false);
                     if (tid == 0 && u.first && u.cut)  // the unit's first CTA says which CTAs share it
                         plan.info[blockIdx.x] = make_int4(u.owner, u.t0, u.m, u.head);
                     if (bar_any(!ok)) break;  // last_ref and sum_part are read before the next unit writes them
@@ -765,6 +778,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && abort_flag) set_error(c.status, ERR_WAIT_TIMEOUT);
     if (warp == 4) {
         tc_fence_after();
         tmem_free(tmem, C::tmem_cols);
@@ -774,7 +788,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, NP>::ctas) k_kv_decod
 // Joins the partial sums of the units that k_kv_decode cut: CTA (x, r) row r of the one that its CTA x began, in CTA order.
 constexpr int kJoinThreads = 512;
 
-template <int HD, int RM>
+template <int HD, int RM, class T>
 __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan plan) {
     constexpr int G = kJoinThreads / HD;
     extern __shared__ float weight[];  // [n] of the partials
@@ -821,7 +835,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan 
     for (int q = 0; q < 16; ++q) l += red[1][q];
     const size_t row = size_t(in.y + r / a.group) * a.n_heads + in.w * a.group + r % a.group;
     const bool none = top == -INFINITY && l == 0.f;
-    store_out(a.out, a.type, row * HD + d, none ? 0.f : o / l);
+    put(static_cast<T*>(a.out) + row * HD + d, none ? 0.f : o / l);
     if (a.lse && d == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
 }
 
@@ -840,9 +854,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan 
 //   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
 //                        to 16-bit operands
 //   last warp            issues the MMAs: S of tile i + 1 runs beside the softmax of tile i
-template <int HD, bool F32>
+template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
-    static constexpr int WG = F32 && HD == 128 ? 1 : 2;  // row groups of 128: what TMEM holds of them
+    static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int QP = F32 ? 2 : 1;               // pieces of a query
     static constexpr int NP = F32 ? 3 : 1;               // pieces of a weight
     static constexpr int rows = 128 * WG;
@@ -853,7 +867,8 @@ struct Chunk {
     static constexpr int smem = WG * QP * q_bytes + 4 * kv_bytes + 2 * keys * HD + 1024;
     static constexpr int p_cols = NP * keys / 2;
     static constexpr int s_at = 0, p_at = 64 * WG, o_at = p_at + p_cols * WG;  // TMEM columns
-    static constexpr int tmem_cols = 512;
+    static constexpr int tmem_cols = o_at + HD * WG <= 256 ? 256 : 512;
+    static constexpr int ctas = smem <= 113 * 1024 && tmem_cols == 256 ? 2 : 1;  // per SM
     static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // W and V: bf16 or f16
     static constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
@@ -877,36 +892,11 @@ __device__ __forceinline__ uint2 codes_f16(unsigned w) {
     return make_uint2(reinterpret_cast<const unsigned&>(x), reinterpret_cast<const unsigned&>(y));
 }
 
-// 8 consecutive elements of a query row as f32; vec: the row is 16-byte aligned.
-__device__ __forceinline__ void load_q8(const void* q, KvType t, long long i, bool vec, float (&x)[8]) {
-    if (vec && t == KV_F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + i);
-        const float4 a = __ldg(p), b = __ldg(p + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else if (vec) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(q) + i));
-        const unsigned w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-            if (t == KV_F16) {
-                const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[z]));
-                x[2 * z] = f.x;
-                x[2 * z + 1] = f.y;
-            } else {
-                x[2 * z] = __uint_as_float(w[z] << 16);
-                x[2 * z + 1] = __uint_as_float(w[z] & 0xffff0000u);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int z = 0; z < 8; ++z) x[z] = load_q(q, t, i + z);
-    }
-}
-
-template <int HD, bool F32>
-__global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView c, KvAttnArgs a, KvCall call, ChunkPlan plan) {
-    using C = Chunk<HD, F32>;
-    constexpr int WG = C::WG, QP = C::QP, NP = C::NP;
+template <int HD, class T, int WG>
+__global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::ctas) k_kv_chunk(KvView c, KvAttnArgs a, KvCall call, ChunkPlan plan) {
+    using C = Chunk<HD, T, WG>;
+    constexpr int QP = C::QP, NP = C::NP;
+    constexpr bool F32 = C::F32;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* kb = smem + WG * QP * C::q_bytes;   // 2 buffers
@@ -960,14 +950,14 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
     if (warp == 4 * WG + 4) {
         // ---- MMAs
         bool ok = true;
-        for (int g = 0; g < wgs && nt > 0; ++g) ok = ok && wait_warp(&q_full[g], 0, ab, c.status);
+        for (int g = 0; g < wgs && nt > 0; ++g) ok = ok && wait_warp(&q_full[g], 0, ab);
 #pragma unroll 1
         for (int i = 0; i <= nt && ok && nt > 0; ++i) {
             if (i < nt) {
-                ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab, c.status);
+                ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab);
 #pragma unroll 1
                 for (int g = 0; g < wgs && ok; ++g) {
-                    if (i > 0) ok = wait_warp(&s_free[g], (i - 1) & 1, ab, c.status);
+                    if (i > 0) ok = wait_warp(&s_free[g], (i - 1) & 1, ab);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t qt = sw_lo(uint32_t(warp_same(int(smem_u32(smem + g * QP * C::q_bytes)))));
@@ -985,10 +975,10 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
             }
             if (i > 0 && ok) {
                 const int t = i - 1;
-                ok = wait_warp(&v_full[t & 1], (t >> 1) & 1, ab, c.status);
+                ok = wait_warp(&v_full[t & 1], (t >> 1) & 1, ab);
 #pragma unroll 1
                 for (int g = 0; g < wgs && ok; ++g) {
-                    ok = wait_warp(&p_full[g], t & 1, ab, c.status);
+                    ok = wait_warp(&p_full[g], t & 1, ab);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t vt = sw_lo(uint32_t(warp_same(int(smem_u32(vb + (t & 1) * C::kv_bytes)))));
@@ -1075,7 +1065,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
             }
             if (i + 1 < nt) copy(i + 1);
             page = page_of(i + 2);
-            if (i >= 2) ok = wait_warp(&k_free[i & 1], ((i >> 1) - 1) & 1, ab, c.status);
+            if (i >= 2) ok = wait_warp(&k_free[i & 1], ((i >> 1) - 1) & 1, ab);
             unsigned char* kt = kb + (i & 1) * C::kv_bytes;
 #pragma unroll
             for (int x = 0; x < pieces; ++x) {  // dims 16 g .. of key ct % 64
@@ -1084,7 +1074,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
             }
             fence_async_smem();
             mbar_arrive(&k_full[i & 1]);
-            if (i >= 2) ok = ok && wait_warp(&v_free[i & 1], ((i >> 1) - 1) & 1, ab, c.status);
+            if (i >= 2) ok = ok && wait_warp(&v_free[i & 1], ((i >> 1) - 1) & 1, ab);
             unsigned char* vt = vb + (i & 1) * C::kv_bytes;
 #pragma unroll
             for (int x = 0; x < pieces; ++x) convert(vt, ct % HD, 2 * (ct / HD + x * (128 / HD)), vc[x], F32);
@@ -1100,49 +1090,55 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
         const uint32_t my = tmem + (uint32_t((warp & 3) * 32) << 16);
         float fac = a.scale * kLog2e;  // score = S * fac * ks, log2
         if (nt > 0) {
-            unsigned char* qt = smem + g * QP * C::q_bytes;
-            const long long q0 = (long long)(w.t0 + qi) * a.q_stride + (long long)qh * HD;
-            const int size = a.type == KV_F32 ? 4 : 2;
-            const bool vec = !((reinterpret_cast<uintptr_t>(a.q) | uintptr_t(a.q_stride * size)) & 15);
-            float pre = 1.f, amax = 0.f;  // a power of two brings the row's largest value to [1, 2)
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load_q8(a.q, a.type, q0 + d, vec, x);
+            // the warp's 32 rows, one after the other (coalesced), 8 in flight; lane = HD / 32 dims
+            constexpr int E = HD / 32;
+            unsigned char* qt = smem + g * QP * C::q_bytes + (lane * E / 64) * 128 * 128;
+            const T* q_mine = static_cast<const T*>(a.q) + (long long)(w.t0 + qi) * a.q_stride + (long long)qh * HD;  // this lane's row
+            const bool vec = !((reinterpret_cast<uintptr_t>(a.q) | uintptr_t(a.q_stride * sizeof(T))) & (E * sizeof(T) - 1));
+            auto rows_in = [&](auto aligned) {  // 8 at a time (rows past the end read some other row)
+#pragma unroll 1
+                for (int r8 = 0; r8 < 32; r8 += 8) {
+                    T x[8][E];
 #pragma unroll
-                for (int z = 0; z < 8; ++z) amax = fmaxf(amax, fabsf(x[z]));
-            }
-            const int e = int(__float_as_uint(amax) >> 23);  // biased exponent
-            if (e > 0 && e < 254) {
-                pre = __uint_as_float(unsigned(254 - e) << 23);
-                fac *= __uint_as_float(unsigned(e) << 23);
-            } else if (e != 255) {  // subnormal numbers or zeros; the largest numbers
-                pre = e == 0 ? 0x1p126f : 0x1p-126f;
-                fac *= e == 0 ? 0x1p-126f : 0x1p126f;
-            }
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load_q8(a.q, a.type, q0 + d, vec, x);
+                    for (int y = 0; y < 8; ++y)
+                        load_row<decltype(aligned)::value>(
+                            reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(q_mine), r8 + y)) + lane * E, x[y]);
 #pragma unroll
-                for (int z = 0; z < 8; ++z) x[z] *= pre;
+                    for (int y = 0; y < 8; ++y) {
+                        float f[E], amax = 0.f;
 #pragma unroll
-                for (int z = 0; z < QP; ++z) {
-                    unsigned o[4];
+                        for (int z = 0; z < E; ++z) {
+                            f[z] = to_f(x[y][z]);
+                            amax = fmaxf(amax, fabsf(f[z]));
+                        }
+                        // a power of two brings the row's largest value to [1, 2); 255: not finite, left as it is
+                        const int e = int(__float_as_uint(warp_max_redux(amax)) >> 23);
+                        const int up = e == 255 ? 127 : min(max(254 - e, 1), 253);  // its biased exponent
+                        const float pre = __uint_as_float(unsigned(up) << 23);
+                        if (lane == r8 + y) fac *= __uint_as_float(unsigned(254 - up) << 23);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const __half2 h = __floats2half2_rn(x[2 * y], x[2 * y + 1]);
-                        o[y] = reinterpret_cast<const unsigned&>(h);
-                        if (z + 1 < QP) {
-                            const float2 f = __half22float2(h);
-                            x[2 * y] -= f.x;
-                            x[2 * y + 1] -= f.y;
+                        for (int z = 0; z < E; ++z) f[z] *= pre;
+                        const int row = (warp & 3) * 32 + r8 + y;
+                        unsigned char* to = qt + sw_offset<128>(row, lane * E % 64 / 8) + lane * E % 8 * 2;
+#pragma unroll
+                        for (int z = 0; z < QP; ++z) {
+                            unsigned o[E / 2];
+#pragma unroll
+                            for (int k = 0; k < E / 2; ++k) {
+                                const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+                                o[k] = reinterpret_cast<const unsigned&>(h);
+                                const float2 b = __half22float2(h);
+                                f[2 * k] -= b.x;
+                                f[2 * k + 1] -= b.y;
+                            }
+                            if constexpr (E == 2) *reinterpret_cast<unsigned*>(to + z * C::q_bytes) = o[0];
+                            else *reinterpret_cast<uint2*>(to + z * C::q_bytes) = make_uint2(o[0], o[1]);
                         }
                     }
-                    *reinterpret_cast<uint4*>(qt + z * C::q_bytes + (d / 64) * 128 * 128 + sw_offset<128>(rt, d / 8 % 8)) =
-                        make_uint4(o[0], o[1], o[2], o[3]);
                 }
-            }
+            };
+            if (vec) rows_in(std::true_type{});
+            else rows_in(std::false_type{});
             fence_async_smem();
             mbar_arrive(&q_full[g]);
         }
@@ -1151,7 +1147,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
 #pragma unroll 1
         for (int i = 0; i < nt && ok; ++i) {
             const int key0 = key_base + i * C::keys;
-            ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab, c.status) && wait_warp(&s_full[g], i & 1, ab, c.status);
+            ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab) && wait_warp(&s_full[g], i & 1, ab);
             if (!ok) break;
             tc_fence_after();
             const float4 ks = *reinterpret_cast<const float4*>(scales[i & 3]), vs = *reinterpret_cast<const float4*>(scales[i & 3] + 4);
@@ -1201,7 +1197,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
             ref = now;
             sum = sum * factor * factor;
             if (i > 0) {  // the product of the last tile has read the weights and written O
-                ok = wait_warp(&o_done[g], (i - 1) & 1, ab, c.status);
+                ok = wait_warp(&o_done[g], (i - 1) & 1, ab);
                 if (!ok) break;
                 tc_fence_after();
                 if (__any_sync(0xffffffffu, change) && busy) {
@@ -1259,46 +1255,38 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
             mbar_arrive(&p_full[g]);
         }
         // ---- results
-        if (nt > 0) ok = ok && wait_warp(&o_done[g], (nt - 1) & 1, ab, c.status);
+        if (nt > 0) ok = ok && wait_warp(&o_done[g], (nt - 1) & 1, ab);
         tc_fence_after();
         const bool none = sum == 0.f && ref == -INFINITY;
         const size_t row = size_t(w.t0 + qi) * a.n_heads + qh;
         const bool direct = plan.splits == 1;
         const float factor = (F32 ? 1.f : v_ref) * (direct ? none ? 0.f : 1.f / sum : 1.f);
         if (ok && busy) {
-#pragma unroll 2
-            for (int x = 0; x < HD; x += 16) {
-                int o[16] = {};
-                __syncwarp();
+            // 32 rows x 32 dims at a time through shared memory (the queries are no longer read), so that rows leave whole
+            float* turn = reinterpret_cast<float*>(smem + g * QP * C::q_bytes) + (warp & 3) * 1024;
+            const unsigned write = __ballot_sync(0xffffffffu, valid && (direct || !none));
+            const long long to_mine = direct ? (long long)row * HD : ((long long)row * plan.splits + split) * HD;
+#pragma unroll 1
+            for (int x = 0; x < HD; x += 32) {
+                int o[32];
                 if (nt > 0) {
                     tmem_ld(my + C::o_at + g * HD + x, o);
                     tmem_ld_wait();
                     tmem_ready(o);
                 }
-                float y[16];
 #pragma unroll
-                for (int z = 0; z < 16; ++z) y[z] = none ? 0.f : __int_as_float(o[z]) * factor;
-                if (!valid || (!direct && none)) continue;
-                if (!direct || a.type == KV_F32) {
-                    float* to = direct ? static_cast<float*>(a.out) + row * HD + x : plan.o + (row * plan.splits + split) * HD + x;
-#pragma unroll
-                    for (int z = 0; z < 16; z += 4) *reinterpret_cast<float4*>(to + z) = make_float4(y[z], y[z + 1], y[z + 2], y[z + 3]);
-                } else {
-                    unsigned h[8];
-#pragma unroll
-                    for (int z = 0; z < 8; ++z) {
-                        if (a.type == KV_F16) {
-                            const __half2 v = __floats2half2_rn(y[2 * z], y[2 * z + 1]);
-                            h[z] = reinterpret_cast<const unsigned&>(v);
-                        } else {
-                            const __nv_bfloat162 v = __floats2bfloat162_rn(y[2 * z], y[2 * z + 1]);
-                            h[z] = reinterpret_cast<const unsigned&>(v);
-                        }
+                for (int z = 0; z < 32; ++z) turn[lane * 32 + (z ^ lane)] = none ? 0.f : __int_as_float(o[z]) * factor;
+                __syncwarp();
+                auto rows_out = [&](auto* out) {
+#pragma unroll 8
+                    for (int y = 0; y < 32; ++y) {
+                        const long long to = __shfl_sync(0xffffffffu, to_mine, y);
+                        if (write >> y & 1) put(out + to + x + lane, turn[y * 32 + (lane ^ y)]);
                     }
-                    uint4* to = reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.out) + row * HD + x);
-                    to[0] = make_uint4(h[0], h[1], h[2], h[3]);
-                    to[1] = make_uint4(h[4], h[5], h[6], h[7]);
-                }
+                };
+                if (!direct) rows_out(plan.o);
+                else rows_out(static_cast<T*>(a.out));
+                __syncwarp();
             }
             if (valid) {
                 if (!direct)
@@ -1311,6 +1299,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && abort_flag) set_error(c.status, ERR_WAIT_TIMEOUT);
     if (warp == 4 * WG + 4) {
         tc_fence_after();
         tmem_free(tmem, C::tmem_cols);
@@ -1318,7 +1307,7 @@ __global__ void __launch_bounds__(Chunk<HD, F32>::threads, 1) k_kv_chunk(KvView 
 }
 
 // Joins the stretches of k_kv_chunk: a warp per (token, head), in order.  Stretches without a key have sum 0 and no O.
-template <int HD>
+template <int HD, class T>
 __global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan plan, long long n_rows) {
     pdl_wait();
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -1340,7 +1329,7 @@ __global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan p
     }
     const bool none = top == -INFINITY && l == 0.f;
 #pragma unroll
-    for (int y = 0; y < HD / 32; ++y) store_out(a.out, a.type, size_t(row) * HD + 32 * y + lane, none ? 0.f : o[y] / l);
+    for (int y = 0; y < HD / 32; ++y) put(static_cast<T*>(a.out) + size_t(row) * HD + 32 * y + lane, none ? 0.f : o[y] / l);
     if (a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
 }
 
@@ -1373,64 +1362,84 @@ DecLaunch dec_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
 }
 
 
-template <int HD, int RM, int NP>
-cudaError_t decode_n(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
-    using C = Dec<HD, RM, NP>;
+template <int HD, int RM, class T>
+cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
+    using C = Dec<HD, RM, T>;
     const DecLaunch l = dec_launch(c, a, call);
     DecPlan p{};
     p.even = l.even;
     if (l.even) {
-        unsigned char* b = static_cast<unsigned char*>(ws);
-        p.o = reinterpret_cast<float*>(b);
+        p.o = static_cast<float*>(ws);
         p.ml = p.o + size_t(l.grid) * 2 * RM * HD;
         p.info = reinterpret_cast<int4*>(p.ml + size_t(l.grid) * 2 * RM * 2);
     }
     // with its static part the shared memory passes the default limit of 48 KB
-    cudaError_t e = cudaFuncSetAttribute(k_kv_decode<HD, RM, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
+    cudaError_t e = cudaFuncSetAttribute(k_kv_decode<HD, RM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(k_kv_decode<HD, RM, NP>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
+    e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
     if (e != cudaSuccess || !l.even) return e;
-    return launch_pdl(k_kv_join<HD, RM>, dim3(unsigned(l.grid), unsigned(a.max_q * a.group)), dim3(kJoinThreads), size_t(l.grid) * 4, st,
-                      true, a, p);
+    return launch_pdl(k_kv_join<HD, RM, T>, dim3(unsigned(l.grid), unsigned(a.max_q * a.group)), dim3(kJoinThreads), size_t(l.grid) * 4,
+                      st, true, a, p);
 }
 
-template <int HD, int RM>
-cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
-    return (a.type == KV_F32 ? decode_n<HD, RM, 3> : decode_n<HD, RM, 2>)(c, a, call, ws, st);
-}
+struct ChunkLaunch {
+    int wg, splits;
+};
 
-// Stretches of keys per row tile of k_kv_chunk: as many as fill the SMs, of at least 16 key tiles (what a CTA's start and the
-// join cost).
-int chunk_splits(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
-    const int rows = 128 * (a.type == KV_F32 && c.hd == 128 ? 1 : 2);
-    // row tiles: of n_tok queries, and a part-filled one per sequence
-    const long long units = c.n_kv * (((long long)call.n_tok * a.group + rows - 1) / rows + call.n - 1);
+// Row groups of 128 per CTA and stretches of keys per row tile.  Two groups share the conversion of K and V, but leave half as
+// many CTAs: taken where those fill the SMs.  Stretches: as many as fill the SMs, of at least 8 key tiles (what a CTA's start
+// and the join cost).
+ChunkLaunch chunk_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
+    ChunkLaunch l;
+    const long long rows = (long long)call.n_tok * a.group;
+    auto units = [&](int wg) { return c.n_kv * ((rows + 128 * wg - 1) / (128 * wg) + call.n - 1); };  // a part-filled tile per sequence
     const long long span = a.window && a.window < a.max_len ? std::min<long long>(a.max_len, (long long)a.window + a.max_q) : a.max_len;
-    return int(std::max<long long>(1, std::min<long long>({(span / 64 + 15) / 16, (2 * 148 + units - 1) / units, 32})));
+    l.wg = (a.type == KV_F32 && c.hd == 128) || units(2) < 148 ? 1 : 2;
+    const long long u = units(l.wg);
+    l.splits = int(std::max<long long>(1, std::min<long long>({(span / 64 + 7) / 8, (2 * 148 + u - 1) / u, 32})));
+    return l;
 }
 
-template <int HD, bool F32>
-cudaError_t chunk_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
-    using C = Chunk<HD, F32>;
+template <int HD, class T, int WG>
+cudaError_t chunk_w(const KvView& c, const KvAttnArgs& a, const KvCall& call, int splits, void* ws, cudaStream_t st) {
+    using C = Chunk<HD, T, WG>;
     ChunkPlan p{};
-    p.splits = chunk_splits(c, a, call);
+    p.splits = splits;
     const long long n_rows = (long long)call.n_tok * a.n_heads;
     if (p.splits > 1) {
         p.o = static_cast<float*>(ws);
         p.ml = p.o + n_rows * p.splits * HD;
     }
     const long long tiles = ((long long)std::min(a.max_q, call.n_tok) * a.group + C::rows - 1) / C::rows;
-    cudaError_t e = launch_pdl(k_kv_chunk<HD, F32>, dim3(unsigned(tiles * p.splits), unsigned(c.n_kv), unsigned(call.n)), dim3(C::threads),
+    cudaError_t e = launch_pdl(k_kv_chunk<HD, T, WG>, dim3(unsigned(tiles * p.splits), unsigned(c.n_kv), unsigned(call.n)), dim3(C::threads),
                                C::smem, st, false, c, a, call, p);
     if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_pdl(k_kv_chunk_join<HD>, dim3(unsigned((n_rows + 7) / 8)), dim3(256), 0, st, true, a, p, n_rows);
+    return launch_pdl(k_kv_chunk_join<HD, T>, dim3(unsigned((n_rows + 7) / 8)), dim3(256), 0, st, true, a, p, n_rows);
+}
+
+template <int HD, class T>
+cudaError_t attn_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
+    if (takes_decode(a)) {
+        const int rm = dec_rm(a);
+        return rm == 4 ? decode_t<HD, 4, T>(c, a, call, ws, st) : rm == 8 ? decode_t<HD, 8, T>(c, a, call, ws, st)
+                                                                        : decode_t<HD, 16, T>(c, a, call, ws, st);
+    }
+    const ChunkLaunch l = chunk_launch(c, a, call);
+    if constexpr (sizeof(T) == 2 || HD == 64)
+        if (l.wg == 2) return chunk_w<HD, T, 2>(c, a, call, l.splits, ws, st);
+    return chunk_w<HD, T, 1>(c, a, call, l.splits, ws, st);
+}
+
+template <class T>
+cudaError_t attn_hd(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
+    return c.hd == 64 ? attn_t<64, T>(c, a, call, ws, st) : attn_t<128, T>(c, a, call, ws, st);
 }
 
 }  // namespace
 
 size_t kv_attn_ws_bytes(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     if (!takes_decode(a)) {
-        const int splits = chunk_splits(c, a, call);
+        const int splits = chunk_launch(c, a, call).splits;
         return splits > 1 ? size_t(call.n_tok) * a.n_heads * splits * (c.hd + 2) * 4 : 0;
     }
     const DecLaunch l = dec_launch(c, a, call);
@@ -1439,14 +1448,8 @@ size_t kv_attn_ws_bytes(const KvView& c, const KvAttnArgs& a, const KvCall& call
 
 cudaError_t launch_kv_attention(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
     if (call.n == 0 || call.n_tok == 0) return cudaSuccess;
-    if (takes_decode(a)) {
-        const int rm = dec_rm(a);
-        if (c.hd == 64)
-            return rm == 4 ? decode_t<64, 4>(c, a, call, ws, st) : rm == 8 ? decode_t<64, 8>(c, a, call, ws, st) : decode_t<64, 16>(c, a, call, ws, st);
-        return rm == 4 ? decode_t<128, 4>(c, a, call, ws, st) : rm == 8 ? decode_t<128, 8>(c, a, call, ws, st) : decode_t<128, 16>(c, a, call, ws, st);
-    }
-    if (c.hd == 64) return a.type == KV_F32 ? chunk_t<64, true>(c, a, call, ws, st) : chunk_t<64, false>(c, a, call, ws, st);
-    return a.type == KV_F32 ? chunk_t<128, true>(c, a, call, ws, st) : chunk_t<128, false>(c, a, call, ws, st);
+    return a.type == KV_F32 ? attn_hd<float>(c, a, call, ws, st)
+         : a.type == KV_F16 ? attn_hd<__half>(c, a, call, ws, st) : attn_hd<__nv_bfloat16>(c, a, call, ws, st);
 }
 
 }  // namespace qb
