@@ -321,7 +321,8 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         constexpr int kLead = C::stages - 1;
         SeqWork w = {};
         int j = first_j, head = first_head, tile = first_tile, at = first_at, end = 0, unit = -1;  // of the next tile to load
-        int key0 = 0, page = -1;  // its first key; lane b < 8: the page of block b (-1: no key of it is seen)
+        int key0 = 0, entry = 0;  // its first key; lane b < 8: the table's entry for block b
+        bool live = false;        // and whether a key of it is seen
         bool ok = true, new_unit = true;
         int s_next = 0, q_next = 0;  // next tile whose scores are to be issued, next unit whose queries are to be waited for
         auto look = [&](int left) {  // the page-table entries of the tile, read an iteration before they are used
@@ -331,8 +332,9 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
             }
             key0 = (w.lo / kTileKeys + tile) * kTileKeys;
             const int lo = max(w.lo, key0), hi = min(w.len, key0 + kTileKeys), b0 = key0 + lane * kKvBlock;
-            page = -1;
-            if (lane < 8 && b0 < hi && b0 + kKvBlock > lo) page = __ldg(c.table + size_t(w.seq) * c.max_pages + (b0 >> c.pt_shift)) & 0x7fffffff;
+            live = lane < 8 && b0 < hi && b0 + kKvBlock > lo;
+            // (not under a condition: the load would be waited for where it ends, instead of an iteration later)
+            entry = __ldg(c.table + size_t(w.seq) * c.max_pages + (live ? b0 >> c.pt_shift : 0));
         };
         auto next_unit = [&]() {
             tile = 0;
@@ -387,12 +389,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         u.owner = u.cut ? deal.owner(at + w.tiles - 1 + (w.tiles > 1 ? kUnitCost : 0)) : 0;
                     }
                 }
-                if (page >= c.n_pages) {  // -1 in the table, or past the pool
-                    set_error(c.status, ERR_BAD_POS);
-                    page = 0;
-                }
-                const long long kt = page < 0 ? 0 : (long long)c.at(page, a.layer, 0, head);
-                const unsigned live = __ballot_sync(0xffffffffu, page >= 0);
+                const bool bad = live && (entry < 0 || entry >= c.n_pages);
+                if (bad) set_error(c.status, ERR_BAD_POS);
+                const long long kt = live ? (long long)c.at(bad ? 0 : entry, a.layer, 0, head) : 0;
+                const unsigned blocks = __ballot_sync(0xffffffffu, live);
                 TileRec& rec = tile_rec[it & 3];
                 if (lane < 8) rec.kt[lane] = kt;
                 if (lane == 0) {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     const int key = kk * 32 + lane;
                     const long long tl = __shfl_sync(0xffffffffu, kt, key / kKvBlock);
                     const int8_t* src = c.codes + (size_t(tl) << (c.pt_shift + (HD == 64 ? 6 : 7))) + (key & (c.pt - 1)) * 16;
-                    if (live >> (key / kKvBlock) & 1)
+                    if (blocks >> (key / kKvBlock) & 1)
 #pragma unroll
                         for (int g = 0; g < HD / 16; ++g)
                             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + sw_offset<HD>(key, g)),
@@ -864,11 +864,11 @@ struct Chunk {
     static constexpr int keys = 64;
     // operands in swizzled rows of 128 bytes: of a query piece and of K, HD / 64 slabs of 64 dims; of V, a row per dim
     static constexpr int q_bytes = 128 * HD * 2, kv_bytes = keys * HD * 2;
-    static constexpr int smem = WG * QP * q_bytes + 4 * kv_bytes + 2 * keys * HD + 1024;
+    static constexpr int smem = WG * QP * q_bytes + 4 * kv_bytes + 2 * keys * HD;
     static constexpr int p_cols = NP * keys / 2;
     static constexpr int s_at = 0, p_at = 64 * WG, o_at = p_at + p_cols * WG;  // TMEM columns
     static constexpr int tmem_cols = o_at + HD * WG <= 256 ? 256 : 512;
-    static constexpr int ctas = smem <= 113 * 1024 && tmem_cols == 256 ? 2 : 1;  // per SM
+    static constexpr int ctas = smem <= 112 * 1024 && tmem_cols == 256 ? 2 : 1;  // per SM (with 1 KB static and 1 KB of the system's each)
     static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // W and V: bf16 or f16
     static constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
@@ -897,8 +897,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
     using C = Chunk<HD, T, WG>;
     constexpr int QP = C::QP, NP = C::NP;
     constexpr bool F32 = C::F32;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* kb = smem + WG * QP * C::q_bytes;   // 2 buffers
     unsigned char* vb = kb + 2 * C::kv_bytes;          // 2 buffers
     unsigned char* codes = vb + 2 * C::kv_bytes;       // of the next tile: K's pieces, V's pieces, 16 bytes each, by thread
@@ -1002,28 +1001,26 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
         constexpr int pieces = HD / 32;  // of K and of V, each thread
         const int ct = tid - 128 * WG, k_shift = c.pt_shift + (HD == 64 ? 6 : 7);
         const uint32_t mine = smem_u32(codes) + ct * 16;
-        auto page_of = [&](int i) {  // lane b < 4: page of block b of tile i; 0 where no key is seen
+        // (loads are not made under a condition: they would be waited for where it ends)
+        int entry = 0;             // lane b < 4 (and every 4th): the table's entry for block b of the next tile to copy
+        bool seen = false;         // and whether a key of it is seen (what lies in the cache beyond may be anything)
+        float ks = 0.f, vs = 0.f;  // the copied tile's scales, where seen
+        bool scaled = false;
+        auto look = [&](int i) {
             const int k = key_base + i * C::keys + (lane & 3) * kKvBlock;
-            int page = 0;
-            if (i < nt && k < hi && k + kKvBlock > lo) {
-                page = __ldg(c.table + size_t(w.seq) * c.max_pages + (k >> c.pt_shift));
-                if (page < 0 || page >= c.n_pages) {
-                    set_error(c.status, ERR_BAD_POS);
-                    page = 0;
-                }
-            }
-            return page;
+            seen = i < nt && k < hi && k + kKvBlock > lo;
+            entry = __ldg(c.table + size_t(w.seq) * c.max_pages + (seen ? k >> c.pt_shift : 0));
         };
-        int page = page_of(0);  // of the next tile to copy
-        float ks = 0.f, vs = 0.f;  // its scales, in lanes 0 .. 3
         auto copy = [&](int i) {
             const int key0 = key_base + i * C::keys;
-            const size_t kt = c.at(page, a.layer, 0, head);
+            const bool bad = seen && (entry < 0 || entry >= c.n_pages);
+            if (bad) set_error(c.status, ERR_BAD_POS);
+            const size_t kt = c.at(seen && !bad ? entry : 0, a.layer, 0, head);
             const int in_page = ((key0 + (lane & 3) * kKvBlock) & (c.pt - 1)) / kKvBlock;
-            const int b0 = key0 + (lane & 3) * kKvBlock;
-            const bool seen = b0 < hi && b0 + kKvBlock > lo;  // (what lies in the cache beyond may be anything)
-            ks = seen ? __ldg(c.scales + (kt << (c.pt_shift - 4)) + in_page) : 0.f;
-            vs = seen ? __ldg(c.scales + ((kt + c.n_kv) << (c.pt_shift - 4)) + in_page) : 0.f;
+            const float* sc = c.scales + (kt << (c.pt_shift - 4)) + in_page;
+            ks = __ldg(sc);
+            vs = __ldg(sc + (c.n_kv << (c.pt_shift - 4)));
+            scaled = seen;
 #pragma unroll
             for (int x = 0; x < pieces; ++x) {
                 const int key = ct % 64, g = ct / 64 + 2 * x;  // K piece: 16 dims of a key
@@ -1048,8 +1045,11 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             *reinterpret_cast<uint4*>(to + sw_offset<128>(row, chunk + 1)) = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
         };
         bool ok = true;
-        if (nt > 0) copy(0);
-        page = page_of(1);
+        if (nt > 0) {
+            look(0);
+            copy(0);
+            look(1);
+        }
 #pragma unroll 1
         for (int i = 0; i < nt && ok; ++i) {
             asm volatile("cp.async.wait_all;" ::: "memory");
@@ -1060,11 +1060,11 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 vc[x] = reinterpret_cast<const uint4*>(codes)[(pieces + x) * 128 + ct];
             }
             if (ct < 4) {  // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
-                scales[i & 3][ct] = fabsf(vs) < INFINITY ? ks : __int_as_float(0x7fffffff);
-                scales[i & 3][4 + ct] = fabsf(vs) < INFINITY ? vs : 0.f;
+                scales[i & 3][ct] = !scaled ? 0.f : fabsf(vs) < INFINITY ? ks : __int_as_float(0x7fffffff);
+                scales[i & 3][4 + ct] = scaled && fabsf(vs) < INFINITY ? vs : 0.f;
             }
             if (i + 1 < nt) copy(i + 1);
-            page = page_of(i + 2);
+            look(i + 2);
             if (i >= 2) ok = wait_warp(&k_free[i & 1], ((i >> 1) - 1) & 1, ab);
             unsigned char* kt = kb + (i & 1) * C::kv_bytes;
 #pragma unroll
@@ -1278,10 +1278,18 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 for (int z = 0; z < 32; ++z) turn[lane * 32 + (z ^ lane)] = none ? 0.f : __int_as_float(o[z]) * factor;
                 __syncwarp();
                 auto rows_out = [&](auto* out) {
-#pragma unroll 8
-                    for (int y = 0; y < 32; ++y) {
-                        const long long to = __shfl_sync(0xffffffffu, to_mine, y);
-                        if (write >> y & 1) put(out + to + x + lane, turn[y * 32 + (lane ^ y)]);
+#pragma unroll 1
+                    for (int y8 = 0; y8 < 32; y8 += 8) {
+                        float v[8];
+                        long long to[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            v[y] = turn[(y8 + y) * 32 + (lane ^ (y8 + y))];
+                            to[y] = __shfl_sync(0xffffffffu, to_mine, y8 + y);
+                        }
+#pragma unroll
+                        for (int y = 0; y < 8; ++y)
+                            if (write >> (y8 + y) & 1) put(out + to[y] + x + lane, v[y]);
                     }
                 };
                 if (!direct) rows_out(plan.o);
