@@ -36,10 +36,13 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 // The work of all (sequence, kv head) units, in order, is dealt evenly to the CTAs (`even`), whatever the lengths; a
 // unit cut between CTAs leaves partial sums in the workspace and k_kv_join adds them up in CTA order.  Where the host's
 // bound on the lengths keeps a unit short, every CTA takes one unit and nothing is joined.
-//   warp 4     loads K (cp.async; bulk copies of the pages' pieces measured about 0.15 us each, whatever their size) and
+//   warp 8     loads K (cp.async; bulk copies of the pages' pieces measured about 0.15 us each, whatever their size) and
 //              the tile's page list two tiles ahead, and issues the MMAs
-//   warps 0-3  thread = key: scores, weights; thread = dim: V codes (copied one tile ahead) to bf16, and O
-constexpr int kDecThreads = 160;
+//   warps 0-7  thread = key, half of the rows (warps 0-3, 4-7): scores, weights; V codes (copied one tile ahead) to bf16; then
+//              thread = dim: O of the same rows.  (One warp per 32 keys for all rows took half again as long: an SM's few warps
+//              wait on the latency of their own instructions.)
+constexpr int kDecSoft = 256;                 // threads of the softmax warps
+constexpr int kDecThreads = kDecSoft + 32;
 constexpr int kTileKeys = 128;
 constexpr float kDigitMax = 8323072.0f;  // 127 * 256^2: three digits
 constexpr float kLog2e = 1.4426950408889634f;
@@ -62,7 +65,7 @@ struct Dec {
     static constexpr int s_cols = NC <= 16 ? 16 : NC <= 32 ? 32 : 64;  // TMEM column pitch of an S buffer
     static constexpr int tmem_need = 2 * s_cols + WC;
     static constexpr int tmem_cols = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : 256;
-    static constexpr int items = HD / 16;                              // V pieces (a dim's 16 tokens) of a thread
+    static constexpr int items = HD * 8 / kDecSoft;                    // V pieces (a dim's 16 tokens) of a thread
     static constexpr uint32_t idesc_s = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NC >> 3) << 17) | (uint32_t(kTileKeys >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(WC >> 3) << 17) | (uint32_t(HD >> 4) << 24);
     static_assert(tmem_need <= 256, "TMEM allocation");
@@ -151,13 +154,13 @@ __device__ __forceinline__ bool wait_warp(uint64_t* b, unsigned parity, volatile
     return true;
 }
 
-// Barrier of the 128 softmax threads; true for all of them if `bad` holds for one, so that they leave a loop together.
+// Barrier of the softmax threads; true for all of them if `bad` holds for one, so that they leave a loop together.
 __device__ __forceinline__ bool bar_any(bool bad) {
     unsigned r;
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"(bad ? 1u : 0u)
+        : "r"(bad ? 1u : 0u), "n"(kDecSoft)
         : "memory");
     return r != 0;
 }
@@ -187,10 +190,10 @@ struct TileRec {
     int key0, unit, head_of_unit, tail_of_unit;
 };
 
-// The call's work is dealt in units of a tile's time: a unit's first tile counts 1 + kUnitCost (its queries, its sums and its
-// outputs cost about as much as that many tiles), the others 1.  CTA x has [x base + min(x, rem), ...) of it, and the tiles
-// that start there.
-constexpr int kUnitCost = 2;
+// The call's work is dealt in units of a tile's time: a unit's first tile counts 1 + kUnitCost (its queries, sums and outputs
+// take about as long as kUnitCost tiles), the others 1.  CTA x has [x base + min(x, rem), ...) of it, and the tiles that start
+// there.
+constexpr int kUnitCost = 1;
 struct Deal {
     int base, rem;
     __device__ __forceinline__ int begin(int x) const { return x * base + min(x, rem); }
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
     __shared__ __align__(16) float fac[2][RM], first_ref[2][RM], last_ref[RM], sum_part[4][RM];
     __shared__ int row_off[2][RM];  // a row's place in out and lse, from its unit's first
     __shared__ int2 scan_part[4];
-    __shared__ int first_j, first_head, first_tile, first_at, tiles_from, tiles_to;
+    __shared__ int start_j, start_head, start_tile, start_at, tiles_from, tiles_to;
     const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
     volatile int* ab = &abort_flag;
 
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         for (int s = 0; s < 4; ++s) mbar_init(&listed[s], 32);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_done[b], 1);
-            mbar_init(&w_ready[b], 128);
+            mbar_init(&w_ready[b], kDecSoft);
         }
         mbar_init(&o_done, 1);
         mbar_init(&q_ready, 128);
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         if (plan.even) plan.info[blockIdx.x] = make_int4(-1, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 4) tmem_alloc(&tmem_base, C::tmem_cols);
+    if (warp == 8) tmem_alloc(&tmem_base, C::tmem_cols);
     pdl_wait();
     pdl_launch_dependents();
 
@@ -290,10 +293,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 const int cost = w.tiles + kUnitCost, all = cost * c.n_kv;
                 if (begin >= before.x && begin < before.x + all) {
                     const int h = (begin - before.x) / cost, t = tiles_before(begin - before.x - h * cost, w.tiles);
-                    first_j = j;  // t == tiles: the first tile is the next unit's
-                    first_head = h;
-                    first_tile = t;
-                    first_at = before.x + h * cost;
+                    start_j = j;  // t == tiles: the first tile is the next unit's
+                    start_head = h;
+                    start_tile = t;
+                    start_at = before.x + h * cost;
                     tiles_from = before.y + h * w.tiles + t;
                 }
                 if (end > before.x && end <= before.x + all) {
@@ -304,32 +307,49 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 before.y += w.tiles * c.n_kv;
             }
         }
-    } else if (tid == 0) {
-        first_j = blockIdx.x / c.n_kv;
-        first_head = blockIdx.x % c.n_kv;
-        first_tile = first_at = tiles_from = 0;
-        tiles_to = seq_work(c, a, call, first_j).tiles;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    int first_j, first_head, first_tile = 0, first_at = 0, n_tiles;  // of the first tile
+    SeqWork first_w = {};
+    if (plan.even) {
+        n_tiles = tiles_to - tiles_from;
+        first_j = n_tiles > 0 ? start_j : 0;
+        first_head = start_head;
+        first_tile = start_tile;
+        first_at = start_at;
+        first_w = seq_work(c, a, call, first_j);
+        if (n_tiles > 0 && first_tile == first_w.tiles) {  // this CTA's part begins after the start of that unit's last tile
+            first_tile = 0;
+            first_at += first_w.tiles + kUnitCost;
+            if (++first_head == c.n_kv) {
+                first_head = 0;
+                do ++first_j;
+                while (first_j < call.n - 1 && __ldg(call.starts + first_j + 1) <= __ldg(call.starts + first_j));
+                first_w = seq_work(c, a, call, first_j);
+            }
+        }
+    } else {
+        first_j = blockIdx.x / c.n_kv;
+        first_head = blockIdx.x % c.n_kv;
+        first_w = seq_work(c, a, call, first_j);
+        n_tiles = first_w.tiles;
+    }
     const uint32_t tmem = uint32_t(warp_same(int(tmem_base)));
-    const int n_my = warp_same(tiles_to - tiles_from);
+    const int n_my = warp_same(n_tiles);
 
-    if (warp == 4) {
+    if (warp == 8) {
         // ---- loads, two tiles ahead, and MMAs
         constexpr int kLead = C::stages - 1;
-        SeqWork w = {};
+        SeqWork w = first_w;
         int j = first_j, head = first_head, tile = first_tile, at = first_at, end = 0, unit = -1;  // of the next tile to load
         int key0 = 0, entry = 0;  // its first key; lane b < 8: the table's entry for block b
         bool live = false;        // and whether a key of it is seen
         bool ok = true, new_unit = true;
         int s_next = 0, q_next = 0;  // next tile whose scores are to be issued, next unit whose queries are to be waited for
         auto look = [&](int left) {  // the page-table entries of the tile, read an iteration before they are used
-            if (new_unit) {
-                w = seq_work(c, a, call, j);
-                end = min(w.tiles, tile + left);
-            }
+            if (new_unit) end = min(w.tiles, tile + left);
             key0 = (w.lo / kTileKeys + tile) * kTileKeys;
             const int lo = max(w.lo, key0), hi = min(w.len, key0 + kTileKeys), b0 = key0 + lane * kKvBlock;
             live = lane < 8 && b0 < hi && b0 + kKvBlock > lo;
@@ -343,16 +363,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 head = 0;
                 do ++j;
                 while (j < call.n - 1 && __ldg(call.starts + j + 1) <= __ldg(call.starts + j));
+                w = seq_work(c, a, call, j);
             }
         };
-        if (n_my > 0) {
-#pragma unroll 1
-            for (int again = 0; again < 2; ++again) {
-                look(n_my);
-                if (tile < w.tiles) break;
-                next_unit();  // this CTA's part begins after the start of that unit's last tile
-            }
-        }
+        if (n_my > 0) look(n_my);
 #pragma unroll 1
         for (int it = 0; it < n_my + kLead && ok; ++it) {
             const int t = it - kLead;  // the tile to finish
@@ -455,39 +469,48 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
     } else {
         // ---- scores, softmax, outputs: thread = key of the tile, then dim of the head
         constexpr int lanes = HD == 64 ? 16 : 32;  // rows of O^T of a warp (M = 64 leaves the upper half of each quadrant unused)
-        const int dim = warp * lanes + lane;
-        const uint32_t my_tmem = tmem + (uint32_t(warp * 32) << 16);
-        const int vd = tid % HD, vblk = tid / HD;  // V pieces: dim vd of blocks vblk + x * (128 / HD)
+        constexpr int RH = RM / 2;                 // rows of a thread: r0 ..
+        const int half = warp >> 2, quad = warp & 3, r0 = half * RH, kid = tid & 127;
+        const int dim = quad * lanes + lane;
+        const uint32_t my_tmem = tmem + (uint32_t(quad * 32) << 16) + r0;
+        const int vd = tid % HD, vblk = tid / HD;  // V pieces: dim vd of blocks vblk + x * (kDecSoft / HD)
         const int v_shift = c.pt_shift + (HD == 64 ? 6 : 7);  // log2 of a tile's codes
         bool ok = true;   // a wait that gave up is acted on at the next barrier, by all threads together
         int in_tmem = 0;  // tiles whose sum lies in TMEM
         UnitRec u = {};
         int rows = 0, p0 = 0, units = 0;  // rows of the unit, position of its first query, units so far
         unsigned unset = 0;               // rows without a reference: they have seen no key
-        float ref[RM], sum[RM], acc[RM], fq[RM];  // ref and fq are the same in all threads
+        float ref[RH], sum[RH], acc[RH], fq[RH];  // ref and fq are the same in all threads of a half
 #pragma unroll 1
         for (int i = -1; i < n_my; ++i) {
             // the next tile begins a unit: its query digits, 128 / RM threads per row (loaded here, written below, as soon as
             // this tile's scores are done and qd is free)
             constexpr int per_row = 128 / RM, E = HD / per_row;
-            const int qr = tid / per_row, d0 = tid % per_row * E;
+            const int qr = kid / per_row, d0 = kid % per_row * E;  // (threads 0-127)
             bool prep = false;
             int q_rows = 0;
             T x[E];
             if (i + 1 < n_my) {
-                ok = wait_warp(&listed[(i + 1) & 3], ((i + 1) >> 2) & 1, ab) && ok;
-                if (tile_rec[(i + 1) & 3].head_of_unit) {
+                int nu_t0 = first_w.t0, nu_m = first_w.m, nu_head = first_head;  // the first unit's is known before it is listed
+                prep = i < 0;
+                if (i >= 0) {
+                    ok = wait_warp(&listed[(i + 1) & 3], ((i + 1) >> 2) & 1, ab) && ok;
+                    prep = tile_rec[(i + 1) & 3].head_of_unit;
                     const UnitRec& nu = unit_rec[tile_rec[(i + 1) & 3].unit];
-                    prep = true;
-                    q_rows = nu.m * a.group;
+                    nu_t0 = nu.t0;
+                    nu_m = nu.m;
+                    nu_head = nu.head;
+                }
+                if (prep) {
+                    q_rows = nu_m * a.group;
                     // (rows past the unit's read its first: a load under a condition would be waited for right here)
                     const int row = qr < q_rows ? qr : 0;
-                    const T* q = static_cast<const T*>(a.q) + (long long)(nu.t0 + row / a.group) * a.q_stride +
-                                 (nu.head * a.group + row % a.group) * HD + d0;
+                    const T* q = static_cast<const T*>(a.q) + (long long)(nu_t0 + row / a.group) * a.q_stride +
+                                 (nu_head * a.group + row % a.group) * HD + d0;
                     load_row<false>(q, x);
                 }
             }
-            float s[RM], vs = 0.f;  // score less ref, log2
+            float s[RH], vs = 0.f;  // score less ref, log2
             if (i >= 0) {
                 const TileRec& rec = tile_rec[i & 3];
                 if (rec.head_of_unit) {
@@ -498,19 +521,19 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     const float* f = fac[units & 1];
                     ++units;
 #pragma unroll
-                    for (int r = 0; r < RM; ++r) {
+                    for (int r = 0; r < RH; ++r) {
                         ref[r] = sum[r] = acc[r] = 0.f;
-                        fq[r] = f[r];
+                        fq[r] = f[r0 + r];
                     }
                 }
                 ok = wait_warp(&k_full[i % C::stages], (i / C::stages) & 1, ab) && ok;
-                const float ks0 = scales[i & 3][tid >> 4], vs0 = scales[i & 3][8 + (tid >> 4)];
+                const float ks0 = scales[i & 3][kid >> 4], vs0 = scales[i & 3][8 + (kid >> 4)];
                 // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
                 vs = fabsf(vs0) < INFINITY ? vs0 : 0.f;
                 const float ks = fabsf(vs0) < INFINITY ? ks0 : __int_as_float(0x7fffffff);
                 ok = wait_warp(&s_done[i & 1], (i >> 1) & 1, ab) && ok;
                 tc_fence_after();
-                int d2[RM], d1[RM], d0[RM];
+                int d2[RH], d1[RH], d0[RH];
                 const uint32_t at = my_tmem + (i & 1) * C::s_cols;
                 tmem_ld(at, d2);
                 tmem_ld(at + RM, d1);
@@ -521,9 +544,9 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 tmem_ready(d0);
                 tc_fence_before();
 #pragma unroll
-                for (int r = 0; r < RM; ++r) s[r] = fmaf(join_digits(d2[r], d1[r], d0[r]), ks * fq[r], -ref[r]);  // (ref less kShift)
+                for (int r = 0; r < RH; ++r) s[r] = fmaf(join_digits(d2[r], d1[r], d0[r]), ks * fq[r], -ref[r]);  // (ref less kShift)
             }
-            if (prep) {
+            if (prep && half == 0) {
                 struct alignas(E < 4 ? E : 4) Bytes {
                     unsigned char b[E];
                 } digit[3];
@@ -551,80 +574,84 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 if (tid % per_row == 0) fac[units & 1][qr] = fine ? (amax * a.scale) * (kLog2e / kDigitMax) : __int_as_float(0x7fffffff);
                 fence_async_smem();
                 mbar_arrive(&q_ready);
-                if (i < 0 && bar_any(!ok)) break;  // else: fac and row_off are read after the barrier below
+            }
+            if (i < 0) {  // (else: fac and row_off are read after the barrier below)
+                if (n_my > 0) ok = wait_warp(&listed[0], 0, ab) && ok;
+                if (bar_any(!ok)) break;
             }
             if (i >= 0) {
                 const TileRec& rec = tile_rec[i & 3];
-                const int key0 = rec.key0, key = key0 + tid;
+                const int key0 = rec.key0, key = key0 + kid;
                 const bool tail = rec.tail_of_unit;
                 const bool seen = key >= u.lo && key < u.len;  // by some row
                 // do all rows see the whole tile?
                 const bool whole = key0 >= u.lo && key0 + kTileKeys <= u.len &&
                                    (u.m == 1 || (key0 + kTileKeys - 1 <= p0 && (!a.window || key0 > u.len - 1 - a.window)));
+                // queries of this thread's first row; the next row is of the next query after g more
+                const int qi0 = u.m == 1 ? 0 : r0 / a.group, g0 = u.m == 1 ? RM : a.group - r0 % a.group;
                 if (!whole) {
-                    if (u.m == 1) {
+                    int p = p0 + qi0, g = g0;
 #pragma unroll
-                        for (int r = 0; r < RM; ++r) s[r] = seen ? s[r] : -INFINITY;
-                    } else {
-                        int p = p0, g = a.group;
-#pragma unroll
-                        for (int r = 0; r < RM; ++r) {
-                            if (!seen || key > p || (a.window && key <= p - a.window)) s[r] = -INFINITY;
-                            if (--g == 0) {
-                                g = a.group;
-                                ++p;
-                            }
-                        }
-                    }
-                }
-                bool high = in_tmem == kFlush;
-                const unsigned had = unset;
-                unsigned can = 0;  // rows without a reference that see a key of this tile: they take the last one's score
-                if (had) {
-                    int p = p0, g = a.group;
-#pragma unroll
-                    for (int r = 0; r < RM; ++r) {
-                        const int last = min(p, key0 + kTileKeys - 1), lo = a.window ? max(p - a.window + 1, key0) : key0;
-                        if ((had >> r & 1) && last >= lo) {
-                            can |= 1u << r;
-                            if (key == last) first_ref[i & 1][r] = s[r];
-                        }
+                    for (int r = 0; r < RH; ++r) {
+                        if (!seen || key > p || (a.window && key <= p - a.window)) s[r] = -INFINITY;
                         if (--g == 0) {
                             g = a.group;
                             ++p;
                         }
                     }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < RM; ++r) high = high || s[r] > kRaise + kShift;
                 }
-                bool any = bar_any(high || !ok);
-                if (had) {
+                bool high = in_tmem == kFlush;
+                const unsigned had = unset;
+                if (had) {  // rows without a reference that see a key of this tile take the last one's score
+                    unsigned can = 0;
+                    int p = p0, g = u.m == 1 ? RM : a.group;
+#pragma unroll 1
+                    for (int r = 0; r < rows; ++r) {
+                        const int last = min(p, key0 + kTileKeys - 1), lo = a.window ? max(p - a.window + 1, key0) : key0;
+                        if (last >= lo) can |= 1u << r;
+                        if (--g == 0) {
+                            g = a.group;
+                            ++p;
+                        }
+                    }
+                    can &= had;
+                    p = p0 + qi0;
+                    g = g0;
 #pragma unroll
-                    for (int r = 0; r < RM; ++r) {
-                        if (can >> r & 1) {
-                            ref[r] = first_ref[i & 1][r] - kShift;
+                    for (int r = 0; r < RH; ++r) {
+                        if ((can >> (r0 + r) & 1) && key == min(p, key0 + kTileKeys - 1)) first_ref[i & 1][r0 + r] = s[r];
+                        if (--g == 0) {
+                            g = a.group;
+                            ++p;
+                        }
+                    }
+                    const bool stop = bar_any(!ok);
+#pragma unroll
+                    for (int r = 0; r < RH; ++r)
+                        if (can >> (r0 + r) & 1) {
+                            ref[r] = first_ref[i & 1][r0 + r] - kShift;
                             s[r] -= ref[r];
                         }
-                        high = high || s[r] > kRaise + kShift;
-                    }
                     unset &= ~can;
-                    any = bar_any(high) || any;
+                    if (stop) break;
                 }
+#pragma unroll
+                for (int r = 0; r < RH; ++r) high = high || s[r] > kRaise + kShift;
+                const bool any = bar_any(high || !ok);
                 bool waited = false;  // for the product of the tile before, which reads vb and wb
                 if (any) {
                     // O leaves TMEM, and the references that a score passed are raised to the tile's maxima
 #pragma unroll
-                    for (int r = 0; r < RM; ++r) {
+                    for (int r = 0; r < RH; ++r) {
                         const float top = warp_max_redux(s[r]);
-                        if (lane == 0) tile_max[warp][r] = top;
+                        if (lane == 0) tile_max[quad][r0 + r] = top;
                     }
                     if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab) && ok;
                     tc_fence_after();
                     waited = true;
                     if (bar_any(!ok)) break;
                     if (in_tmem) {
-                        int o0[RM], o1[RM], o2[RM];
+                        int o0[RH], o1[RH], o2[RH];
                         const uint32_t at = my_tmem + 2 * C::s_cols;
                         tmem_ld(at, o0);
                         tmem_ld(at + RM, o1);
@@ -635,7 +662,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         if constexpr (NP == 3) tmem_ready(o2);
                         tc_fence_before();
 #pragma unroll
-                        for (int r = 0; r < RM; ++r) {
+                        for (int r = 0; r < RH; ++r) {
                             float o = __int_as_float(o1[r]);
                             if constexpr (NP == 3) o += __int_as_float(o2[r]);
                             acc[r] += o + __int_as_float(o0[r]);
@@ -643,8 +670,9 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         in_tmem = 0;
                     }
 #pragma unroll
-                    for (int r = 0; r < RM; ++r) {
-                        const float top = fmaxf(fmaxf(tile_max[0][r], tile_max[1][r]), fmaxf(tile_max[2][r], tile_max[3][r]));
+                    for (int r = 0; r < RH; ++r) {
+                        const int x = r0 + r;
+                        const float top = fmaxf(fmaxf(tile_max[0][x], tile_max[1][x]), fmaxf(tile_max[2][x], tile_max[3][x]));
                         if (top > kRaise + kShift) {
                             ref[r] += top - kShift;
                             s[r] -= top - kShift;
@@ -654,15 +682,14 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         }
                     }
                 }
-                unsigned w[RM / 2][NP];  // pieces of rows 2 x, 2 x + 1
+                unsigned w[RH / 2][NP];  // pieces of rows 2 x, 2 x + 1 of the half
 #pragma unroll
-                for (int x = 0; x < RM / 2; ++x) {
+                for (int x = 0; x < RH / 2; ++x) {
                     float p[2];
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        const int r = 2 * x + y;
-                        const float e = ex2(s[r]);
-                        sum[r] += e;
+                        const float e = ex2(s[2 * x + y]);
+                        sum[2 * x + y] += e;
                         p[y] = e * vs;
                     }
 #pragma unroll
@@ -679,20 +706,21 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab) && ok;
                     tc_fence_after();
                 }
-                unsigned char* wt = wb + (tid >> 6) * C::w_half + (tid & 7) * 2;
-                const int wc = tid >> 3 & 7;  // 16-byte chunk of the half's rows
+                unsigned char* wt = wb + (kid >> 6) * C::w_half + (kid & 7) * 2;
+                const int wc = kid >> 3 & 7;  // 16-byte chunk of the rows of 64 keys
 #pragma unroll
-                for (int x = 0; x < RM / 2; ++x)
+                for (int x = 0; x < RH / 2; ++x)
 #pragma unroll
                     for (int z = 0; z < NP; ++z) {
-                        *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(z * RM + 2 * x, wc)) = (unsigned short)w[x][z];
-                        *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(z * RM + 2 * x + 1, wc)) = (unsigned short)(w[x][z] >> 16);
+                        const int row = z * RM + r0 + 2 * x;
+                        *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(row, wc)) = (unsigned short)w[x][z];
+                        *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(row + 1, wc)) = (unsigned short)(w[x][z] >> 16);
                     }
                 asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
                 for (int x = 0; x < C::items; ++x) {
-                    const int b = vblk + x * (128 / HD);
-                    const uint4 v = reinterpret_cast<const uint4*>(vc)[x * 128 + tid];
+                    const int b = vblk + x * (kDecSoft / HD);
+                    const uint4 v = reinterpret_cast<const uint4*>(vc)[x * kDecSoft + tid];
                     const uint2 x0 = codes_bf16(v.x), x1 = codes_bf16(v.y), x2 = codes_bf16(v.z), x3 = codes_bf16(v.w);
                     unsigned char* dst = vb + (b >> 2) * C::v_half;
                     *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3))) = make_uint4(x0.x, x0.y, x1.x, x1.y);
@@ -707,14 +735,14 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     ok = wait_warp(&o_done, i & 1, ab) && ok;
                     tc_fence_after();
                     {
-                        int o0[RM], o1[RM], o2[RM];
+                        int o0[RH], o1[RH], o2[RH];
                         const uint32_t at = my_tmem + 2 * C::s_cols;
                         tmem_ld(at, o0);
                         tmem_ld(at + RM, o1);
                         if constexpr (NP == 3) tmem_ld(at + 2 * RM, o2);
                         // meanwhile the sums: at each step a lane keeps half of its rows
 #pragma unroll
-                        for (int h = RM / 2, o = 16; h >= 1; h >>= 1, o >>= 1)
+                        for (int h = RH / 2, o = 16; h >= 1; h >>= 1, o >>= 1)
 #pragma unroll
                             for (int r = 0; r < h; ++r) {
                                 const bool up = lane & o;
@@ -722,8 +750,8 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                                 sum[r] = mine + __shfl_xor_sync(0xffffffffu, other, o);
                             }
 #pragma unroll
-                        for (int o = 16 / RM; o > 0; o >>= 1) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
-                        if (lane % (32 / RM) == 0) sum_part[warp][lane / (32 / RM)] = sum[0];
+                        for (int o = 16 / RH; o > 0; o >>= 1) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+                        if (lane % (32 / RH) == 0) sum_part[quad][r0 + lane / (32 / RH)] = sum[0];
                         tmem_ld_wait();
                         tmem_ready(o0);
                         tmem_ready(o1);
@@ -731,11 +759,11 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         tc_fence_before();
                         in_tmem = 0;
 #pragma unroll
-                        for (int r = 0; r < RM; ++r) {
+                        for (int r = 0; r < RH; ++r) {
                             float o = __int_as_float(o1[r]);
                             if constexpr (NP == 3) o += __int_as_float(o2[r]);
                             acc[r] += o + __int_as_float(o0[r]);
-                            if (tid == 0) last_ref[r] = ref[r];
+                            if (kid == 0) last_ref[r0 + r] = ref[r];
                         }
                     }
                     if (bar_any(!ok)) break;
@@ -752,9 +780,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     }
                     auto put_rows = [&](auto* out, bool own_order) {
 #pragma unroll
-                        for (int r = 0; r < RM; ++r) {
-                            const float o = acc[r] * __shfl_sync(0xffffffffu, inv, r);
-                            if (r < rows && lane < lanes) put(out + size_t(own_order ? r : off[r]) * HD + dim, o);
+                        for (int r = 0; r < RH; ++r) {
+                            const int x = r0 + r;
+                            const float o = acc[r] * __shfl_sync(0xffffffffu, inv, x);
+                            if (x < rows && lane < lanes) put(out + size_t(own_order ? x : off[x]) * HD + dim, o);
                         }
                     };
                     if (u.cut) put_rows(plan.o + slot * HD, true);
@@ -768,10 +797,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 const uint32_t dst = smem_u32(vc) + tid * 16;
 #pragma unroll
                 for (int x = 0; x < C::items; ++x) {
-                    const int b = vblk + x * (128 / HD);
+                    const int b = vblk + x * (kDecSoft / HD);
                     const int8_t* src = c.codes + (size_t(tile_rec[(i + 1) & 3].kt[b] + c.n_kv) << v_shift) +
                                         (((b * kKvBlock) & (c.pt - 1)) * HD + vd * 16);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * 2048), "l"(src) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * kDecSoft * 16), "l"(src) : "memory");
                 }
             }
         }
@@ -779,64 +808,118 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && abort_flag) set_error(c.status, ERR_WAIT_TIMEOUT);
-    if (warp == 4) {
+    if (warp == 8) {
         tc_fence_after();
         tmem_free(tmem, C::tmem_cols);
     }
 }
 
-// Joins the partial sums of the units that k_kv_decode cut: CTA (x, r) row r of the one that its CTA x began, in CTA order.
-constexpr int kJoinThreads = 512;
+// Joins the partial sums of the units that k_kv_decode cut, in CTA order.
+// Few partials to a unit (MANY false): CTA x joins the rows of the unit that CTA x of `parts` began, a warp per row.
+// Many: CTA (x, r) joins row r of the x-th unit that was cut, its threads spread over the partials.  (A CTA per began part and
+// row, most of them without work, took 21 us at 2 units of 222 partials and 7 rows.)
+constexpr int kJoinMany = 512, kJoinFew = 256;  // threads
 
-template <int HD, int RM, class T>
-__global__ void __launch_bounds__(kJoinThreads) k_kv_join(KvAttnArgs a, DecPlan plan) {
-    constexpr int G = kJoinThreads / HD;
-    extern __shared__ float weight[];  // [n] of the partials
-    __shared__ float part[G][HD], red[2][16];
-    const int r = blockIdx.y, tid = threadIdx.x, d = tid % HD, g = tid / HD, warp = tid >> 5, lane = tid & 31;
+template <int HD, int RM, class T, bool MANY>
+__global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnArgs a, DecPlan plan, int parts) {
+    constexpr int warps = (MANY ? kJoinMany : kJoinFew) / 32, G = MANY ? kJoinMany / HD : 1, E = HD / 32;
+    extern __shared__ float weight[];  // [n] of the partials, if MANY
+    __shared__ float part[G][HD], red[2][warps];
+    __shared__ int found;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
-    const int4 in = __ldcg(plan.info + blockIdx.x);  // last CTA, first token, queries, kv head
-    if (in.x < 0 || r >= in.z * a.group) return;
-    const int first = blockIdx.x, n = in.x - first + 1;
-    auto slot = [&](int x) { return size_t(2 * (first + x) + (x == 0)) * RM + r; };
-    float top = -INFINITY;
-    float2 ml = make_float2(-INFINITY, 0.f);
-#pragma unroll 1
-    for (int x = tid; x < n; x += kJoinThreads) {  // one partial each, but for the largest grids
-        ml = __ldcg(reinterpret_cast<const float2*>(plan.ml) + slot(x));
-        weight[x] = ml.x;
-        top = fmaxf(top, ml.x);
-    }
-    top = warp_max_redux(top);
-    if (lane == 0) red[0][warp] = top;
-    __syncthreads();
-    top = warp_max_redux(red[0][lane & 15]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-#pragma unroll 1
-    for (int x = tid; x < n; x += kJoinThreads) {
-        const float w = ex2_full(weight[x] - ref);
-        weight[x] = w;
-        l += w * (n <= kJoinThreads ? ml.y : __ldcg(plan.ml + slot(x) * 2 + 1));
-    }
-    l = warp_sum(l);
-    if (lane == 0) red[1][warp] = l;
-    __syncthreads();
-    float o = 0.f;
-#pragma unroll 8
-    for (int x = g; x < n; x += G) o = fmaf(__ldcg(plan.o + slot(x) * HD + d), weight[x], o);
-    part[g][d] = o;
-    __syncthreads();
-    if (g > 0) return;
+    int first = blockIdx.x;
+    if constexpr (MANY) {
+        if (tid == 0) found = -1;
+        int seen = 0;  // units among the parts before
+        for (int x0 = 0; x0 < parts; x0 += kJoinMany) {
+            const bool began = x0 + tid < parts && __ldcg(&plan.info[x0 + tid].x) >= 0;
+            const unsigned mask = __ballot_sync(0xffffffffu, began);
+            if (lane == 0) red[0][warp] = __int_as_float(__popc(mask));
+            __syncthreads();
+            int before = seen;
 #pragma unroll
-    for (int q = 1; q < G; ++q) o += part[q][d];
-    l = 0.f;
+            for (int q = 0; q < warps; ++q) {
+                const int k = __float_as_int(red[0][q]);
+                if (q < warp) before += k;
+                seen += k;
+            }
+            if (began && before + __popc(mask & ((1u << lane) - 1)) == int(blockIdx.x)) found = x0 + tid;
+            __syncthreads();
+        }
+        first = found;
+        if (first < 0) return;
+    }
+    const int4 in = __ldcg(plan.info + first);  // last CTA, first token, queries, kv head
+    if (in.x < 0) return;
+    const int n = in.x - first + 1, rows = in.z * a.group;
+    auto slot = [&](int x, int r) { return size_t(2 * (first + x) + (x == 0)) * RM + r; };
+    auto row_of = [&](int r) { return size_t(in.y + r / a.group) * a.n_heads + in.w * a.group + r % a.group; };
+    if constexpr (!MANY) {
+        for (int r = warp; r < rows; r += warps) {
+            float top = -INFINITY, l = 0.f, o[E] = {};
+            for (int x0 = 0; x0 < n; x0 += 32) {  // a partial per lane
+                const int k = min(n - x0, 32);
+                const float2 ml = lane < k ? __ldcg(reinterpret_cast<const float2*>(plan.ml) + slot(x0 + lane, r))
+                                           : make_float2(-INFINITY, 0.f);
+                const float t = fmaxf(top, warp_max_redux(ml.x)), ref = t == -INFINITY ? 0.f : t;
+                const float w = ex2_full(ml.x - ref), f = ex2_full(top - ref);
+                top = t;
+                l = l * f + warp_sum(ml.y * w);
 #pragma unroll
-    for (int q = 0; q < 16; ++q) l += red[1][q];
-    const size_t row = size_t(in.y + r / a.group) * a.n_heads + in.w * a.group + r % a.group;
-    const bool none = top == -INFINITY && l == 0.f;
-    put(static_cast<T*>(a.out) + row * HD + d, none ? 0.f : o / l);
-    if (a.lse && d == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+                for (int e = 0; e < E; ++e) o[e] *= f;
+#pragma unroll 4
+                for (int x = 0; x < k; ++x) {
+                    float v[E];
+                    load_row<true>(plan.o + slot(x0 + x, r) * HD + lane * E, v);
+                    const float wx = __shfl_sync(0xffffffffu, w, x);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], wx, o[e]);
+                }
+            }
+            const bool none = top == -INFINITY && l == 0.f;
+            T* out = static_cast<T*>(a.out) + row_of(r) * HD + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) put(out + e, none ? 0.f : o[e] / l);
+            if (a.lse && lane == 0) a.lse[row_of(r)] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+        }
+    } else {
+        const int d = tid % HD, g = tid / HD, r = blockIdx.y;
+        if (r >= rows) return;
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int x = tid; x < n; x += kJoinMany) top = fmaxf(top, weight[x] = __ldcg(plan.ml + slot(x, r) * 2));
+        top = warp_max_redux(top);
+        if (lane == 0) red[0][warp] = top;
+        __syncthreads();
+        top = warp_max_redux(lane < warps ? red[0][lane] : -INFINITY);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float l = 0.f;
+#pragma unroll 1
+        for (int x = tid; x < n; x += kJoinMany) {
+            const float w = ex2_full(weight[x] - ref);
+            weight[x] = w;
+            l += w * __ldcg(plan.ml + slot(x, r) * 2 + 1);
+        }
+        l = warp_sum(l);
+        if (lane == 0) red[1][warp] = l;
+        __syncthreads();
+        float o = 0.f;
+#pragma unroll 16
+        for (int x = g; x < n; x += G) o = fmaf(__ldcg(plan.o + slot(x, r) * HD + d), weight[x], o);
+        part[g][d] = o;
+        __syncthreads();
+        if (g == 0) {
+#pragma unroll
+            for (int q = 1; q < G; ++q) o += part[q][d];
+            l = 0.f;
+#pragma unroll
+            for (int q = 0; q < warps; ++q) l += red[1][q];
+            const bool none = top == -INFINITY && l == 0.f;
+            put(static_cast<T*>(a.out) + row_of(r) * HD + d, none ? 0.f : o / l);
+            if (a.lse && d == 0) a.lse[row_of(r)] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- many query rows per kv head (chunks of a prompt, drafts)
@@ -1363,8 +1446,8 @@ DecLaunch dec_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     // a unit's tiles, at most; a window ends anywhere in its first and last tile
     const long long span = a.window && a.window < a.max_len ? (long long)a.window + a.max_q : a.max_len;
     const long long tiles = std::max(1LL, (span + kTileKeys - 1) / kTileKeys + (a.window != 0));
-    l.even = tiles > 8;
     const int ctas = c.hd == 64 && dec_rm(a) <= 8 ? 3 : 2;  // per SM, as the kernel's
+    l.even = tiles > 8;
     l.grid = int(l.even ? std::min<long long>(148 * ctas, std::max<long long>(1, (long long)l.units * tiles / 2)) : (long long)l.units);
     return l;
 }
@@ -1386,8 +1469,11 @@ cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, v
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
     if (e != cudaSuccess || !l.even) return e;
-    return launch_pdl(k_kv_join<HD, RM, T>, dim3(unsigned(l.grid), unsigned(a.max_q * a.group)), dim3(kJoinThreads), size_t(l.grid) * 4,
-                      st, true, a, p);
+    // more than 32 partials to a unit: a CTA per row, else a warp
+    if (size_t(l.grid) > l.units * 32)
+        return launch_pdl(k_kv_join<HD, RM, T, true>, dim3(unsigned(l.units), unsigned(a.max_q * a.group)), dim3(kJoinMany),
+                          size_t(l.grid) * 4, st, true, a, p, int(l.grid));
+    return launch_pdl(k_kv_join<HD, RM, T, false>, dim3(unsigned(l.grid)), dim3(kJoinFew), 0, st, true, a, p, int(l.grid));
 }
 
 struct ChunkLaunch {

@@ -134,8 +134,10 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
 // TMEM -> registers: this warp's 32 lanes, N consecutive 32-bit columns from taddr (tmem_ld_wait before use).
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&v)[N]) {
-    static_assert(N == 4 || N == 8 || N == 16 || N == 32, "columns of a load");
-    if constexpr (N == 4) {
+    static_assert(N == 2 || N == 4 || N == 8 || N == 16 || N == 32, "columns of a load");
+    if constexpr (N == 2) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(taddr));
+    } else if constexpr (N == 4) {
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                      : "r"(taddr));
