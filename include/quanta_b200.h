@@ -227,6 +227,18 @@ int qnt_batch_init(qnt_model* m, int max_seqs, int ctx_len);
 int qnt_prefill_batch(qnt_model* m, int seq, const int* tokens, int n, int* next_id);
 int qnt_decode_batch(qnt_model* m, const int* seq_ids, const int* tokens, int n, int* next_ids);
 int qnt_batch_reset(qnt_model* m, int seq);
+/* Batched serving from the paged 8-bit KV cache (qnt_kv_cache): sequences take pages of page_tokens positions from one pool
+ * of n_pages as they grow, at a bit more than half of the f16 caches' bytes per position, and share a common prefix.
+ *   qnt_batch_init_paged  instead of qnt_batch_init; prefill, decode and reset are the same calls.  A call that would need
+ *                         more pages than are free returns QNT_ERR_RANGE and leaves its sequences as they were (a prefill
+ *                         of more than 512 tokens: with those of its 512-token chunks that found room)
+ *   qnt_batch_fork        the empty sequence dst takes over src's positions: full pages are shared, a part-filled last page
+ *                         is copied
+ *   qnt_batch_resize      the pages in use are moved together and into a pool of n_pages, which replaces the old one
+ *                         (QNT_ERR_RANGE: more are in use) */
+int qnt_batch_init_paged(qnt_model* m, int max_seqs, int ctx_len, int n_pages, int page_tokens);
+int qnt_batch_fork(qnt_model* m, int src, int dst);
+int qnt_batch_resize(qnt_model* m, int n_pages);
 
 /* Sampler (engine/src/sampler.h:20-38): Sampler::sample (sampler.cpp:22-85) on logits that are already in device
  * memory -- repetition penalty -> greedy argmax (first max) or top-k -> softmax(T) -> min-p -> top-p -> xorshift64*

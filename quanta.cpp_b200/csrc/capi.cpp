@@ -567,6 +567,21 @@ int qnt_batch_reset(qnt_model* m, int seq) {
     return engine_code(m->eng, m->eng.batch_reset(seq));
 }
 
+int qnt_batch_init_paged(qnt_model* m, int max_seqs, int ctx_len, int n_pages, int page_tokens) {
+    if (!m) return set_err(QNT_ERR_INVALID, "null model");
+    return engine_code(m->eng, m->eng.batch_init_paged(max_seqs, ctx_len, n_pages, page_tokens));
+}
+
+int qnt_batch_fork(qnt_model* m, int src, int dst) {
+    if (!m) return set_err(QNT_ERR_INVALID, "null model");
+    return engine_code(m->eng, m->eng.batch_fork(src, dst));
+}
+
+int qnt_batch_resize(qnt_model* m, int n_pages) {
+    if (!m) return set_err(QNT_ERR_INVALID, "null model");
+    return engine_code(m->eng, m->eng.batch_resize(n_pages));
+}
+
 int qnt_model_debug_buffer(qnt_model* m, int what, float* out) {
     if (!m || !out) return set_err(QNT_ERR_INVALID, "null argument");
     return m->eng.debug_buffer(what, out);

@@ -1,9 +1,11 @@
 #include "engine.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <functional>
+#include <numeric>
 #include <stdexcept>
 
 namespace qb {
@@ -18,8 +20,7 @@ Engine::~Engine() {
     if (st_) cudaStreamSynchronize(st_);
     for (auto& g : graphs_) cudaGraphExecDestroy(g.second);
     for (void* p : allocs_) cudaFree(p);
-    cudaFree(bkcache_);
-    cudaFree(bvcache_);
+    batch_free();
     if (st_) cudaStreamDestroy(st_);
 }
 
@@ -449,14 +450,38 @@ int Engine::launch_matmul(const DMat& W, const TcMap* wmap, bool ffn_in, int n, 
     return 0;
 }
 
-int Engine::launch_chunk(int n, const int* pos_dev, int pos_bound, TokMap tm) {
+int Engine::launch_chunk(int n, const int* pos_dev, int pos_bound, TokMap tm, const KvCall* paged, int max_q) {
     const int dim = hp_.dim;
     const int kv_dim = hp_.n_kv_heads * hp_.head_dim;
+    KvAttnArgs ka{};
+    if (paged) {
+        ka.q = Q_;
+        ka.out = ATT_;
+        ka.q_stride = (long long)hp_.n_heads * hp_.head_dim;
+        ka.type = KV_F32;
+        ka.n_heads = hp_.n_heads;
+        ka.group = hp_.n_heads / hp_.n_kv_heads;
+        ka.scale = layers_.empty() ? 0.f : layers_[0].aa.scale;
+        ka.max_q = max_q;
+        ka.max_len = pos_bound;
+        const size_t need = kv_attn_ws_bytes(kv_, ka, *paged);
+        if (need > kv_ws_bytes_) {
+            cudaStreamSynchronize(st_);
+            cudaFree(kv_ws_);
+            kv_ws_ = nullptr;
+            kv_ws_bytes_ = 0;
+            QB_TRY(cudaMalloc(&kv_ws_, need));
+            kv_ws_bytes_ = need;
+        }
+    }
     for (size_t l = 0; l < layers_.size(); ++l) {
         const Layer& L = layers_[l];
         QkvArgs qa = L.qa;
         AttnArgs aa = L.aa;
-        if (tm.pos) {  // the batch caches: this layer's slice of sequence 0 (tok_off adds the token's sequence)
+        if (paged) {  // K and V rows by token (tok_off takes the position out), quantized below
+            qa.kcache = kv_rows_;
+            qa.vcache = kv_rows_ + size_t(kChunk) * kv_dim;
+        } else if (tm.pos) {  // the batch caches: this layer's slice of sequence 0 (tok_off adds the token's sequence)
             qa.kcache = bkcache_ + l * size_t(bctx_) * kv_dim;
             qa.vcache = bvcache_ + l * size_t(bctx_) * kv_dim;
             aa.kcache = qa.kcache;
@@ -475,7 +500,14 @@ int Engine::launch_chunk(int n, const int* pos_dev, int pos_bound, TokMap tm) {
         qo.dx = DX_;
         qo.dxt = DXT_;
         qo.ldt = kChunk;
-        QB_TRY(launch_attn_prefill(aa, Q_, pos_dev, n, pos_bound, ATT_, st_, pdl_, tm, &qo));
+        if (paged) {
+            QB_TRY(launch_kv_append(kv_, int(l), qa.kcache, qa.vcache, KV_F16, kv_dim, kv_dim, *paged, max_q, st_));
+            ka.layer = int(l);
+            QB_TRY(launch_kv_attention(kv_, ka, *paged, kv_ws_, st_));
+            QB_TRY(launch_norm_quant_rows(ATT_, nullptr, n, hp_.n_heads * hp_.head_dim, hp_.norm_eps, XQ_, DX_, DXT_, kChunk, st_, false));
+        } else {
+            QB_TRY(launch_attn_prefill(aa, Q_, pos_dev, n, pos_bound, ATT_, st_, pdl_, tm, &qo));
+        }
         if (int r = launch_matmul(L.o, L.tc ? &L.t_o : nullptr, false, n, R_, true)) return r;
         QB_TRY(launch_norm_quant_rows(X_, L.ffn_norm, n, dim, hp_.norm_eps, XQ_, DX_, DXT_, kChunk, st_, pdl_));
         if (tc_swiglu_ && L.tc && n >= kTcChunkMin && !hadamard_) {  // SwiGLU + quantize in the matmul's epilogue
@@ -999,7 +1031,7 @@ namespace qb {
 
 // ---------------------------------------------------------------- batched serving
 
-int Engine::batch_init(int max_seqs, int ctx) {
+int Engine::batch_supported(int max_seqs, int ctx) {
     if (max_seqs <= 0 || ctx <= 1 || ctx > ctx_) {
         err_ = "batch_init: need max_seqs > 0 and 1 < ctx <= the model's context length";
         return -1;
@@ -1013,10 +1045,23 @@ int Engine::batch_init(int max_seqs, int ctx) {
             err_ = "batched serving needs tensor-core sources for every layer";
             return -4;
         }
-    cudaStreamSynchronize(st_);
-    cudaFree(bkcache_);
-    cudaFree(bvcache_);
+    return 0;
+}
+
+void Engine::batch_free() {
+    if (st_) cudaStreamSynchronize(st_);
+    for (void* p : {(void*)bkcache_, (void*)bvcache_, kv_pool_, kv_mem_, kv_ws_}) cudaFree(p);
     bkcache_ = bvcache_ = nullptr;
+    kv_pool_ = kv_mem_ = kv_ws_ = nullptr;
+    kv_ws_bytes_ = 0;
+    kv_ = KvView{};
+    bmax_ = bctx_ = 0;
+    blens_.clear();
+}
+
+int Engine::batch_init(int max_seqs, int ctx) {
+    if (int r = batch_supported(max_seqs, ctx)) return r;
+    batch_free();
     const size_t kv_dim = size_t(hp_.n_kv_heads) * hp_.head_dim;
     const size_t elems = size_t(max_seqs) * hp_.n_layers * size_t(ctx) * kv_dim;
     cudaError_t e = cudaMalloc(&bkcache_, elems * 2);
@@ -1033,10 +1078,163 @@ int Engine::batch_init(int max_seqs, int ctx) {
     return 0;
 }
 
+// ---- paged caches
+
+bool Engine::paged_pool(int n_pages, KvView* v, void** mem) {
+    v->n_pages = n_pages;
+    const size_t codes = align_up(size_t(n_pages) * v->page_codes(), 256);
+    const size_t scales = align_up(size_t(n_pages) * size_t(v->page_scales()) * 4, 256), refs = align_up(size_t(n_pages) * 4, 256);
+    if (cudaMalloc(mem, codes + scales + refs + kv_page_ws_bytes(*v)) != cudaSuccess) {
+        cudaGetLastError();
+        *mem = nullptr;
+        return false;
+    }
+    char* p = static_cast<char*>(*mem);
+    v->codes = reinterpret_cast<int8_t*>(p);
+    v->scales = reinterpret_cast<float*>(p + codes);
+    v->refs = reinterpret_cast<int*>(p + codes + scales);
+    return cudaMemsetAsync(p, 0, codes + scales + refs, st_) == cudaSuccess;
+}
+
+int Engine::batch_init_paged(int max_seqs, int ctx, int n_pages, int page_tokens) {
+    if (int r = batch_supported(max_seqs, ctx)) return r;
+    if (max_seqs > kKvMaxSeqs || n_pages <= 0 || n_pages > kKvMaxPages ||
+        (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) {
+        err_ = "batch_init_paged: at most " + std::to_string(kKvMaxSeqs) + " sequences, 1 .. " + std::to_string(kKvMaxPages) +
+               " pages of 16, 32, 64 or 128 positions";
+        return -1;
+    }
+    if (hp_.head_dim != 64 && hp_.head_dim != 128) {
+        err_ = "batch_init_paged: head_dim must be 64 or 128";
+        return -4;
+    }
+    batch_free();
+    KvView v{};
+    v.n_layers = hp_.n_layers;
+    v.n_kv = hp_.n_kv_heads;
+    v.hd = hp_.head_dim;
+    v.pt = page_tokens;
+    while ((1 << v.pt_shift) < page_tokens) ++v.pt_shift;
+    v.max_seqs = max_seqs;
+    v.max_pages = (ctx + page_tokens - 1) / page_tokens;
+    v.status = status_;
+    v.n_pages = n_pages;
+    // kv_mem_: table, lens, the call's lists, K and V rows
+    const size_t table = align_up(size_t(max_seqs) * v.max_pages * 4, 256), lens = align_up(size_t(max_seqs) * 4, 256);
+    const size_t list = align_up(size_t(kChunk + 1) * 4, 256), rows = size_t(2) * kChunk * hp_.n_kv_heads * hp_.head_dim * 2;
+    bool ok = paged_pool(n_pages, &v, &kv_pool_) && cudaMalloc(&kv_mem_, table + lens + 3 * list + rows) == cudaSuccess;
+    if (ok) {
+        char* p = static_cast<char*>(kv_mem_);
+        v.table = reinterpret_cast<int*>(p);
+        v.lens = reinterpret_cast<int*>(p + table);
+        p += table + lens;
+        kv_seqs_ = reinterpret_cast<int*>(p);
+        kv_starts_ = reinterpret_cast<int*>(p + list);
+        kv_extra_ = reinterpret_cast<int*>(p + 2 * list);
+        kv_rows_ = reinterpret_cast<__half*>(p + 3 * list);
+        ok = cudaMemsetAsync(v.table, 0xff, table, st_) == cudaSuccess && cudaMemsetAsync(v.lens, 0, lens, st_) == cudaSuccess;
+    }
+    if (!ok) {
+        cudaGetLastError();
+        batch_free();
+        err_ = "paged KV caches: out of device memory";
+        return -2;
+    }
+    kv_ = v;
+    bmax_ = max_seqs;
+    bctx_ = ctx;
+    blens_.assign(size_t(max_seqs), 0);
+    return 0;
+}
+
+int Engine::paged_check(long long extra) {
+    long long pages = extra;  // at most: shared pages count for each of their sequences
+    for (int len : blens_) pages += (len + kv_.pt - 1) >> kv_.pt_shift;
+    if (pages <= kv_.n_pages) return 0;
+    const cudaError_t e = cudaStreamSynchronize(st_);
+    if (e != cudaSuccess) return cuda_fail(e, "kernel");
+    const unsigned s = read_status();
+    if (s == 0) return 0;
+    err_ = s == ERR_CAPACITY ? "paged KV caches: no free pages left" : "device status error bits 0x" + std::to_string(s);
+    return s == ERR_CAPACITY ? -5 : -6;
+}
+
+int Engine::paged_reserve(const int* seqs, const int* starts, int n) {
+    h_extra_.resize(size_t(n));
+    long long pages = 0;
+    for (int i = 0; i < n; ++i) {
+        h_extra_[size_t(i)] = starts[i + 1] - starts[i];
+        const int len = blens_[size_t(seqs[i])];
+        pages += ((len + h_extra_[size_t(i)] + kv_.pt - 1) >> kv_.pt_shift) - ((len + kv_.pt - 1) >> kv_.pt_shift);
+    }
+    cudaMemcpyAsync(kv_seqs_, seqs, size_t(n) * 4, cudaMemcpyHostToDevice, st_);
+    cudaMemcpyAsync(kv_starts_, starts, size_t(n + 1) * 4, cudaMemcpyHostToDevice, st_);
+    cudaMemcpyAsync(kv_extra_, h_extra_.data(), size_t(n) * 4, cudaMemcpyHostToDevice, st_);
+    QB_TRY(launch_kv_reserve(kv_, kv_seqs_, kv_extra_, n, kv_page_ws(), st_));
+    return paged_check(pages);
+}
+
+int Engine::batch_fork(int src, int dst) {
+    if (!kv_.codes) {
+        err_ = "batch_fork: batch_init_paged first";
+        return -1;
+    }
+    if (src < 0 || src >= bmax_ || dst < 0 || dst >= bmax_ || src == dst || blens_[size_t(dst)] != 0) {
+        err_ = "batch_fork: needs two sequences, the second one empty";
+        return -1;
+    }
+    const int len = blens_[size_t(src)];
+    cudaMemcpyAsync(kv_seqs_, &src, 4, cudaMemcpyHostToDevice, st_);
+    cudaMemcpyAsync(kv_extra_, &dst, 4, cudaMemcpyHostToDevice, st_);
+    QB_TRY(launch_kv_fork(kv_, kv_seqs_, kv_extra_, 1, kv_page_ws(), st_));
+    if (int r = paged_check(len & (kv_.pt - 1) ? 1 : 0)) return r;
+    blens_[size_t(dst)] = len;
+    return 0;
+}
+
+int Engine::batch_resize(int n_pages) {
+    if (!kv_.codes || n_pages <= 0 || n_pages > kKvMaxPages) {
+        err_ = "batch_resize: batch_init_paged first, and 1 .. " + std::to_string(kKvMaxPages) + " pages";
+        return -1;
+    }
+    QB_TRY(launch_kv_compact(kv_, kv_page_ws(), st_));  // the pages in use are now the first ones
+    h_extra_.resize(size_t(kv_.n_pages));
+    cudaMemcpyAsync(h_extra_.data(), kv_.refs, size_t(kv_.n_pages) * 4, cudaMemcpyDeviceToHost, st_);
+    if (int r = sync_check()) return r;
+    const size_t used = size_t(std::count_if(h_extra_.begin(), h_extra_.end(), [](int r) { return r > 0; }));
+    if (used > size_t(n_pages)) {
+        err_ = "batch_resize: " + std::to_string(used) + " pages are in use";
+        return -5;
+    }
+    KvView v = kv_;
+    void* mem = nullptr;
+    if (!paged_pool(n_pages, &v, &mem)) {
+        cudaFree(mem);
+        err_ = "batch_resize: out of device memory";
+        return -2;
+    }
+    cudaError_t e = cudaMemcpyAsync(v.codes, kv_.codes, used * v.page_codes(), cudaMemcpyDeviceToDevice, st_);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(v.scales, kv_.scales, used * size_t(v.page_scales()) * 4, cudaMemcpyDeviceToDevice, st_);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(v.refs, kv_.refs, used * 4, cudaMemcpyDeviceToDevice, st_);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st_);
+    if (e != cudaSuccess) {
+        cudaFree(mem);
+        return cuda_fail(e, "batch_resize");
+    }
+    cudaFree(kv_pool_);
+    kv_pool_ = mem;
+    kv_ = v;
+    return 0;
+}
+
 int Engine::batch_reset(int seq) {
     if (seq < 0 || seq >= bmax_) {
         err_ = "batch_reset: bad sequence id";
         return -1;
+    }
+    if (kv_.codes && blens_[size_t(seq)] > 0) {
+        cudaMemcpyAsync(kv_seqs_, &seq, 4, cudaMemcpyHostToDevice, st_);
+        QB_TRY(launch_kv_free(kv_, kv_seqs_, 1, st_));
     }
     blens_[size_t(seq)] = 0;
     return 0;
@@ -1069,14 +1267,21 @@ int Engine::batch_prefill(int seq, const int* tokens, int n, int* next_id) {
     for (int i = 0; i < n; i += kChunk) {
         const int m = std::min(kChunk, n - i);
         h_pos_.resize(size_t(m));
-        h_off_.assign(size_t(m), stride * seq);
+        // paged: the row of token t in kv_rows_, less its position's
+        h_off_.assign(size_t(m), kv_.codes ? -(long long)(len + i) * hp_.n_kv_heads * hp_.head_dim : stride * seq);
         for (int t = 0; t < m; ++t) h_pos_[size_t(t)] = len + i + t;
+        if (kv_.codes) {
+            h_starts_ = {0, m};
+            if (int r = paged_reserve(&seq, h_starts_.data(), 1)) return r;
+        }
         cudaMemcpyAsync(tokens_, tokens + i, size_t(m) * 4, cudaMemcpyHostToDevice, st_);
         cudaMemcpyAsync(tok_pos_, h_pos_.data(), size_t(m) * 4, cudaMemcpyHostToDevice, st_);
         cudaMemcpyAsync(tok_off_, h_off_.data(), size_t(m) * 8, cudaMemcpyHostToDevice, st_);
         QB_TRY(launch_embed(embed_, tokens_, m, X_, status_, st_, false));
-        if (int r = launch_chunk(m, pos_, len + i + m, TokMap{tok_pos_, tok_off_})) return r;
+        const KvCall call{kv_seqs_, kv_starts_, 1, m};
+        if (int r = launch_chunk(m, pos_, len + i + m, TokMap{tok_pos_, tok_off_}, kv_.codes ? &call : nullptr, m)) return r;
         cudaStreamSynchronize(st_);  // the host position arrays are rewritten by the next chunk
+        if (kv_.codes) blens_[size_t(seq)] = len + i + m;  // as the device has it, if a later chunk finds no room
         last = m - 1;
     }
     blens_[size_t(seq)] = len + n;
@@ -1112,14 +1317,20 @@ int Engine::batch_decode(const int* seq_ids, const int* tokens, int n, int* next
             return -5;
         }
         h_pos_[size_t(i)] = blens_[size_t(s)];
-        h_off_[size_t(i)] = stride * s;
+        h_off_[size_t(i)] = kv_.codes ? (i - (long long)h_pos_[size_t(i)]) * hp_.n_kv_heads * hp_.head_dim : stride * s;
         bound = std::max(bound, blens_[size_t(s)] + 1);
+    }
+    if (kv_.codes) {
+        h_starts_.resize(size_t(n) + 1);
+        std::iota(h_starts_.begin(), h_starts_.end(), 0);
+        if (int r = paged_reserve(seq_ids, h_starts_.data(), n)) return r;
     }
     cudaMemcpyAsync(tokens_, tokens, size_t(n) * 4, cudaMemcpyHostToDevice, st_);
     cudaMemcpyAsync(tok_pos_, h_pos_.data(), size_t(n) * 4, cudaMemcpyHostToDevice, st_);
     cudaMemcpyAsync(tok_off_, h_off_.data(), size_t(n) * 8, cudaMemcpyHostToDevice, st_);
     QB_TRY(launch_embed(embed_, tokens_, n, X_, status_, st_, false));
-    if (int r = launch_chunk(n, pos_, bound, TokMap{tok_pos_, tok_off_})) return r;
+    const KvCall call{kv_seqs_, kv_starts_, n, n};
+    if (int r = launch_chunk(n, pos_, bound, TokMap{tok_pos_, tok_off_}, kv_.codes ? &call : nullptr, 1)) return r;
     if (int r = batch_head(n, next_ids)) return r;
     for (int i = 0; i < n; ++i) blens_[size_t(seq_ids[i])] += 1;
     return 0;

@@ -16,6 +16,7 @@
 #include "device_layout.h"
 #include "gemm_tc.h"
 #include "head_kernels.h"
+#include "kv_cache.h"
 #include "layer_kernels.h"
 #include "qnt_file.h"
 
@@ -98,6 +99,12 @@ public:
     // greedy next token (std::max_element over the logits: first maximum among ids < n_valid).
     int batch_decode(const int* seq_ids, const int* tokens, int n, int* next_ids);
     int batch_reset(int seq);
+    // The same with the caches in pages of one pool, 8-bit (kv_cache.h): memory follows the positions in use, not
+    // max_seqs * ctx.  fork: the empty sequence dst continues from src's positions (full pages shared);
+    // resize: the pages in use move to a pool of n_pages.
+    int batch_init_paged(int max_seqs, int ctx, int n_pages, int page_tokens);
+    int batch_fork(int src, int dst);
+    int batch_resize(int n_pages);
     int batch_len(int seq) const { return seq >= 0 && seq < int(blens_.size()) ? blens_[size_t(seq)] : -1; }
 
     const HParams& hparams() const { return hp_; }
@@ -147,8 +154,17 @@ private:
     DMat upload_fused(const std::vector<const HostTensor*>& parts, int mode);
     DMat upload_packed(const HostTensor* packed, const std::vector<const HostTensor*>& parts, int mode);
     int launch_layers_decode(const int* pos_dev);
-    // positions of the chunk stay below pos_bound; with tm.pos set, tokens of the batch caches (their own positions)
-    int launch_chunk(int n, const int* pos_dev, int pos_bound, TokMap tm = TokMap{});
+    // positions of the chunk stay below pos_bound; with tm.pos set, tokens of the batch caches (their own positions),
+    // and with paged too, of the paged ones: the call's sequences, each with at most max_q of the tokens
+    int launch_chunk(int n, const int* pos_dev, int pos_bound, TokMap tm = TokMap{}, const KvCall* paged = nullptr, int max_q = 0);
+    int batch_supported(int max_seqs, int ctx);
+    void batch_free();
+    // a pool of n_pages pages for v's sizes (codes, scales, refs, zeroed; workspace); false: no memory
+    bool paged_pool(int n_pages, KvView* v, void** mem);
+    // the pages for extra tokens of sequences (host lists; starts: [n + 1] rows) and their device lists
+    int paged_reserve(const int* seqs, const int* starts, int n);
+    // waits for the call's status if the pages of all sequences, extra more of them, could pass the pool
+    int paged_check(long long extra);
     int batch_head(int n, int* host_ids);  // greedy ids of the n rows of X_
     // Head pass: full or shortlist; n_list > 0 also produces the sampler's stage-1 lists (with the penalty of the
     // marked must ids when penal).
@@ -244,6 +260,14 @@ private:
     // batched serving
     int bmax_ = 0, bctx_ = 0;
     __half *bkcache_ = nullptr, *bvcache_ = nullptr;  // [seq][layer][bctx][kv_dim]
+    KvView kv_{};                         // the paged caches (codes null: the f16 ones)
+    void *kv_pool_ = nullptr, *kv_mem_ = nullptr;  // codes, scales, refs and the page operations' workspace; the rest
+    __half* kv_rows_ = nullptr;           // K and V rows of a chunk before they are quantized, [2][kChunk][kv_dim]
+    int *kv_seqs_ = nullptr, *kv_starts_ = nullptr, *kv_extra_ = nullptr;  // lists of a call, [kChunk + 1] each
+    void* kv_ws_ = nullptr;
+    size_t kv_ws_bytes_ = 0;
+    void* kv_page_ws() const { return kv_.refs + (size_t(kv_.n_pages) + 63) / 64 * 64; }
+    std::vector<int> h_starts_, h_extra_;
     std::vector<int> blens_;
     int* tok_pos_ = nullptr;              // [kChunk] device
     long long* tok_off_ = nullptr;        // [kChunk] device

@@ -130,6 +130,9 @@ def lib() -> C.CDLL:
         L.qnt_prefill_batch.argtypes = [P, I, P, I, C.POINTER(I)]
         L.qnt_decode_batch.argtypes = [P, P, P, I, P]
         L.qnt_batch_reset.argtypes = [P, I]
+        L.qnt_batch_init_paged.argtypes = [P, I, I, I, I]
+        L.qnt_batch_fork.argtypes = [P, I, I]
+        L.qnt_batch_resize.argtypes = [P, I]
         L.qnt_sampler_create.argtypes = [C.POINTER(SamplerParamsC), C.POINTER(P)]
         L.qnt_sampler_sample.argtypes = [P, P, I, P, I, C.POINTER(I), P]
         L.qnt_sampler_free.argtypes = [P]
@@ -625,6 +628,19 @@ class Model:
 
     def batch_reset(self, seq: int):
         _check(lib().qnt_batch_reset(self.h, seq))
+
+    # the same with the paged 8-bit KV cache: prefill_batch, decode_batch and batch_reset as above
+    def batch_init_paged(self, max_seqs: int, ctx_len: int, n_pages: int, page_tokens: int = 64):
+        """Sequences take pages of page_tokens positions from one pool as they grow."""
+        _check(lib().qnt_batch_init_paged(self.h, max_seqs, ctx_len, n_pages, page_tokens))
+
+    def batch_fork(self, src: int, dst: int):
+        """The empty sequence dst takes over src's positions (a shared prefix, another answer)."""
+        _check(lib().qnt_batch_fork(self.h, src, dst))
+
+    def batch_resize(self, n_pages: int):
+        """Moves the pages in use into a pool of n_pages, which replaces the old one."""
+        _check(lib().qnt_batch_resize(self.h, n_pages))
 
     def session_begin(self, prompt, sp: SamplerParams, shortlist: bool = True, batch_prefill: bool = True):
         p = np.ascontiguousarray(prompt, np.int32)
