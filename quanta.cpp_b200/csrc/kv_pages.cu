@@ -40,16 +40,44 @@ __device__ __forceinline__ int kv_page(const KvView& c, int seq, int pos) {
 
 // ---------------------------------------------------------------- append
 
-// One warp per (block of 16 tokens, K or V, head); the block's 16 * hd codes pass through shared memory in their
-// layout, so that they leave as 16-byte stores.  VEC: rows are read 4 elements at a time (aligned rows).
+// A warp takes one (block of 16 tokens, K or V, head) after another.  A lane holds 8 dims of HD / 16 tokens that follow one
+// another, so that the new values are read once, in whole rows, and a lane's codes already make 8 bytes of a token's dims (K)
+// or 4 or 8 of a dim's tokens (V); through shared memory (rows padded by 16 bytes) they leave as the layout's 16-byte pieces.
+// VEC: a lane's dims are read in 16-byte loads (aligned rows).
 constexpr int kAppendWarps = 4;
+
+// |x| of 8 values, the largest (a NaN if one is), as f32
+__device__ __forceinline__ float amax8(const float (&a)[8], float m) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(a[i]));
+    return m;
+}
+__device__ __forceinline__ __half2 amax8(const __half (&a)[8], __half2 m) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) m = __hmax2_nan(m, __habs2(__halves2half2(a[i], a[i + 1])));
+    return m;
+}
+__device__ __forceinline__ __nv_bfloat162 amax8(const __nv_bfloat16 (&a)[8], __nv_bfloat162 m) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) m = __hmax2_nan(m, __habs2(__halves2bfloat162(a[i], a[i + 1])));
+    return m;
+}
+__device__ __forceinline__ float amax_of(float m) { return m; }
+__device__ __forceinline__ float amax_of(__half2 m) { return max_nan(__low2float(m), __high2float(m)); }
+__device__ __forceinline__ float amax_of(__nv_bfloat162 m) { return max_nan(__low2float(m), __high2float(m)); }
+template <class T> struct AmaxType { using t = float; };
+template <> struct AmaxType<__half> { using t = __half2; };
+template <> struct AmaxType<__nv_bfloat16> { using t = __nv_bfloat162; };
 
 template <class T, int HD, bool VEC>
 __global__ void __launch_bounds__(32 * kAppendWarps) k_kv_append(KvView c, int layer, const T* __restrict__ k,
                                                                  const T* __restrict__ v, long long k_stride,
-                                                                 long long v_stride, KvCall call, int max_new) {
-    constexpr int kPer = HD * kKvBlock / 32;  // values of a lane
-    __shared__ __align__(16) int8_t tiles[kAppendWarps][kKvBlock * HD];
+                                                                 long long v_stride, KvCall call, int max_new, int group) {
+    constexpr int TPL = HD / 16, LPR = HD / 8;  // tokens of a lane, lanes of a row
+    struct alignas(16) Row {
+        T a[8];
+    };
+    __shared__ __align__(16) unsigned char tiles[kAppendWarps][HD * 18];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int j = blockIdx.y;
     const int t0 = __ldg(call.starts + j), m = min(__ldg(call.starts + j + 1), call.n_tok) - t0, seq = __ldg(call.seqs + j);
@@ -63,77 +91,99 @@ __global__ void __launch_bounds__(32 * kAppendWarps) k_kv_append(KvView c, int l
         set_error(c.status, ERR_BAD_POS);
         return;
     }
-    const int b0 = (p0 / kKvBlock + int(blockIdx.x)) * kKvBlock;  // first position of this block
-    if (b0 >= p1) return;
-    const int page = kv_page(c, seq, b0);
-    if (page < 0) return;
-    const int in_page = b0 & (c.pt - 1), kept = max(p0 - b0, 0), end = min(p1 - b0, kKvBlock);
-    int8_t* tile = tiles[warp];
-    for (int task = blockIdx.z * kAppendWarps + warp; task < 2 * c.n_kv; task += gridDim.z * kAppendWarps) {
-        const int kind = task / c.n_kv, head = task % c.n_kv;
+    const int block0 = p0 / kKvBlock + int(blockIdx.x) * group, blocks = min(group, (p1 - 1) / kKvBlock + 1 - block0);
+    if (blocks <= 0) return;
+    const int tasks = blocks * 2 * c.n_kv, step = gridDim.z * kAppendWarps;
+    unsigned char* tile = tiles[warp];
+    const int d0 = lane % LPR * 8, tb = lane / LPR * TPL;
+
+#pragma unroll 1
+    for (int task = blockIdx.z * kAppendWarps + warp; task < tasks; task += step) {
+        const int b0 = (block0 + task / (2 * c.n_kv)) * kKvBlock, kh = task % (2 * c.n_kv), kind = kh >= c.n_kv;
+        const int head = kind ? kh - c.n_kv : kh;
+        const int page = kv_page(c, seq, b0);
+        if (page < 0) continue;  // reported
+        const int in_page = b0 & (c.pt - 1), kept = max(p0 - b0, 0), end = min(p1 - b0, kKvBlock);  // tokens [kept, end) are new
         const size_t at = c.at(page, layer, kind, head);
         int8_t* codes = c.codes + at * c.tile();
         float* scale = c.scales + at * (c.pt / kKvBlock) + in_page / kKvBlock;
-        const T* x = (kind ? v : k) + head * HD;
+        const float before = *scale;
+        const T* src = (kind ? v : k) + head * HD + d0;
         const long long stride = kind ? v_stride : k_stride;
-        const float old = kept ? *scale : 0.f;
-        // the lane's values: 4 consecutive dims of a token, 32 * 4 / HD tokens at a time
-        float val[kPer];
-        float amax = 0.f;
+        Row raw[TPL];
+        typename AmaxType<T>::t most = {};
 #pragma unroll
-        for (int u = 0; u < kPer / 4; ++u) {
-            const int e = (u * 32 + lane) * 4, t = e / HD, d = e % HD;
-            const bool is_new = t >= kept && t < end;
-            const T* src = x + (long long)(t0 + b0 + t - p0) * stride + d;
-            if constexpr (VEC) {
-                struct alignas(4 * sizeof(T)) V4 {
-                    T a[4];
-                } w = {};
-                if (is_new) w = *reinterpret_cast<const V4*>(src);
+        for (int u = 0; u < TPL; ++u) {
+            // (tokens that are not new read the nearest one: a load under a condition would be waited for right here)
+            const int t = min(max(tb + u, kept), end - 1);
+            const T* row = src + (long long)(t0 + b0 + t - p0) * stride;
+            if constexpr (VEC) raw[u] = *reinterpret_cast<const Row*>(row);
+            else
 #pragma unroll
-                for (int i = 0; i < 4; ++i) val[4 * u + i] = is_new ? to_f(w.a[i]) : 0.f;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) val[4 * u + i] = is_new ? to_f(src[i]) : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) amax = max_nan(amax, fabsf(val[4 * u + i]));
+                for (int i = 0; i < 8; ++i) raw[u].a[i] = row[i];
         }
+        const float old = kept ? before : 0.f;
+#pragma unroll
+        for (int u = 0; u < TPL; ++u) most = amax8(raw[u].a, most);
+        float amax = amax_of(most);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const float d = max_nan(old, fmul(amax, 1.0f / 127.0f));
         const float inv = d > 0.f ? __frcp_rn(d) : 0.f;
         const bool fine = d > 0.f && d < INFINITY && inv < INFINITY;
-        const float ratio = fine ? fdiv(old, d) : 0.f;
-        // the block's codes in their layout: 16-byte piece i is K: dims 16 (i / 16) .. of token i % 16, V: dim i's tokens
+        // the block's 16-byte pieces: K: dims 16 (i / 16) .. of token i % 16, V: dim i's tokens
         const int pitch = kind ? HD : c.pt, first = kind ? in_page / kKvBlock * HD : in_page;
-        auto piece = [&](int i) { return kind ? codes + size_t(first + i) * 16 : codes + (size_t(i / 16) * pitch + first + i % 16) * 16; };
+        auto piece = [&](int i) {
+            return reinterpret_cast<uint4*>(kind ? codes + size_t(first + i) * 16
+                                                 : codes + (size_t(i / 16) * pitch + first + i % 16) * 16);
+        };
+        auto in_tile = [&](int i) { return tile + i * 16 + (kind ? i / 8 : i / 16) * 16; };
         __syncwarp();
+        if (kept) {
+            const float ratio = fine ? fdiv(old, d) : 0.f;
 #pragma unroll
-        for (int u = 0; u < HD / 32; ++u) {
-            const int i = u * 32 + lane;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (kept) {
-                w = *reinterpret_cast<const uint4*>(piece(i));
+            for (int u = 0; u < HD / 32; ++u) {
+                const int i = u * 32 + lane;
+                uint4 w = *piece(i);
                 if (d != old) {
                     int8_t* b = reinterpret_cast<int8_t*>(&w);
 #pragma unroll
                     for (int z = 0; z < 16; ++z) b[z] = int8_t(__float2int_rn(fmul(float(b[z]), ratio)));
                 }
+                *reinterpret_cast<uint4*>(in_tile(i)) = w;
             }
-            *reinterpret_cast<uint4*>(tile + i * 16) = w;
+            __syncwarp();
         }
-        __syncwarp();
+        // A code is the low byte of 1.5 * 2^23 + x * (1 / d), rounded to an integer by that sum.  |x / d| <= 127 (1 + 2^-20), also
+        // where d is subnormal (1 / d is finite from 2^-128 on): it never rounds to 128.
+        const int used = fine ? end : 0;  // the later tokens' codes are 0
+        unsigned q[TPL][8];
 #pragma unroll
-        for (int u = 0; u < kPer / 4; ++u) {
-            const int e = (u * 32 + lane) * 4, t = e / HD, dim = e % HD;
-            if (t >= kept) {
+        for (int u = 0; u < TPL; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float y = fminf(fmaxf(fmul(val[4 * u + i], inv), -127.f), 127.f);
-                    const int8_t code = t < end && fine ? int8_t(__float2int_rn(y)) : int8_t(0);
-                    const int dd = dim + i;
-                    tile[kind ? dd * 16 + t : (dd / 16) * 256 + t * 16 + dd % 16] = code;
+            for (int i = 0; i < 8; ++i) q[u][i] = __float_as_uint(fadd(fmul(to_f(raw[u].a[i]), inv), 12582912.f));
+        auto pack = [](unsigned a, unsigned b, unsigned e, unsigned f) {
+            return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(e, f, 0x0040), 0x5410);
+        };
+        auto below = [](int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1; };  // mask of the first n bytes
+        if (kind == 0) {
+#pragma unroll
+            for (int u = 0; u < TPL; ++u) {
+                const unsigned on = tb + u < used ? ~0u : 0u;
+                if (tb + u >= kept)
+                    *reinterpret_cast<uint2*>(in_tile(d0 / 16 * 16 + tb + u) + d0 % 16) =
+                        make_uint2(pack(q[u][0], q[u][1], q[u][2], q[u][3]) & on, pack(q[u][4], q[u][5], q[u][6], q[u][7]) & on);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < TPL / 4; ++h) {
+                const unsigned on = below(used - tb - 4 * h), stay = below(kept - tb - 4 * h);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    unsigned* to = reinterpret_cast<unsigned*>(in_tile(d0 + i) + tb) + h;
+                    unsigned w = pack(q[4 * h][i], q[4 * h + 1][i], q[4 * h + 2][i], q[4 * h + 3][i]) & on;
+                    if (kept) w = (w & ~stay) | (*to & stay);
+                    *to = w;
                 }
             }
         }
@@ -141,7 +191,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) k_kv_append(KvView c, int l
 #pragma unroll
         for (int u = 0; u < HD / 32; ++u) {
             const int i = u * 32 + lane;
-            *reinterpret_cast<uint4*>(piece(i)) = *reinterpret_cast<const uint4*>(tile + i * 16);
+            *piece(i) = *reinterpret_cast<const uint4*>(in_tile(i));
         }
         if (lane == 0) *scale = d;
     }
@@ -149,14 +199,27 @@ __global__ void __launch_bounds__(32 * kAppendWarps) k_kv_append(KvView c, int l
 
 // ---------------------------------------------------------------- read
 
-constexpr int kReadRows = 64, kReadWarps = 8;
+constexpr int kReadRows = 32, kReadWarps = 8;
 
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// One CTA per 64 output rows.  Rows of one block of 16 tokens make a segment; a warp takes (segment, head), so that a V
-// piece (one dim's 16 tokens) is loaded once for all its rows and every row is written by consecutive lanes.
+// One CTA per 32 output rows.  Rows of one block of 16 tokens make a segment; a warp takes (segment, K or V, head): a lane reads
+// its dims of all tokens before it writes the first, and rows are written whole by the warp (HD = 64: two K rows at a time).
+// (With 64 rows, K and V to one warp and loads between the stores: 99 us for 17k rows of 8 heads of 128, bf16 to f32.)
+
+// 4 codes -> f32, exactly: 2^23 + 128 + code in the mantissa, less 2^23 + 128
+__device__ __forceinline__ void codes_f32(unsigned w, float (&x)[4]) {
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + i)) - 8388736.f;
+}
+template <class T, int N>
+struct alignas(N * sizeof(T)) Vals {
+    T a[N];
+};
+
 template <class T, int HD>
 __global__ void __launch_bounds__(32 * kReadWarps) k_kv_read(KvView c, int layer, const int* __restrict__ first, KvCall call,
                                                              T* __restrict__ k_out, T* __restrict__ v_out) {
@@ -200,44 +263,55 @@ __global__ void __launch_bounds__(32 * kReadWarps) k_kv_read(KvView c, int layer
     }
     __syncthreads();
     const size_t pitch = size_t(c.n_kv) * HD;
-    for (int task = warp; task < n_seg * c.n_kv; task += kReadWarps) {
-        const int s = task / c.n_kv, head = task % c.n_kv, r0 = seg_row[s], m = seg_row[s + 1] - r0;
+    for (int task = warp; task < n_seg * 2 * c.n_kv; task += kReadWarps) {
+        const int s = task / (2 * c.n_kv), kh = task % (2 * c.n_kv), kind = kh >= c.n_kv, head = kind ? kh - c.n_kv : kh;
+        const int r0 = seg_row[s], m = seg_row[s + 1] - r0;
         const int page = page_of[r0], in_page = pos_of[r0] & (c.pt - 1), t0 = in_page & 15;
-        T* ko = k_out + (size_t(row0 + r0) * c.n_kv + head) * HD;
-        T* vo = v_out + (size_t(row0 + r0) * c.n_kv + head) * HD;
+        T* out = (kind ? v_out : k_out) + (size_t(row0 + r0) * c.n_kv + head) * HD;
         if (page < 0) {  // reported; the rows read as 0
             for (int t = 0; t < m; ++t)
-                for (int d = lane; d < HD; d += 32) {
-                    put(ko + t * pitch + d, 0.f);
-                    put(vo + t * pitch + d, 0.f);
-                }
+                for (int d = lane; d < HD; d += 32) put(out + t * pitch + d, 0.f);
             continue;
         }
-        const size_t ak = c.at(page, layer, 0, head), av = c.at(page, layer, 1, head);
-        const int8_t* kc = c.codes + ak * c.tile();
-        const int8_t* vc = c.codes + av * c.tile();
-        const float ks = __ldg(c.scales + ak * (c.pt / kKvBlock) + in_page / kKvBlock);
-        const float vs = __ldg(c.scales + av * (c.pt / kKvBlock) + in_page / kKvBlock);
-        for (int e = lane * 4; e < m * HD; e += 128) {  // 4 dims of a row
-            const int t = e / HD, d = e % HD;
-            const char4 w = *reinterpret_cast<const char4*>(kc + (size_t(d / 16) * c.pt + in_page + t) * 16 + d % 16);
-            struct alignas(4 * sizeof(T)) V4 {
-                T a[4];
-            } o;
-            put(&o.a[0], fmul(float(w.x), ks));
-            put(&o.a[1], fmul(float(w.y), ks));
-            put(&o.a[2], fmul(float(w.z), ks));
-            put(&o.a[3], fmul(float(w.w), ks));
-            *reinterpret_cast<V4*>(ko + t * pitch + d) = o;
-        }
+        const size_t at = c.at(page, layer, kind, head);
+        const int8_t* codes = c.codes + at * c.tile();
+        const float scale = __ldg(c.scales + at * (c.pt / kKvBlock) + in_page / kKvBlock);
+        if (kind == 0) {
+            constexpr int R = 128 / HD;  // rows at a time
+            const int d = lane * 4 % HD, up = lane * 4 / HD;
+            unsigned w[kKvBlock / R];
 #pragma unroll
-        for (int d = lane; d < HD; d += 32) {
-            const uint4 w = *reinterpret_cast<const uint4*>(vc + (size_t(in_page / 16) * HD + d) * 16);
-            const unsigned word[4] = {w.x, w.y, w.z, w.w};
+            for (int u = 0; u < kKvBlock / R; ++u)
+                w[u] = *reinterpret_cast<const unsigned*>(codes + (size_t(d / 16) * c.pt + in_page + min(u * R + up, m - 1)) * 16 + d % 16);
 #pragma unroll
-            for (int t = 0; t < kKvBlock; ++t)
-                if (t >= t0 && t < t0 + m)
-                    put(vo + (t - t0) * pitch + d, fmul(float(int8_t(word[t / 4] >> (8 * (t % 4)))), vs));
+            for (int u = 0; u < kKvBlock / R; ++u) {
+                float x[4];
+                codes_f32(w[u], x);
+                Vals<T, 4> o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) put(&o.a[i], fmul(x[i], scale));
+                if (u * R + up < m) *reinterpret_cast<Vals<T, 4>*>(out + (u * R + up) * pitch + d) = o;
+            }
+        } else {
+            constexpr int N = HD / 32;  // dims of a lane
+            uint4 w[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                w[i] = *reinterpret_cast<const uint4*>(codes + (size_t(in_page / 16) * HD + lane * N + i) * 16);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {  // 4 tokens at a time
+                float x[N][4];
+#pragma unroll
+                for (int i = 0; i < N; ++i) codes_f32(h == 0 ? w[i].x : h == 1 ? w[i].y : h == 2 ? w[i].z : w[i].w, x[i]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const int t = h * 4 + z - t0;
+                    Vals<T, N> o;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) put(&o.a[i], fmul(x[i][z], scale));
+                    if (t >= 0 && t < m) *reinterpret_cast<Vals<T, N>*>(out + t * pitch + lane * N) = o;
+                }
+            }
         }
     }
 }
@@ -577,14 +651,17 @@ int page_parts(const KvView& c) { return int((c.page_codes() + 16383) / 16384); 
 template <class T, int HD>
 cudaError_t append_t(const KvView& c, int layer, const void* k, const void* v, long long ks, long long vs, const KvCall& call,
                      int max_new, cudaStream_t st) {
-    constexpr uintptr_t A = 4 * sizeof(T);
     const bool vec = !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | uintptr_t(ks * sizeof(T)) |
-                        uintptr_t(vs * sizeof(T))) % A);
-    const dim3 grid(unsigned((max_new + kKvBlock - 1) / kKvBlock + 1), unsigned(call.n),
-                    unsigned((2 * c.n_kv + kAppendWarps - 1) / kAppendWarps));
+                        uintptr_t(vs * sizeof(T))) % 16);
+    // a CTA takes up to 4 blocks of all heads, where that leaves CTAs enough; else a block of kAppendWarps tasks
+    const long long blocks = (max_new + kKvBlock - 1) / kKvBlock + 1;
+    const bool many = blocks * call.n >= 4 * 4 * 148;
+    const int group = many ? 4 : 1;
+    const dim3 grid(unsigned((blocks + group - 1) / group), unsigned(call.n),
+                    many ? 1u : unsigned((2 * c.n_kv + kAppendWarps - 1) / kAppendWarps));
     auto kern = vec ? k_kv_append<T, HD, true> : k_kv_append<T, HD, false>;
     return launch_pdl(kern, grid, dim3(32 * kAppendWarps), 0, st, false, c, layer, static_cast<const T*>(k),
-                      static_cast<const T*>(v), ks, vs, call, max_new);
+                      static_cast<const T*>(v), ks, vs, call, max_new, group);
 }
 
 template <class T, int HD>
