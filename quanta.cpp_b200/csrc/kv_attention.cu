@@ -816,42 +816,42 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
 
 // Joins the partial sums of the units that k_kv_decode cut, in CTA order.
 // Few partials to a unit (MANY false): CTA x joins the rows of the unit that CTA x of `parts` began, a warp per row.
-// Many: CTA (x, r) joins row r of the x-th unit that was cut, its threads spread over the partials.  (A CTA per began part and
-// row, most of them without work, took 21 us at 2 units of 222 partials and 7 rows.)
+// Many: CTA (x, r) joins row r of the x-th unit that was cut, its threads spread over the partials.  Its time is that of its
+// few loads, one after the other, so that they are as few as can be: the parts' records, then sums and values together.
+// (2 units of 222 partials, 7 rows of 64: a CTA per began part and row, most of them without work, 21 us; the maxima, the sums
+// and the values read one after the other, 11 us.)
 constexpr int kJoinMany = 512, kJoinFew = 256;  // threads
 
 template <int HD, int RM, class T, bool MANY>
 __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnArgs a, DecPlan plan, int parts) {
     constexpr int warps = (MANY ? kJoinMany : kJoinFew) / 32, G = MANY ? kJoinMany / HD : 1, E = HD / 32;
-    extern __shared__ float weight[];  // [n] of the partials, if MANY
-    __shared__ float part[G][HD], red[2][warps];
-    __shared__ int found;
+    __shared__ float weight[MANY ? kJoinMany : 1], part[G][HD], red[2][warps];
+    __shared__ int4 unit;
+    __shared__ int unit_first;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     int first = blockIdx.x;
-    if constexpr (MANY) {
-        if (tid == 0) found = -1;
-        int seen = 0;  // units among the parts before
-        for (int x0 = 0; x0 < parts; x0 += kJoinMany) {
-            const bool began = x0 + tid < parts && __ldcg(&plan.info[x0 + tid].x) >= 0;
-            const unsigned mask = __ballot_sync(0xffffffffu, began);
-            if (lane == 0) red[0][warp] = __int_as_float(__popc(mask));
-            __syncthreads();
-            int before = seen;
-#pragma unroll
-            for (int q = 0; q < warps; ++q) {
-                const int k = __float_as_int(red[0][q]);
-                if (q < warp) before += k;
-                seen += k;
-            }
-            if (began && before + __popc(mask & ((1u << lane) - 1)) == int(blockIdx.x)) found = x0 + tid;
-            __syncthreads();
+    int4 in;  // last CTA, first token, queries, kv head
+    if constexpr (MANY) {  // parts <= kJoinMany
+        in = tid < parts ? __ldcg(plan.info + tid) : make_int4(-1, 0, 0, 0);
+        if (tid == 0) unit_first = -1;
+        const unsigned mask = __ballot_sync(0xffffffffu, in.x >= 0);
+        if (lane == 0) red[0][warp] = __int_as_float(__popc(mask));
+        __syncthreads();
+        const int k = lane < warp ? __float_as_int(red[0][lane]) : 0;
+        const int before = __reduce_add_sync(0xffffffffu, k) + __popc(mask & ((1u << lane) - 1));
+        if (in.x >= 0 && before == int(blockIdx.x)) {
+            unit = in;
+            unit_first = tid;
         }
-        first = found;
+        __syncthreads();
+        first = unit_first;
         if (first < 0) return;
+        in = unit;
+    } else {
+        in = __ldcg(plan.info + first);
+        if (in.x < 0) return;
     }
-    const int4 in = __ldcg(plan.info + first);  // last CTA, first token, queries, kv head
-    if (in.x < 0) return;
     const int n = in.x - first + 1, rows = in.z * a.group;
     auto slot = [&](int x, int r) { return size_t(2 * (first + x) + (x == 0)) * RM + r; };
     auto row_of = [&](int r) { return size_t(in.y + r / a.group) * a.n_heads + in.w * a.group + r % a.group; };
@@ -886,27 +886,26 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
     } else {
         const int d = tid % HD, g = tid / HD, r = blockIdx.y;
         if (r >= rows) return;
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int x = tid; x < n; x += kJoinMany) top = fmaxf(top, weight[x] = __ldcg(plan.ml + slot(x, r) * 2));
-        top = warp_max_redux(top);
+        constexpr int U = 32;  // values read along with the sums
+        const float2 ml = tid < n ? __ldcg(reinterpret_cast<const float2*>(plan.ml) + slot(tid, r)) : make_float2(-INFINITY, 0.f);
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = __ldcg(plan.o + slot(min(g + u * G, n - 1), r) * HD + d);
+        float top = warp_max_redux(ml.x);
         if (lane == 0) red[0][warp] = top;
         __syncthreads();
         top = warp_max_redux(lane < warps ? red[0][lane] : -INFINITY);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float l = 0.f;
-#pragma unroll 1
-        for (int x = tid; x < n; x += kJoinMany) {
-            const float w = ex2_full(weight[x] - ref);
-            weight[x] = w;
-            l += w * __ldcg(plan.ml + slot(x, r) * 2 + 1);
-        }
-        l = warp_sum(l);
+        const float w = ex2_full(ml.x - (top == -INFINITY ? 0.f : top));
+        weight[tid] = w;
+        float l = warp_sum(ml.y * w);
         if (lane == 0) red[1][warp] = l;
         __syncthreads();
         float o = 0.f;
-#pragma unroll 16
-        for (int x = g; x < n; x += G) o = fmaf(__ldcg(plan.o + slot(x, r) * HD + d), weight[x], o);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (g + u * G < n) o = fmaf(v[u], weight[g + u * G], o);
+#pragma unroll 4
+        for (int x = g + U * G; x < n; x += G) o = fmaf(__ldcg(plan.o + slot(x, r) * HD + d), weight[x], o);
         part[g][d] = o;
         __syncthreads();
         if (g == 0) {
@@ -965,6 +964,12 @@ struct ChunkPlan {
     float* ml;   // [n_tok * n_heads][splits][2] maximum (log2) and sum, if splits > 1
     float* o;    // [n_tok * n_heads][splits][HD]
 };
+
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 // 4 int8 codes -> 4 f16, exactly: 1024 + (code + 128), less 1152.
 __device__ __forceinline__ uint2 codes_f16(unsigned w) {
@@ -1171,7 +1176,8 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
         const bool valid = r < rows, busy = r0 + g * 128 + (warp & 3) * 32 < rows;  // busy: the warp has rows
         const int qi = valid ? r / a.group : 0, qh = head * a.group + (valid ? r % a.group : 0), pos = p0 + qi;
         const uint32_t my = tmem + (uint32_t((warp & 3) * 32) << 16);
-        float fac = a.scale * kLog2e;  // score = S * fac * ks, log2
+        float fac = fabsf(a.scale) * kLog2e;  // score = S * fac * ks, log2 (the queries carry the scale's sign)
+        const float sign = copysignf(1.f, a.scale);
         if (nt > 0) {
             // the warp's 32 rows, one after the other (coalesced), 8 in flight; lane = HD / 32 dims
             constexpr int E = HD / 32;
@@ -1197,7 +1203,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                         // a power of two brings the row's largest value to [1, 2); 255: not finite, left as it is
                         const int e = int(__float_as_uint(warp_max_redux(amax)) >> 23);
                         const int up = e == 255 ? 127 : min(max(254 - e, 1), 253);  // its biased exponent
-                        const float pre = __uint_as_float(unsigned(up) << 23);
+                        const float pre = __uint_as_float(unsigned(up) << 23) * sign;
                         if (lane == r8 + y) fac *= __uint_as_float(unsigned(254 - up) << 23);
 #pragma unroll
                         for (int z = 0; z < E; ++z) f[z] *= pre;
@@ -1242,24 +1248,29 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             tmem_ready(s1);
             tc_fence_before();
             mbar_arrive(&s_free[g]);
-            const float f[4] = {ks.x * fac, ks.y * fac, ks.z * fac, ks.w * fac};
-            float s[64];
+            float f[4] = {ks.x * fac, ks.y * fac, ks.z * fac, ks.w * fac};  // none below 0
+            float s[64];  // scores less the factor f of their 16 keys
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
-                s[k] = __int_as_float(s0[k]) * f[k / 16];
-                s[k + 32] = __int_as_float(s1[k]) * f[2 + k / 16];
+                s[k] = __int_as_float(s0[k]);
+                s[k + 32] = __int_as_float(s1[k]);
             }
             // do all of the warp's rows see the whole tile?  (rows past the end do as they like)
             const bool whole = key0 + C::keys - 1 <= pos && (!a.window || key0 > pos - a.window);
             if (!__all_sync(0xffffffffu, whole)) {
                 const int last = pos - key0, first = a.window ? last - a.window + 1 : -1;
 #pragma unroll
-                for (int k = 0; k < 64; ++k)
-                    if (k > last || k < first) s[k] = -INFINITY;
+                for (int k = 0; k < 64; ++k) s[k] = k > last || k < first ? -INFINITY : s[k] * f[k / 16];
+                f[0] = f[1] = f[2] = f[3] = 1.f;
             }
-            float top = s[0];
+            float top = -INFINITY;
 #pragma unroll
-            for (int k = 1; k < 64; ++k) top = fmaxf(top, s[k]);
+            for (int b = 0; b < 4; ++b) {
+                float m = s[16 * b];
+#pragma unroll
+                for (int k = 1; k < 15; k += 2) m = fmaxf(fmaxf(m, s[16 * b + k]), s[16 * b + k + 1]);
+                top = fmaxf(top, fmaxf(m, s[16 * b + 15]) * f[b]);
+            }
             const bool up = top > ref + kChunkRaise;
             const float now = up ? top : ref;
             float factor = up ? ex2(0.5f * (ref - now)) : 1.f;  // the square root of O's: that may be below 2^-126
@@ -1303,15 +1314,19 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     float p[16];
+                    const unsigned long long f2 = f2_pack(f[b], f[b]), base2 = f2_pack(-base, -base), vr2 = f2_pack(vr[b], vr[b]);
+                    unsigned long long part[2] = {0, 0};  // two keys at a time
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) p[k] = ex2(s[16 * b + k] - base);
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        part[k & 3] += p[k];
-                        p[k] *= vr[b];
+                    for (int k = 0; k < 16; k += 2) {
+                        const float2 x = f2_unpack(f2_fma(f2_pack(s[16 * b + k], s[16 * b + k + 1]), f2, base2));
+                        const unsigned long long e = f2_pack(ex2(x.x), ex2(x.y));
+                        part[k / 2 & 1] = f2_add(part[k / 2 & 1], e);
+                        const float2 y = f2_unpack(f2_mul(e, vr2));
+                        p[k] = y.x;
+                        p[k + 1] = y.y;
                     }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                    const float2 both = f2_unpack(f2_add(part[0], part[1]));
+                    sum += both.x + both.y;
 #pragma unroll
                     for (int z = 0; z < NP; ++z) {
                         unsigned o[8];
@@ -1321,8 +1336,10 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                                 const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * y], p[2 * y + 1]);
                                 o[y] = reinterpret_cast<const unsigned&>(h);
                                 if (z + 1 < NP) {
-                                    p[2 * y] -= __uint_as_float(o[y] << 16);
-                                    p[2 * y + 1] -= __uint_as_float(o[y] & 0xffff0000u);
+                                    const float2 left = f2_unpack(f2_add(f2_pack(p[2 * y], p[2 * y + 1]),
+                                                                     f2_pack(-__uint_as_float(o[y] << 16), -__uint_as_float(o[y] & 0xffff0000u))));
+                                    p[2 * y] = left.x;
+                                    p[2 * y + 1] = left.y;
                                 }
                             } else {
                                 const __half2 h = __floats2half2_rn(p[2 * y], p[2 * y + 1]);
@@ -1470,9 +1487,10 @@ cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, v
     e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
     if (e != cudaSuccess || !l.even) return e;
     // more than 32 partials to a unit: a CTA per row, else a warp
+    static_assert(148 * C::ctas <= kJoinMany, "a record per thread");
     if (size_t(l.grid) > l.units * 32)
-        return launch_pdl(k_kv_join<HD, RM, T, true>, dim3(unsigned(l.units), unsigned(a.max_q * a.group)), dim3(kJoinMany),
-                          size_t(l.grid) * 4, st, true, a, p, int(l.grid));
+        return launch_pdl(k_kv_join<HD, RM, T, true>, dim3(unsigned(l.units), unsigned(a.max_q * a.group)), dim3(kJoinMany), 0,
+                          st, true, a, p, int(l.grid));
     return launch_pdl(k_kv_join<HD, RM, T, false>, dim3(unsigned(l.grid)), dim3(kJoinFew), 0, st, true, a, p, int(l.grid));
 }
 
