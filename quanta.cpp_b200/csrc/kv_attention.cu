@@ -46,7 +46,9 @@ constexpr int kDecThreads = kDecSoft + 32;
 constexpr int kTileKeys = 128;
 constexpr float kDigitMax = 8323072.0f;  // 127 * 256^2: three digits
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFlush = 16;               // tiles whose O stays in TMEM
+// Tiles whose O stays in TMEM before registers take it over: the tensor cores add with their sums cut off, not rounded, a bias of
+// about 2^-26 for each of a tile's 8 steps.  (float32, 5 tiles: 5.5e-7 of the result; 16 tiles pass what 16-bit results show.)
+template <class T> constexpr int kFlush = sizeof(T) == 4 ? 4 : 16;
 constexpr float kShift = 32.f;           // log2: weights are exp(s - ref) 2^kShift, so that none that f32 can hold is flushed
 constexpr float kRaise = 32.f;           // log2: how far a score may pass the reference
 
@@ -600,7 +602,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         }
                     }
                 }
-                bool high = in_tmem == kFlush;
+                bool high = in_tmem == kFlush<T>;
                 const unsigned had = unset;
                 if (had) {  // rows without a reference that see a key of this tile take the last one's score
                     unsigned can = 0;
@@ -928,11 +930,12 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 // tile for all rows.
 // A query row is scaled by a power of two and is the sum of f16 pieces: two for float32 (2^-23 of the row's largest value), one,
 // exactly, for 16-bit types.  A weight W = exp(s - ref) vs is
-//   float32 queries: the sum of three bf16 pieces (24 bits, f32's range); V in bf16
-//   16-bit queries: one f16 (11 bits cost as much as the result's own rounding to f16); V in f16.  vs is divided by a power
-//     of two near the first tile's largest, and W held below 2^15, so that f16's range serves.
+//   float32 queries: the sum of three bf16 pieces (24 bits, f32's range); V in bf16.  The tensor cores' sums are cut off, not
+//     rounded (12 steps a tile: 1e-6 of the result after 8 tiles), so O moves every other tile to a total in shared memory.
+//   16-bit queries: f16, one (bf16 results) or the sum of two (11 bits would cost as much again as f16's own rounding); V in
+//     f16.  vs is divided by a power of two near the first tile's largest, and W held below 2^15, so that f16's range serves.
 //   warps 0 .. 4 WG - 1  softmax, thread = row: S from TMEM, weights back to TMEM (the A operand of the second product); the
-//                        reference of a row is raised only when a score passes it by 2^4 (O is then scaled in TMEM)
+//                        reference of a row is raised only when a score passes it by far (O is then scaled)
 //   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
 //                        to 16-bit operands
 //   last warp            issues the MMAs: S of tile i + 1 runs beside the softmax of tile i
@@ -940,24 +943,30 @@ template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and f
 struct Chunk {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int QP = F32 ? 2 : 1;               // pieces of a query
-    static constexpr int NP = F32 ? 3 : 1;               // pieces of a weight
+    static constexpr int NP = F32 ? 3 : std::is_same<T, __half>::value ? 2 : 1;  // pieces of a weight
+    static constexpr int flush = F32 ? 2 : 1 << 30;      // tiles whose O stays in TMEM
     static constexpr int rows = 128 * WG;
     static constexpr int threads = 128 * WG + 128 + 32;
     static constexpr int keys = 64;
     // operands in swizzled rows of 128 bytes: of a query piece and of K, HD / 64 slabs of 64 dims; of V, a row per dim
     static constexpr int q_bytes = 128 * HD * 2, kv_bytes = keys * HD * 2;
-    static constexpr int smem = WG * QP * q_bytes + 4 * kv_bytes + 2 * keys * HD;
+    static constexpr int total_at = WG * QP * q_bytes + 4 * kv_bytes + 2 * keys * HD;
+    static constexpr int smem = total_at + (F32 ? WG * HD * 128 * 4 : 0);
     static constexpr int p_cols = NP * keys / 2;
     static constexpr int s_at = 0, p_at = 64 * WG, o_at = p_at + p_cols * WG;  // TMEM columns
     static constexpr int tmem_cols = o_at + HD * WG <= 256 ? 256 : 512;
-    static constexpr int ctas = smem <= 112 * 1024 && tmem_cols == 256 ? 2 : 1;  // per SM (with 1 KB static and 1 KB of the system's each)
+    // per SM, with 1 KB static and 1 KB of the system's each.  (float32: two would leave a thread 96 registers, which it spills:
+    // 31 us instead of 25 for 512 queries of 14 heads of 64 over 512 keys.)
+    static constexpr int ctas = !F32 && smem <= 112 * 1024 && tmem_cols == 256 ? 2 : 1;
     static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // W and V: bf16 or f16
     static constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
-    static constexpr float shift = F32 ? kShift : 7.f;   // log2: weights carry 2^shift
+    // log2.  Weights carry 2^shift; a row's reference follows its scores when one passes it by more than raise (every raise has
+    // the warp's O pass through its registers: with 4 instead of 7 every other tile did, 1.3 times the time).  16-bit weights,
+    // at most 2^(7 + 7) times V's scale over its reference (at most 2), stay below f16's 65504.
+    static constexpr float shift = F32 ? kShift : 7.f, raise = F32 ? 10.f : 7.f;
     static_assert(o_at + HD * WG <= 512, "TMEM");
 };
-constexpr float kChunkRaise = 4.f;
 
 struct ChunkPlan {
     int splits;  // stretches of keys per row tile
@@ -1075,7 +1084,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                         for (int k = 0; k < C::keys / 16; ++k)
                             mma_f16_ts<sw_hi<128>, C::idesc_o>(tmem + C::o_at + g * HD,
                                                                tmem + C::p_at + g * C::p_cols + z * (C::keys / 2) + k * 8, vt + 2 * k,
-                                                               t > 0 || z > 0 || k > 0);
+                                                               t % C::flush > 0 || z > 0 || k > 0);
                     mma_commit_elect(&o_done[g]);
                     if (g == wgs - 1) mma_commit_elect(&v_free[t & 1]);
                 }
@@ -1231,6 +1240,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             fence_async_smem();
             mbar_arrive(&q_full[g]);
         }
+        float* total = reinterpret_cast<float*>(smem + C::total_at) + g * HD * 128 + rt;  // (float32) [dim][row]
         float ref = -INFINITY, sum = 0.f, v_ref = 0.f, v_inv = 0.f;  // v_ref: 16-bit weights carry vs / v_ref
         bool ok = true;
 #pragma unroll 1
@@ -1271,7 +1281,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 for (int k = 1; k < 15; k += 2) m = fmaxf(fmaxf(m, s[16 * b + k]), s[16 * b + k + 1]);
                 top = fmaxf(top, fmaxf(m, s[16 * b + 15]) * f[b]);
             }
-            const bool up = top > ref + kChunkRaise;
+            const bool up = top > ref + C::raise;
             const float now = up ? top : ref;
             float factor = up ? ex2(0.5f * (ref - now)) : 1.f;  // the square root of O's: that may be below 2^-126
             if (ref == -INFINITY) factor = 0.f;  // (an infinite score as the first reference)
@@ -1279,7 +1289,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             bool change = up;
             if (!F32) {  // the same in all threads
                 const float v_max = fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w));
-                if (v_max > 16.f * v_ref) {
+                if (v_max > 2.f * v_ref) {
                     const int e = min(max(int(__float_as_uint(v_max) >> 23), 1), 253);
                     const float next = __uint_as_float(unsigned(e) << 23);
                     if (v_ref > 0.f) v_factor = v_ref / next;
@@ -1294,7 +1304,8 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 ok = wait_warp(&o_done[g], (i - 1) & 1, ab);
                 if (!ok) break;
                 tc_fence_after();
-                if (__any_sync(0xffffffffu, change) && busy) {
+                const bool out = F32 && i % C::flush == 0;  // O moves to the total: the next product starts anew
+                if ((out || __any_sync(0xffffffffu, change)) && busy) {
 #pragma unroll 1
                     for (int x = 0; x < HD; x += 16) {
                         int o[16];
@@ -1302,9 +1313,18 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                         tmem_ld_wait();
                         tmem_ready(o);
                         unsigned n[16];
+                        float* tt = total + x * 128;
 #pragma unroll
-                        for (int z = 0; z < 16; ++z) n[z] = __float_as_uint(__int_as_float(o[z]) * v_factor * factor * factor);
-                        tmem_st(my + C::o_at + g * HD + x, n);
+                        for (int z = 0; z < 16; ++z) {
+                            float y = __int_as_float(o[z]);
+                            if constexpr (F32) {
+                                const float t = i > C::flush ? tt[z * 128] : 0.f;
+                                if (out) y += t;
+                                if (i > C::flush || out) tt[z * 128] = (out ? y : t) * factor * factor;
+                            }
+                            n[z] = __float_as_uint(y * v_factor * factor * factor);
+                        }
+                        if (!out) tmem_st(my + C::o_at + g * HD + x, n);
                     }
                 }
             }
@@ -1344,6 +1364,11 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                             } else {
                                 const __half2 h = __floats2half2_rn(p[2 * y], p[2 * y + 1]);
                                 o[y] = reinterpret_cast<const unsigned&>(h);
+                                if (z + 1 < NP) {
+                                    const float2 b = __half22float2(h), left = f2_unpack(f2_add(f2_pack(p[2 * y], p[2 * y + 1]), f2_pack(-b.x, -b.y)));
+                                    p[2 * y] = left.x;
+                                    p[2 * y + 1] = left.y;
+                                }
                             }
                         }
                         tmem_st(my + C::p_at + g * C::p_cols + z * (C::keys / 2) + b * 8, o);
@@ -1373,6 +1398,10 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                     tmem_ld(my + C::o_at + g * HD + x, o);
                     tmem_ld_wait();
                     tmem_ready(o);
+                }
+                if (F32 && nt > C::flush) {
+#pragma unroll
+                    for (int z = 0; z < 32; ++z) o[z] = __float_as_int(__int_as_float(o[z]) + total[(x + z) * 128]);
                 }
 #pragma unroll
                 for (int z = 0; z < 32; ++z) turn[lane * 32 + (z ^ lane)] = none ? 0.f : __int_as_float(o[z]) * factor;
