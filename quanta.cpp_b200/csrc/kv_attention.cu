@@ -932,8 +932,11 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 // exactly, for 16-bit types.  A weight W = exp(s - ref) vs is
 //   float32 queries: the sum of three bf16 pieces (24 bits, f32's range); V in bf16.  The tensor cores' sums are cut off, not
 //     rounded (12 steps a tile: 1e-6 of the result after 8 tiles), so O moves every other tile to a total in shared memory.
-//   16-bit queries: f16, one (bf16 results) or the sum of two (11 bits would cost as much again as f16's own rounding); V in
-//     f16.  vs is divided by a power of two near the first tile's largest, and W held below 2^15, so that f16's range serves.
+//   bf16 queries: two bf16 pieces (16 bits).  f16 would lose weights below 2^-31 of the largest, which a bf16 result still shows
+//     where the key ahead has a 0 for V.
+//   f16 queries: the sum of two f16 (11 bits would cost as much again as the result's own rounding); V in f16, in fewer
+//     instructions than bf16.  vs is divided by a power of two near the first tile's largest, and W held below 2^15, so that f16's
+//     range serves.
 //   warps 0 .. 4 WG - 1  softmax, thread = row: S from TMEM, weights back to TMEM (the A operand of the second product); the
 //                        reference of a row is raised only when a score passes it by far (O is then scaled)
 //   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
@@ -941,9 +944,9 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 //   last warp            issues the MMAs: S of tile i + 1 runs beside the softmax of tile i
 template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
-    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
     static constexpr int QP = F32 ? 2 : 1;               // pieces of a query
-    static constexpr int NP = F32 ? 3 : std::is_same<T, __half>::value ? 2 : 1;  // pieces of a weight
+    static constexpr int NP = F32 ? 3 : 2;               // pieces of a weight
     static constexpr int flush = F32 ? 2 : 1 << 30;      // tiles whose O stays in TMEM
     static constexpr int rows = 128 * WG;
     static constexpr int threads = 128 * WG + 128 + 32;
@@ -958,13 +961,13 @@ struct Chunk {
     // per SM, with 1 KB static and 1 KB of the system's each.  (float32: two would leave a thread 96 registers, which it spills:
     // 31 us instead of 25 for 512 queries of 14 heads of 64 over 512 keys.)
     static constexpr int ctas = !F32 && smem <= 112 * 1024 && tmem_cols == 256 ? 2 : 1;
-    static constexpr uint32_t fmt = F32 ? (1u << 7) | (1u << 10) : 0u;       // W and V: bf16 or f16
+    static constexpr uint32_t fmt = F16 ? 0u : (1u << 7) | (1u << 10);       // W and V: f16 or bf16
     static constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     // log2.  Weights carry 2^shift; a row's reference follows its scores when one passes it by more than raise (every raise has
-    // the warp's O pass through its registers: with 4 instead of 7 every other tile did, 1.3 times the time).  16-bit weights,
-    // at most 2^(7 + 7) times V's scale over its reference (at most 2), stay below f16's 65504.
-    static constexpr float shift = F32 ? kShift : 7.f, raise = F32 ? 10.f : 7.f;
+    // the warp's O pass through its registers: with 4 instead of 7 every other tile did, 1.3 times the time).  f16 weights, at
+    // most 2^(7 + 7) times V's scale over its reference (at most 2), stay below f16's 65504.
+    static constexpr float shift = F16 ? 7.f : kShift, raise = F16 ? 7.f : 10.f;
     static_assert(o_at + HD * WG <= 512, "TMEM");
 };
 
@@ -993,7 +996,7 @@ template <int HD, class T, int WG>
 __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::ctas) k_kv_chunk(KvView c, KvAttnArgs a, KvCall call, ChunkPlan plan) {
     using C = Chunk<HD, T, WG>;
     constexpr int QP = C::QP, NP = C::NP;
-    constexpr bool F32 = C::F32;
+    constexpr bool F32 = C::F32, F16 = C::F16;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* kb = smem + WG * QP * C::q_bytes;   // 2 buffers
     unsigned char* vb = kb + 2 * C::kv_bytes;          // 2 buffers
@@ -1174,7 +1177,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             if (i >= 2) ok = ok && wait_warp(&v_free[i & 1], ((i >> 1) - 1) & 1, ab);
             unsigned char* vt = vb + (i & 1) * C::kv_bytes;
 #pragma unroll
-            for (int x = 0; x < pieces; ++x) convert(vt, ct % HD, 2 * (ct / HD + x * (128 / HD)), vc[x], F32);
+            for (int x = 0; x < pieces; ++x) convert(vt, ct % HD, 2 * (ct / HD + x * (128 / HD)), vc[x], !F16);
             fence_async_smem();
             mbar_arrive(&v_full[i & 1]);
         }
@@ -1241,7 +1244,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             mbar_arrive(&q_full[g]);
         }
         float* total = reinterpret_cast<float*>(smem + C::total_at) + g * HD * 128 + rt;  // (float32) [dim][row]
-        float ref = -INFINITY, sum = 0.f, v_ref = 0.f, v_inv = 0.f;  // v_ref: 16-bit weights carry vs / v_ref
+        float ref = -INFINITY, sum = 0.f, v_ref = 0.f, v_inv = 0.f;  // v_ref: f16 weights carry vs / v_ref
         bool ok = true;
 #pragma unroll 1
         for (int i = 0; i < nt && ok; ++i) {
@@ -1287,7 +1290,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             if (ref == -INFINITY) factor = 0.f;  // (an infinite score as the first reference)
             float v_factor = 1.f;
             bool change = up;
-            if (!F32) {  // the same in all threads
+            if (F16) {  // the same in all threads
                 const float v_max = fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w));
                 if (v_max > 2.f * v_ref) {
                     const int e = min(max(int(__float_as_uint(v_max) >> 23), 1), 253);
@@ -1330,7 +1333,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             }
             if (busy) {
                 const float base = (ref == -INFINITY ? 0.f : ref) - C::shift;
-                const float vr[4] = {F32 ? vs.x : vs.x * v_inv, F32 ? vs.y : vs.y * v_inv, F32 ? vs.z : vs.z * v_inv, F32 ? vs.w : vs.w * v_inv};
+                const float vr[4] = {F16 ? vs.x * v_inv : vs.x, F16 ? vs.y * v_inv : vs.y, F16 ? vs.z * v_inv : vs.z, F16 ? vs.w * v_inv : vs.w};
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     float p[16];
@@ -1352,7 +1355,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                         unsigned o[8];
 #pragma unroll
                         for (int y = 0; y < 8; ++y) {
-                            if constexpr (F32) {
+                            if constexpr (!F16) {
                                 const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * y], p[2 * y + 1]);
                                 o[y] = reinterpret_cast<const unsigned&>(h);
                                 if (z + 1 < NP) {
@@ -1385,7 +1388,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
         const bool none = sum == 0.f && ref == -INFINITY;
         const size_t row = size_t(w.t0 + qi) * a.n_heads + qh;
         const bool direct = plan.splits == 1;
-        const float factor = (F32 ? 1.f : v_ref) * (direct ? none ? 0.f : 1.f / sum : 1.f);
+        const float factor = (F16 ? v_ref : 1.f) * (direct ? none ? 0.f : 1.f / sum : 1.f);
         if (ok && busy) {
             // 32 rows x 32 dims at a time through shared memory (the queries are no longer read), so that rows leave whole
             float* turn = reinterpret_cast<float*>(smem + g * QP * C::q_bytes) + (warp & 3) * 1024;
