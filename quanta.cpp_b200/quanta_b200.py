@@ -324,6 +324,8 @@ class PagedKV:
         self._p = C.byref(self._c)
         self._types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
         self._ws, self._need = {}, {}
+        self._lib, self._index = lib(), codes.device.index  # a call's host time counts where few tokens are decoded
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._page_ws = lib().qnt_kv_page_workspace(self._p)
         if self._page_ws == 0:
             raise QntError(-1, lib().qnt_last_error().decode(errors="replace"))
@@ -340,7 +342,7 @@ class PagedKV:
 
     def _stream(self, stream):
         if stream is None:
-            return self._torch.cuda.current_stream(self.device).cuda_stream
+            return self._raw_stream(self._index) if self._raw_stream else self._torch.cuda.current_stream(self.device).cuda_stream
         return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
     def _workspace(self, stream: int, need: int):
@@ -372,7 +374,7 @@ class PagedKV:
             raise ValueError("one extra per sequence")
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
-        _check(lib().qnt_kv_reserve(self._p, seqs.data_ptr(), extra.data_ptr(), n, w, nb, s))
+        _check(self._lib.qnt_kv_reserve(self._p, seqs.data_ptr(), extra.data_ptr(), n, w, nb, s))
 
     def fork(self, src, dst, stream=None):
         """Empty sequences dst become copies of src: full pages shared, a part-filled last page copied."""
@@ -381,24 +383,24 @@ class PagedKV:
             raise ValueError("one dst per src")
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
-        _check(lib().qnt_kv_fork(self._p, src.data_ptr(), dst.data_ptr(), n, w, nb, s))
+        _check(self._lib.qnt_kv_fork(self._p, src.data_ptr(), dst.data_ptr(), n, w, nb, s))
 
     def free(self, seqs, stream=None):
         """The sequences give back their pages and become empty."""
-        _check(lib().qnt_kv_free(self._p, seqs.data_ptr(), self._list(seqs), self._stream(stream)))
+        _check(self._lib.qnt_kv_free(self._p, seqs.data_ptr(), self._list(seqs), self._stream(stream)))
 
     def compact(self, stream=None):
         """The pages in use move together to the lowest indices."""
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
-        _check(lib().qnt_kv_compact(self._p, w, nb, s))
+        _check(self._lib.qnt_kv_compact(self._p, w, nb, s))
 
     def copy_pages(self, src, dst, stream=None):
         """Codes and scales of pages src over those of pages dst, all layers."""
         n = self._list(src, dst)
         if dst.numel() != n:
             raise ValueError("one dst per src")
-        _check(lib().qnt_kv_copy(self._p, src.data_ptr(), dst.data_ptr(), n, self._stream(stream)))
+        _check(self._lib.qnt_kv_copy(self._p, src.data_ptr(), dst.data_ptr(), n, self._stream(stream)))
 
     def append(self, layer: int, k, v, seqs, starts, max_new: int | None = None, stream=None):
         """Quantizes rows k, v [tokens, n_kv_heads, head_dim] into a layer, as the last positions of their sequences
@@ -409,7 +411,7 @@ class PagedKV:
         n, m = self._list(seqs, starts), k.shape[0]
         if starts.numel() != n + 1:
             raise ValueError("starts must have one entry more than seqs")
-        _check(lib().qnt_kv_append(self._p, layer, k.data_ptr(), v.data_ptr(), dt, k.stride(0), v.stride(0), seqs.data_ptr(),
+        _check(self._lib.qnt_kv_append(self._p, layer, k.data_ptr(), v.data_ptr(), dt, k.stride(0), v.stride(0), seqs.data_ptr(),
                                    starts.data_ptr(), n, m, m if max_new is None else max_new, self._stream(stream)))
 
     def read(self, layer: int, seqs, first, starts, n_tok: int, dtype=None, stream=None):
@@ -422,9 +424,9 @@ class PagedKV:
         n = self._list(seqs, first, starts)
         if first.numel() != n or starts.numel() != n + 1:
             raise ValueError("one first per sequence, and one entry more in starts")
-        k = t.empty((n_tok, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        k = self.scales.new_empty((n_tok, self.n_kv_heads, self.head_dim), dtype=dtype)
         v = t.empty_like(k)
-        _check(lib().qnt_kv_read(self._p, layer, seqs.data_ptr(), first.data_ptr(), starts.data_ptr(), n, n_tok, k.data_ptr(),
+        _check(self._lib.qnt_kv_read(self._p, layer, seqs.data_ptr(), first.data_ptr(), starts.data_ptr(), n, n_tok, k.data_ptr(),
                                  v.data_ptr(), self._types[dtype], self._stream(stream)))
         return k, v
 
@@ -433,7 +435,6 @@ class PagedKV:
         """Attention of q [tokens, n_heads, head_dim] over the cache of their sequences; query i of a sequence's m sits at
         position lens - m + i and sees the positions up to its own (the last `window` of them, if window > 0).  max_q bounds
         a sequence's queries, max_len its length.  Returns out (q's type), or (out, lse) with lse float32 [tokens, n_heads]."""
-        t = self._torch
         dt = self._rows("q", q)
         n_tok, heads = q.shape[0], q.shape[1]
         n = self._list(seqs, starts)
@@ -444,19 +445,19 @@ class PagedKV:
         if need is None:
             if len(self._need) > 4096:
                 self._need.clear()
-            need = self._need[key] = lib().qnt_kv_attention_workspace(self._p, heads, n, n_tok, max_q, max_len)
+            need = self._need[key] = self._lib.qnt_kv_attention_workspace(self._p, heads, n, n_tok, max_q, max_len)
         s = self._stream(stream)
         w, nb = self._workspace(s, need)
-        out = t.empty((n_tok, heads, self.head_dim), dtype=q.dtype, device=self.device)
-        ls = t.empty((n_tok, heads), dtype=t.float32, device=self.device) if lse else None
-        _check(lib().qnt_kv_attention(self._p, layer, q.data_ptr(), dt, q.stride(0), heads, seqs.data_ptr(), starts.data_ptr(), n,
+        out = self._torch.empty_like(q)  # (a token's heads are contiguous and tokens do not overlap: so is this)
+        ls = self.scales.new_empty((n_tok, heads)) if lse else None
+        _check(self._lib.qnt_kv_attention(self._p, layer, q.data_ptr(), dt, q.stride(0), heads, seqs.data_ptr(), starts.data_ptr(), n,
                                       n_tok, max_q, max_len, self.head_dim ** -0.5 if scale is None else scale, window,
                                       out.data_ptr(), None if ls is None else ls.data_ptr(), w, nb, s))
         return (out, ls) if lse else out
 
     def check(self, stream=None):
         """Waits for the stream and raises the error that earlier calls on this cache ran into, if any."""
-        _check(lib().qnt_kv_check(self._p, self._stream(stream)))
+        _check(self._lib.qnt_kv_check(self._p, self._stream(stream)))
 
 
 def bench_mma_i8(iters: int = 4096) -> float:
