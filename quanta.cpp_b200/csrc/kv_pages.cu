@@ -655,6 +655,16 @@ __global__ void __launch_bounds__(256) k_kv_copy(KvView c, const int* __restrict
     if (a != b) copy_page(c, a, b, blockIdx.x, gridDim.x);
 }
 
+// A planning kernel's launch; large pools and many sequences pass the default limit of shared memory (48 KB, static included).
+template <class... KArgs, class... Args>
+cudaError_t launch_plan(void (*kernel)(KArgs...), int ctas, int threads, size_t smem, cudaStream_t st, Args... args) {
+    if (smem > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(kernel, dim3(unsigned(ctas)), dim3(unsigned(threads)), smem, st, false, args...);
+}
+
 size_t plan_smem(const KvView& c, int n) { return plan_words(c) * 4 + size_t(c.max_seqs) * 4 + size_t(n) * 4; }
 
 // A page in parts of about 16 KB, so that one page's copy spreads over several SMs.
@@ -713,8 +723,7 @@ size_t kv_page_ws_bytes(const KvView& c) { return (size_t(c.n_pages) * 3 + size_
 
 cudaError_t launch_kv_reserve(const KvView& c, const int* seqs, const int* extra, int n, void* ws, cudaStream_t st) {
     if (n == 0) return cudaSuccess;
-    return launch_pdl(k_kv_reserve, dim3(1), dim3(kPlanThreads), plan_smem(c, n), st, false, c, seqs, extra, n,
-                      static_cast<int*>(ws));
+    return launch_plan(k_kv_reserve, 1, kPlanThreads, plan_smem(c, n), st, c, seqs, extra, n, static_cast<int*>(ws));
 }
 
 cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int n, void* ws, cudaStream_t st) {
@@ -722,7 +731,7 @@ cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int 
     int* ok = static_cast<int*>(ws);
     int* fresh = ok + 4;
     int* list = fresh + c.max_seqs;
-    cudaError_t e = launch_pdl(k_kv_fork_plan, dim3(1), dim3(kPlanThreads), plan_smem(c, 0), st, false, c, src, dst, n, ok, fresh, list);
+    cudaError_t e = launch_plan(k_kv_fork_plan, 1, kPlanThreads, plan_smem(c, 0), st, c, src, dst, n, ok, fresh, list);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_kv_fork, dim3(unsigned(page_parts(c)), unsigned(n)), dim3(256), 0, st, true, c, src, dst,
                       static_cast<const int*>(ok), static_cast<const int*>(fresh));
@@ -730,7 +739,7 @@ cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int 
 
 cudaError_t launch_kv_free(const KvView& c, const int* seqs, int n, cudaStream_t st) {
     if (n == 0) return cudaSuccess;
-    return launch_pdl(k_kv_free, dim3(unsigned(n < 148 ? n : 148)), dim3(256), size_t(c.max_seqs) * 4, st, false, c, seqs, n);
+    return launch_plan(k_kv_free, n < 148 ? n : 148, 256, size_t(c.max_seqs) * 4, st, c, seqs, n);
 }
 
 cudaError_t launch_kv_compact(const KvView& c, void* ws, cudaStream_t st) {
@@ -738,7 +747,7 @@ cudaError_t launch_kv_compact(const KvView& c, void* ws, cudaStream_t st) {
     int* from = moves + 4;
     int* to = from + c.n_pages;
     int* map = to + c.n_pages;
-    cudaError_t e = launch_pdl(k_kv_compact_plan, dim3(1), dim3(kPlanThreads), plan_words(c) * 4, st, false, c, moves, from, to, map);
+    cudaError_t e = launch_plan(k_kv_compact_plan, 1, kPlanThreads, plan_words(c) * 4, st, c, moves, from, to, map);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_kv_compact, dim3(148 * 8), dim3(256), 0, st, true, c, static_cast<const int*>(moves),
                       static_cast<const int*>(from), static_cast<const int*>(to), static_cast<const int*>(map), page_parts(c));

@@ -39,3 +39,33 @@ def test_single_tokens_among_chunks(qb, name, kv, group, hd):
     check_attention(c, 0, queries(sum(news), kv * group, hd, name), list(range(20)), news, name=name)
     check_attention(c, 0, queries(sum(news), kv * group, hd, name), list(range(20)), news, window=777, name=name)
 
+
+
+def test_page_operations_of_the_largest_cache(qb):
+    """2^20 pages and 8192 sequences: reserve, fork, free and compact, each over thousands of sequences in a call."""
+    import torch
+    n_pages, most = 1 << 20, 8192
+    c = qb.PagedKV.empty(1, 1, 64, n_pages, most, 64, 16)
+    rng = np.random.default_rng(0)
+    lens = rng.integers(0, 900, most).astype(np.int32)
+    half = most // 2
+    lens[half:] = 0
+    seqs = torch.randperm(most, device="cuda").to(torch.int32)
+    c.reserve(seqs, torch.tensor(lens, device="cuda")[seqs.long()])
+    c.check()
+    used = int(((lens + 15) // 16).sum())
+    assert c.lens.tolist() == lens.tolist() and int((c.refs > 0).sum()) == used and int((c.refs[:used] == 1).sum()) == used
+    src = torch.arange(half, device="cuda", dtype=torch.int32)
+    c.fork(src, src + half)
+    c.check()
+    own = int((lens[:half] % 16 != 0).sum())
+    assert c.lens[half:].tolist() == lens[:half].tolist() and int((c.refs > 0).sum()) == used + own
+    assert int(c.refs.sum()) == 2 * used
+    c.free(src)
+    c.check()
+    assert int((c.refs > 0).sum()) == used and int((c.refs > 1).sum()) == 0
+    c.compact()
+    c.check()
+    assert int((c.refs[:used] == 1).sum()) == used
+    pages = c.table[half:][c.table[half:] >= 0]
+    assert int((c.table[:half] >= 0).sum()) == 0 and torch.equal(pages.sort().values, torch.arange(used, device="cuda", dtype=torch.int32))
