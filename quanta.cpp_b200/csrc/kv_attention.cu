@@ -39,8 +39,15 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 //   warp 8     loads K (cp.async; bulk copies of the pages' pieces measured about 0.15 us each, whatever their size) and
 //              the tile's page list two tiles ahead, and issues the MMAs
 //   warps 0-7  thread = key, half of the rows (warps 0-3, 4-7): scores, weights; V codes (copied one tile ahead) to bf16; then
-//              thread = dim: O of the same rows.  (One warp per 32 keys for all rows took half again as long: an SM's few warps
-//              wait on the latency of their own instructions.)
+//              thread = dim: O of the same rows
+//
+// Bound by: instructions and their latency.  The codes are read once, at HBM's rate a tile would take 0.35 us of an SM (HD 64),
+// and the MMAs are short; but a tile's codes, scores and weights pass through about 5000 warp instructions (HD 128, 4 rows; a
+// fifth of them turn V codes into bf16), issued at half the SM's rate.  Measured (HBM figures of the codes and scales):
+//   192 sequences up to 8191, bf16, 4 rows of 128:  123 us, 2.9 TB/s (four softmax warps of all rows instead of eight of half: 141)
+//   1 sequence of 131071, f16, 7 rows of 64:         25.5 us with the join
+//   256 sequences of 640, f32, 7 rows of 64:         32.8 us
+//   1 sequence of 130, f32:                          10.2 us, start (4 us), two tiles and the outputs one after the other
 constexpr int kDecSoft = 256;                 // threads of the softmax warps
 constexpr int kDecThreads = kDecSoft + 32;
 constexpr int kTileKeys = 128;
@@ -942,6 +949,13 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 //   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
 //                        to 16-bit operands
 //   last warp            issues the MMAs: S of tile i + 1 runs beside the softmax of tile i
+//
+// Bound by: the softmax's chain per tile (S out of TMEM, maximum, exp, pieces, weights into TMEM: about 3000 cycles for a CTA
+// alone) and, with two CTAs to an SM, instructions: about 4200 warp instructions per 128 x 64 scores, half of the issue rate; the
+// tensor cores are busy a quarter of the time at most.  Measured:
+//   8 prompts of 2048, 32/8 heads of 128:  f16 622 us, bf16 602 us (442 and 457 TFLOP/s of what causal rows need)
+//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 119 us, 216 TFLOP/s
+//   1 prompt of 512, f32, 14/2 heads of 64: 21.8 us, 56 CTAs of 1 to 8 tiles
 template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
     static constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
@@ -1447,29 +1461,37 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
 }
 
 // Joins the stretches of k_kv_chunk: a warp per (token, head), in order.  Stretches without a key have sum 0 and no O.
+// (476 tokens of 32 heads of 128, 2 stretches: 7.3 us, latency.)
 template <int HD, class T>
 __global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan plan, long long n_rows) {
     pdl_wait();
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= n_rows) return;
-    const float2* ml = reinterpret_cast<const float2*>(plan.ml) + row * plan.splits;
-    float top = -INFINITY;
-    for (int x = 0; x < plan.splits; ++x) top = fmaxf(top, __ldcg(ml + x).x);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o[HD / 32] = {};
+    constexpr int E = HD / 32;
+    // a stretch per lane (splits <= 32)
+    const float2 ml = lane < plan.splits ? __ldcg(reinterpret_cast<const float2*>(plan.ml) + row * plan.splits + lane)
+                                         : make_float2(-INFINITY, 0.f);
+    const unsigned live = __ballot_sync(0xffffffffu, !(ml.x == -INFINITY && ml.y == 0.f));
+    const float top = warp_max_redux(ml.x), w = ex2_full(ml.x - (top == -INFINITY ? 0.f : top)), l = warp_sum(ml.y * w);
+    const float* src = plan.o + row * plan.splits * HD + lane * E;
+    float o[E] = {};
+#pragma unroll 2
     for (int x = 0; x < plan.splits; ++x) {
-        const float2 p = __ldcg(ml + x);
-        if (p.x == -INFINITY && p.y == 0.f) continue;
-        const float w = ex2_full(p.x - ref);
-        l += p.y * w;
-        const float* src = plan.o + (row * plan.splits + x) * HD + lane;
+        float v[E];
+        load_row<true>(src + x * HD, v);
+        const float wx = __shfl_sync(0xffffffffu, w, x);
 #pragma unroll
-        for (int y = 0; y < HD / 32; ++y) o[y] = fmaf(__ldcg(src + 32 * y), w, o[y]);
+        for (int e = 0; e < E; ++e) o[e] = live >> x & 1 ? fmaf(v[e], wx, o[e]) : o[e];
     }
     const bool none = top == -INFINITY && l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+    struct alignas(E * sizeof(T)) Out {
+        T v[E];
+    } out;
 #pragma unroll
-    for (int y = 0; y < HD / 32; ++y) put(static_cast<T*>(a.out) + size_t(row) * HD + 32 * y + lane, none ? 0.f : o[y] / l);
+    for (int e = 0; e < E; ++e) put(&out.v[e], none ? 0.f : o[e] * inv);
+    *reinterpret_cast<Out*>(static_cast<T*>(a.out) + row * HD + lane * E) = out;
     if (a.lse && lane == 0) a.lse[row] = none ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
 }
 
@@ -1477,6 +1499,7 @@ __global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan p
 
 constexpr int kDecRows = 16;  // most query rows (queries x heads of a kv head) of k_kv_decode
 
+// (256 x 640 f32, 14 rows of 64: 45.9 us against k_kv_chunk's 96.5; 64 x 4000 bf16, 16 rows of 128: 200 against 337.)
 bool takes_decode(const KvAttnArgs& a) { return (long long)a.max_q * a.group <= kDecRows; }
 
 int dec_rm(const KvAttnArgs& a) {
@@ -1496,11 +1519,12 @@ DecLaunch dec_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     const long long span = a.window && a.window < a.max_len ? (long long)a.window + a.max_q : a.max_len;
     const long long tiles = std::max(1LL, (span + kTileKeys - 1) / kTileKeys + (a.window != 0));
     const int ctas = c.hd == 64 && dec_rm(a) <= 8 ? 3 : 2;  // per SM, as the kernel's
+    // Units of up to 8 tiles are not dealt: cutting them costs more than an uneven last wave (32 x 2 units of 640 keys: 19.3 us, dealt
+    // 21.5; 256 x 2: 34.9, dealt 39.9; of 1100 keys 25.4 either way; of 1500 dealt 25.6, a CTA each 29.7; of 2000 27.6, 36.8).
     l.even = tiles > 8;
     l.grid = int(l.even ? std::min<long long>(148 * ctas, std::max<long long>(1, (long long)l.units * tiles / 2)) : (long long)l.units);
     return l;
 }
-
 
 template <int HD, int RM, class T>
 cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, void* ws, cudaStream_t st) {
@@ -1531,7 +1555,8 @@ struct ChunkLaunch {
 };
 
 // Row groups of 128 per CTA and stretches of keys per row tile.  Two groups share the conversion of K and V, but leave half as
-// many CTAs: taken where those fill the SMs.  Stretches: as many as fill the SMs, of at least 8 key tiles (what a CTA's start
+// many CTAs: taken where those fill the SMs (8 prompts of 2048, f16, 8 kv heads of 128: 622 us, one group 708; 16 of 512, f32,
+// 2 of 64: 85, 113; a single one, f16: 27.6, one group 25.6).  Stretches: as many as fill the SMs, of at least 8 key tiles (what a CTA's start
 // and the join cost).
 ChunkLaunch chunk_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     ChunkLaunch l;

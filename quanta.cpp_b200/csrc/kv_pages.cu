@@ -330,6 +330,11 @@ __global__ void __launch_bounds__(32 * kReadWarps) k_kv_read(KvView c, int layer
 
 // ---------------------------------------------------------------- page bookkeeping
 
+// The planning kernels are one CTA each: what they look over (a reference count per page, a mark per sequence) is small, and the
+// lowest free pages, in order, are a prefix sum.  Bound by latency: about 10 dependent rounds of loads and barriers.  Measured:
+// free of 64 sequences and reserve for 256 in a pool of 32768 pages 17.4 us a pair with the host's part (kernels 5.6 and 13 us);
+// fork of 4 sequences to 64: 22.5 us (plan 9, copies of 50 MB at 3.2 TB/s behind it); compact of 2048 pages of 393 KB with 1229
+// in use: 78 us (plan 10), 5.7 TB/s of HBM, by page copies of 16 KB a CTA.
 constexpr int kPlanThreads = 1024;
 
 // Exclusive prefix sum of one value per thread of the CTA; *total gets the sum.
