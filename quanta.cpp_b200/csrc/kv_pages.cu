@@ -332,9 +332,9 @@ __global__ void __launch_bounds__(32 * kReadWarps) k_kv_read(KvView c, int layer
 
 // The planning kernels are one CTA each: what they look over (a reference count per page, a mark per sequence) is small, and the
 // lowest free pages, in order, are a prefix sum.  Bound by latency: about 10 dependent rounds of loads and barriers.  Measured:
-// free of 64 sequences and reserve for 256 in a pool of 32768 pages 17.4 us a pair with the host's part (kernels 5.6 and 13 us);
-// fork of 4 sequences to 64: 22.5 us (plan 9, copies of 50 MB at 3.2 TB/s behind it); compact of 2048 pages of 393 KB with 1229
-// in use: 78 us (plan 10), 5.7 TB/s of HBM, by page copies of 16 KB a CTA.
+// free of 64 sequences and reserve for 256 in a pool of 32768 pages 17 us a pair with the host's part (kernels 4 and 10 us);
+// fork of 4 sequences to 64: 22 us (plan 7.5, copies of 25 MB 12 us); compact of 2048 pages of 393 KB with 1229 in use: 78 us
+// (plan 7.6), moves at 5.7 TB/s of HBM, 16 KB of a page to a CTA.
 constexpr int kPlanThreads = 1024;
 
 // Exclusive prefix sum of one value per thread of the CTA; *total gets the sum.
@@ -350,19 +350,15 @@ __device__ __forceinline__ int cta_scan(int x, int* total) {
     __syncthreads();
     if (lane == 31) part[warp] = inc;
     __syncthreads();
-    int mine = 0, sum = 0;
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) {
-        if (w < warp) mine += part[w];
-        sum += part[w];
-    }
-    *total = sum;
-    return mine + inc - x;
+    const int p = lane < int(blockDim.x >> 5) ? part[lane] : 0;
+    *total = __reduce_add_sync(0xffffffffu, p);
+    return __reduce_add_sync(0xffffffffu, lane < warp ? p : 0) + inc - x;
 }
 
 // words[g] = bit i set where page 32 g + i is free (pages past the pool are not).
 __device__ __forceinline__ void free_bitmap(const KvView& c, unsigned* words, int n_words) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    constexpr int U = 8;  // loads in flight
+    constexpr int U = 16;  // loads in flight
     for (int g0 = warp * U; g0 < n_words; g0 += warps * U) {
         int r[U];
 #pragma unroll
@@ -495,13 +491,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
     for (int i = i0; i < i1; ++i) fresh[i] = (c.lens[src[i]] & (c.pt - 1)) ? list[r++] : -1;
 }
 
+constexpr int kPagePart = 16384;  // bytes of a page that a CTA copies
+
 // Copies a page's codes and scales, all layers; part `part` of `parts`.
 __device__ __forceinline__ void copy_page(const KvView& c, int from, int to, int part, int parts) {
     const size_t n16 = c.page_codes() / 16;
     const uint4* a = reinterpret_cast<const uint4*>(c.codes + size_t(from) * c.page_codes());
     uint4* b = reinterpret_cast<uint4*>(c.codes + size_t(to) * c.page_codes());
     const size_t per = (n16 + parts - 1) / parts, i0 = size_t(part) * per, i1 = min(i0 + per, n16);
-    constexpr int U = 8;
+    constexpr int U = 4;  // 256 threads read a part of 16 KB at once
     for (size_t i = i0 + threadIdx.x; i < i1; i += size_t(U) * blockDim.x) {
         uint4 w[U];
 #pragma unroll
@@ -516,18 +514,39 @@ __device__ __forceinline__ void copy_page(const KvView& c, int from, int to, int
         c.scales[size_t(to) * ns + i] = c.scales[size_t(from) * ns + i];
 }
 
-// Fork, second half: grid (parts of a page, pairs); part 0 also writes the pair's table row and counts its pages.
-__global__ void __launch_bounds__(256) k_kv_fork(KvView c, const int* __restrict__ src, const int* __restrict__ dst,
-                                                 const int* __restrict__ ok, const int* __restrict__ fresh) {
+// Fork, second half: grid (parts of a page, pairs); part 0 also writes the pair's table row and counts its pages.  The plan
+// changes neither the sources' lengths nor their pages, so a part of at most 16 KB is read while the plan still runs.
+constexpr int kForkThreads = 256;
+
+__global__ void __launch_bounds__(kForkThreads) k_kv_fork(KvView c, const int* __restrict__ src, const int* __restrict__ dst,
+                                                          const int* __restrict__ ok, const int* __restrict__ fresh) {
+    constexpr int U = kPagePart / 16 / kForkThreads;
+    const int i = blockIdx.y, s = src[i], d = dst[i], s0 = s >= 0 && s < c.max_seqs ? s : 0;  // (a bad one is refused by the plan)
+    const int len = c.lens[s0], parts = gridDim.x;
+    const int* from = c.table + size_t(s0) * c.max_pages;
+    const int last = from[min(max(len >> c.pt_shift, 0), c.max_pages - 1)];  // the part-filled page, if there is one
+    const bool known = last >= 0 && last < c.n_pages;
+    const size_t n16 = c.page_codes() / 16, per = (n16 + parts - 1) / parts, i0 = blockIdx.x * per, i1 = min(i0 + per, n16);
+    const uint4* codes = reinterpret_cast<const uint4*>(c.codes + size_t(known ? last : 0) * c.page_codes());
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = __ldcs(codes + min(i0 + u * kForkThreads + threadIdx.x, i1 - 1));
     pdl_wait();
-    if (!__ldcg(ok)) return;
-    const int i = blockIdx.y, s = src[i], d = dst[i], len = c.lens[s], to = __ldcg(fresh + i);
+    const int go = __ldcg(ok), to = __ldcg(fresh + i);
+    if (!go) return;
     const int full = min(len >> c.pt_shift, to >= 0 ? c.max_pages - 1 : c.max_pages);
-    const int* from = c.table + size_t(s) * c.max_pages;
     if (to >= 0) {
-        const int p = from[full];
-        if (p >= 0 && p < c.n_pages) copy_page(c, p, to, blockIdx.x, gridDim.x);
-        else if (threadIdx.x == 0) set_error(c.status, ERR_BAD_POS);
+        if (known) {
+            uint4* out = reinterpret_cast<uint4*>(c.codes + size_t(to) * c.page_codes());
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i0 + u * kForkThreads + threadIdx.x < i1) __stcs(out + i0 + u * kForkThreads + threadIdx.x, w[u]);
+            const int ns = c.page_scales();
+            for (int x = blockIdx.x * kForkThreads + threadIdx.x; x < ns; x += parts * kForkThreads)
+                c.scales[size_t(to) * ns + x] = c.scales[size_t(last) * ns + x];
+        } else if (threadIdx.x == 0) {
+            set_error(c.status, ERR_BAD_POS);
+        }
     }
     if (blockIdx.x == 0) {
         int* row = c.table + size_t(d) * c.max_pages;
@@ -673,7 +692,7 @@ cudaError_t launch_plan(void (*kernel)(KArgs...), int ctas, int threads, size_t 
 size_t plan_smem(const KvView& c, int n) { return plan_words(c) * 4 + size_t(c.max_seqs) * 4 + size_t(n) * 4; }
 
 // A page in parts of about 16 KB, so that one page's copy spreads over several SMs.
-int page_parts(const KvView& c) { return int((c.page_codes() + 16383) / 16384); }
+int page_parts(const KvView& c) { return int((c.page_codes() + kPagePart - 1) / kPagePart); }
 
 template <class T, int HD>
 cudaError_t append_t(const KvView& c, int layer, const void* k, const void* v, long long ks, long long vs, const KvCall& call,
@@ -738,7 +757,7 @@ cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int 
     int* list = fresh + c.max_seqs;
     cudaError_t e = launch_plan(k_kv_fork_plan, 1, kPlanThreads, plan_smem(c, 0), st, c, src, dst, n, ok, fresh, list);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_kv_fork, dim3(unsigned(page_parts(c)), unsigned(n)), dim3(256), 0, st, true, c, src, dst,
+    return launch_pdl(k_kv_fork, dim3(unsigned(page_parts(c)), unsigned(n)), dim3(kForkThreads), 0, st, true, c, src, dst,
                       static_cast<const int*>(ok), static_cast<const int*>(fresh));
 }
 
