@@ -954,8 +954,8 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 // alone) and, with two CTAs to an SM, instructions: about 4200 warp instructions per 128 x 64 scores, half of the issue rate; the
 // tensor cores are busy a quarter of the time at most.  Measured:
 //   8 prompts of 2048, 32/8 heads of 128:  f16 622 us, bf16 602 us (442 and 457 TFLOP/s of what causal rows need)
-//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 119 us, 216 TFLOP/s
-//   1 prompt of 512, f32, 14/2 heads of 64: 21.8 us, 56 CTAs of 1 to 8 tiles
+//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 115 us, 223 TFLOP/s
+//   1 prompt of 512, f32, 14/2 heads of 64: 18.4 us with the join, 112 CTAs of up to 4 tiles
 template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
     static constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
@@ -1556,8 +1556,8 @@ struct ChunkLaunch {
 
 // Row groups of 128 per CTA and stretches of keys per row tile.  Two groups share the conversion of K and V, but leave half as
 // many CTAs: taken where those fill the SMs (8 prompts of 2048, f16, 8 kv heads of 128: 622 us, one group 708; 16 of 512, f32,
-// 2 of 64: 85, 113; a single one, f16: 27.6, one group 25.6).  Stretches: as many as fill the SMs, of at least 8 key tiles (what a CTA's start
-// and the join cost).
+// 2 of 64: 85, 113; a single one, f16: 27.6, one group 25.6).  Stretches: as many as fill the SMs twice, of at least 4 key tiles
+// (a prompt of 512, 2 kv heads of 64: f32 23.5 us, of at least 8 tiles 26.6; f16 23.6, 25.6).
 ChunkLaunch chunk_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     ChunkLaunch l;
     const long long rows = (long long)call.n_tok * a.group;
@@ -1565,7 +1565,7 @@ ChunkLaunch chunk_launch(const KvView& c, const KvAttnArgs& a, const KvCall& cal
     const long long span = a.window && a.window < a.max_len ? std::min<long long>(a.max_len, (long long)a.window + a.max_q) : a.max_len;
     l.wg = (a.type == KV_F32 && c.hd == 128) || units(2) < 148 ? 1 : 2;
     const long long u = units(l.wg);
-    l.splits = int(std::max<long long>(1, std::min<long long>({(span / 64 + 7) / 8, (2 * 148 + u - 1) / u, 32})));
+    l.splits = int(std::max<long long>(1, std::min<long long>({(span / 64 + 3) / 4, (2 * 148 + u - 1) / u, 32})));
     return l;
 }
 

@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(32 * kReadWarps) k_kv_read(KvView c, int layer
 // The planning kernels are one CTA each: what they look over (a reference count per page, a mark per sequence) is small, and the
 // lowest free pages, in order, are a prefix sum.  Bound by latency: about 10 dependent rounds of loads and barriers.  Measured:
 // free of 64 sequences and reserve for 256 in a pool of 32768 pages 17 us a pair with the host's part (kernels 4 and 10 us);
-// fork of 4 sequences to 64: 22 us (plan 7.5, copies of 25 MB 12 us); compact of 2048 pages of 393 KB with 1229 in use: 78 us
-// (plan 7.6), moves at 5.7 TB/s of HBM, 16 KB of a page to a CTA.
+// fork of 4 sequences to 64: 18.6 us (plan 7.5, copies of 25 MB 12 us); compact of 2048 pages of 393 KB with 1229 in use: 81 us
+// (plan 7.6), moves at 5.4 TB/s of HBM, 16 KB of a page to a CTA.
 constexpr int kPlanThreads = 1024;
 
 // Exclusive prefix sum of one value per thread of the CTA; *total gets the sum.
