@@ -1537,10 +1537,8 @@ cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, v
         p.ml = p.o + size_t(l.grid) * 2 * RM * HD;
         p.info = reinterpret_cast<int4*>(p.ml + size_t(l.grid) * 2 * RM * 2);
     }
-    // with its static part the shared memory passes the default limit of 48 KB
-    cudaError_t e = cudaFuncSetAttribute(k_kv_decode<HD, RM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
+    static_assert(C::smem > 48 * 1024, "launch_pdl raises the limit");
+    cudaError_t e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
     if (e != cudaSuccess || !l.even) return e;
     // more than 32 partials to a unit: a CTA per row, else a warp
     static_assert(148 * C::ctas <= kJoinMany, "a record per thread");

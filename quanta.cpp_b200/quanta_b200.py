@@ -323,7 +323,7 @@ class PagedKV:
                            scales.data_ptr(), refs.data_ptr(), table.data_ptr(), lens.data_ptr(), self._status.data_ptr())
         self._p = C.byref(self._c)
         self._types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-        self._ws, self._need = {}, {}
+        self._ws, self._need, self._i32 = {}, {}, i32
         self._lib, self._index = lib(), codes.device.index  # a call's host time counts where few tokens are decoded
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._page_ws = lib().qnt_kv_page_workspace(self._p)
@@ -354,18 +354,20 @@ class PagedKV:
         return ws.data_ptr(), ws.numel()
 
     def _list(self, *lists):
-        n = lists[0].numel()
         for t in lists:
-            if not (t.is_cuda and t.dtype == self._torch.int32 and t.is_contiguous()):
+            if t.dtype is not self._i32 or not t.is_cuda or not t.is_contiguous():
                 raise TypeError("sequence lists must be contiguous int32 CUDA tensors")
-        return n
+        return lists[0].numel()
 
     def _rows(self, name, x, heads=None):
-        if not (x.is_cuda and x.dim() == 3 and x.dtype in self._types and x.stride(2) == 1 and x.shape[2] == self.head_dim and
-                x.stride(1) == self.head_dim and (heads is None or x.shape[1] == heads)):
+        """The type and the token stride of rows [tokens, heads, head_dim]."""
+        shape, st, hd = x.shape, x.stride(), self.head_dim
+        dt = self._types.get(x.dtype)
+        if not (len(st) == 3 and st[2] == 1 and st[1] == hd and shape[2] == hd and dt is not None and x.is_cuda and
+                (heads is None or shape[1] == heads)):
             raise TypeError(f"{name} must be a float32, float16 or bfloat16 CUDA tensor [tokens, heads, {self.head_dim}] whose "
                             "heads are contiguous within a token")
-        return self._types[x.dtype]
+        return dt, st[0]
 
     def reserve(self, seqs, extra, stream=None):
         """lens[seqs] += extra, with the pages for it."""
@@ -405,14 +407,16 @@ class PagedKV:
     def append(self, layer: int, k, v, seqs, starts, max_new: int | None = None, stream=None):
         """Quantizes rows k, v [tokens, n_kv_heads, head_dim] into a layer, as the last positions of their sequences
         (reserve first); max_new bounds a sequence's new tokens."""
-        dt = self._rows("k", k, self.n_kv_heads)
-        if self._rows("v", v, self.n_kv_heads) != dt or v.shape[0] != k.shape[0]:
+        dt, ks = self._rows("k", k, self.n_kv_heads)
+        vt, vs = self._rows("v", v, self.n_kv_heads)
+        m = k.shape[0]
+        if vt != dt or v.shape[0] != m:
             raise TypeError("k and v must have the same type and number of tokens")
-        n, m = self._list(seqs, starts), k.shape[0]
+        n = self._list(seqs, starts)
         if starts.numel() != n + 1:
             raise ValueError("starts must have one entry more than seqs")
-        _check(self._lib.qnt_kv_append(self._p, layer, k.data_ptr(), v.data_ptr(), dt, k.stride(0), v.stride(0), seqs.data_ptr(),
-                                   starts.data_ptr(), n, m, m if max_new is None else max_new, self._stream(stream)))
+        _check(self._lib.qnt_kv_append(self._p, layer, k.data_ptr(), v.data_ptr(), dt, ks, vs, seqs.data_ptr(),
+                                       starts.data_ptr(), n, m, m if max_new is None else max_new, self._stream(stream)))
 
     def read(self, layer: int, seqs, first, starts, n_tok: int, dtype=None, stream=None):
         """Values of positions first[j] + i of sequence seqs[j] as rows starts[j] + i: (K, V) [n_tok, n_kv_heads, head_dim]
@@ -435,8 +439,8 @@ class PagedKV:
         """Attention of q [tokens, n_heads, head_dim] over the cache of their sequences; query i of a sequence's m sits at
         position lens - m + i and sees the positions up to its own (the last `window` of them, if window > 0).  max_q bounds
         a sequence's queries, max_len its length.  Returns out (q's type), or (out, lse) with lse float32 [tokens, n_heads]."""
-        dt = self._rows("q", q)
-        n_tok, heads = q.shape[0], q.shape[1]
+        dt, stride = self._rows("q", q)
+        n_tok, heads = q.shape[:2]
         n = self._list(seqs, starts)
         if starts.numel() != n + 1:
             raise ValueError("starts must have one entry more than seqs")
@@ -450,7 +454,7 @@ class PagedKV:
         w, nb = self._workspace(s, need)
         out = self._torch.empty_like(q)  # (a token's heads are contiguous and tokens do not overlap: so is this)
         ls = self.scales.new_empty((n_tok, heads)) if lse else None
-        _check(self._lib.qnt_kv_attention(self._p, layer, q.data_ptr(), dt, q.stride(0), heads, seqs.data_ptr(), starts.data_ptr(), n,
+        _check(self._lib.qnt_kv_attention(self._p, layer, q.data_ptr(), dt, stride, heads, seqs.data_ptr(), starts.data_ptr(), n,
                                       n_tok, max_q, max_len, self.head_dim ** -0.5 if scale is None else scale, window,
                                       out.data_ptr(), None if ls is None else ls.data_ptr(), w, nb, s))
         return (out, ls) if lse else out
