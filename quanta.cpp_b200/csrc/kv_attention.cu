@@ -36,20 +36,19 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 // The work of all (sequence, kv head) units, in order, is dealt evenly to the CTAs (`even`), whatever the lengths; a
 // unit cut between CTAs leaves partial sums in the workspace and k_kv_join adds them up in CTA order.  Where the host's
 // bound on the lengths keeps a unit short, every CTA takes one unit and nothing is joined.
-//   warp 8     loads K (cp.async; bulk copies of the pages' pieces measured about 0.15 us each, whatever their size) and
-//              the tile's page list two tiles ahead, and issues the MMAs
-//   warps 0-7  thread = key, half of the rows (warps 0-3, 4-7): scores, weights; V codes (copied one tile ahead) to bf16; then
-//              thread = dim: O of the same rows
+//   softmax warps  thread = key: scores, weights; then thread = dim: O.  Up to 4 rows: 4 warps; else 8, half of the rows each, which
+//                  also take the V codes (copied one tile ahead) to bf16
+//   4 V warps      (up to 4 rows) that instead
+//   last warp      loads K (cp.async; bulk copies of the pages' pieces measured about 0.15 us each, whatever their size) and
+//                  the tile's page list two tiles ahead, and issues the MMAs
 //
 // Bound by: instructions and their latency.  The codes are read once, at HBM's rate a tile would take 0.35 us of an SM (HD 64),
 // and the MMAs are short; but a tile's codes, scores and weights pass through about 5000 warp instructions (HD 128, 4 rows; a
 // fifth of them turn V codes into bf16), issued at half the SM's rate.  Measured (HBM figures of the codes and scales):
-//   192 sequences up to 8191, bf16, 4 rows of 128:  123 us, 2.9 TB/s (four softmax warps of all rows instead of eight of half: 141)
+//   192 sequences up to 8191, bf16, 4 rows of 128:  117 us, 3.1 TB/s (the V codes in 8 softmax warps: 123, in 4: 141)
 //   1 sequence of 131071, f16, 7 rows of 64:         25.5 us with the join
-//   256 sequences of 640, f32, 7 rows of 64:         32.8 us
+//   256 sequences of 640, f32, 7 rows of 64:         32.8 us (V warps beside 4 softmax warps of 8 rows, which spill: 47)
 //   1 sequence of 130, f32:                          10.2 us, start (4 us), two tiles and the outputs one after the other
-constexpr int kDecSoft = 256;                 // threads of the softmax warps
-constexpr int kDecThreads = kDecSoft + 32;
 constexpr int kTileKeys = 128;
 constexpr float kDigitMax = 8323072.0f;  // 127 * 256^2: three digits
 constexpr float kLog2e = 1.4426950408889634f;
@@ -64,6 +63,10 @@ struct Dec {
     static constexpr int NP = sizeof(T) == 4 ? 3 : 2;                  // pieces of a weight
     static constexpr int NC = (3 * RM + 15) / 16 * 16;                 // columns of S
     static constexpr int WC = (NP * RM + 15) / 16 * 16;                // columns of O
+    static constexpr bool v_warps = RM == 4;
+    static constexpr int soft = v_warps ? 128 : 256;                   // threads of the softmax warps
+    static constexpr int v_threads = v_warps ? 128 : soft;             // threads that take V codes to bf16
+    static constexpr int threads = soft + (v_warps ? v_threads : 0) + 32;
     static constexpr int stages = 3;                                   // K tiles
     static constexpr int ctas = HD == 64 && RM <= 8 ? 3 : 2;           // per SM: shared memory, registers
     static constexpr int k_bytes = kTileKeys * HD;
@@ -74,7 +77,7 @@ struct Dec {
     static constexpr int s_cols = NC <= 16 ? 16 : NC <= 32 ? 32 : 64;  // TMEM column pitch of an S buffer
     static constexpr int tmem_need = 2 * s_cols + WC;
     static constexpr int tmem_cols = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : 256;
-    static constexpr int items = HD * 8 / kDecSoft;                    // V pieces (a dim's 16 tokens) of a thread
+    static constexpr int items = HD * 8 / v_threads;                   // V pieces (a dim's 16 tokens) of a thread
     static constexpr uint32_t idesc_s = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(NC >> 3) << 17) | (uint32_t(kTileKeys >> 4) << 24);
     static constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(WC >> 3) << 17) | (uint32_t(HD >> 4) << 24);
     static_assert(tmem_need <= 256, "TMEM allocation");
@@ -164,12 +167,13 @@ __device__ __forceinline__ bool wait_warp(uint64_t* b, unsigned parity, volatile
 }
 
 // Barrier of the softmax threads; true for all of them if `bad` holds for one, so that they leave a loop together.
+template <int THREADS>
 __device__ __forceinline__ bool bar_any(bool bad) {
     unsigned r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"(bad ? 1u : 0u), "n"(kDecSoft)
+        : "r"(bad ? 1u : 0u), "n"(THREADS)
         : "memory");
     return r != 0;
 }
@@ -214,9 +218,9 @@ struct Deal {
 __device__ __forceinline__ int tiles_before(int part, int tiles) { return part <= 0 ? 0 : min(tiles, max(1, part - kUnitCost)); }
 
 template <int HD, int RM, class T>
-__global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode(KvView c, KvAttnArgs a, KvCall call, DecPlan plan) {
+__global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas) k_kv_decode(KvView c, KvAttnArgs a, KvCall call, DecPlan plan) {
     using C = Dec<HD, RM, T>;
-    constexpr int NP = C::NP;
+    constexpr int NP = C::NP, last = C::threads / 32 - 1;  // the loading warp
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* vb = smem + C::stages * C::k_bytes;
@@ -242,7 +246,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         for (int s = 0; s < 4; ++s) mbar_init(&listed[s], 32);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_done[b], 1);
-            mbar_init(&w_ready[b], kDecSoft);
+            mbar_init(&w_ready[b], C::threads - 32);
         }
         mbar_init(&o_done, 1);
         mbar_init(&q_ready, 128);
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         if (plan.even) plan.info[blockIdx.x] = make_int4(-1, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc(&tmem_base, C::tmem_cols);
+    if (warp == last) tmem_alloc(&tmem_base, C::tmem_cols);
     pdl_wait();
     pdl_launch_dependents();
 
@@ -346,9 +350,29 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         n_tiles = first_w.tiles;
     }
     const uint32_t tmem = uint32_t(warp_same(int(tmem_base)));
+    // V pieces of a thread: dim vd of blocks vblk + x * (v_threads / HD)
+    const int v_tid = C::v_warps ? tid & 127 : tid, vd = v_tid % HD, vblk = v_tid / HD;
+    const int v_shift = c.pt_shift + (HD == 64 ? 6 : 7);  // log2 of a tile's codes
+    auto copy_v = [&](int i) {  // (any codes where no key is seen: their weights are 0)
+        const uint32_t dst = smem_u32(vc) + v_tid * 16;
+#pragma unroll
+        for (int x = 0; x < C::items; ++x) {
+            const int b = vblk + x * (C::v_threads / HD);
+            const int8_t* src = c.codes + (size_t(tile_rec[i & 3].kt[b] + c.n_kv) << v_shift) +
+                                (((b * kKvBlock) & (c.pt - 1)) * HD + vd * 16);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * C::v_threads * 16), "l"(src) : "memory");
+        }
+    };
+    auto put_v = [&](int x, const uint4& v) {
+        const int b = vblk + x * (C::v_threads / HD);
+        const uint2 x0 = codes_bf16(v.x), x1 = codes_bf16(v.y), x2 = codes_bf16(v.z), x3 = codes_bf16(v.w);
+        unsigned char* dst = vb + (b >> 2) * C::v_half;
+        *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3))) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+        *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3) + 1)) = make_uint4(x2.x, x2.y, x3.x, x3.y);
+    };
     const int n_my = warp_same(n_tiles);
 
-    if (warp == 8) {
+    if (warp == last) {
         // ---- loads, two tiles ahead, and MMAs
         constexpr int kLead = C::stages - 1;
         SeqWork w = first_w;
@@ -475,15 +499,36 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
         for (unsigned i = 0; i < kWaitLimit && !__all_sync(0xffffffffu, mbar_try(&fin, 0)); ++i) {
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (C::v_warps && tid >= C::soft) {
+        // ---- V codes to bf16
+        bool ok = n_my == 0 || wait_warp(&listed[0], 0, ab);
+        if (n_my > 0 && ok) copy_v(0);
+#pragma unroll 1
+        for (int i = 0; i < n_my && ok; ++i) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            uint4 v[C::items];
+#pragma unroll
+            for (int x = 0; x < C::items; ++x) v[x] = reinterpret_cast<const uint4*>(vc)[x * C::v_threads + v_tid];
+            if (i + 1 < n_my) {
+                ok = wait_warp(&listed[(i + 1) & 3], ((i + 1) >> 2) & 1, ab);
+                if (!ok) break;
+                copy_v(i + 1);
+            }
+            if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab);  // the product of the tile before has read vb
+            if (!ok) break;
+#pragma unroll
+            for (int x = 0; x < C::items; ++x) put_v(x, v[x]);
+            fence_async_smem();
+            mbar_arrive(&w_ready[i & 1]);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ---- scores, softmax, outputs: thread = key of the tile, then dim of the head
         constexpr int lanes = HD == 64 ? 16 : 32;  // rows of O^T of a warp (M = 64 leaves the upper half of each quadrant unused)
-        constexpr int RH = RM / 2;                 // rows of a thread: r0 ..
+        constexpr int RH = RM * 128 / C::soft;     // rows of a thread: r0 ..
         const int half = warp >> 2, quad = warp & 3, r0 = half * RH, kid = tid & 127;
         const int dim = quad * lanes + lane;
         const uint32_t my_tmem = tmem + (uint32_t(quad * 32) << 16) + r0;
-        const int vd = tid % HD, vblk = tid / HD;  // V pieces: dim vd of blocks vblk + x * (kDecSoft / HD)
-        const int v_shift = c.pt_shift + (HD == 64 ? 6 : 7);  // log2 of a tile's codes
         bool ok = true;   // a wait that gave up is acted on at the next barrier, by all threads together
         int in_tmem = 0;  // tiles whose sum lies in TMEM
         UnitRec u = {};
@@ -586,7 +631,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
             }
             if (i < 0) {  // (else: fac and row_off are read after the barrier below)
                 if (n_my > 0) ok = wait_warp(&listed[0], 0, ab) && ok;
-                if (bar_any(!ok)) break;
+                if (bar_any<C::soft>(!ok)) break;
             }
             if (i >= 0) {
                 const TileRec& rec = tile_rec[i & 3];
@@ -634,7 +679,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                             ++p;
                         }
                     }
-                    const bool stop = bar_any(!ok);
+                    const bool stop = bar_any<C::soft>(!ok);
 #pragma unroll
                     for (int r = 0; r < RH; ++r)
                         if (can >> (r0 + r) & 1) {
@@ -646,7 +691,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                 }
 #pragma unroll
                 for (int r = 0; r < RH; ++r) high = high || s[r] > kRaise + kShift;
-                const bool any = bar_any(high || !ok);
+                const bool any = bar_any<C::soft>(high || !ok);
                 bool waited = false;  // for the product of the tile before, which reads vb and wb
                 if (any) {
                     // O leaves TMEM, and the references that a score passed are raised to the tile's maxima
@@ -658,7 +703,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     if (i > 0) ok = wait_warp(&o_done, (i - 1) & 1, ab) && ok;
                     tc_fence_after();
                     waited = true;
-                    if (bar_any(!ok)) break;
+                    if (bar_any<C::soft>(!ok)) break;
                     if (in_tmem) {
                         int o0[RH], o1[RH], o2[RH];
                         const uint32_t at = my_tmem + 2 * C::s_cols;
@@ -725,15 +770,10 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                         *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(row, wc)) = (unsigned short)w[x][z];
                         *reinterpret_cast<unsigned short*>(wt + sw_offset<128>(row + 1, wc)) = (unsigned short)(w[x][z] >> 16);
                     }
-                asm volatile("cp.async.wait_all;" ::: "memory");
+                if constexpr (!C::v_warps) {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-                for (int x = 0; x < C::items; ++x) {
-                    const int b = vblk + x * (kDecSoft / HD);
-                    const uint4 v = reinterpret_cast<const uint4*>(vc)[x * kDecSoft + tid];
-                    const uint2 x0 = codes_bf16(v.x), x1 = codes_bf16(v.y), x2 = codes_bf16(v.z), x3 = codes_bf16(v.w);
-                    unsigned char* dst = vb + (b >> 2) * C::v_half;
-                    *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3))) = make_uint4(x0.x, x0.y, x1.x, x1.y);
-                    *reinterpret_cast<uint4*>(dst + sw_offset<128>(vd, 2 * (b & 3) + 1)) = make_uint4(x2.x, x2.y, x3.x, x3.y);
+                    for (int x = 0; x < C::items; ++x) put_v(x, reinterpret_cast<const uint4*>(vc)[x * C::v_threads + v_tid]);
                 }
                 if (tid == 0) fresh[i & 1] = in_tmem == 0;
                 ++in_tmem;
@@ -775,7 +815,7 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                             if (kid == 0) last_ref[r0 + r] = ref[r];
                         }
                     }
-                    if (bar_any(!ok)) break;
+                    if (bar_any<C::soft>(!ok)) break;
                     const int* off = row_off[(units - 1) & 1];
                     const size_t row0 = size_t(u.t0) * a.n_heads + u.head * a.group;
                     const size_t slot = size_t(2 * blockIdx.x + u.first) * RM;  // if cut
@@ -799,25 +839,16 @@ __global__ void __launch_bounds__(kDecThreads, Dec<HD, RM, T>::ctas) k_kv_decode
                     else put_rows(static_cast<T*>(a.out) + row0 * HD, false);
                     if (tid == 0 && u.first && u.cut)  // the unit's first CTA says which CTAs share it
                         plan.info[blockIdx.x] = make_int4(u.owner, u.t0, u.m, u.head);
-                    if (bar_any(!ok)) break;  // last_ref and sum_part are read before the next unit writes them
+                    if (bar_any<C::soft>(!ok)) break;  // last_ref and sum_part are read before the next unit writes them
                 }
             }
-            if (i + 1 < n_my) {  // V codes of the next tile (any codes where no key is seen: their weights are 0)
-                const uint32_t dst = smem_u32(vc) + tid * 16;
-#pragma unroll
-                for (int x = 0; x < C::items; ++x) {
-                    const int b = vblk + x * (kDecSoft / HD);
-                    const int8_t* src = c.codes + (size_t(tile_rec[(i + 1) & 3].kt[b] + c.n_kv) << v_shift) +
-                                        (((b * kKvBlock) & (c.pt - 1)) * HD + vd * 16);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x * kDecSoft * 16), "l"(src) : "memory");
-                }
-            }
+            if (!C::v_warps && i + 1 < n_my) copy_v(i + 1);
         }
     }
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && abort_flag) set_error(c.status, ERR_WAIT_TIMEOUT);
-    if (warp == 8) {
+    if (warp == last) {
         tc_fence_after();
         tmem_free(tmem, C::tmem_cols);
     }
@@ -1538,7 +1569,7 @@ cudaError_t decode_t(const KvView& c, const KvAttnArgs& a, const KvCall& call, v
         p.info = reinterpret_cast<int4*>(p.ml + size_t(l.grid) * 2 * RM * 2);
     }
     static_assert(C::smem > 48 * 1024, "launch_pdl raises the limit");
-    cudaError_t e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(kDecThreads), C::smem, st, false, c, a, call, p);
+    cudaError_t e = launch_pdl(k_kv_decode<HD, RM, T>, dim3(unsigned(l.grid)), dim3(C::threads), C::smem, st, false, c, a, call, p);
     if (e != cudaSuccess || !l.even) return e;
     // more than 32 partials to a unit: a CTA per row, else a warp
     static_assert(148 * C::ctas <= kJoinMany, "a record per thread");
