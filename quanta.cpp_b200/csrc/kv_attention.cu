@@ -43,12 +43,12 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 //                  the tile's page list two tiles ahead, and issues the MMAs
 //
 // Bound by: instructions and their latency.  The codes are read once, at HBM's rate a tile would take 0.35 us of an SM (HD 64),
-// and the MMAs are short; but a tile's codes, scores and weights pass through about 5000 warp instructions (HD 128, 4 rows; a
-// fifth of them turn V codes into bf16), issued at half the SM's rate.  Measured (HBM figures of the codes and scales):
-//   192 sequences up to 8191, bf16, 4 rows of 128:  117 us, 3.1 TB/s (the V codes in 8 softmax warps: 123, in 4: 141)
+// and the MMAs are short; but a tile's codes, scores and weights pass through about 3800 warp instructions (HD 128, 4 rows; a
+// quarter of them turn V codes into bf16), issued at 43 to 60 % of the SM's rate.  Measured (HBM figures of the codes and scales):
+//   192 sequences up to 8191, bf16, 4 rows of 128:  115 us, 3.2 TB/s (the V codes in 8 softmax warps: 123, in 4: 141)
 //   1 sequence of 131071, f16, 7 rows of 64:         25.5 us with the join
 //   256 sequences of 640, f32, 7 rows of 64:         32.8 us (V warps beside 4 softmax warps of 8 rows, which spill: 47)
-//   1 sequence of 130, f32:                          10.2 us, start (4 us), two tiles and the outputs one after the other
+//   1 sequence of 130, f32:                         10.2 us, start (4 us), two tiles and the outputs one after the other
 constexpr int kTileKeys = 128;
 constexpr float kDigitMax = 8323072.0f;  // 127 * 256^2: three digits
 constexpr float kLog2e = 1.4426950408889634f;
@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 // alone) and, with two CTAs to an SM, instructions: about 4200 warp instructions per 128 x 64 scores, half of the issue rate; the
 // tensor cores are busy a quarter of the time at most.  Measured:
 //   8 prompts of 2048, 32/8 heads of 128:  f16 622 us, bf16 602 us (442 and 457 TFLOP/s of what causal rows need)
-//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 115 us, 223 TFLOP/s
+//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 98 to 115 us with the lengths drawn
 //   1 prompt of 512, f32, 14/2 heads of 64: 18.4 us with the join, 112 CTAs of up to 4 tiles
 template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
@@ -1492,7 +1492,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
 }
 
 // Joins the stretches of k_kv_chunk: a warp per (token, head), in order.  Stretches without a key have sum 0 and no O.
-// (476 tokens of 32 heads of 128, 2 stretches: 7.3 us, latency.)
+// (476 tokens of 32 heads of 128, 2 stretches: 7.7 us, latency.)
 template <int HD, class T>
 __global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan plan, long long n_rows) {
     pdl_wait();
