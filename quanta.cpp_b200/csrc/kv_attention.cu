@@ -31,7 +31,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 // the small ones beside a much larger one.)  V codes become bf16 on their way through registers.
 // The softmax reference `ref` of a row is the score of the last key that it sees in its first tile (so the largest weight is
 // at least 1), raised only when a score passes it by 2^32: f32 and bf16 have the range, most tiles need no maximum over the
-// CTA, and O stays in TMEM; every 16 tiles it joins f32 registers, which bounds the tensor cores' accumulation error.
+// CTA, and O stays in TMEM; every 16 tiles (float32: 4) it joins f32 registers, which bounds the accumulation error.
 //
 // The work of all (sequence, kv head) units, in order, is dealt evenly to the CTAs (`even`), whatever the lengths; a
 // unit cut between CTAs leaves partial sums in the workspace and k_kv_join adds them up in CTA order.  Where the host's
