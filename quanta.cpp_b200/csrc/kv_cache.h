@@ -5,9 +5,9 @@
 //   codes  [page][layer][2: K, V][kv head][page_tokens * head_dim]
 //            K tile [head_dim / 16][page_tokens][16 dims], V tile [page_tokens / 16][head_dim][16 tokens]
 //   scales [page][layer][2][kv head][page_tokens / 16]
-// Both tiles are stored as the tensor cores' unswizzled K-major operands (8 rows of 16 bytes make a 128-byte core
-// matrix): K with a row per token and the dims contiguous, V with a row per dim and the tokens contiguous, so that a
-// tile goes from HBM to tcgen05.mma with plain bulk copies and no conversion.
+// Both tiles are made of 16-byte pieces along the contraction of the product that reads them: K's of a token's dims, V's of a
+// dim's tokens.  A piece goes to its place in the tensor cores' K-major operand with one copy (K codes as they are, as int8; V
+// codes as bf16 or f16), pieces that follow one another are read by lanes that do, and an append writes whole pieces.
 #pragma once
 
 #include <cuda_runtime.h>
