@@ -92,7 +92,9 @@ struct DecPlan {
 
 // A call's sequence j: its rows and the keys that they see together.
 struct SeqWork {
-    int seq, t0, m, len, lo, tiles;  // keys [lo, len), in tiles of 128 from lo & ~127; tiles >= 1 where m > 0
+    // keys [lo, len), in tiles of 128 from lo & ~127; tiles >= 1 where m > 0.  A sequence that the call cannot have (reported)
+    // has m = 0 like one without rows, and seq 0, so that its row of the page table may be read.
+    int seq, t0, m, len, lo, tiles;
 };
 
 __device__ __forceinline__ SeqWork seq_work(const KvView& c, const KvAttnArgs& a, const KvCall& call, int j) {
@@ -102,7 +104,7 @@ __device__ __forceinline__ SeqWork seq_work(const KvView& c, const KvAttnArgs& a
     const int len = min(max(__ldg(c.lens + (known ? seq : 0)), 0), c.max_pages << c.pt_shift);
     w.t0 = t0;
     w.m = t0 < 0 ? 0 : max(min(t1, call.n_tok) - t0, 0);
-    w.seq = seq;
+    w.seq = known ? seq : 0;
     if (w.m > 0 && (!known || w.m > a.max_q)) {
         set_error(c.status, ERR_BAD_POS);
         w.m = 0;
@@ -110,6 +112,16 @@ __device__ __forceinline__ SeqWork seq_work(const KvView& c, const KvAttnArgs& a
     w.len = w.m > 0 ? len : 0;
     w.lo = a.window ? max(0, w.len - w.m + 1 - a.window) : 0;
     w.tiles = w.m == 0 ? 0 : w.len > 0 ? (w.len - 1) / kTileKeys - w.lo / kTileKeys + 1 : 1;
+    return w;
+}
+// The next sequence of the call, after j, that has tiles; j becomes its number.  (The last one's where there is none: tiles 0.)
+__device__ __forceinline__ SeqWork next_work(const KvView& c, const KvAttnArgs& a, const KvCall& call, int& j) {
+    SeqWork w;
+    do {
+        do ++j;  // without rows: passed by the starts alone
+        while (j < call.n - 1 && __ldg(call.starts + j + 1) <= __ldg(call.starts + j));
+        w = seq_work(c, a, call, j);
+    } while (w.tiles == 0 && j < call.n - 1);
     return w;
 }
 
@@ -338,9 +350,7 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
             first_at += first_w.tiles + kUnitCost;
             if (++first_head == c.n_kv) {
                 first_head = 0;
-                do ++first_j;
-                while (first_j < call.n - 1 && __ldg(call.starts + first_j + 1) <= __ldg(call.starts + first_j));
-                first_w = seq_work(c, a, call, first_j);
+                first_w = next_work(c, a, call, first_j);
             }
         }
     } else {
@@ -394,9 +404,7 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
             at += w.tiles + kUnitCost;
             if (++head == c.n_kv) {
                 head = 0;
-                do ++j;
-                while (j < call.n - 1 && __ldg(call.starts + j + 1) <= __ldg(call.starts + j));
-                w = seq_work(c, a, call, j);
+                w = next_work(c, a, call, j);
             }
         };
         if (n_my > 0) look(n_my);
