@@ -29,8 +29,9 @@ int make_view(const qnt_kv_cache* c, qb::KvView* v) {
     if ((long long)c->max_pages * pt > (1 << 30) || (long long)c->max_pages * c->max_seqs > (1 << 30) ||
         (long long)c->n_layers * c->n_kv_heads > (1 << 20))
         return set_err(QNT_ERR_UNSUPPORTED, "kv cache: page table or sequence too long");
-    if (!aligned(c->codes, 16) || !aligned(c->scales, 4) || !aligned(c->refs, 4) || !aligned(c->table, 4) || !aligned(c->lens, 4))
-        return set_err(QNT_ERR_INVALID, "kv cache: codes must be 16-byte aligned");
+    if (!aligned(c->codes, 16) || !aligned(c->scales, 4) || !aligned(c->refs, 4) || !aligned(c->table, 4) || !aligned(c->lens, 4) ||
+        !aligned(c->status, 4))
+        return set_err(QNT_ERR_INVALID, "kv cache: codes must be 16-byte aligned, the other arrays to their elements");
     v->codes = c->codes;
     v->scales = c->scales;
     v->refs = c->refs;
@@ -57,6 +58,8 @@ int make_type(int dtype, qb::KvType* t) {
     return set_err(QNT_ERR_UNSUPPORTED, "dtype must be QNT_F32, QNT_F16 or QNT_BF16");
 }
 
+uintptr_t size_of(qb::KvType t) { return t == qb::KV_F32 ? 4 : 2; }
+
 int check_layer(const qb::KvView& v, int layer) {
     return layer >= 0 && layer < v.n_layers ? QNT_OK : set_err(QNT_ERR_INVALID, "layer out of range");
 }
@@ -64,12 +67,14 @@ int check_layer(const qb::KvView& v, int layer) {
 int check_call(const qb::KvView& v, const int* seqs, const int* starts, int n, int n_tok) {
     if (n < 0 || n_tok < 0 || n > v.max_seqs) return set_err(QNT_ERR_INVALID, "bad count of sequences or tokens");
     if (n > 0 && (!seqs || !starts)) return set_err(QNT_ERR_INVALID, "null sequence list");
+    if (!aligned(seqs, 4) || !aligned(starts, 4)) return set_err(QNT_ERR_INVALID, "sequence lists must be aligned to their elements");
     return QNT_OK;
 }
 
 int check_list(const qb::KvView& v, const void* a, const void* b, int n) {
     if (n < 0 || n > v.max_seqs) return set_err(QNT_ERR_INVALID, "bad count of sequences");
     if (n > 0 && (!a || !b)) return set_err(QNT_ERR_INVALID, "null sequence list");
+    if (!aligned(a, 4) || !aligned(b, 4)) return set_err(QNT_ERR_INVALID, "sequence lists must be aligned to their elements");
     return QNT_OK;
 }
 
@@ -126,6 +131,7 @@ int qnt_kv_append(const qnt_kv_cache* cache, int layer, const void* k, const voi
     if (!k || !v || max_new <= 0) return set_err(QNT_ERR_INVALID, "null rows or max_new <= 0");
     if (n_tok > 1 && (k_stride < (long long)c.n_kv * c.hd || v_stride < (long long)c.n_kv * c.hd))
         return set_err(QNT_ERR_INVALID, "k_stride or v_stride is smaller than a token's heads");
+    if (!aligned(k, size_of(t)) || !aligned(v, size_of(t))) return set_err(QNT_ERR_INVALID, "k and v must be aligned to their elements");
     return done(qb::launch_kv_append(c, layer, k, v, t, k_stride, v_stride, qb::KvCall{seqs, starts, n, n_tok},
                                      max_new < n_tok ? max_new : n_tok, stream_of(stream)), "kv append");
 }
@@ -139,8 +145,8 @@ int qnt_kv_read(const qnt_kv_cache* cache, int layer, const int* seqs, const int
     if (int r = make_type(dtype, &t)) return r;
     if (int r = check_call(c, seqs, starts, n, n_tok)) return r;
     if (n == 0 || n_tok == 0) return QNT_OK;
-    if (!first || !k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16))
-        return set_err(QNT_ERR_INVALID, "outputs must be 16-byte aligned");
+    if (!first || !k_out || !v_out || !aligned(first, 4) || !aligned(k_out, 16) || !aligned(v_out, 16))
+        return set_err(QNT_ERR_INVALID, "first and outputs: not null, outputs 16-byte aligned, first to its elements");
     return done(qb::launch_kv_read(c, layer, first, qb::KvCall{seqs, starts, n, n_tok}, k_out, v_out, t, stream_of(stream)),
                 "kv read");
 }
@@ -170,6 +176,7 @@ int qnt_kv_attention(const qnt_kv_cache* cache, int layer, const void* q, int dt
     if (int r = attn_args(c, layer, q, dtype, q_stride, n_heads, n, n_tok, max_q, max_len, scale, window, out, lse, &a)) return r;
     if (n == 0 || n_tok == 0) return QNT_OK;
     if (!q || !out || !aligned(out, 16)) return set_err(QNT_ERR_INVALID, "null q, or out not 16-byte aligned");
+    if (!aligned(q, size_of(a.type)) || !aligned(lse, 4)) return set_err(QNT_ERR_INVALID, "q and lse must be aligned to their elements");
     const qb::KvCall call{seqs, starts, n, n_tok};
     if (int r = check_ws(workspace, workspace_bytes, qb::kv_attn_ws_bytes(c, a, call))) return r;
     return done(qb::launch_kv_attention(c, a, call, workspace, stream_of(stream)), "kv attention");
@@ -215,7 +222,7 @@ int qnt_kv_compact(const qnt_kv_cache* cache, void* workspace, size_t workspace_
 int qnt_kv_copy(const qnt_kv_cache* cache, const int* src, const int* dst, int n, void* stream) {
     qb::KvView c;
     if (int r = make_view(cache, &c)) return r;
-    if (n < 0 || n > 65535 || (n > 0 && (!src || !dst))) return set_err(QNT_ERR_INVALID, "bad page list (at most 65535 pages)");
+    if (n < 0 || n > 65535 || (n > 0 && (!src || !dst)) || !aligned(src, 4) || !aligned(dst, 4)) return set_err(QNT_ERR_INVALID, "bad page list (at most 65535 pages)");
     return done(qb::launch_kv_copy(c, src, dst, n, stream_of(stream)), "kv copy");
 }
 
