@@ -70,7 +70,8 @@ struct KvAttnArgs {
     void* out;      // [n_tok][n_heads][hd]
     float* lse;     // [n_tok][n_heads] or null
     KvType type;    // of q and out
-    int layer, n_heads, group, window;
+    int layer, n_heads, group;
+    int window;  // 0: none, else below max_pages * pt
     float scale;
     int max_q, max_len;  // host bounds: queries of a sequence, length of a sequence
 };

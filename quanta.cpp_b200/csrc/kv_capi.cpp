@@ -108,7 +108,8 @@ int attn_args(const qb::KvView& v, int layer, const void* q, int dtype, long lon
     a->layer = layer;
     a->n_heads = n_heads;
     a->group = n_heads / v.n_kv;
-    a->window = window;
+    // a window that holds every position a sequence can have is none (and sums with it stay in range)
+    a->window = window >= v.max_pages * v.pt ? 0 : window;
     a->scale = scale;
     a->max_q = max_q;
     a->max_len = max_len;
