@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "kv_cache.h"
@@ -1554,9 +1555,9 @@ struct DecLaunch {
 DecLaunch dec_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     DecLaunch l;
     l.units = size_t(call.n) * c.n_kv;
-    // a unit's tiles, at most; a window ends anywhere in its first and last tile
-    const long long span = a.window && a.window < a.max_len ? (long long)a.window + a.max_q : a.max_len;
-    const long long tiles = std::max(1LL, (span + kTileKeys - 1) / kTileKeys + (a.window != 0));
+    // a unit's tiles, at most: never more with a window (which may begin and end within a tile) than without
+    const auto tiles_of = [](long long keys) { return std::max(1LL, (keys + kTileKeys - 1) / kTileKeys); };
+    const long long tiles = std::min(tiles_of(a.max_len), a.window ? tiles_of((long long)a.window + a.max_q) + 1 : LLONG_MAX);
     const int ctas = c.hd == 64 && dec_rm(a) <= 8 ? 3 : 2;  // per SM, as the kernel's
     // Units of up to 8 tiles are not dealt: cutting them costs more than an uneven last wave (32 x 2 units of 640 keys: 19.3 us, dealt
     // 21.5; 256 x 2: 34.9, dealt 39.9; of 1100 keys 25.4 either way; of 1500 dealt 25.6, a CTA each 29.7; of 2000 27.6, 36.8).

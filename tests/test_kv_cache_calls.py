@@ -1,8 +1,13 @@
-"""CPU checks of the calls on the paged KV cache: addresses that a kernel could not read are refused before any device work."""
+"""CPU checks of the calls on the paged KV cache: addresses that a kernel could not read are refused before any device work, and
+the workspace that a call is told to bring is the one it takes."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 
+from conftest import ROOT
 from test_kv_cache_abi import AT, INVALID, cache, refused
 
 
@@ -37,3 +42,38 @@ def test_lists_are_aligned_to_their_elements(qb):
         refused(qb, L.qnt_kv_copy(p, seqs, starts, 1, None), INVALID, "page list")
     refused(qb, L.qnt_kv_read(p, 0, AT, odd, AT, 1, 1, AT, AT, 0, None), INVALID, "aligned")
     refused(qb, L.qnt_kv_free(p, odd, 1, None), INVALID, "aligned")
+
+
+# In a process that sees no GPU, whatever the machine: a call that is not refused for its workspace ends with CUDA's own error.
+DEMANDS = """
+import ctypes as C, itertools, sys
+sys.path[:0] = {paths!r}
+import quanta_b200 as qb
+from test_kv_cache_abi import AT, cache
+L, short, calls = qb.lib(), [], 0
+for (kv, group, hd), (n, m), page in itertools.product([(8, 4, 128), (2, 7, 64), (1, 1, 64), (1, 40, 128), (2, 2, 64)],
+                                                       [(1, 1), (1, 4), (8, 1), (64, 1), (256, 1), (5, 2), (3, 60), (40, 300)], [16, 64]):
+    for max_len in [1, 100, 128, 896, 897, 1000, 1023, 1024, 1025, 1152, 1153, 4096, 4200, 8000, 70000]:
+        c = cache(qb, n_kv_heads=kv, head_dim=hd, page_tokens=page, max_seqs=300, max_pages=-(-max_len // page) + 5)
+        p = C.byref(c)
+        have = L.qnt_kv_attention_workspace(p, kv * group, n, n * m, m, max_len)
+        for window in sorted({{0, 1, 100, 128, 900, 1000, 1023, 4096, 8192, max_len - 1, max_len, max_len + 1, max_len - m, max_len + 79,
+                              max_len + 200, 2 ** 31 - 1}} - {{-1}} - set(range(-400, 0))):
+            for dtype in (0, 1, 4):
+                rc = L.qnt_kv_attention(p, 0, AT, dtype, kv * group * hd, kv * group, AT, AT, n, n * m, m, max_len, 1.0, window, AT, None,
+                                        AT, have, None)
+                calls += 1
+                why = L.qnt_last_error().decode()
+                assert rc != 0, "a GPU was seen"
+                if "workspace" in why:
+                    short.append((kv, group, hd, n, m, max_len, window, dtype, have, why))
+print(calls, len(short), short[:5])
+sys.exit(1 if short else 0)
+"""
+
+
+def test_the_workspace_that_is_asked_for_is_enough_with_any_window(qb):
+    paths = [str(ROOT / "quanta.cpp_b200"), str(ROOT / "tests")]
+    r = subprocess.run([sys.executable, "-c", DEMANDS.format(paths=paths)], env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True,
+                       text=True, timeout=600)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
