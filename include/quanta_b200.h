@@ -231,7 +231,9 @@ int qnt_batch_reset(qnt_model* m, int seq);
  * of n_pages as they grow, at a bit more than half of the f16 caches' bytes per position, and share a common prefix.
  *   qnt_batch_init_paged  instead of qnt_batch_init; prefill, decode and reset are the same calls.  A call that would need
  *                         more pages than are free returns QNT_ERR_RANGE and leaves its sequences as they were (a prefill
- *                         of more than 512 tokens: with those of its 512-token chunks that found room)
+ *                         of more than 512 tokens: with those of its 512-token chunks that found room).  A token id outside
+ *                         the embedding is QNT_ERR_DEVICE as above, and changes nothing.  After any other QNT_ERR_DEVICE or
+ *                         QNT_ERR_CUDA the call's sequences have its positions without their values: reset them
  *   qnt_batch_fork        the empty sequence dst takes over src's positions: full pages are shared, a part-filled last page
  *                         is copied
  *   qnt_batch_resize      the pages in use are moved together and into a pool of n_pages, which replaces the old one

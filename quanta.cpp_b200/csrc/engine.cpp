@@ -453,27 +453,7 @@ int Engine::launch_matmul(const DMat& W, const TcMap* wmap, bool ffn_in, int n, 
 int Engine::launch_chunk(int n, const int* pos_dev, int pos_bound, TokMap tm, const KvCall* paged, int max_q) {
     const int dim = hp_.dim;
     const int kv_dim = hp_.n_kv_heads * hp_.head_dim;
-    KvAttnArgs ka{};
-    if (paged) {
-        ka.q = Q_;
-        ka.out = ATT_;
-        ka.q_stride = (long long)hp_.n_heads * hp_.head_dim;
-        ka.type = KV_F32;
-        ka.n_heads = hp_.n_heads;
-        ka.group = hp_.n_heads / hp_.n_kv_heads;
-        ka.scale = layers_.empty() ? 0.f : layers_[0].aa.scale;
-        ka.max_q = max_q;
-        ka.max_len = pos_bound;
-        const size_t need = kv_attn_ws_bytes(kv_, ka, *paged);
-        if (need > kv_ws_bytes_) {
-            cudaStreamSynchronize(st_);
-            cudaFree(kv_ws_);
-            kv_ws_ = nullptr;
-            kv_ws_bytes_ = 0;
-            QB_TRY(cudaMalloc(&kv_ws_, need));
-            kv_ws_bytes_ = need;
-        }
-    }
+    KvAttnArgs ka = paged ? paged_attn(max_q, pos_bound) : KvAttnArgs{};
     for (size_t l = 0; l < layers_.size(); ++l) {
         const Layer& L = layers_[l];
         QkvArgs qa = L.qa;
@@ -1147,6 +1127,26 @@ int Engine::batch_init_paged(int max_seqs, int ctx, int n_pages, int page_tokens
     return 0;
 }
 
+KvAttnArgs Engine::paged_attn(int max_q, int max_len) const {
+    KvAttnArgs a{};
+    a.q = Q_;
+    a.out = ATT_;
+    a.q_stride = (long long)hp_.n_heads * hp_.head_dim;
+    a.type = KV_F32;
+    a.n_heads = hp_.n_heads;
+    a.group = hp_.n_heads / hp_.n_kv_heads;
+    a.scale = layers_.empty() ? 0.f : layers_[0].aa.scale;
+    a.max_q = max_q;
+    a.max_len = max_len;
+    return a;
+}
+
+int Engine::paged_tokens(const int* tokens, int n) {
+    if (std::all_of(tokens, tokens + n, [this](int t) { return t >= 0 && t < embed_.rows; })) return 0;
+    err_ = "paged KV caches: token id outside the embedding";
+    return -6;
+}
+
 int Engine::paged_check(long long extra) {
     long long pages = extra;  // at most: shared pages count for each of their sequences
     for (int len : blens_) pages += (len + kv_.pt - 1) >> kv_.pt_shift;
@@ -1155,11 +1155,20 @@ int Engine::paged_check(long long extra) {
     if (e != cudaSuccess) return cuda_fail(e, "kernel");
     const unsigned s = read_status();
     if (s == 0) return 0;
-    err_ = s == ERR_CAPACITY ? "paged KV caches: no free pages left" : "device status error bits 0x" + std::to_string(s);
-    return s == ERR_CAPACITY ? -5 : -6;
+    err_ = s & ERR_CAPACITY ? "paged KV caches: no free pages left" : "device status error bits 0x" + std::to_string(s);
+    return s & ERR_CAPACITY ? -5 : -6;
 }
 
-int Engine::paged_reserve(const int* seqs, const int* starts, int n) {
+int Engine::paged_reserve(const int* seqs, const int* starts, int n, int max_q, int bound) {
+    const size_t need = kv_attn_ws_bytes(kv_, paged_attn(max_q, bound), KvCall{nullptr, nullptr, n, starts[n]});
+    if (need > kv_ws_bytes_) {  // before anything changes
+        cudaStreamSynchronize(st_);
+        cudaFree(kv_ws_);
+        kv_ws_ = nullptr;
+        kv_ws_bytes_ = 0;
+        QB_TRY(cudaMalloc(&kv_ws_, need));
+        kv_ws_bytes_ = need;
+    }
     h_extra_.resize(size_t(n));
     long long pages = 0;
     for (int i = 0; i < n; ++i) {
@@ -1171,7 +1180,10 @@ int Engine::paged_reserve(const int* seqs, const int* starts, int n) {
     cudaMemcpyAsync(kv_starts_, starts, size_t(n + 1) * 4, cudaMemcpyHostToDevice, st_);
     cudaMemcpyAsync(kv_extra_, h_extra_.data(), size_t(n) * 4, cudaMemcpyHostToDevice, st_);
     QB_TRY(launch_kv_reserve(kv_, kv_seqs_, kv_extra_, n, kv_page_ws(), st_));
-    return paged_check(pages);
+    const int r = paged_check(pages);
+    if (r != -5)  // the device's lengths have grown, whatever becomes of the step: so do the host's
+        for (int i = 0; i < n; ++i) blens_[size_t(seqs[i])] += h_extra_[size_t(i)];
+    return r;
 }
 
 int Engine::batch_fork(int src, int dst) {
@@ -1187,9 +1199,9 @@ int Engine::batch_fork(int src, int dst) {
     cudaMemcpyAsync(kv_seqs_, &src, 4, cudaMemcpyHostToDevice, st_);
     cudaMemcpyAsync(kv_extra_, &dst, 4, cudaMemcpyHostToDevice, st_);
     QB_TRY(launch_kv_fork(kv_, kv_seqs_, kv_extra_, 1, kv_page_ws(), st_));
-    if (int r = paged_check(len & (kv_.pt - 1) ? 1 : 0)) return r;
-    blens_[size_t(dst)] = len;
-    return 0;
+    const int r = paged_check(len & (kv_.pt - 1) ? 1 : 0);
+    if (r != -5) blens_[size_t(dst)] = len;
+    return r;
 }
 
 int Engine::batch_resize(int n_pages) {
@@ -1262,6 +1274,8 @@ int Engine::batch_prefill(int seq, const int* tokens, int n, int* next_id) {
         err_ = "batch_prefill: sequence exceeds its context";
         return -5;
     }
+    if (kv_.codes)
+        if (int r = paged_tokens(tokens, n)) return r;
     const long long stride = (long long)hp_.n_layers * bctx_ * hp_.n_kv_heads * hp_.head_dim;
     int last = 0;
     for (int i = 0; i < n; i += kChunk) {
@@ -1272,7 +1286,7 @@ int Engine::batch_prefill(int seq, const int* tokens, int n, int* next_id) {
         for (int t = 0; t < m; ++t) h_pos_[size_t(t)] = len + i + t;
         if (kv_.codes) {
             h_starts_ = {0, m};
-            if (int r = paged_reserve(&seq, h_starts_.data(), 1)) return r;
+            if (int r = paged_reserve(&seq, h_starts_.data(), 1, m, len + i + m)) return r;
         }
         cudaMemcpyAsync(tokens_, tokens + i, size_t(m) * 4, cudaMemcpyHostToDevice, st_);
         cudaMemcpyAsync(tok_pos_, h_pos_.data(), size_t(m) * 4, cudaMemcpyHostToDevice, st_);
@@ -1281,7 +1295,6 @@ int Engine::batch_prefill(int seq, const int* tokens, int n, int* next_id) {
         const KvCall call{kv_seqs_, kv_starts_, 1, m};
         if (int r = launch_chunk(m, pos_, len + i + m, TokMap{tok_pos_, tok_off_}, kv_.codes ? &call : nullptr, m)) return r;
         cudaStreamSynchronize(st_);  // the host position arrays are rewritten by the next chunk
-        if (kv_.codes) blens_[size_t(seq)] = len + i + m;  // as the device has it, if a later chunk finds no room
         last = m - 1;
     }
     blens_[size_t(seq)] = len + n;
@@ -1300,6 +1313,8 @@ int Engine::batch_decode(const int* seq_ids, const int* tokens, int n, int* next
         err_ = "batch_decode: need 1 <= n <= " + std::to_string(kChunk) + " sequences";
         return -1;
     }
+    if (kv_.codes)
+        if (int r = paged_tokens(tokens, n)) return r;
     const long long stride = (long long)hp_.n_layers * bctx_ * hp_.n_kv_heads * hp_.head_dim;
     h_pos_.resize(size_t(n));
     h_off_.resize(size_t(n));
@@ -1323,7 +1338,7 @@ int Engine::batch_decode(const int* seq_ids, const int* tokens, int n, int* next
     if (kv_.codes) {
         h_starts_.resize(size_t(n) + 1);
         std::iota(h_starts_.begin(), h_starts_.end(), 0);
-        if (int r = paged_reserve(seq_ids, h_starts_.data(), n)) return r;
+        if (int r = paged_reserve(seq_ids, h_starts_.data(), n, 1, bound)) return r;
     }
     cudaMemcpyAsync(tokens_, tokens, size_t(n) * 4, cudaMemcpyHostToDevice, st_);
     cudaMemcpyAsync(tok_pos_, h_pos_.data(), size_t(n) * 4, cudaMemcpyHostToDevice, st_);
@@ -1332,7 +1347,8 @@ int Engine::batch_decode(const int* seq_ids, const int* tokens, int n, int* next
     const KvCall call{kv_seqs_, kv_starts_, n, n};
     if (int r = launch_chunk(n, pos_, bound, TokMap{tok_pos_, tok_off_}, kv_.codes ? &call : nullptr, 1)) return r;
     if (int r = batch_head(n, next_ids)) return r;
-    for (int i = 0; i < n; ++i) blens_[size_t(seq_ids[i])] += 1;
+    if (!kv_.codes)
+        for (int i = 0; i < n; ++i) blens_[size_t(seq_ids[i])] += 1;
     return 0;
 }
 

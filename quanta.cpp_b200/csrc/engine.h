@@ -161,8 +161,12 @@ private:
     void batch_free();
     // a pool of n_pages pages for v's sizes (codes, scales, refs, zeroed; workspace); false: no memory
     bool paged_pool(int n_pages, KvView* v, void** mem);
-    // the pages for extra tokens of sequences (host lists; starts: [n + 1] rows) and their device lists
-    int paged_reserve(const int* seqs, const int* starts, int n);
+    // attention over the paged caches for a chunk: at most max_q tokens of a sequence, no sequence past max_len
+    KvAttnArgs paged_attn(int max_q, int max_len) const;
+    int paged_tokens(const int* tokens, int n);  // an error where an id is outside the embedding
+    // the workspace, the pages and the positions for more tokens of sequences (host lists; starts: [n + 1] rows; max_q and bound
+    // as of paged_attn), and the call's device lists.  Refused for lack of pages (-5) or memory it changes nothing.
+    int paged_reserve(const int* seqs, const int* starts, int n, int max_q, int bound);
     // waits for the call's status if the pages of all sequences, extra more of them, could pass the pool
     int paged_check(long long extra);
     int batch_head(int n, int* host_ids);  // greedy ids of the n rows of X_
