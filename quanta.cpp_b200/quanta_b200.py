@@ -300,7 +300,8 @@ class PagedKV:
     Sequence lists (seqs, starts, extra, ...) are contiguous int32 CUDA tensors: tokens starts[j] .. starts[j + 1] - 1 of a
     call belong to sequence seqs[j].  Work is queued on `stream` (default: torch's current stream), nothing waits; errors
     that kernels find (no free pages, a sequence out of range) are raised by check().  Calls that write the cache must be
-    ordered against its other calls; the object's workspaces are one per stream."""
+    ordered against its other calls; the object's workspaces are one per stream, and live as long as the object: a graph that
+    captured calls is replayed while the object exists, ordered against the calls on the stream that it was captured on."""
 
     def __init__(self, codes, scales, refs, table, lens):
         import torch
@@ -323,7 +324,7 @@ class PagedKV:
                            scales.data_ptr(), refs.data_ptr(), table.data_ptr(), lens.data_ptr(), self._status.data_ptr())
         self._p = C.byref(self._c)
         self._types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-        self._ws, self._need, self._i32 = {}, {}, i32
+        self._ws, self._kept, self._need, self._i32 = {}, [], {}, i32
         self._lib, self._index = lib(), codes.device.index  # a call's host time counts where few tokens are decoded
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._page_ws = lib().qnt_kv_page_workspace(self._p)
@@ -348,9 +349,11 @@ class PagedKV:
     def _workspace(self, stream: int, need: int):
         ws = self._ws.get(stream)
         if ws is None or ws.numel() < need:
-            if ws is not None:  # kernels queued on `stream` may still use the old one
-                ws.record_stream(self._torch.cuda.ExternalStream(stream, device=self.device))
-            ws = self._ws[stream] = self._torch.empty(max(need, self._page_ws, 1 << 20), dtype=self._torch.uint8, device=self.device)
+            size = max(need, self._page_ws, 1 << 20)
+            if ws is not None:  # the old one stays: queued kernels and captured graphs still write to it
+                self._kept.append(ws)
+                size = max(size, 2 * ws.numel())  # (all of the old ones together are less than the new one)
+            ws = self._ws[stream] = self._torch.empty(size, dtype=self._torch.uint8, device=self.device)
         return ws.data_ptr(), ws.numel()
 
     def _list(self, *lists):
