@@ -11,6 +11,7 @@ loudly when either is missing.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from dataclasses import dataclass
@@ -290,6 +291,9 @@ def sample_noalloc(sp: SamplerParams, rng_state: int, logits, n_valid: int | Non
     return tok.value, state.value
 
 
+_NOTHING = contextlib.nullcontext()
+
+
 class PagedKV:
     """The paged 8-bit KV cache (qnt_kv_*): many sequences in pages of one pool, int8 codes with a f32 scale for each block
     of 16 tokens, K or V, layer and kv head.  The arrays are torch CUDA tensors that the caller may keep and look at:
@@ -298,10 +302,12 @@ class PagedKV:
         scales float32 [n_pages, n_layers, 2, n_kv_heads, page_tokens / 16]
         refs int32 [n_pages], table int32 [max_seqs, max_pages], lens int32 [max_seqs]
     Sequence lists (seqs, starts, extra, ...) are contiguous int32 CUDA tensors: tokens starts[j] .. starts[j + 1] - 1 of a
-    call belong to sequence seqs[j].  Work is queued on `stream` (default: torch's current stream), nothing waits; errors
-    that kernels find (no free pages, a sequence out of range) are raised by check().  Calls that write the cache must be
-    ordered against its other calls; the object's workspaces are one per stream, and live as long as the object: a graph that
-    captured calls is replayed while the object exists, ordered against the calls on the stream that it was captured on."""
+    call belong to sequence seqs[j].  Work is queued on `stream` (a torch stream or a cudaStream_t's number; default: torch's
+    current stream), nothing waits.  With another stream than the current one a call is as if made within torch.cuda.stream(stream):
+    its outputs belong to that stream, and what it reads has to be ready there.  Errors that kernels find (no free pages, a
+    sequence out of range) are raised by check().  Calls that write the cache must be ordered against its other calls; the
+    object's workspaces are one per stream, and live as long as the object: a graph that captured calls is replayed while the
+    object exists, ordered against the calls on the stream that it was captured on."""
 
     def __init__(self, codes, scales, refs, table, lens):
         import torch
@@ -346,6 +352,13 @@ class PagedKV:
             return self._raw_stream(self._index) if self._raw_stream else self._torch.cuda.current_stream(self.device).cuda_stream
         return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
+    def _allocating_on(self, stream):
+        """Within it torch allocates for work on this stream: from its own pool, whose memory no other stream still uses."""
+        cuda = self._torch.cuda
+        if not hasattr(stream, "cuda_stream"):
+            stream = cuda.ExternalStream(int(stream), device=self.device) if int(stream) else cuda.default_stream(self.device)
+        return cuda.stream(stream)
+
     def _workspace(self, stream: int, need: int):
         ws = self._ws.get(stream)
         if ws is None or ws.numel() < need:
@@ -353,7 +366,8 @@ class PagedKV:
             if ws is not None:  # the old one stays: queued kernels and captured graphs still write to it
                 self._kept.append(ws)
                 size = max(size, 2 * ws.numel())  # (all of the old ones together are less than the new one)
-            ws = self._ws[stream] = self._torch.empty(size, dtype=self._torch.uint8, device=self.device)
+            with self._allocating_on(stream):
+                ws = self._ws[stream] = self._torch.empty(size, dtype=self._torch.uint8, device=self.device)
         return ws.data_ptr(), ws.numel()
 
     def _list(self, *lists):
@@ -431,8 +445,9 @@ class PagedKV:
         n = self._list(seqs, first, starts)
         if first.numel() != n or starts.numel() != n + 1:
             raise ValueError("one first per sequence, and one entry more in starts")
-        k = self.scales.new_empty((n_tok, self.n_kv_heads, self.head_dim), dtype=dtype)
-        v = t.empty_like(k)
+        with _NOTHING if stream is None else self._allocating_on(stream):
+            k = self.scales.new_empty((n_tok, self.n_kv_heads, self.head_dim), dtype=dtype)
+            v = t.empty_like(k)
         _check(self._lib.qnt_kv_read(self._p, layer, seqs.data_ptr(), first.data_ptr(), starts.data_ptr(), n, n_tok, k.data_ptr(),
                                  v.data_ptr(), self._types[dtype], self._stream(stream)))
         return k, v
@@ -455,8 +470,9 @@ class PagedKV:
             need = self._need[key] = self._lib.qnt_kv_attention_workspace(self._p, heads, n, n_tok, max_q, max_len)
         s = self._stream(stream)
         w, nb = self._workspace(s, need)
-        out = self._torch.empty_like(q)  # (a token's heads are contiguous and tokens do not overlap: so is this)
-        ls = self.scales.new_empty((n_tok, heads)) if lse else None
+        with _NOTHING if stream is None else self._allocating_on(stream):
+            out = self._torch.empty_like(q)  # (a token's heads are contiguous and tokens do not overlap: so is this)
+            ls = self.scales.new_empty((n_tok, heads)) if lse else None
         _check(self._lib.qnt_kv_attention(self._p, layer, q.data_ptr(), dt, stride, heads, seqs.data_ptr(), starts.data_ptr(), n,
                                       n_tok, max_q, max_len, self.head_dim ** -0.5 if scale is None else scale, window,
                                       out.data_ptr(), None if ls is None else ls.data_ptr(), w, nb, s))

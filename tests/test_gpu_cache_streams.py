@@ -39,3 +39,35 @@ def test_a_graph_keeps_its_workspace(qb):
         assert torch.equal(out, want)
     assert all(bool((t == 7).all()) for t in taken)
     c.check()
+
+
+@pytest.mark.parametrize("call", ["attention", "read"])
+def test_outputs_on_a_stream_of_their_own(qb, call):
+    """With stream=, nothing that the current stream still has queued reaches the outputs."""
+    c = make(qb, [2000] * 8, 2, 64, 64, seed=51)
+    side = torch.cuda.Stream()
+    q, seqs, starts = queries(8, 14, 64, "f32"), ints(range(8)), ints(range(9))
+    rows, first = ints(range(0, 801, 100)), ints([0] * 8)
+    run = {"attention": lambda s: c.attention(0, q, seqs, starts, 1, 2000, lse=True, stream=s),
+           "read": lambda s: c.read(0, seqs, first, rows, 800, stream=s)}[call]
+    want = [x.clone() for x in run(None)]
+    run(side)  # (the side stream's workspace)
+    torch.cuda.synchronize()
+    shapes = [x.shape for x in want]
+    for _ in range(3):
+        blocks = [torch.empty(s, device="cuda") for s in shapes for _ in range(4)]
+        torch.cuda._sleep(20_000_000)  # about 10 ms: the fills below are still queued when the call runs
+        for b in blocks:
+            b.fill_(7.0)
+        del b, blocks
+        got = run(side)
+        torch.cuda.synchronize()
+        for a, w in zip(got, want):
+            assert torch.equal(a, w)
+    by_number = run(side.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, w) for a, w in zip(by_number, want))
+    torch.cuda.synchronize()
+    on_default = run(0)  # the legacy default stream
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, w) for a, w in zip(on_default, want))
