@@ -11,7 +11,6 @@ loudly when either is missing.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 from dataclasses import dataclass
@@ -291,9 +290,6 @@ def sample_noalloc(sp: SamplerParams, rng_state: int, logits, n_valid: int | Non
     return tok.value, state.value
 
 
-_NOTHING = contextlib.nullcontext()
-
-
 class PagedKV:
     """The paged 8-bit KV cache (qnt_kv_*): many sequences in pages of one pool, int8 codes with a f32 scale for each block
     of 16 tokens, K or V, layer and kv head.  The arrays are torch CUDA tensors that the caller may keep and look at:
@@ -333,6 +329,7 @@ class PagedKV:
         self._ws, self._kept, self._need, self._i32 = {}, [], {}, i32
         self._lib, self._index = lib(), codes.device.index  # a call's host time counts where few tokens are decoded
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         self._page_ws = lib().qnt_kv_page_workspace(self._p)
         if self._page_ws == 0:
             raise QntError(-1, lib().qnt_last_error().decode(errors="replace"))
@@ -370,20 +367,30 @@ class PagedKV:
                 ws = self._ws[stream] = self._torch.empty(size, dtype=self._torch.uint8, device=self.device)
         return ws.data_ptr(), ws.numel()
 
+    def _run(self, call, *args):
+        """A launching call of the library: on the cache's device, whichever is current."""
+        if self._current_device() == self._index:
+            rc = call(*args)
+        else:
+            with self._torch.cuda.device(self._index):
+                rc = call(*args)
+        if rc:
+            _check(rc)
+
     def _list(self, *lists):
         for t in lists:
-            if t.dtype is not self._i32 or not t.is_cuda or not t.is_contiguous():
-                raise TypeError("sequence lists must be contiguous int32 CUDA tensors")
+            if t.dtype is not self._i32 or t.get_device() != self._index or not t.is_contiguous():
+                raise TypeError("sequence lists must be contiguous int32 CUDA tensors on the cache's device")
         return lists[0].numel()
 
     def _rows(self, name, x, heads=None):
         """The type and the token stride of rows [tokens, heads, head_dim]."""
         shape, st, hd = x.shape, x.stride(), self.head_dim
         dt = self._types.get(x.dtype)
-        if not (len(st) == 3 and st[2] == 1 and st[1] == hd and shape[2] == hd and dt is not None and x.is_cuda and
-                (heads is None or shape[1] == heads)):
-            raise TypeError(f"{name} must be a float32, float16 or bfloat16 CUDA tensor [tokens, heads, {self.head_dim}] whose "
-                            "heads are contiguous within a token")
+        if not (len(st) == 3 and st[2] == 1 and st[1] == hd and shape[2] == hd and dt is not None and
+                x.get_device() == self._index and (heads is None or shape[1] == heads)):
+            raise TypeError(f"{name} must be a float32, float16 or bfloat16 CUDA tensor [tokens, heads, {self.head_dim}] on the "
+                            "cache's device whose heads are contiguous within a token")
         return dt, st[0]
 
     def reserve(self, seqs, extra, stream=None):
@@ -393,7 +400,7 @@ class PagedKV:
             raise ValueError("one extra per sequence")
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
-        _check(self._lib.qnt_kv_reserve(self._p, seqs.data_ptr(), extra.data_ptr(), n, w, nb, s))
+        self._run(self._lib.qnt_kv_reserve, self._p, seqs.data_ptr(), extra.data_ptr(), n, w, nb, s)
 
     def fork(self, src, dst, stream=None):
         """Empty sequences dst become copies of src: full pages shared, a part-filled last page copied."""
@@ -402,24 +409,24 @@ class PagedKV:
             raise ValueError("one dst per src")
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
-        _check(self._lib.qnt_kv_fork(self._p, src.data_ptr(), dst.data_ptr(), n, w, nb, s))
+        self._run(self._lib.qnt_kv_fork, self._p, src.data_ptr(), dst.data_ptr(), n, w, nb, s)
 
     def free(self, seqs, stream=None):
         """The sequences give back their pages and become empty."""
-        _check(self._lib.qnt_kv_free(self._p, seqs.data_ptr(), self._list(seqs), self._stream(stream)))
+        self._run(self._lib.qnt_kv_free, self._p, seqs.data_ptr(), self._list(seqs), self._stream(stream))
 
     def compact(self, stream=None):
         """The pages in use move together to the lowest indices."""
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
-        _check(self._lib.qnt_kv_compact(self._p, w, nb, s))
+        self._run(self._lib.qnt_kv_compact, self._p, w, nb, s)
 
     def copy_pages(self, src, dst, stream=None):
         """Codes and scales of pages src over those of pages dst, all layers."""
         n = self._list(src, dst)
         if dst.numel() != n:
             raise ValueError("one dst per src")
-        _check(self._lib.qnt_kv_copy(self._p, src.data_ptr(), dst.data_ptr(), n, self._stream(stream)))
+        self._run(self._lib.qnt_kv_copy, self._p, src.data_ptr(), dst.data_ptr(), n, self._stream(stream))
 
     def append(self, layer: int, k, v, seqs, starts, max_new: int | None = None, stream=None):
         """Quantizes rows k, v [tokens, n_kv_heads, head_dim] into a layer, as the last positions of their sequences
@@ -432,8 +439,8 @@ class PagedKV:
         n = self._list(seqs, starts)
         if starts.numel() != n + 1:
             raise ValueError("starts must have one entry more than seqs")
-        _check(self._lib.qnt_kv_append(self._p, layer, k.data_ptr(), v.data_ptr(), dt, ks, vs, seqs.data_ptr(),
-                                       starts.data_ptr(), n, m, m if max_new is None else max_new, self._stream(stream)))
+        self._run(self._lib.qnt_kv_append, self._p, layer, k.data_ptr(), v.data_ptr(), dt, ks, vs, seqs.data_ptr(),
+                  starts.data_ptr(), n, m, m if max_new is None else max_new, self._stream(stream))
 
     def read(self, layer: int, seqs, first, starts, n_tok: int, dtype=None, stream=None):
         """Values of positions first[j] + i of sequence seqs[j] as rows starts[j] + i: (K, V) [n_tok, n_kv_heads, head_dim]
@@ -445,11 +452,16 @@ class PagedKV:
         n = self._list(seqs, first, starts)
         if first.numel() != n or starts.numel() != n + 1:
             raise ValueError("one first per sequence, and one entry more in starts")
-        with _NOTHING if stream is None else self._allocating_on(stream):
-            k = self.scales.new_empty((n_tok, self.n_kv_heads, self.head_dim), dtype=dtype)
+        shape = (n_tok, self.n_kv_heads, self.head_dim)
+        if stream is None:
+            k = self.scales.new_empty(shape, dtype=dtype)
             v = t.empty_like(k)
-        _check(self._lib.qnt_kv_read(self._p, layer, seqs.data_ptr(), first.data_ptr(), starts.data_ptr(), n, n_tok, k.data_ptr(),
-                                 v.data_ptr(), self._types[dtype], self._stream(stream)))
+        else:
+            with self._allocating_on(stream):
+                k = self.scales.new_empty(shape, dtype=dtype)
+                v = t.empty_like(k)
+        self._run(self._lib.qnt_kv_read, self._p, layer, seqs.data_ptr(), first.data_ptr(), starts.data_ptr(), n, n_tok, k.data_ptr(),
+                  v.data_ptr(), self._types[dtype], self._stream(stream))
         return k, v
 
     def attention(self, layer: int, q, seqs, starts, max_q: int, max_len: int, scale: float | None = None, window: int = 0,
@@ -470,17 +482,21 @@ class PagedKV:
             need = self._need[key] = self._lib.qnt_kv_attention_workspace(self._p, heads, n, n_tok, max_q, max_len)
         s = self._stream(stream)
         w, nb = self._workspace(s, need)
-        with _NOTHING if stream is None else self._allocating_on(stream):
+        if stream is None:
             out = self._torch.empty_like(q)  # (a token's heads are contiguous and tokens do not overlap: so is this)
             ls = self.scales.new_empty((n_tok, heads)) if lse else None
-        _check(self._lib.qnt_kv_attention(self._p, layer, q.data_ptr(), dt, stride, heads, seqs.data_ptr(), starts.data_ptr(), n,
-                                      n_tok, max_q, max_len, self.head_dim ** -0.5 if scale is None else scale, window,
-                                      out.data_ptr(), None if ls is None else ls.data_ptr(), w, nb, s))
+        else:
+            with self._allocating_on(stream):
+                out = self._torch.empty_like(q)
+                ls = self.scales.new_empty((n_tok, heads)) if lse else None
+        self._run(self._lib.qnt_kv_attention, self._p, layer, q.data_ptr(), dt, stride, heads, seqs.data_ptr(), starts.data_ptr(), n,
+                  n_tok, max_q, max_len, self.head_dim ** -0.5 if scale is None else scale, window,
+                  out.data_ptr(), None if ls is None else ls.data_ptr(), w, nb, s)
         return (out, ls) if lse else out
 
     def check(self, stream=None):
         """Waits for the stream and raises the error that earlier calls on this cache ran into, if any."""
-        _check(self._lib.qnt_kv_check(self._p, self._stream(stream)))
+        self._run(self._lib.qnt_kv_check, self._p, self._stream(stream))
 
 
 def bench_mma_i8(iters: int = 4096) -> float:

@@ -1,9 +1,11 @@
 """CPU checks of the calls on the paged KV cache: addresses that a kernel could not read are refused before any device work, and
 the workspace that a call is told to bring is the one it takes."""
+import contextlib
 import ctypes as C
 import os
 import subprocess
 import sys
+import types
 
 import pytest
 
@@ -77,3 +79,61 @@ def test_the_workspace_that_is_asked_for_is_enough_with_any_window(qb):
     r = subprocess.run([sys.executable, "-c", DEMANDS.format(paths=paths)], env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True,
                        text=True, timeout=600)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+class FakeCuda:
+    def __init__(self):
+        self.now = 0
+
+    def current_device(self):
+        return self.now
+
+    @contextlib.contextmanager
+    def device(self, index):
+        was, self.now = self.now, index
+        yield
+        self.now = was
+
+
+def on(index, dtype, shape=(4,)):
+    """What PagedKV looks at of a tensor on a device."""
+    strides = [1] * len(shape)
+    for i in range(len(shape) - 2, -1, -1):
+        strides[i] = strides[i + 1] * shape[i + 1]
+    return types.SimpleNamespace(dtype=dtype, shape=shape, stride=lambda: tuple(strides), is_cuda=index >= 0, get_device=lambda: index,
+                                 is_contiguous=lambda: True, numel=lambda: shape[0], data_ptr=lambda: AT,
+                                 device=types.SimpleNamespace(type="cuda", index=index))
+
+
+def test_a_cache_on_another_device_than_the_current_one(qb):
+    """Calls run on the cache's device and its stream; tensors of another device are refused.  (A second device is not needed: the
+    library and torch's device are stood in for.)"""
+    cuda, calls = FakeCuda(), []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *args: calls.append((name, cuda.now, args)) or 0
+
+    kv = qb.PagedKV.__new__(qb.PagedKV)
+    kv._torch, kv._lib, kv._index, kv._raw_stream = types.SimpleNamespace(cuda=cuda), Lib(), 1, lambda i: 70 + i
+    kv._current_device = cuda.current_device
+    kv._i32, kv._types, kv._p, kv._page_ws = "int32", {"f16": qb.F16}, None, 64
+    kv._ws, kv._kept, kv._need = {71: on(1, "uint8", (1 << 20,))}, [], {}
+    kv.n_kv_heads, kv.head_dim = 2, 64
+    here, there, rows = on(1, "int32"), on(0, "int32"), on(1, "f16", (3, 2, 64))
+    kv.free(here)
+    kv.reserve(here, here)
+    kv.fork(here, here)
+    kv.copy_pages(here, here)
+    kv.compact()
+    kv.append(0, rows, rows, on(1, "int32", (3,)), here)
+    kv.check()
+    assert [c[0] for c in calls] == ["qnt_kv_" + n for n in "free reserve fork copy compact append check".split()]
+    assert all(now == 1 and args[-1] == 71 for _, now, args in calls) and cuda.now == 0
+    n = len(calls)
+    for bad in (lambda: kv.free(there), lambda: kv.reserve(here, there), lambda: kv.fork(there, here), lambda: kv.free(on(-1, "int32")),
+                lambda: kv.append(0, rows, on(0, "f16", (3, 2, 64)), on(1, "int32", (3,)), here),
+                lambda: kv.attention(0, on(0, "f16", (3, 2, 64)), on(1, "int32", (3,)), here, 1, 9)):
+        with pytest.raises(TypeError, match="device"):
+            bad()
+    assert len(calls) == n
