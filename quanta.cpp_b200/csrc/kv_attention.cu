@@ -975,15 +975,14 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 // A CTA takes 128 WG query rows (token-major: row r is query r / group, head r % group of the kv head) and a stretch of keys,
 // 64 at a time.  S = Q K^T and O += W V run on the 16-bit tensor cores; K and V codes become 16-bit numbers, exactly, once per
 // tile for all rows.
-// A query row is scaled by a power of two and is the sum of f16 pieces: two for float32 (2^-23 of the row's largest value), one,
-// exactly, for 16-bit types.  A weight W = exp(s - ref) vs is
-//   float32 queries: the sum of three bf16 pieces (24 bits, f32's range); V in bf16.  The tensor cores' sums are cut off, not
-//     rounded (12 steps a tile: 1e-6 of the result after 8 tiles), so O moves every other tile to a total in shared memory.
-//   bf16 queries: two bf16 pieces (16 bits).  f16 would lose weights below 2^-31 of the largest, which a bf16 result still shows
-//     where the key ahead has a 0 for V.
-//   f16 queries: the sum of two f16 (11 bits would cost as much again as the result's own rounding); V in f16, in fewer
-//     instructions than bf16.  vs is divided by a power of two near the first tile's largest, and W held below 2^15, so that f16's
-//     range serves.
+// A query row is scaled by a power of two that brings its largest value to [1, 2), and is the sum of f16 pieces: two for float32
+// (2^-23 of the row's largest value), one for 16-bit types (their 11 bits or fewer, to 2^-25 of the row's largest value).  A weight
+// W = exp(s - ref) vs is a sum of bf16 pieces, which have f32's range:
+//   float32 queries: three (24 bits).  The tensor cores' sums are cut off, not rounded (12 steps a tile: 1e-6 of the result after 8
+//     tiles), so O moves every other tile to a total in shared memory.
+//   16-bit queries: two (16 bits; 8 or 11 would cost as much again as the result's own rounding).
+// (f16 weights for f16 queries lost small ones: those of keys behind one whose V is 0, and all weights where a block's V, even one
+// that the row does not see, was 2^20 times the others'.)
 //   warps 0 .. 4 WG - 1  softmax, thread = row: S from TMEM, weights back to TMEM (the A operand of the second product); the
 //                        reference of a row is raised only when a score passes it by far (O is then scaled)
 //   next 4 warps         codes and scales of the next tile on their way (cp.async into each thread's own places), this one's
@@ -998,7 +997,7 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 //   1 prompt of 512, f32, 14/2 heads of 64: 18.4 us with the join, 112 CTAs of up to 4 tiles
 template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
-    static constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
+    static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int QP = F32 ? 2 : 1;               // pieces of a query
     static constexpr int NP = F32 ? 3 : 2;               // pieces of a weight
     static constexpr int flush = F32 ? 2 : 1 << 30;      // tiles whose O stays in TMEM
@@ -1015,13 +1014,11 @@ struct Chunk {
     // per SM, with 1 KB static and 1 KB of the system's each.  (float32: two would leave a thread 96 registers, which it spills:
     // 31 us instead of 25 for 512 queries of 14 heads of 64 over 512 keys.)
     static constexpr int ctas = !F32 && smem <= 112 * 1024 && tmem_cols == 256 ? 2 : 1;
-    static constexpr uint32_t fmt = F16 ? 0u : (1u << 7) | (1u << 10);       // W and V: f16 or bf16
     static constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(keys >> 3) << 17) | (uint32_t(128 >> 4) << 24);
-    static constexpr uint32_t idesc_o = (1u << 4) | fmt | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    static constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     // log2.  Weights carry 2^shift; a row's reference follows its scores when one passes it by more than raise (every raise has
-    // the warp's O pass through its registers: with 4 instead of 7 every other tile did, 1.3 times the time).  f16 weights, at
-    // most 2^(7 + 7) times V's scale over its reference (at most 2), stay below f16's 65504.
-    static constexpr float shift = F16 ? 7.f : kShift, raise = F16 ? 7.f : 10.f;
+    // the warp's O pass through its registers: with 4 every other tile did, 1.3 times the time).
+    static constexpr float shift = kShift, raise = 10.f;
     static_assert(o_at + HD * WG <= 512, "TMEM");
 };
 
@@ -1050,7 +1047,7 @@ template <int HD, class T, int WG>
 __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::ctas) k_kv_chunk(KvView c, KvAttnArgs a, KvCall call, ChunkPlan plan) {
     using C = Chunk<HD, T, WG>;
     constexpr int QP = C::QP, NP = C::NP;
-    constexpr bool F32 = C::F32, F16 = C::F16;
+    constexpr bool F32 = C::F32;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* kb = smem + WG * QP * C::q_bytes;   // 2 buffers
     unsigned char* vb = kb + 2 * C::kv_bytes;          // 2 buffers
@@ -1190,7 +1187,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (pieces + x) * 2048), "l"(src) : "memory");
             }
         };
-        auto convert = [&](unsigned char* to, int row, int chunk, const uint4& v, bool bf16) {  // 16 codes -> chunks `chunk`, + 1 of a row
+        auto convert = [&](unsigned char* to, int row, int chunk, const uint4& v, bool bf16) {  // 16 codes -> 16-byte chunks `chunk`, + 1 of a row
             uint2 x[4];
             const unsigned w4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -1231,7 +1228,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             if (i >= 2) ok = ok && wait_warp(&v_free[i & 1], ((i >> 1) - 1) & 1, ab);
             unsigned char* vt = vb + (i & 1) * C::kv_bytes;
 #pragma unroll
-            for (int x = 0; x < pieces; ++x) convert(vt, ct % HD, 2 * (ct / HD + x * (128 / HD)), vc[x], !F16);
+            for (int x = 0; x < pieces; ++x) convert(vt, ct % HD, 2 * (ct / HD + x * (128 / HD)), vc[x], true);
             fence_async_smem();
             mbar_arrive(&v_full[i & 1]);
         }
@@ -1298,7 +1295,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             mbar_arrive(&q_full[g]);
         }
         float* total = reinterpret_cast<float*>(smem + C::total_at) + g * HD * 128 + rt;  // (float32) [dim][row]
-        float ref = -INFINITY, sum = 0.f, v_ref = 0.f, v_inv = 0.f;  // v_ref: f16 weights carry vs / v_ref
+        float ref = -INFINITY, sum = 0.f;
         bool ok = true;
 #pragma unroll 1
         for (int i = 0; i < nt && ok; ++i) {
@@ -1342,19 +1339,6 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             const float now = up ? top : ref;
             float factor = up ? ex2(0.5f * (ref - now)) : 1.f;  // the square root of O's: that may be below 2^-126
             if (ref == -INFINITY) factor = 0.f;  // (an infinite score as the first reference)
-            float v_factor = 1.f;
-            bool change = up;
-            if (F16) {  // the same in all threads
-                const float v_max = fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w));
-                if (v_max > 2.f * v_ref) {
-                    const int e = min(max(int(__float_as_uint(v_max) >> 23), 1), 253);
-                    const float next = __uint_as_float(unsigned(e) << 23);
-                    if (v_ref > 0.f) v_factor = v_ref / next;
-                    v_ref = next;
-                    v_inv = __uint_as_float(unsigned(254 - e) << 23);
-                    change = true;
-                }
-            }
             ref = now;
             sum = sum * factor * factor;
             if (i > 0) {  // the product of the last tile has read the weights and written O
@@ -1362,7 +1346,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 if (!ok) break;
                 tc_fence_after();
                 const bool out = F32 && i % C::flush == 0;  // O moves to the total: the next product starts anew
-                if ((out || __any_sync(0xffffffffu, change)) && busy) {
+                if ((out || __any_sync(0xffffffffu, up)) && busy) {
 #pragma unroll 1
                     for (int x = 0; x < HD; x += 16) {
                         int o[16];
@@ -1379,7 +1363,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                                 if (out) y += t;
                                 if (i > C::flush || out) tt[z * 128] = (out ? y : t) * factor * factor;
                             }
-                            n[z] = __float_as_uint(y * v_factor * factor * factor);
+                            n[z] = __float_as_uint(y * factor * factor);
                         }
                         if (!out) tmem_st(my + C::o_at + g * HD + x, n);
                     }
@@ -1387,7 +1371,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             }
             if (busy) {
                 const float base = (ref == -INFINITY ? 0.f : ref) - C::shift;
-                const float vr[4] = {F16 ? vs.x * v_inv : vs.x, F16 ? vs.y * v_inv : vs.y, F16 ? vs.z * v_inv : vs.z, F16 ? vs.w * v_inv : vs.w};
+                const float vr[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     float p[16];
@@ -1409,23 +1393,13 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                         unsigned o[8];
 #pragma unroll
                         for (int y = 0; y < 8; ++y) {
-                            if constexpr (!F16) {
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * y], p[2 * y + 1]);
-                                o[y] = reinterpret_cast<const unsigned&>(h);
-                                if (z + 1 < NP) {
-                                    const float2 left = f2_unpack(f2_add(f2_pack(p[2 * y], p[2 * y + 1]),
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * y], p[2 * y + 1]);
+                            o[y] = reinterpret_cast<const unsigned&>(h);
+                            if (z + 1 < NP) {
+                                const float2 left = f2_unpack(f2_add(f2_pack(p[2 * y], p[2 * y + 1]),
                                                                      f2_pack(-__uint_as_float(o[y] << 16), -__uint_as_float(o[y] & 0xffff0000u))));
-                                    p[2 * y] = left.x;
-                                    p[2 * y + 1] = left.y;
-                                }
-                            } else {
-                                const __half2 h = __floats2half2_rn(p[2 * y], p[2 * y + 1]);
-                                o[y] = reinterpret_cast<const unsigned&>(h);
-                                if (z + 1 < NP) {
-                                    const float2 b = __half22float2(h), left = f2_unpack(f2_add(f2_pack(p[2 * y], p[2 * y + 1]), f2_pack(-b.x, -b.y)));
-                                    p[2 * y] = left.x;
-                                    p[2 * y + 1] = left.y;
-                                }
+                                p[2 * y] = left.x;
+                                p[2 * y + 1] = left.y;
                             }
                         }
                         tmem_st(my + C::p_at + g * C::p_cols + z * (C::keys / 2) + b * 8, o);
@@ -1442,7 +1416,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
         const bool none = sum == 0.f && ref == -INFINITY;
         const size_t row = size_t(w.t0 + qi) * a.n_heads + qh;
         const bool direct = plan.splits == 1;
-        const float factor = (F16 ? v_ref : 1.f) * (direct ? none ? 0.f : 1.f / sum : 1.f);
+        const float factor = direct ? none ? 0.f : 1.f / sum : 1.f;
         if (ok && busy) {
             // 32 rows x 32 dims at a time through shared memory (the queries are no longer read), so that rows leave whole
             float* turn = reinterpret_cast<float*>(smem + g * QP * C::q_bytes) + (warp & 3) * 1024;

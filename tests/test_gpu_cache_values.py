@@ -1,0 +1,37 @@
+"""Attention over the paged 8-bit KV cache where values, scales or queries are unusual: scales of either sign and of very different
+size, values and queries that are not finite.  Bounds as in test_gpu_kv_cache.py."""
+import pytest
+
+from test_gpu_kv_cache import TYPES, check_attention, ints, make, queries
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_row_does_not_depend_on_values_it_cannot_see(qb, name, hd):
+    """The last block's V, far larger than the others', is seen by the last queries alone: the rows before it keep their bits."""
+    c = make(qb, [320, 1000], 2, hd, 64, seed=43)
+    q, seqs, starts = queries(250, 4, hd, name), ints([0, 1]), ints([0, 200, 250])
+    c.scales[..., 1, :, :] = torch.where(c.scales[..., 1, :, :] > 0, 2.0 ** -12, c.scales[..., 1, :, :])
+    good = c.attention(0, q, seqs, starts, 200, 1000)
+    for s, n in ((0, 320), (1, 1000)):
+        c.scales[c.table[s, (n - 1) // 64].long(), 0, 1, :, (n - 1) % 64 // 16] = 2.0 ** 9
+    out = c.attention(0, q, seqs, starts, 200, 1000)
+    c.check()
+    assert torch.equal(out[:184], good[:184]) and torch.equal(out[200:242], good[200:242])
+    assert not torch.equal(out, good)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m", [1, 2, 60])
+def test_large_values_of_keys_without_weight(qb, name, m):
+    """The first block's V is 2^21 times the others', but its keys lie far behind in every score."""
+    c = make(qb, [700], 1, 64, 64, seed=44)
+    v = c.scales[:, 0, 1]
+    v.copy_(torch.where(v > 0, 2.0 ** -12, v))
+    p = c.table[0, 0].long()
+    c.scales[p, 0, 1, 0, 0], c.scales[p, 0, 0, 0, 0] = 2.0 ** 9, 1.0
+    c.codes[p, 0, 0, 0].view(4, 64, 16)[:, :16] = -127  # K of positions 0 .. 15
+    check_attention(c, 0, queries(m, 8, 64, name).abs(), [0], [m], name=name)
