@@ -1263,11 +1263,11 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                             f[z] = to_f(x[y][z]);
                             amax = fmaxf(amax, fabsf(f[z]));
                         }
-                        // a power of two brings the row's largest value to [1, 2); 255: not finite, left as it is
+                        // a power of two brings the row's largest value to [1, 2); 255: not finite, its scores are NaN
                         const int e = int(__float_as_uint(warp_max_redux(amax)) >> 23);
                         const int up = e == 255 ? 127 : min(max(254 - e, 1), 253);  // its biased exponent
                         const float pre = __uint_as_float(unsigned(up) << 23) * sign;
-                        if (lane == r8 + y) fac *= __uint_as_float(unsigned(254 - up) << 23);
+                        if (lane == r8 + y) fac *= e == 255 ? __int_as_float(0x7fffffff) : __uint_as_float(unsigned(254 - up) << 23);
 #pragma unroll
                         for (int z = 0; z < E; ++z) f[z] *= pre;
                         const int row = (warp & 3) * 32 + r8 + y;

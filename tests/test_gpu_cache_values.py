@@ -35,3 +35,22 @@ def test_large_values_of_keys_without_weight(qb, name, m):
     c.scales[p, 0, 1, 0, 0], c.scales[p, 0, 0, 0, 0] = 2.0 ** 9, 1.0
     c.codes[p, 0, 0, 0].view(4, 64, 16)[:, :16] = -127  # K of positions 0 .. 15
     check_attention(c, 0, queries(m, 8, 64, name).abs(), [0], [m], name=name)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m", [1, 30])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_an_infinite_query_is_nan_whatever_its_scores(qb, name, m, sign):
+    """All scores -inf (or +inf): the softmax of them is no number, as with scores of both signs."""
+    c = make(qb, [300], 2, 64, 64, seed=45)
+    c.codes[:, :, 0] = -5  # K
+    q = queries(m, 6, 64, name).abs() + 0.1
+    good = c.attention(0, q, ints([0]), ints([0, m]), m, 300)
+    q2 = q.clone()
+    q2[0, 2, 7] = sign * float("inf")
+    out = c.attention(0, q2, ints([0]), ints([0, m]), m, 300)
+    c.check()
+    assert out[0, 2].isnan().all()
+    keep = torch.ones(m, 6, dtype=torch.bool, device="cuda")
+    keep[0, 2] = False
+    assert torch.equal(out[keep], good[keep])
