@@ -1052,7 +1052,10 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
     unsigned char* kb = smem + WG * QP * C::q_bytes;   // 2 buffers
     unsigned char* vb = kb + 2 * C::kv_bytes;          // 2 buffers
     unsigned char* codes = vb + 2 * C::kv_bytes;       // of the next tile: K's pieces, V's pieces, 16 bytes each, by thread
-    __shared__ uint64_t q_full[WG], k_full[2], v_full[2], k_free[2], v_free[2], s_full[WG], s_free[WG], p_full[WG], o_done[WG], fin;
+    // A wait on a phase's parity must come before the phase after it ends.  The softmax warps wait on scales_full, which comes
+    // round every 4 tiles (converted at most 2 ahead of the weights), and not on k_full: K of tile i + 2 may be there as soon as
+    // the scores of tile i are, however late a softmax warp is to look.
+    __shared__ uint64_t q_full[WG], k_full[2], v_full[2], k_free[2], v_free[2], scales_full[4], s_full[WG], s_free[WG], p_full[WG], o_done[WG], fin;
     __shared__ __align__(16) float scales[4][8];       // of a tile's 4 blocks: K's, V's
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag;
@@ -1086,6 +1089,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             mbar_init(&k_free[b], 1);
             mbar_init(&v_free[b], 1);
         }
+        for (int b = 0; b < 4; ++b) mbar_init(&scales_full[b], 4);
         mbar_init(&fin, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1213,6 +1217,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             if (ct < 4) {  // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
                 scales[i & 3][ct] = !scaled ? 0.f : fabsf(vs) < INFINITY ? ks : __int_as_float(0x7fffffff);
                 scales[i & 3][4 + ct] = scaled && fabsf(vs) < INFINITY ? vs : 0.f;
+                mbar_arrive(&scales_full[i & 3]);
             }
             if (i + 1 < nt) copy(i + 1);
             look(i + 2);
@@ -1300,7 +1305,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
 #pragma unroll 1
         for (int i = 0; i < nt && ok; ++i) {
             const int key0 = key_base + i * C::keys;
-            ok = wait_warp(&k_full[i & 1], (i >> 1) & 1, ab) && wait_warp(&s_full[g], i & 1, ab);
+            ok = wait_warp(&scales_full[i & 3], (i >> 2) & 1, ab) && wait_warp(&s_full[g], i & 1, ab);
             if (!ok) break;
             tc_fence_after();
             const float4 ks = *reinterpret_cast<const float4*>(scales[i & 3]), vs = *reinterpret_cast<const float4*>(scales[i & 3] + 4);
