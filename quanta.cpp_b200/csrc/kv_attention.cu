@@ -1317,15 +1317,17 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             tmem_ready(s1);
             tc_fence_before();
             mbar_arrive(&s_free[g]);
-            float f[4] = {ks.x * fac, ks.y * fac, ks.z * fac, ks.w * fac};  // none below 0
+            float f[4] = {ks.x * fac, ks.y * fac, ks.z * fac, ks.w * fac};
             float s[64];  // scores less the factor f of their 16 keys
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
                 s[k] = __int_as_float(s0[k]);
                 s[k + 32] = __int_as_float(s1[k]);
             }
-            // do all of the warp's rows see the whole tile?  (rows past the end do as they like)
-            const bool whole = key0 + C::keys - 1 <= pos && (!a.window || key0 > pos - a.window);
+            // do all of the warp's rows see the whole tile, and is no factor below 0 (none that an append makes), so that the
+            // maximum may be taken before it?  (rows past the end do as they like)
+            const bool whole = key0 + C::keys - 1 <= pos && (!a.window || key0 > pos - a.window) &&
+                               fminf(fminf(ks.x, ks.y), fminf(ks.z, ks.w)) >= 0.f;
             if (!__all_sync(0xffffffffu, whole)) {
                 const int last = pos - key0, first = a.window ? last - a.window + 1 : -1;
 #pragma unroll

@@ -2,7 +2,7 @@
 size, values and queries that are not finite.  Bounds as in test_gpu_kv_cache.py."""
 import pytest
 
-from test_gpu_kv_cache import TYPES, check_attention, ints, make, queries
+from test_gpu_kv_cache import SMALL, TYPES, check_attention, ints, make, queries
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -54,3 +54,24 @@ def test_an_infinite_query_is_nan_whatever_its_scores(qb, name, m, sign):
     keep = torch.ones(m, 6, dtype=torch.bool, device="cuda")
     keep[0, 2] = False
     assert torch.equal(out[keep], good[keep])
+
+
+# lengths and queries of each sequence: single tokens in a CTA each, dealt out and joined by a warp and by a CTA a row; chunks whole and in stretches
+SHAPES = {"few": ([200, 150, 90], [1, 1, 1]), "dealt": ([1500] * 20, [1] * 20), "long": ([9000], [1]), "chunk": ([200, 150, 300], [40, 150, 30]),
+          "stretches": ([3000], [60])}
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("which, std", [("some", 1.5), ("some", 40.0), ("all", 1.5), ("all", 40.0)])
+def test_scales_of_either_sign(qb, monkeypatch, shape, name, which, std):
+    """value = code * scale whatever the scale's sign; also with scores far apart (results below 2^-126 may then read 0: where all
+    keys but those with weights of 1e-60 have a 0 for V)."""
+    monkeypatch.setitem(SMALL, name, SMALL[name] + 2.0 ** -126)
+    lens, news = SHAPES[shape]
+    c = make(qb, lens, 2, 64, 64, seed=41)
+    g = torch.Generator(device="cuda").manual_seed(42)
+    flip = torch.rand(c.scales.shape, generator=g, device="cuda") < (0.4 if which == "some" else 2.0)
+    c.scales.copy_(torch.where(flip, -c.scales, c.scales))
+    check_attention(c, 0, queries(sum(news), 6, 64, name, std=std), list(range(len(lens))), news, name=name)
+    check_attention(c, 0, queries(sum(news), 6, 64, name, std=std), list(range(len(lens))), news, name=name, window=77)
