@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
     __shared__ __align__(16) float tile_max[4][RM];
     __shared__ __align__(16) float fac[2][RM], first_ref[2][RM], last_ref[RM], sum_part[4][RM];
     __shared__ int row_off[2][RM];  // a row's place in out and lse, from its unit's first
+    __shared__ unsigned nan_rows[2];  // by unit: rows that see a V scale which is not finite
     __shared__ int2 scan_part[4];
     __shared__ int start_j, start_head, start_tile, start_at, tiles_from, tiles_to;
     const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
         mbar_init(&q_ready, 128);
         mbar_init(&fin, 1);
         abort_flag = 0;
+        nan_rows[0] = nan_rows[1] = 0;
         tiles_from = tiles_to = 0;
         if (plan.even) plan.info[blockIdx.x] = make_int4(-1, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -590,10 +592,8 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
                     }
                 }
                 ok = wait_warp(&k_full[i % C::stages], (i / C::stages) & 1, ab) && ok;
-                const float ks0 = scales[i & 3][kid >> 4], vs0 = scales[i & 3][8 + (kid >> 4)];
-                // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
-                vs = fabsf(vs0) < INFINITY ? vs0 : 0.f;
-                const float ks = fabsf(vs0) < INFINITY ? ks0 : __int_as_float(0x7fffffff);
+                const float ks = scales[i & 3][kid >> 4];
+                vs = scales[i & 3][8 + (kid >> 4)];
                 ok = wait_warp(&s_done[i & 1], (i >> 1) & 1, ab) && ok;
                 tc_fence_after();
                 int d2[RH], d1[RH], d0[RH];
@@ -662,6 +662,14 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
                             ++p;
                         }
                     }
+                }
+                // a V scale that is not finite stays out of the products (a weight of 0 would be NaN), and is noted for the rows that see it
+                if (!(fabsf(vs) < INFINITY)) {
+                    vs = 0.f;
+                    unsigned hit = 0;
+#pragma unroll
+                    for (int r = 0; r < RH; ++r) hit |= unsigned(s[r] != -INFINITY) << (r0 + r);
+                    if (hit) atomicOr(&nan_rows[units & 1], hit);
                 }
                 bool high = in_tmem == kFlush<T>;
                 const unsigned had = unset;
@@ -831,7 +839,8 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
                     const int rr = lane % RM;  // lane r of a warp looks after row r
                     const float l = (sum_part[0][rr] + sum_part[1][rr]) + (sum_part[2][rr] + sum_part[3][rr]);
                     const bool none = (unset >> rr & 1) && l == 0.f;
-                    const float inv = u.cut ? 1.f : none ? 0.f : __fdividef(1.f, l);
+                    const float inv = nan_rows[units & 1] >> rr & 1 ? __int_as_float(0x7fffffff)
+                                      : u.cut ? 1.f : none ? 0.f : __fdividef(1.f, l);
                     if (tid < rows) {
                         if (u.cut) reinterpret_cast<float2*>(plan.ml)[slot + tid] = make_float2(none ? -INFINITY : last_ref[tid], l);
                         else if (a.lse) a.lse[row0 + off[tid]] = none ? -INFINITY : (last_ref[tid] + __log2f(l)) * (1.f / kLog2e);
@@ -849,6 +858,7 @@ __global__ void __launch_bounds__(Dec<HD, RM, T>::threads, Dec<HD, RM, T>::ctas)
                     if (tid == 0 && u.first && u.cut)  // the unit's first CTA says which CTAs share it
                         plan.info[blockIdx.x] = make_int4(u.owner, u.t0, u.m, u.head);
                     if (bar_any<C::soft>(!ok)) break;  // last_ref and sum_part are read before the next unit writes them
+                    if (tid == 0) nan_rows[units & 1] = 0;  // (for the unit after the next)
                 }
             }
             if (!C::v_warps && i + 1 < n_my) copy_v(i + 1);
@@ -1214,9 +1224,9 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
                 kc[x] = reinterpret_cast<const uint4*>(codes)[x * 128 + ct];
                 vc[x] = reinterpret_cast<const uint4*>(codes)[(pieces + x) * 128 + ct];
             }
-            if (ct < 4) {  // a scale that is not finite makes the scores NaN of the rows that see it, and stays out of the products
-                scales[i & 3][ct] = !scaled ? 0.f : fabsf(vs) < INFINITY ? ks : __int_as_float(0x7fffffff);
-                scales[i & 3][4 + ct] = scaled && fabsf(vs) < INFINITY ? vs : 0.f;
+            if (ct < 4) {
+                scales[i & 3][ct] = scaled ? ks : 0.f;
+                scales[i & 3][4 + ct] = scaled ? vs : 0.f;
                 mbar_arrive(&scales_full[i & 3]);
             }
             if (i + 1 < nt) copy(i + 1);
@@ -1301,7 +1311,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
         }
         float* total = reinterpret_cast<float*>(smem + C::total_at) + g * HD * 128 + rt;  // (float32) [dim][row]
         float ref = -INFINITY, sum = 0.f;
-        bool ok = true;
+        bool ok = true, sees_nan = false;
 #pragma unroll 1
         for (int i = 0; i < nt && ok; ++i) {
             const int key0 = key_base + i * C::keys;
@@ -1309,6 +1319,17 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             if (!ok) break;
             tc_fence_after();
             const float4 ks = *reinterpret_cast<const float4*>(scales[i & 3]), vs = *reinterpret_cast<const float4*>(scales[i & 3] + 4);
+            float vr[4] = {vs.x, vs.y, vs.z, vs.w};
+            if (!(fabsf((vs.x + vs.y) + (vs.z + vs.w)) < INFINITY)) {
+                // a V scale that is not finite stays out of the products (a weight of 0 would be NaN); rows that see it are NaN
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (!(fabsf(vr[b]) < INFINITY)) {
+                        const int k = key0 + b * kKvBlock;
+                        sees_nan = sees_nan || (k <= pos && (!a.window || k + kKvBlock - 1 > pos - a.window));
+                        vr[b] = 0.f;
+                    }
+            }
             int s0[32], s1[32];
             tmem_ld(my + C::s_at + g * 64, s0);
             tmem_ld(my + C::s_at + g * 64 + 32, s1);
@@ -1378,7 +1399,6 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
             }
             if (busy) {
                 const float base = (ref == -INFINITY ? 0.f : ref) - C::shift;
-                const float vr[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     float p[16];
@@ -1423,7 +1443,7 @@ __global__ void __launch_bounds__(Chunk<HD, T, WG>::threads, Chunk<HD, T, WG>::c
         const bool none = sum == 0.f && ref == -INFINITY;
         const size_t row = size_t(w.t0 + qi) * a.n_heads + qh;
         const bool direct = plan.splits == 1;
-        const float factor = direct ? none ? 0.f : 1.f / sum : 1.f;
+        const float factor = sees_nan ? __int_as_float(0x7fffffff) : direct ? none ? 0.f : 1.f / sum : 1.f;
         if (ok && busy) {
             // 32 rows x 32 dims at a time through shared memory (the queries are no longer read), so that rows leave whole
             float* turn = reinterpret_cast<float*>(smem + g * QP * C::q_bytes) + (warp & 3) * 1024;

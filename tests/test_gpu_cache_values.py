@@ -75,3 +75,26 @@ def test_scales_of_either_sign(qb, monkeypatch, shape, name, which, std):
     c.scales.copy_(torch.where(flip, -c.scales, c.scales))
     check_attention(c, 0, queries(sum(news), 6, 64, name, std=std), list(range(len(lens))), news, name=name)
     check_attention(c, 0, queries(sum(news), 6, 64, name, std=std), list(range(len(lens))), news, name=name, window=77)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_lse_does_not_depend_on_values(qb, shape, name, bad):
+    """A V scale that is not finite: NaN for the queries that see it, whose lse (of scores alone) stays what it was."""
+    lens, news = SHAPES[shape]
+    c = make(qb, lens, 2, 64, 64, seed=40)
+    q, starts = queries(sum(news), 6, 64, name), [0]
+    for m in news:
+        starts.append(starts[-1] + m)
+    args = (0, q, ints(range(len(lens))), ints(starts), max(news), max(lens))
+    good, gl = c.attention(*args, lse=True)
+    at, pos = len(lens) - 1, lens[-1] - 20  # head 1 of the last sequence, the block of this position
+    c.scales[c.table[at, pos // 64].long(), 0, 1, 1, pos % 64 // 16] = bad
+    out, lse = c.attention(*args, lse=True)
+    c.check()
+    assert torch.equal(lse, gl)
+    hit = torch.zeros(sum(news), 6, dtype=torch.bool, device="cuda")
+    first = starts[-2] + max(0, pos // 16 * 16 - (lens[-1] - news[-1]))  # the first query that sees the block
+    hit[first:, 3:] = True
+    assert out[hit].isnan().all() and torch.equal(out[~hit], good[~hit])
