@@ -291,8 +291,10 @@ int qnt_sampler_sample_noalloc(const qnt_sampler_params* sp, uint64_t* rng_state
  *   refs    [n_pages]: how many sequences use the page (0: free)
  *   table   [max_seqs][max_pages]: the page of positions k * page_tokens .. of a sequence, -1 past its pages
  *   lens    [max_seqs]: positions of the sequence; it holds ceil(len / page_tokens) pages
+ *           (refs, table and lens change through the calls below: a length lowered by hand would lose its pages)
  *   status  one word of error bits that kernels set (qnt_kv_check reports and clears them)
- * An empty cache: refs and lens 0, table -1, status 0; codes and scales need no initial values.
+ * An empty cache: refs and lens 0, table -1, status 0; codes and scales need no initial values.  An append makes scales of 0 and
+ * above; the caller may write scales of either sign.
  * Limits: head_dim 64 or 128; page_tokens 16, 32, 64 or 128; n_pages <= 1048576; max_seqs <= 8192.
  *
  * Every call queues its work on `stream` (a cudaStream_t, NULL = legacy default) and returns.  All pointers are device
@@ -343,7 +345,10 @@ int qnt_kv_copy(const qnt_kv_cache* cache, const int* src, const int* dst, int n
  *                     n_kv_heads).  q: token t, head h, dim d at t * q_stride + h * head_dim + d; out [n_tok][n_heads]
  *                     [head_dim] of the same dtype, 16-byte aligned; lse (may be NULL) [n_tok][n_heads] f32: log of the
  *                     sum of exp(score).  A query that sees nothing gets out 0 and lse -inf.  max_q bounds m; max_len
- *                     bounds lens (a longer sequence is still read whole, only less evenly spread).
+ *                     bounds lens (a longer sequence is still read whole, only less evenly spread).  lse is of the scores
+ *                     alone; a V scale that is not finite makes out NaN where it is seen, a query that is not finite
+ *                     makes out NaN.  (Weights carry up to 2^64 in f32: V below 2^40 in magnitude cannot overflow on the
+ *                     way.)
  *                     workspace: qnt_kv_attention_workspace bytes for the same counts, 16-byte aligned, contents
  *                     irrelevant. */
 int qnt_kv_append(const qnt_kv_cache* cache, int layer, const void* k, const void* v, int dtype, long long k_stride,

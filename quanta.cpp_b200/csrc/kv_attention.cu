@@ -46,8 +46,8 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 // Bound by: instructions and their latency.  The codes are read once, at HBM's rate a tile would take 0.35 us of an SM (HD 64),
 // and the MMAs are short; but a tile's codes, scores and weights pass through about 3800 warp instructions (HD 128, 4 rows; a
 // quarter of them turn V codes into bf16), issued at 43 to 60 % of the SM's rate.  Measured (HBM figures of the codes and scales):
-//   192 sequences up to 8191, bf16, 4 rows of 128:  115 us, 3.2 TB/s (the V codes in 8 softmax warps: 123, in 4: 141)
-//   1 sequence of 131071, f16, 7 rows of 64:         25.5 us with the join
+//   192 sequences up to 8191, bf16, 4 rows of 128:  115 us, 3.1 TB/s (the V codes in 8 softmax warps: 123, in 4: 141)
+//   1 sequence of 131071, f16, 7 rows of 64:         25.3 us with the join
 //   256 sequences of 640, f32, 7 rows of 64:         32.8 us (V warps beside 4 softmax warps of 8 rows, which spill: 47)
 //   1 sequence of 130, f32:                         10.2 us, start (4 us), two tiles and the outputs one after the other
 constexpr int kTileKeys = 128;
@@ -1002,9 +1002,10 @@ __global__ void __launch_bounds__(MANY ? kJoinMany : kJoinFew) k_kv_join(KvAttnA
 // Bound by: the softmax's chain per tile (S out of TMEM, maximum, exp, pieces, weights into TMEM: about 3000 cycles for a CTA
 // alone) and, with two CTAs to an SM, instructions: about 4200 warp instructions per 128 x 64 scores, half of the issue rate; the
 // tensor cores are busy a quarter of the time at most.  Measured:
-//   8 prompts of 2048, 32/8 heads of 128:  f16 622 us, bf16 602 us (442 and 457 TFLOP/s of what causal rows need)
-//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 98 to 115 us with the lengths drawn
-//   1 prompt of 512, f32, 14/2 heads of 64: 18.4 us with the join, 112 CTAs of up to 4 tiles
+//   8 prompts of 2048, 32/8 heads of 128:  f16 607 us, bf16 609 us (453 and 451 TFLOP/s of what causal rows need)
+//   6 sequences up to 8191 with 5 .. 509 queries, f16, 32/8 heads of 128, window 4096: 89 to 121 us with the sequences' order
+//     (every row tile has the same number of stretches, whatever its keys)
+//   1 prompt of 512, f32, 14/2 heads of 64: 18.4 to 19.1 us with the join, 112 CTAs of up to 4 tiles
 template <int HD, class T, int WG>  // WG row groups of 128 (two of HD 128 and float32 pass TMEM)
 struct Chunk {
     static constexpr bool F32 = sizeof(T) == 4;
@@ -1540,7 +1541,7 @@ __global__ void __launch_bounds__(256) k_kv_chunk_join(KvAttnArgs a, ChunkPlan p
 
 constexpr int kDecRows = 16;  // most query rows (queries x heads of a kv head) of k_kv_decode
 
-// (256 x 640 f32, 14 rows of 64: 45.9 us against k_kv_chunk's 96.5; 64 x 4000 bf16, 16 rows of 128: 200 against 337.)
+// (256 x 640 f32, 14 rows of 64: 46 us against k_kv_chunk's 103; 64 x 4000 bf16, 16 rows of 128: 200 against 336.)
 bool takes_decode(const KvAttnArgs& a) { return (long long)a.max_q * a.group <= kDecRows; }
 
 int dec_rm(const KvAttnArgs& a) {
@@ -1594,9 +1595,9 @@ struct ChunkLaunch {
 };
 
 // Row groups of 128 per CTA and stretches of keys per row tile.  Two groups share the conversion of K and V, but leave half as
-// many CTAs: taken where those fill the SMs (8 prompts of 2048, f16, 8 kv heads of 128: 622 us, one group 708; 16 of 512, f32,
-// 2 of 64: 85, 113; a single one, f16: 27.6, one group 25.6).  Stretches: as many as fill the SMs twice, of at least 4 key tiles
-// (a prompt of 512, 2 kv heads of 64: f32 23.5 us, of at least 8 tiles 26.6; f16 23.6, 25.6).
+// many CTAs: taken where those fill the SMs (8 prompts of 2048, f16, 8 kv heads of 128: 607 us, one group 674; 16 of 512, f32,
+// 2 of 64: 88, 117; a single one, f32: 23.5 with one group, 27.6 with two).  Stretches: as many as fill the SMs twice, of at least
+// 4 key tiles (a prompt of 512, 2 kv heads of 64: f32 23.5 us, of at least 8 tiles 27.4; f16 23.6, 24.6).
 ChunkLaunch chunk_launch(const KvView& c, const KvAttnArgs& a, const KvCall& call) {
     ChunkLaunch l;
     const long long rows = (long long)call.n_tok * a.group;
