@@ -361,9 +361,10 @@ def _plain_reorder(s, case):
     i = torch.arange(n, device="cuda")
     parent = i - i % b + parents  # its place in the list
     rows, lens, old = s["table"][seqs][parent], s["lens"][seqs].long()[parent], s["table"][seqs]
-    # the first of a parent's children takes over its part-filled page, the others get copies
+    # one child takes over its parent's part-filled page (the parent itself if it goes on, else the first), the others get copies
     first = torch.full((n,), n, device="cuda").scatter_reduce_(0, parent, i, "amin")
-    copy = ((lens % pt > 0) & (first[parent] != i)).nonzero()[:, 0]
+    heir = torch.where(parent == i, i, first)
+    copy = ((lens % pt > 0) & (heir[parent] != i)).nonzero()[:, 0]
     at = lens // pt
     src = rows[copy, at[copy]].long()
     rows[copy, at[copy]] = -1
