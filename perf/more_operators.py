@@ -10,6 +10,7 @@ operand of the quantized matrix products.  The cache (reorder cases): codes int8
 `own` false: the plain forms, elementary torch operations in 32 bits (angles and candidates' scores in 64: far positions and
 candidates next to each other need them).  `own` true: quanta.cpp_b200's operators.
 """
+import functools
 import math
 import sys
 from pathlib import Path
@@ -261,6 +262,7 @@ def _cache_inputs(case, gen):
     return s
 
 
+@functools.cache
 def _package():
     at = str(Path(__file__).resolve().parent.parent / "quanta.cpp_b200")
     if at not in sys.path:
