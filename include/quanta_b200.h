@@ -29,7 +29,7 @@ extern "C" {
 #define QNT_F16 1
 #define QNT_Q8_0 2
 #define QNT_Q4_0 3
-/* activations only (the qnt_kv_* entries); no .qnt tensor has this type */
+/* activations only (the qnt_kv_*, norm, rope and beam entries); no .qnt tensor has this type */
 #define QNT_BF16 4
 
 const char* qnt_last_error(void);
@@ -76,6 +76,48 @@ int qnt_quantize_q8_host(const float* x, int n, int8_t* q, float* d);
 int qnt_matvec_host(const qnt_dtensor* W, const int8_t* qx, const float* dx, int r0, int r1, float* out);
 int qnt_matmul_host(const qnt_dtensor* W, const int8_t* qx, const float* dx, int n, int r0, int r1, float* out, int ldo,
                     int impl);
+
+/* ---------------------------------------------------------------- around a decoder layer's products
+ *
+ * For models that a caller composes of the operators of this file: the engine's own layers fuse the reference's forms of these
+ * (engine/src/ops_ref.cpp:69-83, 194-199), whose sums are in element order, bit for bit.  Device pointers; work is queued on `stream` (a
+ * cudaStream_t, NULL = legacy default); nothing is allocated, so the calls can be captured into a graph. */
+
+/* RMS norm with the residual's addition, 8-bit rows out (the operand of qnt_matvec / qnt_matmul):
+ *   h = x + residual (f32; residual := h, rounded to its type; NULL: h = x),  y = h / sqrt(mean h^2 + eps) * weight,
+ *   per 32 values: d = max |y| / 127,  q = y / d to the nearest integer, halves away from zero.
+ * x [n_tok][n] at x_stride, of dtype QNT_F32, QNT_F16 or QNT_BF16; residual [n_tok][n] at residual_stride, of x's dtype or
+ * QNT_F32, not x itself; weight f32 [n]; q [n_tok][n] and d [n_tok][n / 32], 16-byte aligned; n a multiple of 32, at most 32768.
+ * Sums are in f32 (h below 10^18).  A value that is not finite makes its block read as NaN (its row, where h is not). */
+int qnt_rms_norm_q8(const void* x, int dtype, long long x_stride, void* residual, int residual_dtype, long long residual_stride,
+                    const float* weight, float eps, int n_tok, int n, int8_t* q, float* d, void* stream);
+
+/* The values q * d of 8-bit rows (the inverse of qnt_quantize_q8 and qnt_rms_norm_q8): out [n_tok][n] of dtype, 16-byte aligned
+ * like q; one rounding of the f32 product. */
+int qnt_dequantize_q8(const int8_t* q, const float* d, int n_tok, int n, void* out, int dtype, void* stream);
+
+/* Rotary positions of query and key heads (either may be NULL with 0 heads): pair i of a head's first rotary_dim dims, (i, i +
+ * rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), turns by positions[t] * turns[i] revolutions and is multiplied by `scale`; the
+ * dims behind are copied.  Token t, head h, dim i at t * stride + h * head_dim + i (elements) of dtype QNT_F32, QNT_F16 or QNT_BF16; an
+ * output may be its input (with one stride), and must not overlap it otherwise.  turns: f64 [rotary_dim / 2] = frequency / (2 pi),
+ * with whatever scaling for long contexts; the revolution count is formed in f64, so that far positions keep their angles.
+ * positions int32 [n_tok], of any sign.  head_dim even, at most 1024. */
+int qnt_rope(const void* q, long long q_stride, void* q_out, long long q_out_stride, int n_heads, const void* k, long long k_stride,
+             void* k_out, long long k_out_stride, int n_kv_heads, int dtype, int head_dim, int rotary_dim, int interleaved,
+             const double* turns, float scale, const int* positions, int n_tok, void* stream);
+
+/* The selection of a beam search's next step: of each group's candidates (b, t), beam b < beams and token t < vocab,
+ *     s(b, t) = scores[group][b] + logit(b, t) - log sum_u exp(logit(b, u))
+ * the k best: out_scores, tokens and parents (the beams) [groups][k], best first, equal ones by the lowest b * vocab + t.
+ * logits: row group * beams + b at that times stride (elements), of dtype QNT_F32, QNT_F16 or QNT_BF16.  ended (may be NULL)
+ * [groups][beams]: such a beam has one candidate, its own score with token end_id.  Candidates that are -inf or no numbers (a
+ * forbidden token, a row with NaN or +inf, a score that is not finite) come behind all others, with score -inf, in order of their
+ * places.  Scores are formed and compared in f64.  k <= 64, beams <= 1024, beams * vocab < 2^31.
+ * workspace: qnt_beam_workspace bytes, 16-byte aligned, contents irrelevant. */
+size_t qnt_beam_workspace(int groups, int beams, int vocab, int k);
+int qnt_beam_select(const void* logits, int dtype, long long stride, const float* scores, const uint8_t* ended, int end_id,
+                    int groups, int beams, int vocab, int k, float* out_scores, int* tokens, int* parents, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- model level (engine/src/model.h) */
 
@@ -317,6 +359,11 @@ typedef struct qnt_kv_cache {
  *   qnt_kv_fork     sequence dst[i] (empty) becomes a copy of src[i]: full pages are shared (refs + 1), a part-filled last
  *                   page is copied in every layer, so that both can go on; distinct dst, none of them also a src
  *   qnt_kv_free     the sequences give back their pages (refs - 1) and become empty (distinct sequences)
+ *   qnt_kv_reorder  sequence seqs[i] becomes what sequence seqs[i - i % group + parents[i]] was before the call (n distinct
+ *                   sequences in whole groups; 0 <= parents[i] < group): a beam search's step.  Full pages are shared; a
+ *                   part-filled last page goes to one child (the parent itself if it goes on, else the first), the others
+ *                   get copies of its filled blocks of 16 positions, in every layer; pages that nothing uses any more
+ *                   are given back, to this call's copies first.  Its workspace: qnt_kv_reorder_workspace bytes.
  *   qnt_kv_compact  the n pages in use move to indices 0 .. n - 1 (only those at or past n move); table and refs follow
  *   qnt_kv_copy     page src[i]'s codes and scales, all layers, over page dst[i]'s (no dst twice, none also a src)
  * workspace: qnt_kv_page_workspace bytes, 16-byte aligned, contents irrelevant. */
@@ -325,6 +372,9 @@ int qnt_kv_reserve(const qnt_kv_cache* cache, const int* seqs, const int* extra,
                    void* stream);
 int qnt_kv_fork(const qnt_kv_cache* cache, const int* src, const int* dst, int n, void* workspace, size_t workspace_bytes,
                 void* stream);
+size_t qnt_kv_reorder_workspace(const qnt_kv_cache* cache);
+int qnt_kv_reorder(const qnt_kv_cache* cache, const int* seqs, const int* parents, int n, int group, void* workspace,
+                   size_t workspace_bytes, void* stream);
 int qnt_kv_free(const qnt_kv_cache* cache, const int* seqs, int n, void* stream);
 int qnt_kv_compact(const qnt_kv_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
 int qnt_kv_copy(const qnt_kv_cache* cache, const int* src, const int* dst, int n, void* stream);

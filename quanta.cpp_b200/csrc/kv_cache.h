@@ -60,6 +60,9 @@ cudaError_t launch_kv_read(const KvView& c, int layer, const int* first, const K
 size_t kv_page_ws_bytes(const KvView& c);
 cudaError_t launch_kv_reserve(const KvView& c, const int* seqs, const int* extra, int n, void* ws, cudaStream_t st);
 cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int n, void* ws, cudaStream_t st);
+// Sequence seqs[i] becomes what seqs[i - i % group + parents[i]] was (kv_reorder_ws_bytes(c) bytes of ws).
+size_t kv_reorder_ws_bytes(const KvView& c);
+cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* parents, int n, int group, void* ws, cudaStream_t st);
 cudaError_t launch_kv_free(const KvView& c, const int* seqs, int n, cudaStream_t st);
 cudaError_t launch_kv_compact(const KvView& c, void* ws, cudaStream_t st);
 cudaError_t launch_kv_copy(const KvView& c, const int* src, const int* dst, int n, cudaStream_t st);

@@ -206,6 +206,22 @@ int qnt_kv_fork(const qnt_kv_cache* cache, const int* src, const int* dst, int n
     return done(qb::launch_kv_fork(c, src, dst, n, workspace, stream_of(stream)), "kv fork");
 }
 
+size_t qnt_kv_reorder_workspace(const qnt_kv_cache* cache) {
+    qb::KvView c;
+    return make_view(cache, &c) ? 0 : qb::kv_reorder_ws_bytes(c);
+}
+
+int qnt_kv_reorder(const qnt_kv_cache* cache, const int* seqs, const int* parents, int n, int group, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    qb::KvView c;
+    if (int r = make_view(cache, &c)) return r;
+    if (int r = check_list(c, seqs, parents, n)) return r;
+    if (n > 0 && (group <= 0 || n % group)) return set_err(QNT_ERR_INVALID, "kv reorder: the list must be whole groups");
+    if (n == 0) return QNT_OK;
+    if (int r = check_ws(workspace, workspace_bytes, qb::kv_reorder_ws_bytes(c))) return r;
+    return done(qb::launch_kv_reorder(c, seqs, parents, n, group, workspace, stream_of(stream)), "kv reorder");
+}
+
 int qnt_kv_free(const qnt_kv_cache* cache, const int* seqs, int n, void* stream) {
     qb::KvView c;
     if (int r = make_view(cache, &c)) return r;

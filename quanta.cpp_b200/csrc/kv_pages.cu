@@ -491,6 +491,156 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
     for (int i = i0; i < i1; ++i) fresh[i] = (c.lens[src[i]] & (c.pt - 1)) ? list[r++] : -1;
 }
 
+// Reorder, first half.  Sequence i of the list takes over what sequence parent(i) = i - i % group + parents[i] of it held before
+// the call.  Of a parent's children one is the heir of its part-filled page: the parent itself if it goes on, else the first;
+// the others get copies in fresh pages.  plan[0] = copies (-1: the call is refused), plan[1 + 3 r ..] = {from, to, blocks of 16
+// positions} of copy r.  rows, len: workspace for the list's new table rows and lengths, all read before one is written.  Pages that no
+// sequence uses any more are free for the copies of the same call.
+__global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, const int* __restrict__ seqs,
+                                                                  const int* __restrict__ parents, int n, int group,
+                                                                  int* __restrict__ plan, int* __restrict__ rows,
+                                                                  int* __restrict__ len, int* __restrict__ list) {
+    extern __shared__ __align__(16) unsigned smem[];
+    pdl_launch_dependents();
+    unsigned* words = smem;
+    int* mark = reinterpret_cast<int*>(words + plan_words(c));
+    int* heir = mark + c.max_seqs;  // of each place of the list: who gets its part-filled page
+    uint16_t* base = reinterpret_cast<uint16_t*>(heir + n);  // copies of entries 0 .. i (at most kKvMaxSeqs)
+    __shared__ int bad;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+    if (tid == 0) bad = 0;
+    for (int s = tid; s < c.max_seqs; s += blockDim.x) mark[s] = 0;
+    for (int i = tid; i < n; i += blockDim.x) heir[i] = INT_MAX;
+    __syncthreads();
+    auto parent = [&](int i) { return i - i % group + parents[i]; };
+    for (int i = tid; i < n; i += blockDim.x) {
+        const int s = seqs[i], p = parents[i];
+        if (s < 0 || s >= c.max_seqs || p < 0 || p >= group || atomicExch(mark + s, 1)) {
+            bad = int(ERR_BAD_POS);
+            continue;
+        }
+        const int l = c.lens[s];
+        if (l < 0 || l > c.max_pages << c.pt_shift) bad = int(ERR_BAD_POS);
+        const int j = parent(i);
+        atomicMin(heir + j, j == i ? -1 : i);  // (-1: itself)
+    }
+    __syncthreads();
+    const int per = (n + int(blockDim.x) - 1) / int(blockDim.x);
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    int want = 0;
+    if (!bad) {
+        int mine = 0;
+        for (int i = i0; i < i1; ++i) {
+            const int j = parent(i);
+            len[i] = c.lens[seqs[j]];
+            mine += (len[i] & (c.pt - 1)) && heir[j] != (j == i ? -1 : i);
+            base[i] = uint16_t(mine);
+        }
+        const int before = cta_scan(mine, &want);
+        for (int i = i0; i < i1; ++i) base[i] = uint16_t(base[i] + before);
+    }
+    __syncthreads();
+    if (bad) {
+        if (tid == 0) {
+            set_error(c.status, ERR_BAD_POS);
+            plan[0] = -1;
+        }
+        return;
+    }
+    // the pages that the rows lose and gain; sign -1 takes it back
+    auto count = [&](int sign) {
+        for (int i = warp; i < n; i += warps) {
+            const int j = parent(i);
+            const bool copy = base[i] != (i ? base[i - 1] : 0);
+            if (j == i && !copy) continue;
+            const int* old = c.table + size_t(seqs[i]) * c.max_pages;
+            const int* now = c.table + size_t(seqs[j]) * c.max_pages;
+            const int n_now = (len[i] + c.pt - 1) >> c.pt_shift, n_old = (c.lens[seqs[i]] + c.pt - 1) >> c.pt_shift;
+            for (int k = lane; k < max(n_old, n_now); k += 32) {
+                const int a = k < n_old ? old[k] : -1;
+                int b = k < n_now ? now[k] : -1;
+                if (sign > 0) rows[size_t(i) * c.max_pages + k] = b;
+                if (copy && k == n_now - 1) {
+                    if (sign > 0 && (b < 0 || b >= c.n_pages)) bad = int(ERR_BAD_POS);
+                    b = -1;  // a fresh page
+                }
+                if (a == b) continue;
+                if (a >= 0 && a < c.n_pages) atomicSub(c.refs + a, sign);
+                if (b >= 0 && b < c.n_pages) atomicAdd(c.refs + b, sign);
+            }
+        }
+    };
+    count(1);
+    __syncthreads();
+    if (!bad && want > 0 && lowest_free(c, words, want, list) < want && tid == 0) bad = int(ERR_CAPACITY);
+    __syncthreads();
+    if (bad) {
+        count(-1);
+        if (tid == 0) {
+            set_error(c.status, unsigned(bad));
+            plan[0] = -1;
+        }
+        return;
+    }
+    for (int i = warp; i < n; i += warps) {
+        const int j = parent(i), r = (i ? base[i - 1] : 0);
+        const bool copy = base[i] != r;
+        if (j == i && !copy) continue;
+        int* row = c.table + size_t(seqs[i]) * c.max_pages;
+        const int n_now = (len[i] + c.pt - 1) >> c.pt_shift, n_old = (c.lens[seqs[i]] + c.pt - 1) >> c.pt_shift;
+        for (int k = lane; k < max(n_old, n_now); k += 32) {
+            int p = rows[size_t(i) * c.max_pages + k];
+            if (copy && k == n_now - 1) {
+                plan[1 + 3 * r] = p;
+                p = list[r];
+                plan[2 + 3 * r] = p;
+                plan[3 + 3 * r] = ((len[i] & (c.pt - 1)) + kKvBlock - 1) / kKvBlock;
+                c.refs[p] = 1;
+            }
+            row[k] = p;
+        }
+        __syncwarp();
+        if (lane == 0) c.lens[seqs[i]] = len[i];
+    }
+    if (tid == 0) plan[0] = want;
+}
+
+// Reorder, second half: the filled blocks of the copied pages, in every layer and head.  Grid (parts, copies at most); a warp takes
+// one tile after another: of a K tile hd / 16 stretches of `fill` blocks, of a V tile one.
+constexpr int kReorderWarps = 8;
+
+__global__ void __launch_bounds__(32 * kReorderWarps) k_kv_reorder(KvView c, const int* __restrict__ plan) {
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = __ldcg(plan), tiles = c.n_layers * 2 * c.n_kv, blocks = c.pt / kKvBlock;
+    for (int r = blockIdx.y; r < n; r += gridDim.y) {
+        const int from = __ldcg(plan + 1 + 3 * r), to = __ldcg(plan + 2 + 3 * r), fill = __ldcg(plan + 3 + 3 * r);
+        const int pieces = fill * c.hd, strip = fill * kKvBlock;  // of 16 bytes: of a tile, and of one of K's stretches
+        const unsigned magic = unsigned((0x100000000ULL + strip - 1) / strip);
+        for (int tile = blockIdx.x * kReorderWarps + warp; tile < tiles; tile += gridDim.x * kReorderWarps) {
+            const size_t a = size_t(from) * tiles + tile, b = size_t(to) * tiles + tile;
+            const uint4* src = reinterpret_cast<const uint4*>(c.codes + a * c.tile());
+            uint4* dst = reinterpret_cast<uint4*>(c.codes + b * c.tile());
+            const bool is_v = tile / c.n_kv & 1;
+            constexpr int U = 8;
+            for (int y0 = lane; y0 < pieces; y0 += 32 * U) {
+                uint4 w[U];
+                int at[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int y = min(y0 + 32 * u, pieces - 1), s = int(__umulhi(unsigned(y), magic));  // y / strip
+                    at[u] = is_v ? y : s * c.pt + y - s * strip;
+                    w[u] = __ldcs(src + at[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (y0 + 32 * u < pieces) __stcs(dst + at[u], w[u]);
+            }
+            if (lane < fill) c.scales[b * blocks + lane] = c.scales[a * blocks + lane];
+        }
+    }
+}
+
 constexpr int kPagePart = 16384;  // bytes of a page that a CTA copies
 
 // Copies a page's codes and scales, all layers; part `part` of `parts`.
@@ -759,6 +909,25 @@ cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int 
     if (e != cudaSuccess) return e;
     return launch_pdl(k_kv_fork, dim3(unsigned(page_parts(c)), unsigned(n)), dim3(kForkThreads), 0, st, true, c, src, dst,
                       static_cast<const int*>(ok), static_cast<const int*>(fresh));
+}
+
+// plan: {from, to, blocks} of each copy, [max_seqs] lengths, [max_seqs][max_pages] rows, [n_pages] list.
+size_t kv_reorder_ws_bytes(const KvView& c) {
+    return (4 + size_t(c.max_seqs) * (3 + 1 + size_t(c.max_pages)) + size_t(c.n_pages)) * 4;
+}
+
+cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* parents, int n, int group, void* ws, cudaStream_t st) {
+    if (n == 0) return cudaSuccess;
+    int* plan = static_cast<int*>(ws);
+    int* len = plan + 4 + size_t(c.max_seqs) * 3;
+    int* rows = len + c.max_seqs;
+    int* list = rows + size_t(c.max_seqs) * c.max_pages;
+    cudaError_t e = launch_plan(k_kv_reorder_plan, 1, kPlanThreads, plan_words(c) * 4 + size_t(c.max_seqs) * 4 + size_t(n) * 6, st, c, seqs,
+                                parents, n, group, plan, rows, len, list);
+    if (e != cudaSuccess) return e;
+    const int parts = (c.n_layers * 2 * c.n_kv + kReorderWarps - 1) / kReorderWarps;
+    return launch_pdl(k_kv_reorder, dim3(unsigned(parts < 1024 ? parts : 1024), unsigned(n)), dim3(32 * kReorderWarps), 0, st, true, c,
+                      static_cast<const int*>(plan));
 }
 
 cudaError_t launch_kv_free(const KvView& c, const int* seqs, int n, cudaStream_t st) {

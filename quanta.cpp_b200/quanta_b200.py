@@ -4,7 +4,9 @@ The names follow the reference's C++ interface (engine/src/model.h, ops.h, sampl
     Model(path, ctx).forward(token, pos, hq) / forward_batch(tokens, pos0, hq) / head(hq) / last_head_rows
     quantize_q8(x) ; DeviceTensor(dtype, rows, cols, raw).matvec(q, d, r0, r1) / .matmul(...)
     Model.generate(prompt, SamplerParams(...), shortlist=True, batch_prefill=True, n_gen=64)
-    PagedKV.empty(...).reserve / append / attention / read / fork / free / compact  the paged 8-bit KV cache (torch tensors)
+    PagedKV.empty(...).reserve / append / attention / read / fork / reorder / free / compact  the paged 8-bit KV cache (torch)
+    rms_norm_q8(x, weight, residual=r), dequantize_q8(q, d), Rope(...)(q, k, positions)  around a layer's products (torch)
+    BeamSelector(k)(logits, scores)  the selection of a beam search's next step (torch)
     synth_model(path, ...)  seeded random-init .qnt writer
 There is no CPU fallback: importing works anywhere, but every call needs libquanta_b200.so and a GPU, and fails
 loudly when either is missing.
@@ -12,6 +14,7 @@ loudly when either is missing.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from dataclasses import dataclass
 from pathlib import Path
@@ -22,7 +25,7 @@ PKG = Path(__file__).resolve().parent
 LIB_DIR = Path(os.environ["QNT_LIB_DIR"]) if os.environ.get("QNT_LIB_DIR") else PKG / "lib"  # timeline.py: lib_stamps
 
 F32, F16, Q8_0, Q4_0 = 0, 1, 2, 3
-BF16 = 4  # activations of the paged KV cache
+BF16 = 4  # activations only: the paged KV cache, norm, rope and beams
 QK = 32
 GEN_SHORTLIST, GEN_BATCH_PREFILL = 1, 2
 
@@ -157,6 +160,9 @@ def lib() -> C.CDLL:
         L.qnt_kv_page_workspace.restype = Z
         L.qnt_kv_reserve.argtypes = [K, P, P, I, P, Z, P]
         L.qnt_kv_fork.argtypes = [K, P, P, I, P, Z, P]
+        L.qnt_kv_reorder_workspace.argtypes = [K]
+        L.qnt_kv_reorder_workspace.restype = Z
+        L.qnt_kv_reorder.argtypes = [K, P, P, I, I, P, Z, P]
         L.qnt_kv_free.argtypes = [K, P, I, P]
         L.qnt_kv_compact.argtypes = [K, P, Z, P]
         L.qnt_kv_copy.argtypes = [K, P, P, I, P]
@@ -166,6 +172,12 @@ def lib() -> C.CDLL:
         L.qnt_kv_attention_workspace.restype = Z
         L.qnt_kv_attention.argtypes = [K, I, P, I, LL, I, P, P, I, I, I, I, F, I, P, P, P, Z, P]
         L.qnt_kv_check.argtypes = [K, P]
+        L.qnt_rms_norm_q8.argtypes = [P, I, LL, P, I, LL, P, F, I, I, P, P, P]
+        L.qnt_dequantize_q8.argtypes = [P, P, I, I, P, I, P]
+        L.qnt_rope.argtypes = [P, LL, P, LL, I, P, LL, P, LL, I, I, I, I, I, P, F, P, I, P]
+        L.qnt_beam_workspace.argtypes = [I, I, I, I]
+        L.qnt_beam_workspace.restype = Z
+        L.qnt_beam_select.argtypes = [P, I, LL, P, P, I, I, I, I, I, P, P, P, P, Z, P]
         _lib = L
     return _lib
 
@@ -326,7 +338,7 @@ class PagedKV:
                            scales.data_ptr(), refs.data_ptr(), table.data_ptr(), lens.data_ptr(), self._status.data_ptr())
         self._p = C.byref(self._c)
         self._types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-        self._ws, self._kept, self._need, self._i32 = {}, [], {}, i32
+        self._ws, self._kept, self._need, self._i32, self._reorder_ws = {}, [], {}, i32, None
         self._lib, self._index = lib(), codes.device.index  # a call's host time counts where few tokens are decoded
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -410,6 +422,19 @@ class PagedKV:
         s = self._stream(stream)
         w, nb = self._workspace(s, self._page_ws)
         self._run(self._lib.qnt_kv_fork, self._p, src.data_ptr(), dst.data_ptr(), n, w, nb, s)
+
+    def reorder(self, seqs, parents, group: int | None = None, stream=None):
+        """A beam search's step: sequence seqs[i] becomes what seqs[i - i % group + parents[i]] was before the call (group: beams of a
+        request, by default the whole list).  Full pages are shared; one child of each parent goes on with its part-filled last
+        page, the others get copies of what it holds; pages that nothing uses any more are free again."""
+        n = self._list(seqs, parents)
+        if parents.numel() != n:
+            raise ValueError("one parent per sequence")
+        if self._reorder_ws is None:
+            self._reorder_ws = self._lib.qnt_kv_reorder_workspace(self._p)
+        s = self._stream(stream)
+        w, nb = self._workspace(s, self._reorder_ws)
+        self._run(self._lib.qnt_kv_reorder, self._p, seqs.data_ptr(), parents.data_ptr(), n, n if group is None else group, w, nb, s)
 
     def free(self, seqs, stream=None):
         """The sequences give back their pages and become empty."""
@@ -497,6 +522,242 @@ class PagedKV:
     def check(self, stream=None):
         """Waits for the stream and raises the error that earlier calls on this cache ran into, if any."""
         self._run(self._lib.qnt_kv_check, self._p, self._stream(stream))
+
+
+class _TorchCalls:
+    """What the operators on torch tensors share: types, streams, and calls on a tensor's device.  Work is queued on `stream` (a torch
+    stream or a cudaStream_t's number; default: torch's current stream of the tensors' device); with another stream than the
+    current one a call is as if made within torch.cuda.stream(stream)."""
+
+    def __init__(self):
+        import torch
+        self.torch = torch
+        self.types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self.lib = lib()
+
+    def stream(self, stream, device: int) -> int:
+        if stream is None:
+            return self.raw_stream(device) if self.raw_stream else self.torch.cuda.current_stream(device).cuda_stream
+        return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+    def allocating_on(self, stream, device: int):
+        cuda = self.torch.cuda
+        if not hasattr(stream, "cuda_stream"):
+            stream = cuda.ExternalStream(int(stream), device=device) if int(stream) else cuda.default_stream(device)
+        return cuda.stream(stream)
+
+    def empty(self, like, stream, *shapes):
+        """New tensors (shape, dtype) for work on the stream."""
+        if stream is None:
+            return [like.new_empty(s, dtype=t) for s, t in shapes]
+        with self.allocating_on(stream, like.get_device()):
+            return [like.new_empty(s, dtype=t) for s, t in shapes]
+
+    def run(self, device: int, call, *args):
+        if self.current_device() == device:
+            rc = call(*args)
+        else:
+            with self.torch.cuda.device(device):
+                rc = call(*args)
+        if rc:
+            _check(rc)
+
+
+_calls = None
+
+
+def _torch_calls() -> _TorchCalls:
+    global _calls
+    if _calls is None:
+        _calls = _TorchCalls()
+    return _calls
+
+
+def rms_norm_q8(x, weight, eps: float = 1e-6, residual=None, stream=None):
+    """RMS norm of rows x [tokens, n] (float32, float16 or bfloat16 CUDA tensor; rows may lie in wider ones) with 8-bit rows out:
+    (q int8 [tokens, n], d float32 [tokens, n / 32]), the operand of the quantized products.  weight float32 [n].  With residual
+    [tokens, n] (x's type or float32), residual += x first, in place, and the sum (before its rounding) is normed."""
+    c = _torch_calls()
+    t, dt, dev = c.torch, c.types.get(x.dtype), x.get_device()
+    if dt is None or dev < 0 or x.dim() != 2 or x.stride(1) != 1:
+        raise TypeError("x must be a float32, float16 or bfloat16 CUDA tensor [tokens, n] whose rows are contiguous")
+    m, n = x.shape
+    if weight.dtype is not t.float32 or weight.get_device() != dev or weight.shape != (n,) or not weight.is_contiguous():
+        raise TypeError(f"weight must be a contiguous float32 CUDA tensor [{n}] on x's device")
+    rp, rt, rs = None, dt, 0
+    if residual is not None:
+        rt = c.types.get(residual.dtype)
+        if residual.shape != x.shape or residual.get_device() != dev or residual.stride(1) != 1 or (rt != dt and rt != F32):
+            raise TypeError("residual must be a CUDA tensor of x's shape, on its device, of its type or float32, whose rows are contiguous")
+        rp, rs = residual.data_ptr(), residual.stride(0)
+    q, d = c.empty(x, stream, ((m, n), t.int8), ((m, n // QK), t.float32))
+    c.run(dev, c.lib.qnt_rms_norm_q8, x.data_ptr(), dt, x.stride(0), rp, rt, rs, weight.data_ptr(), eps, m, n, q.data_ptr(), d.data_ptr(),
+          c.stream(stream, dev))
+    return q, d
+
+
+def dequantize_q8(q, d, dtype=None, stream=None):
+    """The values q * d of 8-bit rows (q int8 [tokens, n], d float32 [tokens, n / 32], contiguous CUDA tensors), as dtype (bfloat16
+    unless said otherwise)."""
+    c = _torch_calls()
+    t, dev = c.torch, q.get_device()
+    dtype = dtype or t.bfloat16
+    dt = c.types.get(dtype)
+    if dt is None:
+        raise TypeError("dtype must be float32, float16 or bfloat16")
+    if q.dtype is not t.int8 or dev < 0 or q.dim() != 2 or not q.is_contiguous() or d.dtype is not t.float32 or \
+            d.get_device() != dev or not d.is_contiguous() or q.shape[1] % QK or d.shape != (q.shape[0], q.shape[1] // QK):
+        raise TypeError("q must be a contiguous int8 CUDA tensor [tokens, n], d a contiguous float32 one [tokens, n / 32] on its device")
+    out, = c.empty(q, stream, (q.shape, dtype))
+    c.run(dev, c.lib.qnt_dequantize_q8, q.data_ptr(), d.data_ptr(), q.shape[0], q.shape[1], out.data_ptr(), dt, c.stream(stream, dev))
+    return out
+
+
+class Rope:
+    """Rotary positions: rope(q, k, positions) rotates the first rotary_dim dims of every head (pairs (i, i + rotary_dim / 2), or with
+    interleaved=True (2 i, 2 i + 1)) by positions * base ** (-2 i / rotary_dim); the other dims are copied.  scaling, for long contexts:
+        dict(kind="linear", factor=)            every frequency divided by the factor
+        dict(kind="ntk", factor=)               base * factor ** (rotary_dim / (rotary_dim - 2))
+        dict(kind="yarn", factor=, original=, beta_fast=32, beta_slow=1, attention=None)  pairs that turn more than beta_fast times
+            within the original context keep their frequency, those below beta_slow have it divided, a ramp between them; rotated
+            values are multiplied by `attention` (0.1 ln factor + 1)
+        dict(kind="bands", factor=, original=, low=1, high=4)  kept from `high` turns within the original context, divided up to
+            `low`, a ramp between them
+    or frequencies= (rotary_dim / 2 radians a position) instead of base and scaling."""
+
+    def __init__(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, scaling: dict | None = None, frequencies=None,
+                 device="cuda"):
+        import torch
+        self.rotary_dim, self.interleaved = int(rotary_dim), bool(interleaved)
+        if self.rotary_dim <= 0 or self.rotary_dim % 2:
+            raise ValueError("rotary_dim must be positive and even")
+        if frequencies is None:
+            f, self.scale = self.frequencies(self.rotary_dim, base, scaling)
+        else:
+            f, self.scale = [float(x) for x in frequencies], 1.0
+            if len(f) != self.rotary_dim // 2 or scaling is not None:
+                raise ValueError("frequencies: one for each pair, and no scaling beside them")
+        self.turns = torch.tensor([x / (2 * math.pi) for x in f], dtype=torch.float64, device=device)  # revolutions a position
+        self._dev, self._turns = self.turns.get_device(), self.turns.data_ptr()
+        self._inter, self._c = int(self.interleaved), None
+
+    @staticmethod
+    def frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None):
+        """(radians a position of each pair, factor on rotated values) of a base and a scaling, in 64 bits."""
+        sc = dict(scaling or {"kind": "none"})
+        kind = sc.pop("kind", None)
+        known = {"none": {}, "linear": {"factor": None}, "ntk": {"factor": None},
+                 "yarn": {"factor": None, "original": None, "beta_fast": 32.0, "beta_slow": 1.0, "attention": 0.0},
+                 "bands": {"factor": None, "original": None, "low": 1.0, "high": 4.0}}
+        if kind not in known or set(sc) - set(known[kind]):
+            raise ValueError(f"scaling: kind none, linear, ntk, yarn or bands with {known.get(kind, {})}, not {scaling}")
+        sc = known[kind] | {k: v for k, v in sc.items() if v is not None}
+        if any(v is None for v in sc.values()) or any(v <= 0 for k, v in sc.items() if k in ("factor", "original", "beta_fast", "beta_slow")):
+            raise ValueError(f"scaling {kind}: needs positive {[k for k in sc if known[kind][k] is None]}")
+        if not base > 1:
+            raise ValueError("base must be above 1")
+        factor = sc.get("factor", 1.0)
+        if kind == "ntk" and rotary_dim > 2:
+            base = base * factor ** (rotary_dim / (rotary_dim - 2))
+        f = [base ** (-2 * i / rotary_dim) for i in range(rotary_dim // 2)]
+        if kind == "linear":
+            return [x / factor for x in f], 1.0
+        if kind == "yarn":
+            lo, hi = (rotary_dim * math.log(sc["original"] / (b * 2 * math.pi)) / (2 * math.log(base)) for b in (sc["beta_fast"], sc["beta_slow"]))
+            lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), rotary_dim - 1)
+            ramp = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(rotary_dim // 2)]
+            return [x * (1 - r) + x / factor * r for x, r in zip(f, ramp)], sc["attention"] or 0.1 * math.log(factor) + 1.0
+        if kind == "bands":
+            if not sc["high"] > sc["low"]:
+                raise ValueError("scaling bands: high must be above low")
+            keep = [min(1.0, max(0.0, (sc["original"] * x / (2 * math.pi) - sc["low"]) / (sc["high"] - sc["low"]))) for x in f]
+            return [x * k + x / factor * (1 - k) for x, k in zip(f, keep)], 1.0
+        return f, 1.0
+
+    def _fits(self, x, tokens):
+        shape, st = x.shape, x.stride()
+        return len(shape) == 3 and st[2] == 1 and (st[1] == shape[2] or shape[1] == 1) and shape[0] == tokens and x.get_device() == self._dev
+
+    def __call__(self, q, k, positions, inplace: bool = False, stream=None):
+        """q [tokens, heads, head_dim] and k [tokens, kv heads, head_dim] (or None) of one type, float32, float16 or bfloat16; heads
+        contiguous within a token, so that they may lie in the rows of one projection's output; positions int32 [tokens].
+        Returns rotated (q, k), new contiguous tensors, or with inplace=True the ones given."""
+        c = self._c
+        if c is None:
+            c = self._c = _torch_calls()
+        dt, tokens = c.types.get(q.dtype), positions.numel()
+        if dt is None or not self._fits(q, tokens) or (k is not None and (k.dtype is not q.dtype or not self._fits(k, tokens) or
+                                                                          k.shape[2] != q.shape[2])):
+            raise TypeError("q and k must be CUDA tensors [tokens, heads, head_dim] of one type, float32, float16 or bfloat16, on the "
+                            "table's device, whose heads are contiguous within a token")
+        if positions.dtype is not c.torch.int32 or positions.get_device() != self._dev or positions.dim() != 1 or not positions.is_contiguous():
+            raise TypeError("positions must be a contiguous int32 CUDA tensor [tokens] on the table's device")
+        if inplace:
+            q_out, k_out = q, k
+        elif k is None:
+            (q_out,), k_out = c.empty(q, stream, (q.shape, q.dtype)), None
+        else:
+            q_out, k_out = c.empty(q, stream, (q.shape, q.dtype), (k.shape, q.dtype))
+        of_k = (None, 0, None, 0, 0) if k is None else (k.data_ptr(), k.stride(0), k_out.data_ptr(), k_out.stride(0), k.shape[1])
+        c.run(self._dev, c.lib.qnt_rope, q.data_ptr(), q.stride(0), q_out.data_ptr(), q_out.stride(0), q.shape[1], *of_k, dt, q.shape[2],
+              self.rotary_dim, self._inter, self._turns, self.scale, positions.data_ptr(), tokens, c.stream(stream, self._dev))
+        return q_out, k_out
+
+
+class BeamSelector:
+    """The selection of a beam search's next step (qnt_beam_select): select(logits, scores, ended) -> (scores float32, tokens int32,
+    parents int32), each [groups, k], best first: of every group's candidates scores[g, b] + log_softmax(logits[g, b])[t] the k best,
+    equal ones by the lowest beam, then token.  An ended beam has one candidate, its own score with token end_id.  Forbidden tokens
+    (logits of -inf) and beams without a finite score come last, with -inf.  With k = beams, PagedKV.reorder takes the parents as
+    they are.  Workspaces are one per stream and live as long as the object: a graph that captured calls is replayed while the
+    object exists, ordered against the calls on the stream that it was captured on."""
+
+    def __init__(self, k: int, end_id: int = -1):
+        self.k, self.end_id = int(k), int(end_id)
+        self._ws, self._kept, self._need, self._c = {}, [], {}, None
+
+    def _workspace(self, c, device, stream, given, need):
+        ws = self._ws.get((device, stream))
+        if ws is None or ws.numel() < need:
+            size = max(need, 1 << 20)
+            if ws is not None:  # the old one stays: queued kernels and captured graphs still write to it
+                self._kept.append(ws)
+                size = max(size, 2 * ws.numel())
+            with c.allocating_on(stream if given is None else given, device):
+                ws = self._ws[device, stream] = c.torch.empty(size, dtype=c.torch.uint8, device=f"cuda:{device}")
+        return ws.data_ptr(), ws.numel()
+
+    def __call__(self, logits, scores, ended=None, stream=None):
+        """logits [groups, beams, vocab] (float32, float16 or bfloat16 CUDA tensor, rows at one distance, which may be wider than
+        vocab), scores float32 [groups, beams], ended bool or uint8 [groups, beams] or None."""
+        c = self._c
+        if c is None:
+            c = self._c = _torch_calls()
+        t, dt, dev = c.torch, c.types.get(logits.dtype), logits.get_device()
+        shape, st = logits.shape, logits.stride()
+        if dt is None or dev < 0 or len(shape) != 3 or (st[2] != 1 and shape[2] != 1):
+            raise TypeError("logits must be a float32, float16 or bfloat16 CUDA tensor [groups, beams, vocab] whose rows are contiguous")
+        g, b, v = shape
+        row = st[1] if b > 1 else st[0]
+        if g > 1 and b > 1 and st[0] != b * row:
+            raise TypeError("the rows of logits must lie at one distance from each other")
+        if scores.dtype is not t.float32 or scores.get_device() != dev or scores.shape != (g, b) or not scores.is_contiguous():
+            raise TypeError("scores must be a contiguous float32 CUDA tensor [groups, beams] on the logits' device")
+        if ended is not None and (ended.dtype not in (t.bool, t.uint8) or ended.get_device() != dev or ended.shape != (g, b) or
+                                  not ended.is_contiguous()):
+            raise TypeError("ended must be a contiguous bool or uint8 CUDA tensor [groups, beams] on the logits' device")
+        k, key = self.k, (g, b, v)
+        need = self._need.get(key)
+        if need is None:
+            need = self._need[key] = c.lib.qnt_beam_workspace(g, b, v, k)
+        s = c.stream(stream, dev)
+        w, nb = self._workspace(c, dev, s, stream, need)
+        out, tokens, parents = c.empty(scores, stream, ((g, k), t.float32), ((g, k), t.int32), ((g, k), t.int32))
+        c.run(dev, c.lib.qnt_beam_select, logits.data_ptr(), dt, row, scores.data_ptr(), None if ended is None else ended.data_ptr(),
+              self.end_id, g, b, v, k, out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), w, nb, s)
+        return out, tokens, parents
 
 
 def bench_mma_i8(iters: int = 4096) -> float:
