@@ -112,7 +112,7 @@ int qnt_rope(const void* q, long long q_stride, void* q_out, long long q_out_str
  * logits: row group * beams + b at that times stride (elements), of dtype QNT_F32, QNT_F16 or QNT_BF16.  ended (may be NULL)
  * [groups][beams]: such a beam has one candidate, its own score with token end_id.  Candidates that are -inf or no numbers (a
  * forbidden token, a row with NaN or +inf, a score that is not finite) come behind all others, with score -inf, in order of their
- * places.  Scores are formed and compared in f64.  k <= 64, beams <= 1024, beams * vocab < 2^31.
+ * places.  Scores are formed and compared in f64.  k <= 64, beams <= 1024, vocab <= 2^30, beams * vocab < 2^31.
  * workspace: qnt_beam_workspace bytes, 16-byte aligned, contents irrelevant. */
 size_t qnt_beam_workspace(int groups, int beams, int vocab, int k);
 int qnt_beam_select(const void* logits, int dtype, long long stride, const float* scores, const uint8_t* ended, int end_id,

@@ -48,7 +48,7 @@ int beam_args(int groups, int beams, int vocab, int k, qb::BeamArgs* a) {
     if (groups < 0 || beams <= 0 || vocab <= 0 || k <= 0) return set_err(QNT_ERR_INVALID, "beam select: sizes must be positive");
     if (k > qb::kBeamMaxK || beams > 1024) return set_err(QNT_ERR_UNSUPPORTED, "beam select: at most 64 candidates and 1024 beams");
     if ((long long)beams * vocab < k) return set_err(QNT_ERR_INVALID, "beam select: fewer than k candidates");
-    if ((long long)beams * vocab > 0x7fffffffLL || (long long)groups * beams * (vocab / 2048 + 2) > 0x7fffffffLL)
+    if (vocab > 1 << 30 || (long long)beams * vocab > 0x7fffffffLL || (long long)groups * beams * (vocab / 2048 + 2) > 0x7fffffffLL)
         return set_err(QNT_ERR_UNSUPPORTED, "beam select: groups x beams x vocab is too large for one call");
     a->groups = groups;
     a->beams = beams;
@@ -136,7 +136,14 @@ int qnt_rope(const void* q, long long q_stride, void* q_out, long long q_out_str
 
 size_t qnt_beam_workspace(int groups, int beams, int vocab, int k) {
     qb::BeamArgs a{};
-    return beam_args(groups, beams, vocab, k, &a) ? 0 : qb::beam_ws_bytes(a);
+    if (beam_args(groups, beams, vocab, k, &a)) return 0;
+    size_t need = 0;
+    for (qb::KvType t : {qb::KV_F32, qb::KV_F16}) {  // whichever type the call will have
+        a.type = t;
+        const size_t b = qb::beam_ws_bytes(a);
+        if (b > need) need = b;
+    }
+    return need;
 }
 
 int qnt_beam_select(const void* logits, int dtype, long long stride, const float* scores, const uint8_t* ended, int end_id,
