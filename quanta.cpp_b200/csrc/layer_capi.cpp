@@ -48,7 +48,7 @@ int beam_args(int groups, int beams, int vocab, int k, qb::BeamArgs* a) {
     if (groups < 0 || beams <= 0 || vocab <= 0 || k <= 0) return set_err(QNT_ERR_INVALID, "beam select: sizes must be positive");
     if (k > qb::kBeamMaxK || beams > 1024) return set_err(QNT_ERR_UNSUPPORTED, "beam select: at most 64 candidates and 1024 beams");
     if ((long long)beams * vocab < k) return set_err(QNT_ERR_INVALID, "beam select: fewer than k candidates");
-    if (vocab > 1 << 30 || (long long)beams * vocab > 0x7fffffffLL || (long long)groups * beams * (vocab / 2048 + 2) > 0x7fffffffLL)
+    if (vocab > 1 << 30 || (long long)beams * vocab > 0x7fffffffLL || (long long)groups * beams * (vocab / 512 + 2) > 0x3fffffffLL)
         return set_err(QNT_ERR_UNSUPPORTED, "beam select: groups x beams x vocab is too large for one call");
     a->groups = groups;
     a->beams = beams;
