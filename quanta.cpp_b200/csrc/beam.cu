@@ -22,8 +22,8 @@ namespace {
 
 constexpr int kTilePieces = 4;       // 16-byte pieces of a lane in a tile
 constexpr int kTileThreads = 256;
-constexpr int kTileCtas = 6;         // on an SM
-constexpr int kMergeThreads = 512;
+constexpr int kTileCtas = 8;         // on an SM
+constexpr int kMergeThreads = 1024;  // at most
 constexpr int kCap = 1024;           // candidates that pass a threshold; more are taken one at a time
 constexpr float kMaxF = 3.402823466e38f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -184,45 +184,18 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas)
     }
 }
 
-// The k-th largest of 32 G values that warp 0 reads (as ordered keys; 0 where there are fewer): with a value of every lane's own
-// known against all others, a rank is a count.
-template <int G>
-__device__ __forceinline__ unsigned kth_of(const unsigned* vals, int k) {
-    const int lane = threadIdx.x & 31;
-    unsigned v[G];
-    int rank[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        v[g] = vals[g * 32 + lane];
-        rank[g] = 0;
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const unsigned o = __shfl_sync(0xffffffffu, v[g], j);
-#pragma unroll
-            for (int h = 0; h < G; ++h) rank[h] += o > v[h];
-        }
-    unsigned least = 0xffffffffu;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-        if (rank[g] < k) least = min(least, v[g]);
-    return __reduce_min_sync(0xffffffffu, least);
-}
-
-// One candidate in the merge's order: a score and its place in the group.
+// A candidate, or the largest one of a tile: its score, its place in the group (which breaks ties) and its row.
 struct Found {
     double score;
-    unsigned at;  // beam * vocab + token
-    unsigned pad;
+    unsigned at;
+    int row;
 };
-__device__ __forceinline__ bool before(double s, unsigned at, double t, unsigned other) { return s > t || (s == t && at < other); }
+__device__ __forceinline__ bool before(const Found& a, const Found& b) { return a.score > b.score || (a.score == b.score && a.at < b.at); }
 
-// Order-preserving key of a score.
-__device__ __forceinline__ unsigned long long order64(double x) {
-    const unsigned long long b = (unsigned long long)__double_as_longlong(x == 0. ? 0. : x);
-    return b ^ (b >> 63 ? ~0ull : 1ull << 63);
+// Order-preserving key of a score, its upper half: enough for a threshold.
+__device__ __forceinline__ unsigned order_hi(double x) {
+    const unsigned b = unsigned(__double2hiint(x == 0. ? 0. : x));
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
 // e^t for t <= 0 as f32: the rounding of t log2 e made good.
@@ -233,7 +206,7 @@ __device__ __forceinline__ float exp_neg(float t) {
 }
 
 // log of the sum of exponentials of a row, by a warp, from its tiles; NaN where the row has no candidates.
-__device__ double join_sums(const Tile* tiles, int n) {
+__device__ __forceinline__ double join_sums(const Tile* tiles, int n) {
     constexpr int N = 8;  // tiles of a lane that are read once
     const int lane = threadIdx.x & 31;
     const float2* in = reinterpret_cast<const float2*>(tiles);
@@ -244,10 +217,11 @@ __device__ double join_sums(const Tile* tiles, int n) {
 #pragma unroll
     for (int u = 0; u < N; ++u) top = fmaxf(top, t[u].x);
     for (int i = lane + 32 * N; i < n; i += 32) top = fmaxf(top, __ldcg(in + i).x);
-    top = warp_max(top);
-    double sum = 0;  // (a tile of forbidden tokens has the sum 0)
+    top = unorder(__reduce_max_sync(0xffffffffu, order(top)));
+    float part = 0.f;  // (a tile of forbidden tokens has the sum 0)
 #pragma unroll
-    for (int u = 0; u < N; ++u) sum += double(t[u].y) * double(exp_neg(t[u].x - top));
+    for (int u = 0; u < N; ++u) part = fmaf(t[u].y, exp_neg(t[u].x - top), part);
+    double sum = double(part);
     for (int i = lane + 32 * N; i < n; i += 32) {
         const float2 v = __ldcg(in + i);
         sum += double(v.y) * double(exp_neg(v.x - top));
@@ -258,7 +232,7 @@ __device__ double join_sums(const Tile* tiles, int n) {
 }
 
 struct MergeShared {
-    unsigned group_top[32 * 4];
+    unsigned group_top[128];
     unsigned threshold;
     int count, redo;
     Found found[kCap];
@@ -266,67 +240,70 @@ struct MergeShared {
     double sums[kMergeThreads / 32];
 };
 
-// best[0 .. n - 1] = the n = min(k + 1, all) best of the items of the CTA's threads, in order; each(f) calls f(score, place) for every
-// item of this thread, the same ones every time.  Items that reach a threshold, the (k + 1)-th largest of the largest of 64 (or 128)
-// groups of threads, are ranked by counting.  `floor`: no item below it is wanted.
-template <class Each>
-__device__ int best_of(MergeShared& sh, int k, double floor, bool has_floor, Each&& each) {
-    constexpr int W = kMergeThreads / 32;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    unsigned least = 0;
-    if (!has_floor) {
-        unsigned top = 0;  // the upper half of the order is enough for a threshold
-        each([&](double sc, unsigned) { top = max(top, unsigned(order64(sc) >> 32)); });
-        const bool small = k < 32;
-        const int of = kMergeThreads / (small ? 64 : 128);  // threads of a group
-        for (int o = 1; o < of; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (tid % of == 0) sh.group_top[tid / of] = top;
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        if (warp == 0) {
-            const unsigned t = small ? kth_of<2>(sh.group_top, k + 1) : kth_of<4>(sh.group_top, k + 1);
-            if (lane == 0) sh.threshold = t;
+// A threshold that at least k + 1 of the CTA's items reach, if there are so many, and not many more: the (k + 1)-th largest of the
+// largest items of 32 (or 128) groups of threads, whose keys are made different by their groups' numbers in the lowest bits.
+// `top`: the key of the largest item of this thread, 0: none.
+__device__ __forceinline__ unsigned threshold_of(MergeShared& sh, int k, unsigned top) {
+    const int tid = threadIdx.x, groups = k < 16 ? 32 : 128, of = blockDim.x / groups;
+    for (int o = 1; o < of; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (tid % of == 0) sh.group_top[tid / of] = (top & ~127u) | unsigned(tid / of);
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (tid < groups) {
+        const unsigned mine = sh.group_top[tid];
+        const uint4* all = reinterpret_cast<const uint4*>(sh.group_top);
+        int rank = 0;
+#pragma unroll 8
+        for (int g = 0; g < groups / 4; ++g) {
+            const uint4 v = all[g];
+            rank += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
         }
-        __syncthreads();
-        least = sh.threshold;
-    } else {
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
+        if (rank == k) sh.threshold = mine & ~127u;
     }
-    each([&](double sc, unsigned at) {
-        if (has_floor ? sc >= floor : unsigned(order64(sc) >> 32) >= least) {
-            const int i = atomicAdd(&sh.count, 1);
-            if (i < kCap) sh.found[i] = Found{sc, at, 0};
-        }
-    });
+    __syncthreads();
+    return sh.threshold;
+}
+
+__device__ __forceinline__ void push(MergeShared& sh, double score, unsigned at, int row) {
+    const int i = atomicAdd(&sh.count, 1);
+    if (i < kCap) sh.found[i] = Found{score, at, row};
+}
+
+// best[0 .. n - 1] = the n = min(k + 1, all) best of the items that have been pushed, in order; where they are too many, of all that
+// each(f) calls f(score, place, row) for.  A warp ranks an item by counting.  Ends synchronised.
+template <class Each>
+__device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     __syncthreads();
     const int n = sh.count;
     if (n <= kCap) {
-        for (int c = tid; c < n; c += kMergeThreads) {
+        for (int c = warp; c < n; c += warps) {
             const Found mine = sh.found[c];
             int rank = 0;
-            for (int o = 0; o < n; ++o) rank += before(sh.found[o].score, sh.found[o].at, mine.score, mine.at);
-            if (rank <= k) sh.best[rank] = mine;
+            for (int o = lane; o < n; o += 32) rank += before(sh.found[o], mine);
+            rank = __reduce_add_sync(0xffffffffu, rank);
+            if (rank <= k && lane == 0) sh.best[rank] = mine;
         }
-    } else {  // very many that reach it: the best one behind the last, k + 1 times
+    } else {  // very many that reach the threshold: the best one behind the last, k + 1 times
         Found last{INFINITY, 0, 0};
         for (int i = 0; i <= k; ++i) {
             Found mine{-INFINITY, UINT_MAX, 0};
-            each([&](double sc, unsigned at) {
-                if ((i == 0 || before(last.score, last.at, sc, at)) && before(sc, at, mine.score, mine.at)) mine = Found{sc, at, 0};
+            each([&](double score, unsigned at, int row) {
+                const Found f{score, at, row};
+                if ((i == 0 || before(last, f)) && before(f, mine)) mine = f;
             });
-#pragma unroll
+#pragma unroll 1
             for (int o = 16; o > 0; o >>= 1) {
-                const double sc = __shfl_xor_sync(0xffffffffu, mine.score, o);
-                const unsigned at = __shfl_xor_sync(0xffffffffu, mine.at, o);
-                if (before(sc, at, mine.score, mine.at)) mine = Found{sc, at, 0};
+                const Found f{__shfl_xor_sync(0xffffffffu, mine.score, o), __shfl_xor_sync(0xffffffffu, mine.at, o),
+                              __shfl_xor_sync(0xffffffffu, mine.row, o)};
+                if (before(f, mine)) mine = f;
             }
             __syncthreads();
             if (lane == 0) sh.found[warp] = mine;
             __syncthreads();
             last = sh.found[0];
-            for (int w = 1; w < W; ++w)
-                if (before(sh.found[w].score, sh.found[w].at, last.score, last.at)) last = sh.found[w];
+            for (int w = 1; w < warps; ++w)
+                if (before(sh.found[w], last)) last = sh.found[w];
             if (tid == 0) sh.best[i] = last;
         }
     }
@@ -334,25 +311,25 @@ __device__ int best_of(MergeShared& sh, int k, double floor, bool has_floor, Eac
     return min(n, k + 1);
 }
 
-// A CTA per group.
-constexpr int kHeld = 4;  // tiles of a thread that are read once
-
+// A CTA per group; bound by the latency of its steps, one behind the other.
 template <class T>
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restrict__ logits, long long stride, int vocab, int beams,
                                                               const float* __restrict__ scores, const uint8_t* __restrict__ ended,
                                                               int end_id, int k, const Tile* __restrict__ tiles, int row_tiles,
                                                               unsigned row_magic, float* __restrict__ out_scores,
                                                               int* __restrict__ tokens, int* __restrict__ parents) {
-    constexpr int U = kTilePieces, V = 16 / sizeof(T), W = kMergeThreads / 32;
+    constexpr int U = kTilePieces, V = 16 / sizeof(T), kHeld = 2;  // tiles of a thread whose scores are formed once
     // Twice the error of a log sum: of a term 2^-22 (the exponential), ln 2 2^-20 (y above -32), 21 * 1.4e-8 (log2 e as f32); 12 roundings
-    // of a tile's sum; 2^-22 of its weight.  In all below 2.2e-6.
-    constexpr double kNear = 5e-6;
+    // of a tile's sum; 2^-22 of its weight and 8 roundings in the row's.  In all below 2.7e-6.
+    constexpr double kNear = 6e-6;
     extern __shared__ double lse[];                                          // [beams]; NaN: no candidates of this row
     float* score = reinterpret_cast<float*>(lse + beams);                    // [beams]
     unsigned char* state = reinterpret_cast<unsigned char*>(score + beams);  // [beams] 1: the sum is formed again, 2: exactly known, 3: none
     __shared__ MergeShared sh;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = blockIdx.x, r0 = group * beams;
-    for (int b = tid; b < beams; b += kMergeThreads) {
+    __shared__ Found tile_of[kBeamMaxK];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = blockDim.x, warps = threads >> 5;
+    const int group = blockIdx.x, r0 = group * beams;
+    for (int b = tid; b < beams; b += threads) {
         const float sc = __ldg(scores + r0 + b);
         const bool over = ended && __ldg(ended + r0 + b);
         score[b] = sc;
@@ -363,40 +340,31 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
     pdl_wait();
     const int n_tiles = beams * row_tiles;
     const Tile* mine = tiles + size_t(r0) * row_tiles;
-    float held[kHeld];
+    auto row_of = [&](int c) { return row_magic ? int(__umulhi(unsigned(c), row_magic)) : c / row_tiles; };
+    float held_top[kHeld];
+    int held_row[kHeld];
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
-        const int c = tid + u * kMergeThreads;
-        held[u] = c < n_tiles ? __ldcg(&mine[c].top) : -INFINITY;
+        const int c = tid + u * threads;
+        held_row[u] = row_of(c);
+        held_top[u] = c < n_tiles ? __ldcg(&mine[c].top) : -INFINITY;
     }
-    for (int b = warp; b < beams; b += W) {
+    for (int b = warp; b < beams; b += warps) {
         const double l = state[b] ? __longlong_as_double(0x7ff8000000000000ll) : join_sums(mine + size_t(b) * row_tiles, row_tiles);
         if (lane == 0) lse[b] = l;
     }
     __syncthreads();
-    auto row_of = [&](unsigned c) { return row_magic ? int(__umulhi(c, row_magic)) : int(c / unsigned(row_tiles)); };
-    // the largest candidates of the group's tiles, with their numbers
-    auto each_tile = [&](auto&& f) {
-        auto one = [&](int c, float top) {
-            const int b = row_of(c);
-            const double l = lse[b];
-            if (l == l && top != -INFINITY) f(double(score[b]) + (double(top) - l), unsigned(c));
-        };
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-            if (tid + u * kMergeThreads < n_tiles) one(tid + u * kMergeThreads, held[u]);
-        for (int c = tid + kHeld * kMergeThreads; c < n_tiles; c += kMergeThreads) one(c, __ldcg(&mine[c].top));
-        if (ended)
-            for (int b = tid; b < beams; b += kMergeThreads)
-                if (state[b] == 2 && lse[b] != lse[b]) f(double(score[b]), unsigned(b) * unsigned(row_tiles));
+    // the score of a tile's largest logit; NaN: none
+    auto value = [&](int row, float x) {
+        return x == -INFINITY ? __longlong_as_double(0x7ff8000000000000ll) : double(score[row]) + (double(x) - lse[row]);
     };
     // Whether two beams' candidates lie too close to each other in best[0 .. n - 1]; then their sums are formed again.
-    auto settle = [&](int n, unsigned per_row) {
-        for (int i = tid; i + 1 < n; i += kMergeThreads) {
-            const unsigned a = sh.best[i].at / per_row, b = sh.best[i + 1].at / per_row;
-            if (a != b && sh.best[i].score - sh.best[i + 1].score < kNear) {
-                if (state[a] == 0) state[a] = 1, sh.redo = 1;
-                if (state[b] == 0) state[b] = 1, sh.redo = 1;
+    auto settle = [&](int n) {
+        for (int i = tid; i + 1 < n; i += threads) {
+            const Found &a = sh.best[i], &b = sh.best[i + 1];
+            if (a.row != b.row && a.score - b.score < kNear) {
+                if (state[a.row] == 0) state[a.row] = 1, sh.redo = 1;
+                if (state[b.row] == 0) state[b.row] = 1, sh.redo = 1;
             }
         }
         __syncthreads();
@@ -407,14 +375,14 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
             float top = -INFINITY;
             for (int i = 0; i < row_tiles; ++i) top = fmaxf(top, __ldcg(&mine[size_t(b) * row_tiles + i].top));
             double sum = 0;
-            for (int t = tid; t < vocab; t += kMergeThreads) sum += exp(double(to_float(row[t])) - double(top));
-#pragma unroll
+            for (int t = tid; t < vocab; t += threads) sum += exp(double(to_float(row[t])) - double(top));
+#pragma unroll 1
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane == 0) sh.sums[warp] = sum;
             __syncthreads();
             if (tid == 0) {
                 double t = 0;
-                for (int w = 0; w < W; ++w) t += sh.sums[w];
+                for (int w = 0; w < warps; ++w) t += sh.sums[w];
                 lse[b] = double(top) + log(t);
                 state[b] = 2;
             }
@@ -424,22 +392,54 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
         __syncthreads();
         return true;
     };
-    int n = best_of(sh, k, 0., false, each_tile);
-    if (settle(n, unsigned(row_tiles))) n = best_of(sh, k, 0., false, each_tile);
+    // the best tiles, by their largest candidates; an ended beam counts as a tile of one candidate
+    int n;
+    do {
+        double held[kHeld];
+        unsigned top = 0;
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            held[u] = tid + u * threads < n_tiles ? value(held_row[u], held_top[u]) : __longlong_as_double(0x7ff8000000000000ll);
+            if (held[u] == held[u]) top = max(top, order_hi(held[u]));
+        }
+        auto others = [&](auto&& f) {
+            for (int c = tid + kHeld * threads; c < n_tiles; c += threads) {
+                const int row = row_of(c);
+                const double v = value(row, __ldcg(&mine[c].top));
+                if (v == v) f(v, unsigned(c), row);
+            }
+            if (ended)
+                for (int b = tid; b < beams; b += threads)
+                    if (state[b] == 2 && lse[b] != lse[b]) f(double(score[b]), unsigned(b) * unsigned(row_tiles), b);
+        };
+        others([&](double v, unsigned, int) { top = max(top, order_hi(v)); });
+        const unsigned least = threshold_of(sh, k, top);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (held[u] == held[u] && order_hi(held[u]) >= least) push(sh, held[u], unsigned(tid + u * threads), held_row[u]);
+        others([&](double v, unsigned at, int row) {
+            if (order_hi(v) >= least) push(sh, v, at, row);
+        });
+        n = rank_found(sh, k, [&](auto&& f) {
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u)
+                if (held[u] == held[u]) f(held[u], unsigned(tid + u * threads), held_row[u]);
+            others(f);
+        });
+    } while (settle(n));
     // the candidates of the k best tiles that reach the last one's largest
     const int open = min(n, k);
     bool bounded = n >= k;
     const double floor = bounded ? sh.best[k - 1].score : 0.;
-    __shared__ unsigned tile_of[kBeamMaxK];
-    for (int i = tid; i < open; i += kMergeThreads) tile_of[i] = sh.best[i].at;
+    for (int i = tid; i < open; i += threads) tile_of[i] = sh.best[i];
     __syncthreads();
     auto each_token = [&](auto&& f) {
-        for (int c = tid; c < open * 32 * U; c += kMergeThreads) {
-            const unsigned tile = tile_of[c / (32 * U)];
-            const int b = row_of(tile), j = int(tile) - b * row_tiles;
+        for (int c = tid; c < open * 32 * U; c += threads) {
+            const Found& tile = tile_of[c / (32 * U)];
+            const int b = tile.row, j = int(tile.at) - b * row_tiles;
             const double l = lse[b], sc = double(score[b]);
             if (l != l) {  // an ended beam
-                if (c % (32 * U) == 0) f(sc, unsigned(b) * unsigned(vocab) + unsigned(end_id));
+                if (c % (32 * U) == 0) f(sc, unsigned(b) * unsigned(vocab) + unsigned(end_id), b);
                 continue;
             }
             const Row<T> row(logits + (r0 + b) * stride);
@@ -450,25 +450,38 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
 #pragma unroll 1
             for (int i = 0; i < V; ++i) {
                 const float v = first_of<T>(x);
-                if (v != -INFINITY) f(sc + (double(v) - l), unsigned(b) * unsigned(vocab) + unsigned(p * V - row.lead + i));
+                if (v != -INFINITY) f(sc + (double(v) - l), unsigned(b) * unsigned(vocab) + unsigned(p * V - row.lead + i), b);
                 x = next_of<T>(x);
             }
         }
     };
-    n = best_of(sh, k, floor, bounded, each_token);
-    if (settle(n, unsigned(vocab))) {
-        bounded = false;  // (the sums have moved a little)
-        n = best_of(sh, k, 0., false, each_token);
+    for (;; bounded = false) {  // (when the sums have moved a little, so may the bound)
+        if (bounded) {
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            each_token([&](double v, unsigned at, int row) {
+                if (v >= floor) push(sh, v, at, row);
+            });
+        } else {
+            unsigned top = 0;
+            each_token([&](double v, unsigned, int) { top = max(top, order_hi(v)); });
+            const unsigned least = threshold_of(sh, k, top);
+            each_token([&](double v, unsigned at, int row) {
+                if (order_hi(v) >= least) push(sh, v, at, row);
+            });
+        }
+        n = rank_found(sh, k, each_token);
+        if (!settle(n)) break;
     }
     const int have = min(n, k);
     out_scores += size_t(group) * k;
     tokens += size_t(group) * k;
     parents += size_t(group) * k;
-    for (int i = tid; i < have; i += kMergeThreads) {
-        const unsigned b = sh.best[i].at / unsigned(vocab);
-        out_scores[i] = float(sh.best[i].score);
-        parents[i] = int(b);
-        tokens[i] = int(sh.best[i].at - b * unsigned(vocab));
+    for (int i = tid; i < have; i += threads) {
+        const Found f = sh.best[i];
+        out_scores[i] = float(f.score);
+        parents[i] = f.row;
+        tokens[i] = int(f.at - unsigned(f.row) * unsigned(vocab));
     }
     // fewer than k: all that are left are -inf, in order of their places; the first k places hold at most `have` of the best
     if (have < k && warp == 0) {
@@ -502,8 +515,11 @@ cudaError_t select_t(const BeamArgs& a, Tile* ws, cudaStream_t st) {
                                static_cast<const T*>(a.logits), a.stride, a.vocab, a.scores, a.ended, row_tiles, tiles, ws);
     if (e != cudaSuccess) return e;
     // c / row_tiles = umulhi(c, ceil(2^32 / row_tiles)) for both below 2^16, row_tiles > 1
-    const bool small = (long long)a.beams * row_tiles < 65536 && row_tiles > 1;
-    return launch_pdl(k_beam_merge<T>, dim3(unsigned(a.groups)), dim3(kMergeThreads), size_t(a.beams) * 13, st, true,
+    const bool small = (long long)a.beams * row_tiles + 2 * kMergeThreads < 65536 && row_tiles > 1;
+    // threads for a tile or two each, as far as that leaves the SMs a CTA per group
+    const int work = a.beams * row_tiles > 128 * a.k ? a.beams * row_tiles : 128 * a.k;
+    const int threads = work > 1024 && a.groups <= 2 * 148 ? 1024 : work > 512 ? 512 : 256;
+    return launch_pdl(k_beam_merge<T>, dim3(unsigned(a.groups)), dim3(unsigned(threads)), size_t(a.beams) * 13, st, true,
                       static_cast<const T*>(a.logits), a.stride, a.vocab, a.beams, a.scores, a.ended, a.end_id, a.k,
                       static_cast<const Tile*>(ws), row_tiles, small ? unsigned((0x100000000ULL + row_tiles - 1) / row_tiles) : 0u,
                       a.out_scores, a.tokens, a.parents);
