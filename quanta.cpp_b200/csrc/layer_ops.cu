@@ -1,4 +1,6 @@
 // RMS norm with the residual's addition and 8-bit rows out, values of 8-bit rows, rotary positions (layer_ops.h).
+#include <type_traits>
+
 #include "layer_ops.h"
 #include "rows.cuh"
 
@@ -11,87 +13,118 @@ bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>
 // ---------------------------------------------------------------- RMS norm to 8-bit rows
 
 // With h = x + r (r: the residual row, h rounded once into it):
-//     y = h * (1 / sqrt(mean h^2 + eps)) * w;  per 32 values: d = max |y| / 127, q = y * (1 / d) to the nearest, halves away from 0
+//     y = h * (1 / sqrt(mean h^2 + eps)) * w;  per 32 values: d = max |y| / 127, q = y / d to the nearest, halves away from 0
 // A CTA per row, which stays in registers between the sum and the rounding: every byte crosses HBM once.  A thread holds R chunks
 // of 8 consecutive values, so that a block of 32 is 4 neighbouring lanes and its maximum two shuffles.  Sums in f32: per thread,
-// then per warp, then over warps (an error of a few 2^-24).  A block with a value that is not finite gets a scale that is not and
-// codes 0: it reads as NaN.
+// then per warp, then over warps (an error of a few 2^-24).  A block with a value that is not finite gets a NaN for its scale.  Next to HBM instructions bound it, so values go in pairs (f32x2), and a code is the low byte of t + 1.5 * 2^23:
+// with t = y * (1 / d, one step up) that addition rounds to the nearest, halves away from 0 as far as t says where they are.
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 8 elements as 4 pairs of f32, and back with one rounding.
+template <class T>
+__device__ __forceinline__ void load_pairs(const T* p, unsigned long long (&x)[4], bool aligned) {
+    float v[8];
+    load_row(p, v, aligned);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = f2_pack(v[2 * i], v[2 * i + 1]);
+}
+template <class T>
+__device__ __forceinline__ void store_pairs(T* p, const unsigned long long (&x)[4], bool aligned) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = f2_unpack(x[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+    store_row(p, v, aligned);
+}
+
 template <class T, class RT, int R, bool VEC>
-__global__ void __launch_bounds__(1024) k_rms_norm_q8(const T* __restrict__ x, long long x_stride, RT* __restrict__ residual,
-                                                      long long residual_stride, const float* __restrict__ weight, float eps,
-                                                      int n, int8_t* __restrict__ q, float* __restrict__ d) {
+__global__ void __launch_bounds__(R == 4 ? 1024 : 512)
+    k_rms_norm_q8(const T* __restrict__ x, long long x_stride, RT* __restrict__ residual, long long residual_stride,
+                  const float* __restrict__ weight, float eps, int n, int8_t* __restrict__ q, float* __restrict__ d) {
     constexpr int C = 8;
     __shared__ float part[32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = n / C;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = n / C, threads = blockDim.x;
     const T* xr = x + blockIdx.x * x_stride;
     RT* rr = residual ? residual + blockIdx.x * residual_stride : nullptr;
-    float h[R][C], w[R][C];
+    unsigned long long h[R][4];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int c = r * int(blockDim.x) + tid;
+        const int c = r * threads + tid;
         if (c < chunks) {
-            load_row(xr + c * C, h[r], VEC);
+            load_pairs(xr + c * C, h[r], VEC);
         } else {
 #pragma unroll
-            for (int i = 0; i < C; ++i) h[r][i] = 0.f;
+            for (int i = 0; i < 4; ++i) h[r][i] = 0;
         }
     }
     if (rr) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int c = r * int(blockDim.x) + tid;
+            const int c = r * threads + tid;
             if (c < chunks) {
-                float b[C];
-                load_row(rr + c * C, b, VEC);
+                unsigned long long b[4];
+                load_pairs(rr + c * C, b, VEC);
 #pragma unroll
-                for (int i = 0; i < C; ++i) h[r][i] = fadd(h[r][i], b[i]);
+                for (int i = 0; i < 4; ++i) h[r][i] = f2_add(h[r][i], b[i]);
+                store_pairs(rr + c * C, h[r], VEC);
             }
         }
     }
+    unsigned long long squares = f2_pack(0.f, 0.f);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int c = r * int(blockDim.x) + tid;
-        if (c < chunks) load_row(weight + c * C, w[r], VEC);
-    }
-    float sum = 0.f;
+        unsigned long long s = f2_mul(h[r][0], h[r][0]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < C; ++i) s = fmaf(h[r][i], h[r][i], s);
-        sum += s;
+        for (int i = 1; i < 4; ++i) s = f2_fma(h[r][i], h[r][i], s);
+        squares = r ? f2_add(squares, s) : s;
     }
-    sum = warp_sum(sum);
-    if (blockDim.x > 32) {
+    const float2 both = f2_unpack(squares);
+    float sum = warp_sum(both.x + both.y);
+    if (threads > 32) {
         if (lane == 0) part[warp] = sum;
         __syncthreads();
-        sum = warp_sum(lane < int(blockDim.x >> 5) ? part[lane] : 0.f);
+        sum = warp_sum(lane < threads >> 5 ? part[lane] : 0.f);
     }
     const float inv = __frsqrt_rn(sum / float(n) + eps);
+    const unsigned long long inv2 = f2_pack(inv, inv), magic = f2_pack(12582912.f, 12582912.f);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int c = r * int(blockDim.x) + tid;
+        const int c = r * threads + tid;
         const bool in = c < chunks;
-        float top = 0.f, y[C];
-        if (in && rr) store_row(rr + c * C, h[r], VEC);
+        unsigned long long w[4];
+        if (in) load_pairs(weight + c * C, w, VEC);
+        float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            y[i] = in ? h[r][i] * inv * w[r][i] : 0.f;
-            top = max_or_nan(top, fabsf(y[i]));
+        for (int i = 0; i < 4; ++i) {
+            w[i] = in ? f2_mul(f2_mul(h[r][i], inv2), w[i]) : 0;  // y
+            const float2 y = f2_unpack(w[i]);
+            top = max_or_nan(top, max_or_nan(fabsf(y.x), fabsf(y.y)));
         }
         top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float scale = div127(top), up = scale > 0.f ? __frcp_rn(scale) : 0.f;
-        const bool fine = top <= 3.402823466e38f && up <= 3.402823466e38f;
-        uint2 codes = make_uint2(0, 0);
+        const float scale = div127(top), step = scale > 0.f ? __frcp_rn(scale) : 0.f;
+        const float up = step > 0.f && step <= 3.402823466e38f ? __uint_as_float(__float_as_uint(step) + 1) : 0.f;
+        const unsigned long long up2 = f2_pack(up, up);
+        unsigned b[8];
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const unsigned b = unsigned(fine ? round_away(fmul(y[i], up)) : 0) & 0xff;
-            (i < 4 ? codes.x : codes.y) |= b << (i % 4 * 8);
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = f2_unpack(f2_add(f2_mul(w[i], up2), magic));
+            b[2 * i] = __float_as_uint(t.x);
+            b[2 * i + 1] = __float_as_uint(t.y);
         }
         if (in) {
+            uint2 codes;
+            codes.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            codes.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
             *reinterpret_cast<uint2*>(q + size_t(blockIdx.x) * n + c * C) = codes;
-            if ((lane & 3) == 0) d[size_t(blockIdx.x) * (n / QK) + c / 4] = scale;
+            if ((lane & 3) == 0) d[size_t(blockIdx.x) * (n / QK) + c / 4] = top <= 3.402823466e38f ? scale : __int_as_float(0x7fc00000);
         }
     }
 }
@@ -114,25 +147,45 @@ cudaError_t norm_t(const NormQ8Args& a, cudaStream_t st) {
 
 // ---------------------------------------------------------------- values of 8-bit rows
 
-// 16 codes (half a block) a thread.
+// 16 bytes of output a thread and step, so that a warp writes whole lines; kDequantAhead steps in flight.  Bound by HBM.
+constexpr int kDequantAhead = 4;
+
 template <class T>
-__global__ void __launch_bounds__(256) k_dequantize_q8(const int8_t* __restrict__ q, const float* __restrict__ d, long long halves,
+__global__ void __launch_bounds__(256) k_dequantize_q8(const int8_t* __restrict__ q, const float* __restrict__ d, long long pieces,
                                                        T* __restrict__ out) {
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= halves) return;
-    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(q) + i);
-    const float s = __ldcs(d + i / 2);
-    const unsigned words[4] = {w.x, w.y, w.z, w.w};
-    float v[16];
+    constexpr int V = 16 / sizeof(T);
+    using Codes = typename std::conditional<V == 8, uint2, unsigned>::type;
+    const long long first = (long long)blockIdx.x * (256 * kDequantAhead) + threadIdx.x;
+    Codes w[kDequantAhead];
+    float s[kDequantAhead];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = fmul(float(int8_t(words[j / 4] >> (j % 4 * 8))), s);
-    store_row(out + i * 16, v, true);
+    for (int u = 0; u < kDequantAhead; ++u) {
+        const long long i = first + u * 256;
+        if (i < pieces) {
+            w[u] = __ldg(reinterpret_cast<const Codes*>(q) + i);
+            s[u] = __ldg(d + i / (QK / V));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kDequantAhead; ++u) {
+        const long long i = first + u * 256;
+        if (i >= pieces) continue;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            unsigned word;
+            if constexpr (V == 8) word = j < 4 ? w[u].x : w[u].y;
+            else word = w[u];
+            v[j] = fmul(float(int8_t(word >> (j % 4 * 8))), s[u]);
+        }
+        store_row(out + i * V, v, true);
+    }
 }
 
 template <class T>
 cudaError_t dequantize_t(const int8_t* q, const float* d, long long n, void* out, cudaStream_t st) {
-    const long long halves = n / 16;
-    return launch_pdl(k_dequantize_q8<T>, dim3(unsigned((halves + 255) / 256)), dim3(256), 0, st, false, q, d, halves,
+    const long long pieces = n * sizeof(T) / 16, per = 256 * kDequantAhead;
+    return launch_pdl(k_dequantize_q8<T>, dim3(unsigned((pieces + per - 1) / per)), dim3(256), 0, st, false, q, d, pieces,
                       static_cast<T*>(out));
 }
 
