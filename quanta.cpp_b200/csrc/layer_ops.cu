@@ -237,13 +237,12 @@ cudaError_t dequantize_t(const int8_t* q, const float* d, long long n, void* out
 
 // Pair (a, b) of a head's first rotary_dim dims at position p: (a cos - b sin, a sin + b cos) * scale at p * turns[i] revolutions;
 // pairs are (i, i + rotary_dim / 2) or (2 i, 2 i + 1).  The revolution count is formed in 64 bits and only its fraction becomes
-// f32, so that an angle is as exact at position 2^31 as at the start.  A CTA takes a few tokens: their cosines and sines go to
-// shared memory once, then all heads of q and k pass through registers, V elements of 16 bytes at a time.  Bound by HBM.
-constexpr int kRopeThreads = 256;
-constexpr int kRopeAhead = 4;  // tasks of a thread whose loads are in flight together
-
-// d = quotient: by a multiplication where the numbers are small (magic != 0), see rope_v.
-__device__ __forceinline__ int quotient(int n, int d, unsigned magic) { return magic ? int(__umulhi(unsigned(n), magic)) : n / d; }
+// f32, so that an angle is as exact at position 2^31 as at the start.  A thread has a token and a unit of its heads (interleaved:
+// V dims of 16 bytes; half layout: V dims and the V that they turn with), forms these pairs' cosines and sines once and takes one
+// head after another, 64 bytes of them in flight; `slots` threads share the heads of a token.  Bound by HBM: 8192 tokens of 32 + 8
+// bf16 heads of 128: 28.9 us, 5.8 TB/s (128 bytes in flight: 44, too many registers; without streaming stores 44; cosines and
+// sines of a CTA's tokens in shared memory and a task of any head: 57).
+constexpr int kRopeThreads = 128;
 
 // VEC: V elements are one access; else they are read one by one.
 template <class T, int V, bool VEC>
@@ -259,7 +258,9 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
 }
 template <class T, int V, bool VEC>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& w) {
-    if constexpr (VEC) {
+    if constexpr (VEC && sizeof(w) == 16) {
+        __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&w));
+    } else if constexpr (VEC) {
         *reinterpret_cast<Pack<T, V>*>(p) = w;
     } else {
 #pragma unroll
@@ -268,84 +269,90 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& w) {
 }
 
 template <class T, int V, bool INTER, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads) k_rope(RopeHeads qh, RopeHeads kh, int head_dim, int rotary_dim, int n_tok,
-                                                       int tok_per_cta, const int* __restrict__ positions,
-                                                       const double* __restrict__ turns, float scale, int units,
-                                                       unsigned units_magic, unsigned heads_magic) {
-    extern __shared__ float2 cs[];  // [tok_per_cta][rotary_dim / 2]
-    const int pairs = rotary_dim / 2, t0 = blockIdx.x * tok_per_cta, toks = min(tok_per_cta, n_tok - t0);
-    for (int t = 0; t < toks; ++t) {
-        const double p = double(__ldg(positions + t0 + t));
-        for (int i = threadIdx.x; i < pairs; i += kRopeThreads) {
-            const double turn = p * __ldg(turns + i);
-            float s, c;
-            sincospif(2.f * float(turn - rint(turn)), &s, &c);
-            cs[t * pairs + i] = make_float2(c * scale, s * scale);
+__global__ void __launch_bounds__(kRopeThreads) k_rope(RopeHeads qh, RopeHeads kh, int head_dim, int rotary_dim, int n_tok, int slots,
+                                                       const int* __restrict__ positions, const double* __restrict__ turns, float scale,
+                                                       int units) {
+    constexpr int P = INTER ? V / 2 : V, AHEAD = INTER ? 4 : 2;  // pairs of a unit, heads in flight
+    const int pairs = rotary_dim / 2, n_rot = INTER ? rotary_dim / V : pairs / V;
+    // thread -> token, slot, unit; units: rotated ones first, then ones (half layout: two) of V dims that are only copied
+    const long long id = (long long)blockIdx.x * kRopeThreads + threadIdx.x;
+    const int per = slots * units, t = int(id / per), in_tok = int(id - (long long)t * per), slot = in_tok / units, u = in_tok - slot * units;
+    if (t >= n_tok) return;
+    const bool rot = u < n_rot;
+    const int at = rot ? u * V : rotary_dim + (u - n_rot) * V, other = rot ? pairs : (units - n_rot) * V;
+    const bool two = !INTER && at + other < head_dim;
+    float c[P], s[P];
+    if (rot) {
+        const double p = double(__ldg(positions + t));
+        const double* turn = turns + (INTER ? at / 2 : at);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const double n = p * __ldg(turn + i);
+            sincospif(2.f * float(n - rint(n)), &s[i], &c[i]);
+            c[i] *= scale;
+            s[i] *= scale;
         }
     }
-    __syncthreads();
-    // a task: a unit of a head; units: rotated ones first (INTER: V elements, else V elements of either half), then V elements that
-    // are only copied
-    const int heads = qh.heads + kh.heads, n_rot = INTER ? rotary_dim / V : pairs / V, tasks = toks * heads * units;
-    for (int task0 = threadIdx.x; task0 < tasks; task0 += kRopeThreads * kRopeAhead) {
-        Pack<T, V> lo[kRopeAhead], hi[kRopeAhead];
-        T* to[kRopeAhead];
-        int trig[kRopeAhead];  // -1: copied
+    auto heads = [&](const RopeHeads& h) {
+        const T* from = static_cast<const T*>(h.in) + t * h.in_stride + at;
+        T* to = static_cast<T*>(h.out) + t * h.out_stride + at;
+#pragma unroll 1
+        for (int h0 = slot; h0 < h.heads; h0 += slots * AHEAD) {
+            Pack<T, V> lo[AHEAD], hi[AHEAD];
 #pragma unroll
-        for (int a = 0; a < kRopeAhead; ++a) {
-            const int task = task0 + a * kRopeThreads;
-            if (task >= tasks) break;
-            const int row = quotient(task, units, units_magic), u = task - row * units;
-            const int t = quotient(row, heads, heads_magic), h = row - t * heads;
-            const bool is_q = h < qh.heads, rot = u < n_rot;
-            const int at = (is_q ? h : h - qh.heads) * head_dim + (rot ? u * V : rotary_dim + (u - n_rot) * V);
-            const T* from = static_cast<const T*>(is_q ? qh.in : kh.in) + (t0 + t) * (is_q ? qh.in_stride : kh.in_stride) + at;
-            to[a] = static_cast<T*>(is_q ? qh.out : kh.out) + (t0 + t) * (is_q ? qh.out_stride : kh.out_stride) + at;
-            trig[a] = rot ? t * pairs + (INTER ? u * V / 2 : u * V) : -1;
-            lo[a] = load_pack<T, V, VEC>(from);
-            if (!INTER && rot) hi[a] = load_pack<T, V, VEC>(from + pairs);
-        }
-#pragma unroll
-        for (int a = 0; a < kRopeAhead; ++a) {
-            if (task0 + a * kRopeThreads >= tasks) break;
-            if (trig[a] >= 0) {
-                if constexpr (INTER) {
-#pragma unroll
-                    for (int i = 0; i < V; i += 2) {
-                        const float2 r = cs[trig[a] + i / 2];
-                        const float x = to_float(lo[a].v[i]), y = to_float(lo[a].v[i + 1]);
-                        lo[a].v[i] = from_float<T>(fmaf(x, r.x, -(y * r.y)));
-                        lo[a].v[i + 1] = from_float<T>(fmaf(x, r.y, y * r.x));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float2 r = cs[trig[a] + i];
-                        const float x = to_float(lo[a].v[i]), y = to_float(hi[a].v[i]);
-                        lo[a].v[i] = from_float<T>(fmaf(x, r.x, -(y * r.y)));
-                        hi[a].v[i] = from_float<T>(fmaf(x, r.y, y * r.x));
-                    }
-                    store_pack<T, V, VEC>(to[a] + pairs, hi[a]);
+            for (int a = 0; a < AHEAD; ++a)
+                if (h0 + a * slots < h.heads) {
+                    const T* x = from + (h0 + a * slots) * head_dim;
+                    lo[a] = load_pack<T, V, VEC>(x);
+                    if (two) hi[a] = load_pack<T, V, VEC>(x + other);
                 }
-            }
-            store_pack<T, V, VEC>(to[a], lo[a]);
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a)
+                if (h0 + a * slots < h.heads) {
+                    T* y = to + (h0 + a * slots) * head_dim;
+                    if (rot) {
+                        float x[V], z[V];
+                        to_floats(lo[a], x);
+                        if constexpr (INTER) {
+#pragma unroll
+                            for (int i = 0; i < P; ++i) {
+                                const float v = x[2 * i], w = x[2 * i + 1];
+                                x[2 * i] = fmaf(v, c[i], -(w * s[i]));
+                                x[2 * i + 1] = fmaf(v, s[i], w * c[i]);
+                            }
+                        } else {
+                            to_floats(hi[a], z);
+#pragma unroll
+                            for (int i = 0; i < P; ++i) {
+                                const float v = x[i], w = z[i];
+                                x[i] = fmaf(v, c[i], -(w * s[i]));
+                                z[i] = fmaf(v, s[i], w * c[i]);
+                            }
+                            hi[a] = from_floats(z, T());
+                        }
+                        lo[a] = from_floats(x, T());
+                    }
+                    store_pack<T, V, VEC>(y, lo[a]);
+                    if (two) store_pack<T, V, VEC>(y + other, hi[a]);
+                }
         }
-    }
+    };
+    heads(qh);
+    heads(kh);
 }
 
 template <class T, int V, bool INTER, bool VEC>
 cudaError_t rope_v(const RopeArgs& a, cudaStream_t st) {
-    const int heads = a.q.heads + a.k.heads, pairs = a.rotary_dim / 2;
-    const bool in_place = a.q.in == a.q.out && a.k.in == a.k.out;
-    const int units = (INTER ? a.rotary_dim : pairs) / V + (in_place ? 0 : (a.head_dim - a.rotary_dim) / V);
-    int per = 1;  // tokens of a CTA: until every SM has several CTAs of it, while a CTA's tasks are few
-    while (per < 8 && a.n_tok / (2 * per) >= 8 * 148 && 2 * per * heads * units <= 8 * kRopeThreads) per *= 2;
-    const bool small = per * heads * units < 65536;  // n / d = umulhi(n, ceil(2^32 / d)) for n, d < 2^16, d > 1
-    const unsigned um = small && units > 1 ? unsigned((0x100000000ULL + units - 1) / units) : 0;
-    const unsigned hm = small && heads > 1 ? unsigned((0x100000000ULL + heads - 1) / heads) : 0;
-    return launch_pdl(k_rope<T, V, INTER, VEC>, dim3(unsigned((a.n_tok + per - 1) / per)), dim3(kRopeThreads),
-                      size_t(per) * pairs * sizeof(float2), st, false, a.q, a.k, a.head_dim, a.rotary_dim, a.n_tok, per, a.positions,
-                      a.turns, a.scale, units, um, hm);
+    const int most = a.q.heads > a.k.heads ? a.q.heads : a.k.heads;
+    const int copied = a.q.in == a.q.out && a.k.in == a.k.out ? 0 : (a.head_dim - a.rotary_dim) / V;
+    const int units = INTER ? a.rotary_dim / V + copied : a.rotary_dim / 2 / V + (copied + 1) / 2;
+    int slots = 1;  // threads that share a token's heads: until there are threads enough for every SM
+    while (slots < most && (long long)a.n_tok * slots * units < 148 * 1024) slots *= 2;
+    if (slots > most) slots = most;
+    const long long threads = (long long)a.n_tok * slots * units, ctas = (threads + kRopeThreads - 1) / kRopeThreads;
+    if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_pdl(k_rope<T, V, INTER, VEC>, dim3(unsigned(ctas)), dim3(kRopeThreads), 0, st, false, a.q, a.k, a.head_dim, a.rotary_dim,
+                      a.n_tok, slots, a.positions, a.turns, a.scale, units);
 }
 
 template <class T, int V>

@@ -32,6 +32,42 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
     T v[N];
 };
 
+// The elements as floats, and floats with one rounding each, two 16-bit ones in one conversion.
+template <class T, int N>
+__device__ __forceinline__ void to_floats(const Pack<T, N>& w, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_float(w.v[i]);
+}
+template <int N>
+__device__ __forceinline__ Pack<float, N> from_floats(const float (&x)[N], float) {
+    Pack<float, N> w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w.v[i] = x[i];
+    return w;
+}
+template <int N>
+__device__ __forceinline__ Pack<__half, N> from_floats(const float (&x)[N], __half) {
+    Pack<__half, N> w;
+    if constexpr (N == 1) {
+        w.v[0] = __float2half_rn(x[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<__half2*>(&w.v[i]) = __floats2half2_rn(x[i], x[i + 1]);
+    }
+    return w;
+}
+template <int N>
+__device__ __forceinline__ Pack<__nv_bfloat16, N> from_floats(const float (&x)[N], __nv_bfloat16) {
+    Pack<__nv_bfloat16, N> w;
+    if constexpr (N == 1) {
+        w.v[0] = __float2bfloat16_rn(x[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<__nv_bfloat162*>(&w.v[i]) = __floats2bfloat162_rn(x[i], x[i + 1]);
+    }
+    return w;
+}
+
 template <class T, int N>
 __device__ __forceinline__ void load_row(const T* p, float (&x)[N], bool aligned) {
     if (aligned) {
@@ -47,10 +83,7 @@ __device__ __forceinline__ void load_row(const T* p, float (&x)[N], bool aligned
 template <class T, int N>
 __device__ __forceinline__ void store_row(T* p, const float (&x)[N], bool aligned) {
     if (aligned) {
-        Pack<T, N> w;
-#pragma unroll
-        for (int i = 0; i < N; ++i) w.v[i] = from_float<T>(x[i]);
-        *reinterpret_cast<Pack<T, N>*>(p) = w;
+        *reinterpret_cast<Pack<T, N>*>(p) = from_floats(x, T());
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) p[i] = from_float<T>(x[i]);
