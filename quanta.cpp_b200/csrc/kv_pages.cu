@@ -494,50 +494,44 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
 // Reorder, first half.  Sequence i of the list takes over what sequence parent(i) = i - i % group + parents[i] of it held before
 // the call.  Of a parent's children one is the heir of its part-filled page: the parent itself if it goes on, else the first;
 // the others get copies in fresh pages.  plan[0] = copies (-1: the call is refused), plan[1 + 3 r ..] = {from, to, blocks of 16
-// positions} of copy r.  rows, len: workspace for the list's new table rows and lengths, all read before one is written.  Pages that no
-// sequence uses any more are free for the copies of the same call.
+// positions} of copy r.  rows, far_len: workspace for the list's new table rows, which are all read before one is written, and for its
+// lengths where shared memory does not hold them (LEN).  Pages that no sequence uses any more are free for the copies of the same
+// call.  One CTA, bound by latency: what an entry needs is looked up by a thread each, once, and a warp has the table rows of
+// kReorderAhead entries in flight (256 sequences of up to 32 pages: 7 us; entry by entry 15).
+constexpr int kReorderAhead = 4;
+
+template <bool LEN>
 __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, const int* __restrict__ seqs,
                                                                   const int* __restrict__ parents, int n, int group,
                                                                   int* __restrict__ plan, int* __restrict__ rows,
-                                                                  int* __restrict__ len, int* __restrict__ list) {
+                                                                  int* __restrict__ far_len) {
     extern __shared__ __align__(16) unsigned smem[];
     pdl_launch_dependents();
     unsigned* words = smem;
-    int* mark = reinterpret_cast<int*>(words + plan_words(c));
-    int* heir = mark + c.max_seqs;  // of each place of the list: who gets its part-filled page
-    uint16_t* base = reinterpret_cast<uint16_t*>(heir + n);  // copies of entries 0 .. i (at most kKvMaxSeqs)
+    int* heir = reinterpret_cast<int*>(words + plan_words(c));  // of each place of the list: who gets its part-filled page
+    int* len = LEN ? heir + n : far_len;                        // of each place, before the call
+    uint16_t* seq = reinterpret_cast<uint16_t*>(heir + (LEN ? 2 : 1) * n);
+    uint16_t* par = seq + n;   // places of the parents
+    uint16_t* base = par + n;  // copies of entries 0 .. i (at most kKvMaxSeqs)
+    __shared__ unsigned mark[kKvMaxSeqs / 32];
     __shared__ int bad;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     if (tid == 0) bad = 0;
-    for (int s = tid; s < c.max_seqs; s += blockDim.x) mark[s] = 0;
+    for (int s = tid; s < kKvMaxSeqs / 32; s += blockDim.x) mark[s] = 0;
     for (int i = tid; i < n; i += blockDim.x) heir[i] = INT_MAX;
     __syncthreads();
-    auto parent = [&](int i) { return i - i % group + parents[i]; };
     for (int i = tid; i < n; i += blockDim.x) {
         const int s = seqs[i], p = parents[i];
-        if (s < 0 || s >= c.max_seqs || p < 0 || p >= group || atomicExch(mark + s, 1)) {
+        if (s < 0 || s >= c.max_seqs || p < 0 || p >= group || (atomicOr(mark + s / 32, 1u << s % 32) >> s % 32 & 1)) {
             bad = int(ERR_BAD_POS);
             continue;
         }
-        const int l = c.lens[s];
+        const int l = c.lens[s], j = i - i % group + p;
         if (l < 0 || l > c.max_pages << c.pt_shift) bad = int(ERR_BAD_POS);
-        const int j = parent(i);
+        seq[i] = uint16_t(s);
+        par[i] = uint16_t(j);
+        len[i] = l;
         atomicMin(heir + j, j == i ? -1 : i);  // (-1: itself)
-    }
-    __syncthreads();
-    const int per = (n + int(blockDim.x) - 1) / int(blockDim.x);
-    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    int want = 0;
-    if (!bad) {
-        int mine = 0;
-        for (int i = i0; i < i1; ++i) {
-            const int j = parent(i);
-            len[i] = c.lens[seqs[j]];
-            mine += (len[i] & (c.pt - 1)) && heir[j] != (j == i ? -1 : i);
-            base[i] = uint16_t(mine);
-        }
-        const int before = cta_scan(mine, &want);
-        for (int i = i0; i < i1; ++i) base[i] = uint16_t(base[i] + before);
     }
     __syncthreads();
     if (bad) {
@@ -547,31 +541,70 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         }
         return;
     }
+    const int per = (n + int(blockDim.x) - 1) / int(blockDim.x);
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    int mine = 0, want;
+    for (int i = i0; i < i1; ++i) {
+        const int j = par[i];
+        mine += (len[j] & (c.pt - 1)) && heir[j] != (j == i ? -1 : i);
+        base[i] = uint16_t(mine);
+    }
+    const int before = cta_scan(mine, &want);
+    for (int i = i0; i < i1; ++i) base[i] = uint16_t(base[i] + before);
+    __syncthreads();
+    // entry i: changed, gets a copy, pages before and after
+    struct Entry {
+        bool changed, copy;
+        int n_old, n_now, r;
+    };
+    auto entry = [&](int i) {
+        Entry e{false, false, 0, 0, 0};
+        if (i < n) {
+            e.r = i ? base[i - 1] : 0;
+            e.copy = base[i] != e.r;
+            e.changed = par[i] != i || e.copy;
+            e.n_old = (len[i] + c.pt - 1) >> c.pt_shift;
+            e.n_now = (len[par[i]] + c.pt - 1) >> c.pt_shift;
+        }
+        return e;
+    };
     // the pages that the rows lose and gain; sign -1 takes it back
     auto count = [&](int sign) {
-        for (int i = warp; i < n; i += warps) {
-            const int j = parent(i);
-            const bool copy = base[i] != (i ? base[i - 1] : 0);
-            if (j == i && !copy) continue;
-            const int* old = c.table + size_t(seqs[i]) * c.max_pages;
-            const int* now = c.table + size_t(seqs[j]) * c.max_pages;
-            const int n_now = (len[i] + c.pt - 1) >> c.pt_shift, n_old = (c.lens[seqs[i]] + c.pt - 1) >> c.pt_shift;
-            for (int k = lane; k < max(n_old, n_now); k += 32) {
-                const int a = k < n_old ? old[k] : -1;
-                int b = k < n_now ? now[k] : -1;
-                if (sign > 0) rows[size_t(i) * c.max_pages + k] = b;
-                if (copy && k == n_now - 1) {
-                    if (sign > 0 && (b < 0 || b >= c.n_pages)) bad = int(ERR_BAD_POS);
-                    b = -1;  // a fresh page
-                }
-                if (a == b) continue;
-                if (a >= 0 && a < c.n_pages) atomicSub(c.refs + a, sign);
-                if (b >= 0 && b < c.n_pages) atomicAdd(c.refs + b, sign);
+        auto one = [&](const Entry& e, int i, int k, int a, int b) {
+            if (sign > 0) rows[size_t(i) * c.max_pages + k] = b;
+            if (e.copy && k == e.n_now - 1) {
+                if (sign > 0 && (b < 0 || b >= c.n_pages)) bad = int(ERR_BAD_POS);
+                b = -1;  // a fresh page
+            }
+            if (a == b) return;
+            if (a >= 0 && a < c.n_pages) atomicSub(c.refs + a, sign);
+            if (b >= 0 && b < c.n_pages) atomicAdd(c.refs + b, sign);
+        };
+        for (int i0 = warp; i0 < n; i0 += warps * kReorderAhead) {
+            int a[kReorderAhead], b[kReorderAhead];
+#pragma unroll
+            for (int u = 0; u < kReorderAhead; ++u) {
+                const int i = i0 + u * warps;
+                const Entry e = entry(i);
+                a[u] = e.changed && lane < e.n_old ? c.table[size_t(seq[i]) * c.max_pages + lane] : -1;
+                b[u] = e.changed && lane < e.n_now ? c.table[size_t(seq[par[i]]) * c.max_pages + lane] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < kReorderAhead; ++u) {
+                const int i = i0 + u * warps;
+                const Entry e = entry(i);
+                if (!e.changed) continue;
+                const int most = max(e.n_old, e.n_now);
+                if (lane < most) one(e, i, lane, a[u], b[u]);
+                for (int k = lane + 32; k < most; k += 32)
+                    one(e, i, k, k < e.n_old ? c.table[size_t(seq[i]) * c.max_pages + k] : -1,
+                        k < e.n_now ? c.table[size_t(seq[par[i]]) * c.max_pages + k] : -1);
             }
         }
     };
     count(1);
     __syncthreads();
+    int* list = heir;  // fresh pages
     if (!bad && want > 0 && lowest_free(c, words, want, list) < want && tid == 0) bad = int(ERR_CAPACITY);
     __syncthreads();
     if (bad) {
@@ -582,25 +615,33 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         }
         return;
     }
-    for (int i = warp; i < n; i += warps) {
-        const int j = parent(i), r = (i ? base[i - 1] : 0);
-        const bool copy = base[i] != r;
-        if (j == i && !copy) continue;
-        int* row = c.table + size_t(seqs[i]) * c.max_pages;
-        const int n_now = (len[i] + c.pt - 1) >> c.pt_shift, n_old = (c.lens[seqs[i]] + c.pt - 1) >> c.pt_shift;
-        for (int k = lane; k < max(n_old, n_now); k += 32) {
-            int p = rows[size_t(i) * c.max_pages + k];
-            if (copy && k == n_now - 1) {
-                plan[1 + 3 * r] = p;
-                p = list[r];
-                plan[2 + 3 * r] = p;
-                plan[3 + 3 * r] = ((len[i] & (c.pt - 1)) + kKvBlock - 1) / kKvBlock;
-                c.refs[p] = 1;
-            }
-            row[k] = p;
+    for (int i0 = warp; i0 < n; i0 += warps * kReorderAhead) {
+        int p[kReorderAhead];
+#pragma unroll
+        for (int u = 0; u < kReorderAhead; ++u) {
+            const int i = i0 + u * warps;
+            const Entry e = entry(i);
+            p[u] = e.changed && lane < max(e.n_old, e.n_now) ? rows[size_t(i) * c.max_pages + lane] : -1;
         }
-        __syncwarp();
-        if (lane == 0) c.lens[seqs[i]] = len[i];
+#pragma unroll
+        for (int u = 0; u < kReorderAhead; ++u) {
+            const int i = i0 + u * warps;
+            const Entry e = entry(i);
+            if (!e.changed) continue;
+            int* row = c.table + size_t(seq[i]) * c.max_pages;
+            for (int k = lane; k < max(e.n_old, e.n_now); k += 32) {
+                int page = k == lane ? p[u] : rows[size_t(i) * c.max_pages + k];
+                if (e.copy && k == e.n_now - 1) {
+                    plan[1 + 3 * e.r] = page;
+                    page = list[e.r];
+                    plan[2 + 3 * e.r] = page;
+                    plan[3 + 3 * e.r] = ((len[par[i]] & (c.pt - 1)) + kKvBlock - 1) / kKvBlock;
+                    c.refs[page] = 1;
+                }
+                row[k] = page;
+            }
+            if (lane == 0) c.lens[seq[i]] = len[par[i]];
+        }
     }
     if (tid == 0) plan[0] = want;
 }
@@ -609,35 +650,35 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
 // one tile after another: of a K tile hd / 16 stretches of `fill` blocks, of a V tile one.
 constexpr int kReorderWarps = 8;
 
-__global__ void __launch_bounds__(32 * kReorderWarps) k_kv_reorder(KvView c, const int* __restrict__ plan) {
+__global__ void __launch_bounds__(32 * kReorderWarps, 6) k_kv_reorder(KvView c, const int* __restrict__ plan) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y;
+    const int tiles = c.n_layers * 2 * c.n_kv, blocks = c.pt / kKvBlock;
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n = __ldcg(plan), tiles = c.n_layers * 2 * c.n_kv, blocks = c.pt / kKvBlock;
-    for (int r = blockIdx.y; r < n; r += gridDim.y) {
-        const int from = __ldcg(plan + 1 + 3 * r), to = __ldcg(plan + 2 + 3 * r), fill = __ldcg(plan + 3 + 3 * r);
-        const int pieces = fill * c.hd, strip = fill * kKvBlock;  // of 16 bytes: of a tile, and of one of K's stretches
-        const unsigned magic = unsigned((0x100000000ULL + strip - 1) / strip);
-        for (int tile = blockIdx.x * kReorderWarps + warp; tile < tiles; tile += gridDim.x * kReorderWarps) {
-            const size_t a = size_t(from) * tiles + tile, b = size_t(to) * tiles + tile;
-            const uint4* src = reinterpret_cast<const uint4*>(c.codes + a * c.tile());
-            uint4* dst = reinterpret_cast<uint4*>(c.codes + b * c.tile());
-            const bool is_v = tile / c.n_kv & 1;
-            constexpr int U = 8;
-            for (int y0 = lane; y0 < pieces; y0 += 32 * U) {
-                uint4 w[U];
-                int at[U];
+    const int n = __ldcg(plan), from = __ldcg(plan + 1 + 3 * r), to = __ldcg(plan + 2 + 3 * r), fill = __ldcg(plan + 3 + 3 * r);
+    if (r >= n) return;
+    const int pieces = fill * c.hd, strip = fill * kKvBlock;  // of 16 bytes: of a tile, and of one of K's stretches
+    const unsigned magic = unsigned((0x100000000ULL + strip - 1) / strip);
+    for (int tile = blockIdx.x * kReorderWarps + warp; tile < tiles; tile += gridDim.x * kReorderWarps) {
+        const size_t a = size_t(from) * tiles + tile, b = size_t(to) * tiles + tile;
+        const uint4* src = reinterpret_cast<const uint4*>(c.codes + a * c.tile());
+        uint4* dst = reinterpret_cast<uint4*>(c.codes + b * c.tile());
+        const bool is_v = tile / c.n_kv & 1;
+        auto place = [&](int y) {
+            const int s = int(__umulhi(unsigned(y), magic));  // y / strip
+            return is_v ? y : s * c.pt + y - s * strip;
+        };
+        float scale;
+        if (lane < fill) scale = c.scales[a * blocks + lane];
+        constexpr int U = 4;
+        for (int y0 = lane; y0 < pieces; y0 += 32 * U) {
+            uint4 w[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int y = min(y0 + 32 * u, pieces - 1), s = int(__umulhi(unsigned(y), magic));  // y / strip
-                    at[u] = is_v ? y : s * c.pt + y - s * strip;
-                    w[u] = __ldcs(src + at[u]);
-                }
+            for (int u = 0; u < U; ++u) w[u] = __ldcs(src + place(min(y0 + 32 * u, pieces - 1)));
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (y0 + 32 * u < pieces) __stcs(dst + at[u], w[u]);
-            }
-            if (lane < fill) c.scales[b * blocks + lane] = c.scales[a * blocks + lane];
+            for (int u = 0; u < U; ++u)
+                if (y0 + 32 * u < pieces) __stcs(dst + place(y0 + 32 * u), w[u]);
         }
+        if (lane < fill) c.scales[b * blocks + lane] = scale;
     }
 }
 
@@ -911,19 +952,19 @@ cudaError_t launch_kv_fork(const KvView& c, const int* src, const int* dst, int 
                       static_cast<const int*>(ok), static_cast<const int*>(fresh));
 }
 
-// plan: {from, to, blocks} of each copy, [max_seqs] lengths, [max_seqs][max_pages] rows, [n_pages] list.
-size_t kv_reorder_ws_bytes(const KvView& c) {
-    return (4 + size_t(c.max_seqs) * (3 + 1 + size_t(c.max_pages)) + size_t(c.n_pages)) * 4;
-}
+// plan: {from, to, blocks} of each copy, [max_seqs] lengths, [max_seqs][max_pages] rows.
+size_t kv_reorder_ws_bytes(const KvView& c) { return (4 + size_t(c.max_seqs) * (3 + 1 + size_t(c.max_pages))) * 4; }
 
 cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* parents, int n, int group, void* ws, cudaStream_t st) {
     if (n == 0) return cudaSuccess;
     int* plan = static_cast<int*>(ws);
     int* len = plan + 4 + size_t(c.max_seqs) * 3;
     int* rows = len + c.max_seqs;
-    int* list = rows + size_t(c.max_seqs) * c.max_pages;
-    cudaError_t e = launch_plan(k_kv_reorder_plan, 1, kPlanThreads, plan_words(c) * 4 + size_t(c.max_seqs) * 4 + size_t(n) * 6, st, c, seqs,
-                                parents, n, group, plan, rows, len, list);
+    // shared memory: free pages, then heirs, lengths, sequences, parents and copies; the largest pools leave the lengths out
+    const size_t all = plan_words(c) * 4 + size_t(n) * 14, less = all - size_t(n) * 4;
+    cudaError_t e = all <= 200 * 1024
+                        ? launch_plan(k_kv_reorder_plan<true>, 1, kPlanThreads, all, st, c, seqs, parents, n, group, plan, rows, len)
+                        : launch_plan(k_kv_reorder_plan<false>, 1, kPlanThreads, less, st, c, seqs, parents, n, group, plan, rows, len);
     if (e != cudaSuccess) return e;
     const int parts = (c.n_layers * 2 * c.n_kv + kReorderWarps - 1) / kReorderWarps;
     return launch_pdl(k_kv_reorder, dim3(unsigned(parts < 1024 ? parts : 1024), unsigned(n)), dim3(32 * kReorderWarps), 0, st, true, c,
