@@ -496,9 +496,16 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
 // the others get copies in fresh pages.  plan[0] = copies (-1: the call is refused), plan[1 + 3 r ..] = {from, to, blocks of 16
 // positions} of copy r.  rows, far_len: workspace for the list's new table rows, which are all read before one is written, and for its
 // lengths where shared memory does not hold them (LEN).  Pages that no sequence uses any more are free for the copies of the same
-// call.  One CTA, bound by latency: what an entry needs is looked up by a thread each, once, and a warp has the table rows of
-// kReorderAhead entries in flight (256 sequences of up to 32 pages: 7 us; entry by entry 15).
+// call.  Bound by latency, and by instructions where one SM has all entries (256 sequences of up to 32 pages: 17 us): many entries
+// go to a cluster of kReorderCtas CTAs.  Each looks up what the entries need and finds the free pages, alike; counting pages and
+// writing rows is dealt out to their warps, which have the table rows of kReorderAhead entries in flight.
 constexpr int kReorderAhead = 4;
+constexpr int kReorderCtas = 8;
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 template <bool LEN>
 __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, const int* __restrict__ seqs,
@@ -515,8 +522,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
     uint16_t* base = par + n;  // copies of entries 0 .. i (at most kKvMaxSeqs)
     __shared__ unsigned mark[kKvMaxSeqs / 32];
     __shared__ int bad;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warps = gridDim.x * (blockDim.x >> 5), warp = blockIdx.x * (blockDim.x >> 5) + (tid >> 5);  // of the cluster
     if (tid == 0) bad = 0;
+    if (tid == 0 && blockIdx.x == 0) plan[0] = 0;
     for (int s = tid; s < kKvMaxSeqs / 32; s += blockDim.x) mark[s] = 0;
     for (int i = tid; i < n; i += blockDim.x) heir[i] = INT_MAX;
     __syncthreads();
@@ -534,8 +543,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         atomicMin(heir + j, j == i ? -1 : i);  // (-1: itself)
     }
     __syncthreads();
-    if (bad) {
-        if (tid == 0) {
+    if (bad) {  // (in every CTA alike)
+        if (tid == 0 && blockIdx.x == 0) {
             set_error(c.status, ERR_BAD_POS);
             plan[0] = -1;
         }
@@ -551,7 +560,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
     }
     const int before = cta_scan(mine, &want);
     for (int i = i0; i < i1; ++i) base[i] = uint16_t(base[i] + before);
-    __syncthreads();
+    const bool alone = gridDim.x == 1;
+    if (alone) __syncthreads();
+    else cluster_sync();  // (every CTA has read the lengths, plan[0] is 0)
     // entry i: changed, gets a copy, pages before and after
     struct Entry {
         bool changed, copy;
@@ -573,7 +584,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         auto one = [&](const Entry& e, int i, int k, int a, int b) {
             if (sign > 0) rows[size_t(i) * c.max_pages + k] = b;
             if (e.copy && k == e.n_now - 1) {
-                if (sign > 0 && (b < 0 || b >= c.n_pages)) bad = int(ERR_BAD_POS);
+                if (sign > 0 && (b < 0 || b >= c.n_pages)) {
+                    if (alone) bad = 1;
+                    else atomicExch(plan, -1);
+                }
                 b = -1;  // a fresh page
             }
             if (a == b) return;
@@ -603,14 +617,16 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         }
     };
     count(1);
-    __syncthreads();
+    if (alone) __syncthreads();
+    else cluster_sync();  // every row has been read, every page counted
     int* list = heir;  // fresh pages
-    if (!bad && want > 0 && lowest_free(c, words, want, list) < want && tid == 0) bad = int(ERR_CAPACITY);
-    __syncthreads();
-    if (bad) {
+    int status = (alone ? bad : __ldcg(plan) < 0) ? int(ERR_BAD_POS) : 0;
+    if (!status && want > 0 && lowest_free(c, words, want, list) < want) status = int(ERR_CAPACITY);
+    if (!alone) cluster_sync();  // every CTA has found the free pages
+    if (status) {  // (in every CTA alike)
         count(-1);
-        if (tid == 0) {
-            set_error(c.status, unsigned(bad));
+        if (tid == 0 && blockIdx.x == 0) {
+            set_error(c.status, unsigned(status));
             plan[0] = -1;
         }
         return;
@@ -643,42 +659,64 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
             if (lane == 0) c.lens[seq[i]] = len[par[i]];
         }
     }
-    if (tid == 0) plan[0] = want;
+    if (tid == 0 && blockIdx.x == 0) plan[0] = want;
 }
 
-// Reorder, second half: the filled blocks of the copied pages, in every layer and head.  Grid (parts, copies at most); a warp takes
-// one tile after another: of a K tile hd / 16 stretches of `fill` blocks, of a V tile one.
-constexpr int kReorderWarps = 8;
+// Reorder, second half: the filled blocks of the copied pages, in every layer and head.  A copy's tiles have `fill` * hd pieces of
+// 16 bytes each (of a K tile hd / 16 stretches, of a V tile one); a task is kReorderThreads * kReorderPieces of them, `parts` tasks
+// at most a copy, taken in turn by as many CTAs as run together (a CTA for each task that there could be: 11 us for 256 sequences,
+// most of it to start CTAs without a task).
+constexpr int kReorderThreads = 256, kReorderPieces = 8, kReorderPerSm = 4;
 
-__global__ void __launch_bounds__(32 * kReorderWarps, 6) k_kv_reorder(KvView c, const int* __restrict__ plan) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y;
-    const int tiles = c.n_layers * 2 * c.n_kv, blocks = c.pt / kKvBlock;
+__global__ void __launch_bounds__(kReorderThreads, kReorderPerSm) k_kv_reorder(KvView c, const int* __restrict__ plan, int parts) {
+    const int tiles = c.n_layers * 2 * c.n_kv, blocks = c.pt / kKvBlock, hd_shift = c.hd == 64 ? 6 : 7;
+    int r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const int step_r = gridDim.x / parts, step_part = gridDim.x - step_r * parts;
     pdl_wait();
-    const int n = __ldcg(plan), from = __ldcg(plan + 1 + 3 * r), to = __ldcg(plan + 2 + 3 * r), fill = __ldcg(plan + 3 + 3 * r);
-    if (r >= n) return;
-    const int pieces = fill * c.hd, strip = fill * kKvBlock;  // of 16 bytes: of a tile, and of one of K's stretches
-    const unsigned magic = unsigned((0x100000000ULL + strip - 1) / strip);
-    for (int tile = blockIdx.x * kReorderWarps + warp; tile < tiles; tile += gridDim.x * kReorderWarps) {
-        const size_t a = size_t(from) * tiles + tile, b = size_t(to) * tiles + tile;
-        const uint4* src = reinterpret_cast<const uint4*>(c.codes + a * c.tile());
-        uint4* dst = reinterpret_cast<uint4*>(c.codes + b * c.tile());
-        const bool is_v = tile / c.n_kv & 1;
-        auto place = [&](int y) {
-            const int s = int(__umulhi(unsigned(y), magic));  // y / strip
-            return is_v ? y : s * c.pt + y - s * strip;
-        };
-        float scale;
-        if (lane < fill) scale = c.scales[a * blocks + lane];
-        constexpr int U = 4;
-        for (int y0 = lane; y0 < pieces; y0 += 32 * U) {
-            uint4 w[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = __ldcs(src + place(min(y0 + 32 * u, pieces - 1)));
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (y0 + 32 * u < pieces) __stcs(dst + place(y0 + 32 * u), w[u]);
+    const int n = __ldcg(plan);
+    int from = 0, to = 0, fill = 0;
+    auto look = [&] {  // (copy 0 .. n - 1; the plan has room for one more than the list's length)
+        from = __ldcg(plan + 1 + 3 * r);
+        to = __ldcg(plan + 2 + 3 * r);
+        fill = __ldcg(plan + 3 + 3 * r);
+    };
+    look();
+    while (r < n) {
+        const int a = from, b = to, now = fill, p = part;
+        r += step_r;
+        part += step_part;
+        if (part >= parts) {
+            part -= parts;
+            ++r;
         }
-        if (lane < fill) c.scales[b * blocks + lane] = scale;
+        if (r < n) look();
+        const unsigned total = unsigned(tiles) * unsigned(now) << hd_shift, strip = unsigned(now) * kKvBlock;
+        const unsigned x0 = unsigned(p) * (kReorderThreads * kReorderPieces) + threadIdx.x;
+        const uint4* src = reinterpret_cast<const uint4*>(c.codes + size_t(a) * c.page_codes());
+        uint4* dst = reinterpret_cast<uint4*>(c.codes + size_t(b) * c.page_codes());
+        auto place = [&](unsigned x) {  // piece x of the copy, among the page's
+            const unsigned tile = (x >> hd_shift) / unsigned(now), y = x - (tile * unsigned(now) << hd_shift);
+            const size_t at = (size_t(tile) << hd_shift) * blocks;
+            if (tile / unsigned(c.n_kv) & 1) return at + y;
+            const unsigned s = y / strip;
+            return at + s * unsigned(c.pt) + (y - s * strip);
+        };
+        if (x0 < total) {
+            uint4 w[kReorderPieces];
+            size_t at[kReorderPieces];
+#pragma unroll
+            for (int u = 0; u < kReorderPieces; ++u) {
+                at[u] = place(min(x0 + u * kReorderThreads, total - 1));
+                w[u] = __ldcs(src + at[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kReorderPieces; ++u)
+                if (x0 + u * kReorderThreads < total) __stcs(dst + at[u], w[u]);
+        }
+        for (int t = p * kReorderThreads + threadIdx.x; t < tiles * now; t += parts * kReorderThreads) {
+            const int tile = t / now, i = tile * blocks + t - tile * now;
+            c.scales[size_t(b) * c.page_scales() + i] = c.scales[size_t(a) * c.page_scales() + i];
+        }
     }
 }
 
@@ -962,13 +1000,27 @@ cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* paren
     int* rows = len + c.max_seqs;
     // shared memory: free pages, then heirs, lengths, sequences, parents and copies; the largest pools leave the lengths out
     const size_t all = plan_words(c) * 4 + size_t(n) * 14, less = all - size_t(n) * 4;
-    cudaError_t e = all <= 200 * 1024
-                        ? launch_plan(k_kv_reorder_plan<true>, 1, kPlanThreads, all, st, c, seqs, parents, n, group, plan, rows, len)
-                        : launch_plan(k_kv_reorder_plan<false>, 1, kPlanThreads, less, st, c, seqs, parents, n, group, plan, rows, len);
+    const bool with_len = all <= 200 * 1024, many = n > 32;
+    auto kern = with_len ? k_kv_reorder_plan<true> : k_kv_reorder_plan<false>;
+    const size_t smem = with_len ? all : less;
+    cudaError_t e = smem > 32 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) : cudaSuccess;
     if (e != cudaSuccess) return e;
-    const int parts = (c.n_layers * 2 * c.n_kv + kReorderWarps - 1) / kReorderWarps;
-    return launch_pdl(k_kv_reorder, dim3(unsigned(parts < 1024 ? parts : 1024), unsigned(n)), dim3(32 * kReorderWarps), 0, st, true, c,
-                      static_cast<const int*>(plan));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(many ? kReorderCtas : 1);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {cfg.gridDim.x, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kern, c, seqs, parents, n, group, plan, rows, len);
+    if (e != cudaSuccess) return e;
+    const size_t per = size_t(kReorderThreads) * kReorderPieces * 16, parts = (c.page_codes() + per - 1) / per, tasks = parts * size_t(n);
+    const size_t most = 148 * kReorderPerSm;
+    return launch_pdl(k_kv_reorder, dim3(unsigned(tasks < most ? tasks : most)), dim3(kReorderThreads), 0, st, true, c,
+                      static_cast<const int*>(plan), int(parts));
 }
 
 cudaError_t launch_kv_free(const KvView& c, const int* seqs, int n, cudaStream_t st) {
