@@ -5,6 +5,7 @@
 
 Outputs (git-ignored, shipped with the repository snapshot):
     quanta.cpp_b200/lib/libquanta_b200.so   CUDA kernels + engine + the C ABI of include/quanta_b200.h
+    quanta.cpp_b200/lib/quanta_b200_torch.so  the operators on torch tensors (csrc/torch_calls.cpp; needs torch's headers)
     quanta.cpp_b200/lib/libqnt_synth.so     seeded random-init .qnt writer
     quanta.cpp_b200/lib/quanta_b200         command-line driver (selftest / gen / bench / checkbatch / checkhead / run)
 Objects go to quanta.cpp_b200/_build/.  Rebuilds only what changed (source or header mtimes).
@@ -85,11 +86,30 @@ def build(verbose: bool = False, jobs: int = 0, stamps: bool = False) -> None:
     ssrc = CSRC / "synth" / "qnt_synth.cpp"
     if _newer(synth, [ssrc, CSRC / "synth" / "qnt_synth.h"]):
         _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-march=x86-64-v3", "-o", str(synth), str(ssrc), "-pthread"])
+    build_torch_calls(so)
     cli_src = CSRC / "cli" / "main.cpp"
     cli = LIB / "quanta_b200"
     if cli_src.exists() and _newer(cli, [cli_src, so] + hdrs):
         _run(["g++", "-O2", "-std=c++17", f"-I{ROOT / 'include'}", "-o", str(cli), str(cli_src), f"-L{LIB}", "-lquanta_b200",
               f"-Wl,-rpath,$ORIGIN", "-pthread"])
+
+
+def build_torch_calls(so: Path) -> None:
+    """The CPython extension over the C ABI for torch tensors; without torch there is nothing that could call it."""
+    src, out = CSRC / "torch_calls.cpp", LIB / "quanta_b200_torch.so"
+    if not _newer(out, [src, ROOT / "include" / "quanta_b200.h"]):
+        return
+    try:
+        import torch
+    except ImportError:
+        return
+    import sysconfig
+    t = Path(torch.__file__).resolve().parent
+    inc = [t / "include", t / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+           Path(NVCC).resolve().parent.parent / "include"]
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
+         [x for i in inc for x in ("-isystem", str(i))] + [f"-I{ROOT / 'include'}", str(src), "-o", str(out), f"-L{t / 'lib'}", "-ltorch_python",
+          "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{so.parent}", "-lquanta_b200", "-Wl,-rpath,$ORIGIN"])
 
 
 if __name__ == "__main__":

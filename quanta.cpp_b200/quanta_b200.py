@@ -524,95 +524,66 @@ class PagedKV:
         self._run(self._lib.qnt_kv_check, self._p, self._stream(stream))
 
 
-class _TorchCalls:
-    """What the operators on torch tensors share: types, streams, and calls on a tensor's device.  Work is queued on `stream` (a torch
-    stream or a cudaStream_t's number; default: torch's current stream of the tensors' device); with another stream than the
-    current one a call is as if made within torch.cuda.stream(stream)."""
-
-    def __init__(self):
-        import torch
-        self.torch = torch
-        self.types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        self.lib = lib()
-
-    def stream(self, stream, device: int) -> int:
-        if stream is None:
-            return self.raw_stream(device) if self.raw_stream else self.torch.cuda.current_stream(device).cuda_stream
-        return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-
-    def allocating_on(self, stream, device: int):
-        cuda = self.torch.cuda
-        if not hasattr(stream, "cuda_stream"):
-            stream = cuda.ExternalStream(int(stream), device=device) if int(stream) else cuda.default_stream(device)
-        return cuda.stream(stream)
-
-    def empty(self, like, stream, *shapes):
-        """New tensors (shape, dtype) for work on the stream."""
-        if stream is None:
-            return [like.new_empty(s, dtype=t) for s, t in shapes]
-        with self.allocating_on(stream, like.get_device()):
-            return [like.new_empty(s, dtype=t) for s, t in shapes]
-
-    def run(self, device: int, call, *args):
-        if self.current_device() == device:
-            rc = call(*args)
-        else:
-            with self.torch.cuda.device(device):
-                rc = call(*args)
-        if rc:
-            _check(rc)
+_torch_module = None
 
 
-_calls = None
+def _torch_calls():
+    """quanta_b200_torch.so: the operators on torch tensors (csrc/torch_calls.cpp)."""
+    global _torch_module
+    if _torch_module is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries come first)
+        lib()
+        p = PKG / "lib" / "quanta_b200_torch.so"
+        if not p.exists():
+            raise RuntimeError(f"{p} is missing: run `python quanta.cpp_b200/build.py` where torch is installed")
+        loader = importlib.machinery.ExtensionFileLoader("quanta_b200_torch", str(p))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("quanta_b200_torch", loader))
+        loader.exec_module(module)
+        _torch_module = module
+    return _torch_module
 
 
-def _torch_calls() -> _TorchCalls:
-    global _calls
-    if _calls is None:
-        _calls = _TorchCalls()
-    return _calls
+def _on_stream(stream, device):
+    """torch.cuda.stream(stream) of a torch stream or a cudaStream_t's number."""
+    from torch import cuda
+    if not hasattr(stream, "cuda_stream"):
+        stream = cuda.ExternalStream(int(stream), device=device) if int(stream) else cuda.default_stream(device)
+    return cuda.stream(stream)
 
 
 def rms_norm_q8(x, weight, eps: float = 1e-6, residual=None, stream=None):
     """RMS norm of rows x [tokens, n] (float32, float16 or bfloat16 CUDA tensor; rows may lie in wider ones) with 8-bit rows out:
     (q int8 [tokens, n], d float32 [tokens, n / 32]), the operand of the quantized products.  weight float32 [n].  With residual
-    [tokens, n] (x's type or float32), residual += x first, in place, and the sum (before its rounding) is normed."""
-    c = _torch_calls()
-    t, dt, dev = c.torch, c.types.get(x.dtype), x.get_device()
-    if dt is None or dev < 0 or x.dim() != 2 or x.stride(1) != 1:
-        raise TypeError("x must be a float32, float16 or bfloat16 CUDA tensor [tokens, n] whose rows are contiguous")
-    m, n = x.shape
-    if weight.dtype is not t.float32 or weight.get_device() != dev or weight.shape != (n,) or not weight.is_contiguous():
-        raise TypeError(f"weight must be a contiguous float32 CUDA tensor [{n}] on x's device")
-    rp, rt, rs = None, dt, 0
-    if residual is not None:
-        rt = c.types.get(residual.dtype)
-        if residual.shape != x.shape or residual.get_device() != dev or residual.stride(1) != 1 or (rt != dt and rt != F32):
-            raise TypeError("residual must be a CUDA tensor of x's shape, on its device, of its type or float32, whose rows are contiguous")
-        rp, rs = residual.data_ptr(), residual.stride(0)
-    q, d = c.empty(x, stream, ((m, n), t.int8), ((m, n // QK), t.float32))
-    c.run(dev, c.lib.qnt_rms_norm_q8, x.data_ptr(), dt, x.stride(0), rp, rt, rs, weight.data_ptr(), eps, m, n, q.data_ptr(), d.data_ptr(),
-          c.stream(stream, dev))
-    return q, d
+    [tokens, n] (x's type or float32), residual += x first, in place, and the sum (before its rounding) is normed.
+    Work is queued on `stream` (a torch stream or a cudaStream_t's number; default: torch's current stream); with another one than
+    the current one the call is as if made within torch.cuda.stream(stream).  So for the functions and objects below."""
+    if stream is not None:
+        with _on_stream(stream, x.device):
+            return rms_norm_q8(x, weight, eps, residual)
+    r = (_torch_module or _torch_calls()).rms_norm_q8(x, weight, eps, residual)
+    return r if r.__class__ is tuple else _check(r)
+
+
+_values = {}  # torch dtype -> number
 
 
 def dequantize_q8(q, d, dtype=None, stream=None):
     """The values q * d of 8-bit rows (q int8 [tokens, n], d float32 [tokens, n / 32], contiguous CUDA tensors), as dtype (bfloat16
     unless said otherwise)."""
-    c = _torch_calls()
-    t, dev = c.torch, q.get_device()
-    dtype = dtype or t.bfloat16
-    dt = c.types.get(dtype)
-    if dt is None:
+    if stream is not None:
+        with _on_stream(stream, q.device):
+            return dequantize_q8(q, d, dtype)
+    if not _values:
+        import torch
+        _values.update({None: BF16, torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    number = _values.get(dtype)
+    if number is None:
         raise TypeError("dtype must be float32, float16 or bfloat16")
-    if q.dtype is not t.int8 or dev < 0 or q.dim() != 2 or not q.is_contiguous() or d.dtype is not t.float32 or \
-            d.get_device() != dev or not d.is_contiguous() or q.shape[1] % QK or d.shape != (q.shape[0], q.shape[1] // QK):
-        raise TypeError("q must be a contiguous int8 CUDA tensor [tokens, n], d a contiguous float32 one [tokens, n / 32] on its device")
-    out, = c.empty(q, stream, (q.shape, dtype))
-    c.run(dev, c.lib.qnt_dequantize_q8, q.data_ptr(), d.data_ptr(), q.shape[0], q.shape[1], out.data_ptr(), dt, c.stream(stream, dev))
-    return out
+    r = (_torch_module or _torch_calls()).dequantize_q8(q, d, number)
+    return _check(r) if r.__class__ is int else r
 
 
 class Rope:
@@ -640,8 +611,7 @@ class Rope:
             if len(f) != self.rotary_dim // 2 or scaling is not None:
                 raise ValueError("frequencies: one for each pair, and no scaling beside them")
         self.turns = torch.tensor([x / (2 * math.pi) for x in f], dtype=torch.float64, device=device)  # revolutions a position
-        self._dev, self._turns = self.turns.get_device(), self.turns.data_ptr()
-        self._inter, self._c = int(self.interleaved), None
+        self._inter = int(self.interleaved)
 
     @staticmethod
     def frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None):
@@ -676,34 +646,15 @@ class Rope:
             return [x * k + x / factor * (1 - k) for x, k in zip(f, keep)], 1.0
         return f, 1.0
 
-    def _fits(self, x, tokens):
-        shape, st = x.shape, x.stride()
-        return len(shape) == 3 and st[2] == 1 and (st[1] == shape[2] or shape[1] == 1) and shape[0] == tokens and x.get_device() == self._dev
-
     def __call__(self, q, k, positions, inplace: bool = False, stream=None):
         """q [tokens, heads, head_dim] and k [tokens, kv heads, head_dim] (or None) of one type, float32, float16 or bfloat16; heads
         contiguous within a token, so that they may lie in the rows of one projection's output; positions int32 [tokens].
         Returns rotated (q, k), new contiguous tensors, or with inplace=True the ones given."""
-        c = self._c
-        if c is None:
-            c = self._c = _torch_calls()
-        dt, tokens = c.types.get(q.dtype), positions.numel()
-        if dt is None or not self._fits(q, tokens) or (k is not None and (k.dtype is not q.dtype or not self._fits(k, tokens) or
-                                                                          k.shape[2] != q.shape[2])):
-            raise TypeError("q and k must be CUDA tensors [tokens, heads, head_dim] of one type, float32, float16 or bfloat16, on the "
-                            "table's device, whose heads are contiguous within a token")
-        if positions.dtype is not c.torch.int32 or positions.get_device() != self._dev or positions.dim() != 1 or not positions.is_contiguous():
-            raise TypeError("positions must be a contiguous int32 CUDA tensor [tokens] on the table's device")
-        if inplace:
-            q_out, k_out = q, k
-        elif k is None:
-            (q_out,), k_out = c.empty(q, stream, (q.shape, q.dtype)), None
-        else:
-            q_out, k_out = c.empty(q, stream, (q.shape, q.dtype), (k.shape, q.dtype))
-        of_k = (None, 0, None, 0, 0) if k is None else (k.data_ptr(), k.stride(0), k_out.data_ptr(), k_out.stride(0), k.shape[1])
-        c.run(self._dev, c.lib.qnt_rope, q.data_ptr(), q.stride(0), q_out.data_ptr(), q_out.stride(0), q.shape[1], *of_k, dt, q.shape[2],
-              self.rotary_dim, self._inter, self._turns, self.scale, positions.data_ptr(), tokens, c.stream(stream, self._dev))
-        return q_out, k_out
+        if stream is not None:
+            with _on_stream(stream, q.device):
+                return self(q, k, positions, inplace)
+        r = (_torch_module or _torch_calls()).rope(q, k, positions, self.turns, self.rotary_dim, self._inter, self.scale, inplace)
+        return r if r.__class__ is tuple else _check(r)
 
 
 class BeamSelector:
@@ -716,48 +667,45 @@ class BeamSelector:
 
     def __init__(self, k: int, end_id: int = -1):
         self.k, self.end_id = int(k), int(end_id)
-        self._ws, self._kept, self._need, self._c = {}, [], {}, None
+        self._ws, self._kept = {}, []
+        self._raw_stream = None
 
-    def _workspace(self, c, device, stream, given, need):
+    def _workspace(self, device, stream, shape):
+        """The stream's workspace, large enough for logits of this shape: (tensor, shapes that it is known to be enough for)."""
+        import torch
+        need = lib().qnt_beam_workspace(*shape, self.k) if len(shape) == 3 else 0
+        if need == 0 and len(shape) == 3 and shape[0] > 0:
+            raise QntError(-1, lib().qnt_last_error().decode(errors="replace"))
         ws = self._ws.get((device, stream))
-        if ws is None or ws.numel() < need:
+        if ws is None or ws[0].numel() < need:
             size = max(need, 1 << 20)
             if ws is not None:  # the old one stays: queued kernels and captured graphs still write to it
-                self._kept.append(ws)
-                size = max(size, 2 * ws.numel())
-            with c.allocating_on(stream if given is None else given, device):
-                ws = self._ws[device, stream] = c.torch.empty(size, dtype=c.torch.uint8, device=f"cuda:{device}")
-        return ws.data_ptr(), ws.numel()
+                self._kept.append(ws[0])
+                size = max(size, 2 * ws[0].numel())
+            ws = self._ws[device, stream] = torch.empty(size, dtype=torch.uint8, device=f"cuda:{device}"), ws[1] if ws else set()
+        if len(ws[1]) > 4096:
+            ws[1].clear()
+        ws[1].add(shape)
+        return ws
 
     def __call__(self, logits, scores, ended=None, stream=None):
         """logits [groups, beams, vocab] (float32, float16 or bfloat16 CUDA tensor, rows at one distance, which may be wider than
         vocab), scores float32 [groups, beams], ended bool or uint8 [groups, beams] or None."""
-        c = self._c
-        if c is None:
-            c = self._c = _torch_calls()
-        t, dt, dev = c.torch, c.types.get(logits.dtype), logits.get_device()
-        shape, st = logits.shape, logits.stride()
-        if dt is None or dev < 0 or len(shape) != 3 or (st[2] != 1 and shape[2] != 1):
-            raise TypeError("logits must be a float32, float16 or bfloat16 CUDA tensor [groups, beams, vocab] whose rows are contiguous")
-        g, b, v = shape
-        row = st[1] if b > 1 else st[0]
-        if g > 1 and b > 1 and st[0] != b * row:
-            raise TypeError("the rows of logits must lie at one distance from each other")
-        if scores.dtype is not t.float32 or scores.get_device() != dev or scores.shape != (g, b) or not scores.is_contiguous():
-            raise TypeError("scores must be a contiguous float32 CUDA tensor [groups, beams] on the logits' device")
-        if ended is not None and (ended.dtype not in (t.bool, t.uint8) or ended.get_device() != dev or ended.shape != (g, b) or
-                                  not ended.is_contiguous()):
-            raise TypeError("ended must be a contiguous bool or uint8 CUDA tensor [groups, beams] on the logits' device")
-        k, key = self.k, (g, b, v)
-        need = self._need.get(key)
-        if need is None:
-            need = self._need[key] = c.lib.qnt_beam_workspace(g, b, v, k)
-        s = c.stream(stream, dev)
-        w, nb = self._workspace(c, dev, s, stream, need)
-        out, tokens, parents = c.empty(scores, stream, ((g, k), t.float32), ((g, k), t.int32), ((g, k), t.int32))
-        c.run(dev, c.lib.qnt_beam_select, logits.data_ptr(), dt, row, scores.data_ptr(), None if ended is None else ended.data_ptr(),
-              self.end_id, g, b, v, k, out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), w, nb, s)
-        return out, tokens, parents
+        if stream is not None:
+            with _on_stream(stream, logits.device):
+                return self(logits, scores, ended)
+        device, shape = logits.get_device(), logits.shape
+        if device < 0:
+            raise TypeError("logits must be a CUDA tensor")
+        if self._raw_stream is None:
+            import torch
+            self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        s = self._raw_stream(device)
+        ws = self._ws.get((device, s))
+        if ws is None or shape not in ws[1]:
+            ws = self._workspace(device, s, shape)
+        r = (_torch_module or _torch_calls()).beam_select(logits, scores, ended, self.end_id, self.k, ws[0])
+        return r if r.__class__ is tuple else _check(r)
 
 
 def bench_mma_i8(iters: int = 4096) -> float:
