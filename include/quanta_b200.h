@@ -284,6 +284,12 @@ int qnt_batch_init_paged(qnt_model* m, int max_seqs, int ctx_len, int n_pages, i
 int qnt_batch_fork(qnt_model* m, int src, int dst);
 int qnt_batch_resize(qnt_model* m, int n_pages);
 
+/* Beam search from the paged cache (qnt_batch_init_paged; sequences 0 .. beams - 1 empty, before and after the call; no
+ * counterpart in the reference): the prompt, then up to n_gen steps of qnt_beam_select over all beams' logits, qnt_kv_reorder and
+ * one batched decode step.  A beam that takes end_id (-1: none) ends with it and stays with its score; the search stops when all
+ * have.  ids [beams][n_gen], lens and scores (sums of log-probabilities) [beams], best first.  beams <= 64; n + n_gen - 1 positions. */
+int qnt_beam_search(qnt_model* m, const int* prompt, int n, int beams, int n_gen, int end_id, int* ids, int* lens, float* scores);
+
 /* Sampler (engine/src/sampler.h:20-38): Sampler::sample (sampler.cpp:22-85) on logits that are already in device
  * memory -- repetition penalty -> greedy argmax (first max) or top-k -> softmax(T) -> min-p -> top-p -> xorshift64*
  * draw, with the reference's float operations, so the same logits, history and seed give the same ids.

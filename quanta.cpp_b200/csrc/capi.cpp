@@ -577,6 +577,15 @@ int qnt_batch_fork(qnt_model* m, int src, int dst) {
     return engine_code(m->eng, m->eng.batch_fork(src, dst));
 }
 
+int qnt_beam_search(qnt_model* m, const int* prompt, int n, int beams, int n_gen, int end_id, int* ids, int* lens, float* scores) {
+    if (!m) return set_err(QNT_ERR_INVALID, "null model");
+    try {
+        return engine_code(m->eng, m->eng.beam_search(prompt, n, beams, n_gen, end_id, ids, lens, scores));
+    } catch (const std::exception& e) {
+        return set_err(QNT_ERR_INVALID, e.what());
+    }
+}
+
 int qnt_batch_resize(qnt_model* m, int n_pages) {
     if (!m) return set_err(QNT_ERR_INVALID, "null model");
     return engine_code(m->eng, m->eng.batch_resize(n_pages));

@@ -1030,10 +1030,10 @@ int Engine::batch_supported(int max_seqs, int ctx) {
 
 void Engine::batch_free() {
     if (st_) cudaStreamSynchronize(st_);
-    for (void* p : {(void*)bkcache_, (void*)bvcache_, kv_pool_, kv_mem_, kv_ws_}) cudaFree(p);
+    for (void* p : {(void*)bkcache_, (void*)bvcache_, kv_pool_, kv_mem_, kv_ws_, beam_mem_}) cudaFree(p);
     bkcache_ = bvcache_ = nullptr;
-    kv_pool_ = kv_mem_ = kv_ws_ = nullptr;
-    kv_ws_bytes_ = 0;
+    kv_pool_ = kv_mem_ = kv_ws_ = beam_mem_ = nullptr;
+    kv_ws_bytes_ = beam_bytes_ = 0;
     kv_ = KvView{};
     bmax_ = bctx_ = 0;
     blens_.clear();
@@ -1313,6 +1313,14 @@ int Engine::batch_decode(const int* seq_ids, const int* tokens, int n, int* next
         err_ = "batch_decode: need 1 <= n <= " + std::to_string(kChunk) + " sequences";
         return -1;
     }
+    if (int r = batch_step(seq_ids, tokens, n)) return r;
+    if (int r = batch_head(n, next_ids)) return r;
+    if (!kv_.codes)
+        for (int i = 0; i < n; ++i) blens_[size_t(seq_ids[i])] += 1;
+    return 0;
+}
+
+int Engine::batch_step(const int* seq_ids, const int* tokens, int n) {
     if (kv_.codes)
         if (int r = paged_tokens(tokens, n)) return r;
     const long long stride = (long long)hp_.n_layers * bctx_ * hp_.n_kv_heads * hp_.head_dim;
@@ -1345,11 +1353,157 @@ int Engine::batch_decode(const int* seq_ids, const int* tokens, int n, int* next
     cudaMemcpyAsync(tok_off_, h_off_.data(), size_t(n) * 8, cudaMemcpyHostToDevice, st_);
     QB_TRY(launch_embed(embed_, tokens_, n, X_, status_, st_, false));
     const KvCall call{kv_seqs_, kv_starts_, n, n};
-    if (int r = launch_chunk(n, pos_, bound, TokMap{tok_pos_, tok_off_}, kv_.codes ? &call : nullptr, 1)) return r;
-    if (int r = batch_head(n, next_ids)) return r;
-    if (!kv_.codes)
-        for (int i = 0; i < n; ++i) blens_[size_t(seq_ids[i])] += 1;
+    return launch_chunk(n, pos_, bound, TokMap{tok_pos_, tok_off_}, kv_.codes ? &call : nullptr, 1);
+}
+
+// ---- beam search
+
+namespace {
+
+// beam_mem_ of `beams` beams over a vocabulary of `rows` (the head's) and a cache: byte offsets.
+struct BeamMemory {
+    size_t logits, select, reorder, scores[2], tokens, parents, ended, end;
+    BeamMemory(int beams, int rows, int vocab, const KvView& kv) {
+        BeamArgs a{};
+        a.groups = 1;
+        a.beams = beams;
+        a.vocab = vocab;
+        a.k = beams;
+        a.type = KV_F32;
+        size_t at = 0;
+        const auto take = [&at](size_t bytes) {
+            const size_t here = at;
+            at = align_up(at + bytes, 256);
+            return here;
+        };
+        logits = take(size_t(beams) * rows * 4);
+        select = take(beam_ws_bytes(a));
+        reorder = take(kv_reorder_ws_bytes(kv));
+        scores[0] = take(size_t(beams) * 4);
+        scores[1] = take(size_t(beams) * 4);
+        tokens = take(size_t(beams) * 4);
+        parents = take(size_t(beams) * 4);
+        ended = take(size_t(beams));
+        end = at;
+    }
+};
+
+}  // namespace
+
+int Engine::beam_memory(int beams) {
+    const size_t need = BeamMemory(beams, lm_head_.rows, n_valid_default(), kv_).end;
+    if (need <= beam_bytes_) return 0;
+    cudaStreamSynchronize(st_);
+    cudaFree(beam_mem_);
+    beam_mem_ = nullptr;
+    beam_bytes_ = 0;
+    if (cudaMalloc(&beam_mem_, need) != cudaSuccess) {
+        cudaGetLastError();
+        beam_mem_ = nullptr;
+        err_ = "beam_search: out of device memory";
+        return -2;
+    }
+    beam_bytes_ = need;
     return 0;
+}
+
+int Engine::beam_search(const int* prompt, int n, int beams, int n_gen, int end_id, int* ids, int* lens, float* scores) {
+    const int vocab = n_valid_default();
+    if (!kv_.codes) {
+        err_ = "beam_search: batch_init_paged first";
+        return -1;
+    }
+    if (!prompt || n <= 0 || beams <= 0 || beams > kBeamMaxK || beams > bmax_ || beams > vocab || n_gen <= 0 || !ids || !lens || !scores) {
+        err_ = "beam_search: needs a prompt, 1 .. " + std::to_string(kBeamMaxK) + " beams (at most the batch's sequences) and n_gen > 0";
+        return -1;
+    }
+    if (std::any_of(blens_.begin(), blens_.begin() + beams, [](int len) { return len != 0; })) {
+        err_ = "beam_search: sequences 0 .. beams - 1 must be empty";
+        return -1;
+    }
+    if ((long long)n + n_gen - 1 > bctx_) {
+        err_ = "beam_search: prompt and answer exceed the context";
+        return -5;
+    }
+    if (int r = beam_memory(beams)) return r;
+    const BeamMemory at(beams, lm_head_.rows, vocab, kv_);
+    char* mem = static_cast<char*>(beam_mem_);
+    BeamArgs a{};
+    a.logits = mem + at.logits;
+    a.stride = lm_head_.rows;
+    a.ended = reinterpret_cast<uint8_t*>(mem + at.ended);
+    a.groups = 1;
+    a.vocab = vocab;
+    a.k = beams;
+    a.end_id = end_id;
+    a.tokens = reinterpret_cast<int*>(mem + at.tokens);
+    a.parents = reinterpret_cast<int*>(mem + at.parents);
+    a.type = KV_F32;
+    const size_t nb = size_t(beams);
+    std::vector<int> seqs(nb), next(nb), from(nb);
+    std::iota(seqs.begin(), seqs.end(), 0);
+    std::vector<std::vector<int>> hyp(nb), grown(nb);
+    std::vector<uint8_t> over(nb, 0), then(nb, 0);
+    std::vector<float> score(nb, 0.f);
+
+    // the rows' logits, the next beams; all of it has run when this returns
+    const auto select = [&](int step) -> int {
+        const int rows = step ? beams : 1;
+        a.scores = reinterpret_cast<float*>(mem + at.scores[step & 1]);
+        a.out_scores = reinterpret_cast<float*>(mem + at.scores[~step & 1]);
+        QB_TRY(launch_norm_quant_rows(X_, final_norm_, rows, hp_.dim, hp_.norm_eps, XQ_, DX_, DXT_, kChunk, st_, false));
+        QB_TRY(launch_matmul_tc(lm_head_, t_head_, tm_x_, rows, 0, lm_head_.rows, reinterpret_cast<float*>(mem + at.logits), lm_head_.rows,
+                                status_, st_, pdl_));
+        a.beams = rows;
+        cudaMemcpyAsync(mem + at.ended, over.data(), size_t(rows), cudaMemcpyHostToDevice, st_);
+        QB_TRY(launch_beam_select(a, mem + at.select, st_));
+        cudaMemcpyAsync(next.data(), a.tokens, size_t(beams) * 4, cudaMemcpyDeviceToHost, st_);
+        cudaMemcpyAsync(from.data(), a.parents, size_t(beams) * 4, cudaMemcpyDeviceToHost, st_);
+        cudaMemcpyAsync(score.data(), a.out_scores, size_t(beams) * 4, cudaMemcpyDeviceToHost, st_);
+        return sync_check();
+    };
+    const auto search = [&]() -> int {
+        if (int r = batch_prefill(0, prompt, n, nullptr)) return r;
+        if ((n - 1) % kChunk > 0)
+            cudaMemcpyAsync(X_, X_ + size_t((n - 1) % kChunk) * hp_.dim, size_t(hp_.dim) * 4, cudaMemcpyDeviceToDevice, st_);
+        cudaMemsetAsync(mem + at.scores[0], 0, 4, st_);
+        for (int step = 0; step < n_gen; ++step) {
+            if (int r = select(step)) return r;
+            for (int i = 0; i < beams; ++i) {
+                const size_t p = size_t(from[size_t(i)]);
+                grown[size_t(i)] = hyp[p];
+                if (!over[p]) grown[size_t(i)].push_back(next[size_t(i)]);
+                then[size_t(i)] = over[p] || next[size_t(i)] == end_id;
+            }
+            hyp.swap(grown);
+            over.swap(then);
+            if (step + 1 == n_gen || std::all_of(over.begin(), over.end(), [](uint8_t o) { return o != 0; })) return 0;
+            if (step == 0) {
+                for (int i = 1; i < beams; ++i)
+                    if (int r = batch_fork(0, i)) return r;
+            } else {
+                cudaMemcpyAsync(kv_seqs_, seqs.data(), size_t(beams) * 4, cudaMemcpyHostToDevice, st_);
+                QB_TRY(launch_kv_reorder(kv_, kv_seqs_, a.parents, beams, beams, mem + at.reorder, st_));
+                if (int r = paged_check(beams - 1)) return r;  // (all have one length: the host's stay)
+            }
+            // (an ended beam goes on with end_id: its row is not looked at)
+            if (int r = batch_step(seqs.data(), next.data(), beams)) return r;
+        }
+        return 0;
+    };
+    const int r = search();
+    const std::string why = err_;
+    for (int i = 0; i < beams; ++i) batch_reset(i);
+    if (r) {
+        err_ = why;
+        return r;
+    }
+    for (int i = 0; i < beams; ++i) {
+        std::copy(hyp[size_t(i)].begin(), hyp[size_t(i)].end(), ids + size_t(i) * n_gen);
+        lens[i] = int(hyp[size_t(i)].size());
+        scores[i] = score[size_t(i)];
+    }
+    return sync_check();
 }
 
 }  // namespace qb

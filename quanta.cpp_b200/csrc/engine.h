@@ -16,6 +16,7 @@
 #include "device_layout.h"
 #include "gemm_tc.h"
 #include "head_kernels.h"
+#include "beam.h"
 #include "kv_cache.h"
 #include "layer_kernels.h"
 #include "qnt_file.h"
@@ -105,6 +106,8 @@ public:
     int batch_init_paged(int max_seqs, int ctx, int n_pages, int page_tokens);
     int batch_fork(int src, int dst);
     int batch_resize(int n_pages);
+    // Beam search from the paged caches: ids [beams][n_gen], lens and scores [beams], best first.
+    int beam_search(const int* prompt, int n, int beams, int n_gen, int end_id, int* ids, int* lens, float* scores);
     int batch_len(int seq) const { return seq >= 0 && seq < int(blens_.size()) ? blens_[size_t(seq)] : -1; }
 
     const HParams& hparams() const { return hp_; }
@@ -170,6 +173,8 @@ private:
     // waits for the call's status if the pages of all sequences, extra more of them, could pass the pool
     int paged_check(long long extra);
     int batch_head(int n, int* host_ids);  // greedy ids of the n rows of X_
+    int batch_step(const int* seq_ids, const int* tokens, int n);  // a decode step up to its rows of X_
+    int beam_memory(int beams);
     // Head pass: full or shortlist; n_list > 0 also produces the sampler's stage-1 lists (with the penalty of the
     // marked must ids when penal).
     // marked: the must ids were marked already (by the step's sampler), so no mark kernel runs
@@ -268,6 +273,8 @@ private:
     void *kv_pool_ = nullptr, *kv_mem_ = nullptr;  // codes, scales, refs and the page operations' workspace; the rest
     __half* kv_rows_ = nullptr;           // K and V rows of a chunk before they are quantized, [2][kChunk][kv_dim]
     int *kv_seqs_ = nullptr, *kv_starts_ = nullptr, *kv_extra_ = nullptr;  // lists of a call, [kChunk + 1] each
+    void* beam_mem_ = nullptr;  // beam search: logits [beams][V], the selection's workspace and results, the reordering's workspace
+    size_t beam_bytes_ = 0;
     void* kv_ws_ = nullptr;
     size_t kv_ws_bytes_ = 0;
     void* kv_page_ws() const { return kv_.refs + (size_t(kv_.n_pages) + 63) / 64 * 64; }

@@ -136,6 +136,7 @@ def lib() -> C.CDLL:
         L.qnt_batch_init_paged.argtypes = [P, I, I, I, I]
         L.qnt_batch_fork.argtypes = [P, I, I]
         L.qnt_batch_resize.argtypes = [P, I]
+        L.qnt_beam_search.argtypes = [P, P, I, I, I, I, P, P, P]
         L.qnt_sampler_create.argtypes = [C.POINTER(SamplerParamsC), C.POINTER(P)]
         L.qnt_sampler_sample.argtypes = [P, P, I, P, I, C.POINTER(I), P]
         L.qnt_sampler_free.argtypes = [P]
@@ -890,6 +891,14 @@ class Model:
     def batch_resize(self, n_pages: int):
         """Moves the pages in use into a pool of n_pages, which replaces the old one."""
         _check(lib().qnt_batch_resize(self.h, n_pages))
+
+    def beam_search(self, prompt, beams: int, n_gen: int, end_id: int = -1):
+        """Beam search from the paged cache (batch_init_paged first; sequences 0 .. beams - 1 must be empty and are so afterwards):
+        (ids, score) of every beam, best first; ids end with end_id where the beam did."""
+        t = np.ascontiguousarray(prompt, np.int32)
+        ids, lens, scores = np.zeros((max(beams, 1), max(n_gen, 1)), np.int32), np.zeros(max(beams, 1), np.int32), np.zeros(max(beams, 1), np.float32)
+        _check(lib().qnt_beam_search(self.h, _ptr(t), t.size, beams, n_gen, end_id, _ptr(ids), _ptr(lens), _ptr(scores)))
+        return [(ids[i, : lens[i]].copy(), float(scores[i])) for i in range(beams)]
 
     def session_begin(self, prompt, sp: SamplerParams, shortlist: bool = True, batch_prefill: bool = True):
         p = np.ascontiguousarray(prompt, np.int32)
