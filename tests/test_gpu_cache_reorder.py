@@ -161,9 +161,11 @@ def test_a_page_that_the_table_has_wrong(qb):
     assert all(torch.equal(a, b) for a, b in zip(before, (c.codes, c.scales, c.refs, c.table, c.lens)))
 
 
-def test_large_pool_and_many_sequences(qb):
-    """Shared memory of the plan past 48 KB; a search of 1024 groups of 8."""
-    c, seqs = beams(qb, 1020, 8, [20] * 1020, [16] * 1020, layers=1, kv=1, page=16, spare=300000, seed=9)
+@pytest.mark.parametrize("pages", [300000, 1 << 20])
+def test_large_pool_and_many_sequences(qb, pages):
+    """Shared memory of the plan past 48 KB, and at its most; a search of 1020 groups of 8."""
+    c, seqs = beams(qb, 1020, 8, [20] * 1020, [16] * 1020, layers=1, kv=1, page=16, spare=pages - 1020 * 9, seed=9)
+    assert c.refs.numel() == pages
     rng = np.random.default_rng(9)
     want = model(c, seqs, p := rng.integers(0, 8, 8160).tolist(), 8)
     c.reorder(ints(seqs), ints(p), 8)
