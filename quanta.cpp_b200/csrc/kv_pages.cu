@@ -668,7 +668,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
 // most of it to start CTAs without a task).
 constexpr int kReorderThreads = 256, kReorderPieces = 8, kReorderPerSm = 4;
 
-__global__ void __launch_bounds__(kReorderThreads, kReorderPerSm) k_kv_reorder(KvView c, const int* __restrict__ plan, int parts) {
+__global__ void __launch_bounds__(kReorderThreads, kReorderPerSm) k_kv_reorder(KvView c, const int* __restrict__ plan, int parts,
+                                                                            unsigned kv_magic) {
     const int tiles = c.n_layers * 2 * c.n_kv, blocks = c.pt / kKvBlock, hd_shift = c.hd == 64 ? 6 : 7;
     int r = blockIdx.x / parts, part = blockIdx.x - r * parts;
     const int step_r = gridDim.x / parts, step_part = gridDim.x - step_r * parts;
@@ -690,16 +691,19 @@ __global__ void __launch_bounds__(kReorderThreads, kReorderPerSm) k_kv_reorder(K
             ++r;
         }
         if (r < n) look();
-        const unsigned total = unsigned(tiles) * unsigned(now) << hd_shift, strip = unsigned(now) * kKvBlock;
+        const unsigned total = unsigned(tiles) * unsigned(now) << hd_shift, magic = now > 1 ? 0xffffffffu / unsigned(now) + 1 : 0;
+        // x / now (x below 2^25, now at most 8), and tile / n_kv
+        auto by_fill = [&](unsigned x) { return now > 1 ? __umulhi(x, magic) : x; };
+        auto by_kv = [&](unsigned t) { return kv_magic ? __umulhi(t, kv_magic) : t / unsigned(c.n_kv); };
         const unsigned x0 = unsigned(p) * (kReorderThreads * kReorderPieces) + threadIdx.x;
         const uint4* src = reinterpret_cast<const uint4*>(c.codes + size_t(a) * c.page_codes());
         uint4* dst = reinterpret_cast<uint4*>(c.codes + size_t(b) * c.page_codes());
         auto place = [&](unsigned x) {  // piece x of the copy, among the page's
-            const unsigned tile = (x >> hd_shift) / unsigned(now), y = x - (tile * unsigned(now) << hd_shift);
+            const unsigned tile = by_fill(x >> hd_shift), y = x - (tile * unsigned(now) << hd_shift);
             const size_t at = (size_t(tile) << hd_shift) * blocks;
-            if (tile / unsigned(c.n_kv) & 1) return at + y;
-            const unsigned s = y / strip;
-            return at + s * unsigned(c.pt) + (y - s * strip);
+            if (by_kv(tile) & 1) return at + y;
+            const unsigned s = by_fill(y / kKvBlock);  // which stretch
+            return at + s * unsigned(c.pt) + (y - s * unsigned(now) * kKvBlock);
         };
         if (x0 < total) {
             uint4 w[kReorderPieces];
@@ -1020,7 +1024,9 @@ cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* paren
     const size_t per = size_t(kReorderThreads) * kReorderPieces * 16, parts = (c.page_codes() + per - 1) / per, tasks = parts * size_t(n);
     const size_t most = 148 * kReorderPerSm;
     return launch_pdl(k_kv_reorder, dim3(unsigned(tasks < most ? tasks : most)), dim3(kReorderThreads), 0, st, true, c,
-                      static_cast<const int*>(plan), int(parts));
+                      static_cast<const int*>(plan), int(parts),
+                      // tile / n_kv = umulhi(tile, ceil(2^32 / n_kv)) where their product is below 2^32, n_kv > 1
+                      c.n_kv > 1 && (long long)c.n_layers * 2 * c.n_kv * c.n_kv < (1LL << 32) ? 0xffffffffu / unsigned(c.n_kv) + 1 : 0u);
 }
 
 cudaError_t launch_kv_free(const KvView& c, const int* seqs, int n, cudaStream_t st) {
