@@ -184,6 +184,29 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
+// the address of a qnt_kv_cache, seqs, parents, group or None, workspace -> 0
+PyObject* kv_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    long long cache, group = -1;
+    if (!arguments(n_args, 5) || !to_long(a[0], &cache) || (a[3] != Py_None && !to_long(a[3], &group))) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *s = tensor_or_null(a[1]), *p = tensor_or_null(a[2]), *ws = tensor_or_null(a[4]);
+        if (!ws) refuse("workspace");
+        for (const at::Tensor* t : {s, p})
+            if (!t || t->scalar_type() != at::kInt || t->device() != ws->device() || !t->is_contiguous())
+                refuse("sequence lists must be contiguous int32 CUDA tensors on the cache's device");
+        const int64_t n = s->numel();
+        if (p->numel() != n) {
+            PyErr_SetString(PyExc_ValueError, "one parent per sequence");
+            return nullptr;
+        }
+        const c10::cuda::CUDAGuard on(ws->device());
+        return PyLong_FromLong(qnt_kv_reorder(reinterpret_cast<const qnt_kv_cache*>(intptr_t(cache)), static_cast<const int*>(s->const_data_ptr()),
+                                              static_cast<const int*>(p->const_data_ptr()), narrow(n),
+                                              a[3] == Py_None ? narrow(n) : narrow(group), ws->mutable_data_ptr(), size_t(ws->nbytes()),
+                                              c10::cuda::getCurrentCUDAStream().stream()));
+    });
+}
+
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
 }
@@ -192,6 +215,7 @@ PyMethodDef methods[] = {{"rms_norm_q8", fast(rms_norm_q8), METH_FASTCALL, nullp
                          {"dequantize_q8", fast(dequantize_q8), METH_FASTCALL, nullptr},
                          {"rope", fast(rope), METH_FASTCALL, nullptr},
                          {"beam_select", fast(beam_select), METH_FASTCALL, nullptr},
+                         {"kv_reorder", fast(kv_reorder), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "quanta_b200_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

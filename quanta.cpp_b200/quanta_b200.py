@@ -428,14 +428,19 @@ class PagedKV:
         """A beam search's step: sequence seqs[i] becomes what seqs[i - i % group + parents[i]] was before the call (group: beams of a
         request, by default the whole list).  Full pages are shared; one child of each parent goes on with its part-filled last
         page, the others get copies of what it holds; pages that nothing uses any more are free again."""
-        n = self._list(seqs, parents)
-        if parents.numel() != n:
-            raise ValueError("one parent per sequence")
+        if stream is not None:
+            with _on_stream(stream, self.device):
+                return self.reorder(seqs, parents, group)
         if self._reorder_ws is None:
             self._reorder_ws = self._lib.qnt_kv_reorder_workspace(self._p)
-        s = self._stream(stream)
-        w, nb = self._workspace(s, self._reorder_ws)
-        self._run(self._lib.qnt_kv_reorder, self._p, seqs.data_ptr(), parents.data_ptr(), n, n if group is None else group, w, nb, s)
+        s = self._stream(None)
+        ws = self._ws.get(s)
+        if ws is None or ws.numel() < self._reorder_ws:
+            self._workspace(s, self._reorder_ws)
+            ws = self._ws[s]
+        rc = (_torch_module or _torch_calls()).kv_reorder(C.addressof(self._c), seqs, parents, group, ws)
+        if rc:
+            _check(rc)
 
     def free(self, seqs, stream=None):
         """The sequences give back their pages and become empty."""
