@@ -8,7 +8,7 @@
 // candidates lie in the k tiles with the best largest candidates (of equal ones the first).  So k_beam_tiles leaves of a tile no
 // more than its largest logit and its sum of exponentials: no warp waits for another, nothing is selected on the way.
 // k_beam_merge, a CTA per group, joins the sums, ranks the tiles and opens the k best of them.  Scores are formed and compared in
-// 64 bits.  The sums carry an error of their f32 exponentials and roundings, below 2.2e-6; where two beams' candidates lie closer
+// 64 bits.  The sums carry an error of their f32 exponentials and roundings, below 2.7e-6; where two beams' candidates lie closer
 // than that could move them, the sums of these beams are formed again in 64 bits.
 #include <climits>
 #include <type_traits>
@@ -120,6 +120,8 @@ struct Tile {
 // A warp per tile, one after another.  Bound by HBM; next to it by instructions: a logit costs half a packed maximum, its conversion,
 // half a packed fused y = x log2 e + c, the exponential and half a packed sum.  c is the f32 next to -top log2 e, and what it lacks
 // is made good in the sum.
+// 256 rows of 151936 bf16 logits: 15.6 us, 5.0 TB/s, where a loop that only reads them takes 13.7 to 14.4 (4 CTAs per SM 17.0 us, the
+// next tile through cp.async 16.7; candidates picked on the way, with thresholds from the tiles before, 30 us and more a call).
 template <class T>
 __global__ void __launch_bounds__(kTileThreads, kTileCtas)
     k_beam_tiles(const T* __restrict__ logits, long long stride, int vocab, const float* __restrict__ scores,
@@ -311,7 +313,9 @@ __device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each) {
     return min(n, k + 1);
 }
 
-// A CTA per group; bound by the latency of its steps, one behind the other.
+// A CTA per group; bound by the latency of its ten or so steps, one behind the other: 5.3 us for one group of 4 rows of 151665 f32
+// logits, 6.2 us for 64 (the k best tiles' ranking is a step of its own: opening every tile above a threshold instead took as long
+// on ordinary groups and 377 us where few beams live and their tiles lie together).
 template <class T>
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restrict__ logits, long long stride, int vocab, int beams,
                                                               const float* __restrict__ scores, const uint8_t* __restrict__ ended,

@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
 // the others get copies in fresh pages.  plan[0] = copies (-1: the call is refused), plan[1 + 3 r ..] = {from, to, blocks of 16
 // positions} of copy r.  rows, far_len: workspace for the list's new table rows, which are all read before one is written, and for its
 // lengths where shared memory does not hold them (LEN).  Pages that no sequence uses any more are free for the copies of the same
-// call.  Bound by latency, and by instructions where one SM has all entries (256 sequences of up to 32 pages: 17 us): many entries
-// go to a cluster of kReorderCtas CTAs.  Each looks up what the entries need and finds the free pages, alike; counting pages and
+// call.  Bound by latency, and by instructions where one SM has all entries: many
+// go to a cluster of kReorderCtas CTAs (256 sequences of up to 32 pages: the call 22 instead of 23 us).  Each looks up what the entries need and finds the free pages, alike; counting pages and
 // writing rows is dealt out to their warps, which have the table rows of kReorderAhead entries in flight.
 constexpr int kReorderAhead = 4;
 constexpr int kReorderCtas = 8;
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
 // Reorder, second half: the filled blocks of the copied pages, in every layer and head.  A copy's tiles have `fill` * hd pieces of
 // 16 bytes each (of a K tile hd / 16 stretches, of a V tile one); a task is kReorderThreads * kReorderPieces of them, `parts` tasks
 // at most a copy, taken in turn by as many CTAs as run together (a CTA for each task that there could be: 11 us for 256 sequences,
-// most of it to start CTAs without a task).
+// most of it to start CTAs without a task, where these take 8).
 constexpr int kReorderThreads = 256, kReorderPieces = 8, kReorderPerSm = 4;
 
 __global__ void __launch_bounds__(kReorderThreads, kReorderPerSm) k_kv_reorder(KvView c, const int* __restrict__ plan, int parts,
