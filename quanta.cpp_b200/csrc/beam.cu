@@ -200,6 +200,16 @@ __device__ __forceinline__ unsigned order_hi(double x) {
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
+// The least score whose key's upper half is `key` or more; all scores for 0.
+__device__ __forceinline__ double least_of(unsigned key) {
+    if (key == 0) return __longlong_as_double(0xfff0000000000000ll);
+    return key >> 31 ? __hiloint2double(int(key ^ 0x80000000u), 0) : __hiloint2double(int(~key), -1);
+}
+
+// Twice the error of a log sum: of a term 2^-22 (the exponential), ln 2 2^-20 (y above -32), 21 * 1.4e-8 (log2 e as f32); 12 roundings
+// of a tile's sum; 2^-22 of its weight and 8 roundings in the row's.  In all below 2.7e-6.
+constexpr double kNear = 6e-6;
+
 // e^t for t <= 0 as f32: the rounding of t log2 e made good.
 __device__ __forceinline__ float exp_neg(float t) {
     t = fmaxf(t, -150.f);
@@ -243,9 +253,10 @@ struct MergeShared {
 };
 
 // A threshold that at least k + 1 of the CTA's items reach, if there are so many, and not many more: the (k + 1)-th largest of the
-// largest items of 32 (or 128) groups of threads, whose keys are made different by their groups' numbers in the lowest bits.
+// largest items of 32 (or 128) groups of threads, whose keys are made different by their groups' numbers in the lowest bits; and less
+// by kNear, so that what the sums' errors could lift above the k-th best passes too.
 // `top`: the key of the largest item of this thread, 0: none.
-__device__ __forceinline__ unsigned threshold_of(MergeShared& sh, int k, unsigned top) {
+__device__ __forceinline__ double threshold_of(MergeShared& sh, int k, unsigned top) {
     const int tid = threadIdx.x, groups = k < 16 ? 32 : 128, of = blockDim.x / groups;
     for (int o = 1; o < of; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (tid % of == 0) sh.group_top[tid / of] = (top & ~127u) | unsigned(tid / of);
@@ -263,7 +274,7 @@ __device__ __forceinline__ unsigned threshold_of(MergeShared& sh, int k, unsigne
         if (rank == k) sh.threshold = mine & ~127u;
     }
     __syncthreads();
-    return sh.threshold;
+    return least_of(sh.threshold) - kNear;
 }
 
 __device__ __forceinline__ void push(MergeShared& sh, double score, unsigned at, int row) {
@@ -323,9 +334,6 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
                                                               unsigned row_magic, float* __restrict__ out_scores,
                                                               int* __restrict__ tokens, int* __restrict__ parents) {
     constexpr int U = kTilePieces, V = 16 / sizeof(T), kHeld = 2;  // tiles of a thread whose scores are formed once
-    // Twice the error of a log sum: of a term 2^-22 (the exponential), ln 2 2^-20 (y above -32), 21 * 1.4e-8 (log2 e as f32); 12 roundings
-    // of a tile's sum; 2^-22 of its weight and 8 roundings in the row's.  In all below 2.7e-6.
-    constexpr double kNear = 6e-6;
     extern __shared__ double lse[];                                          // [beams]; NaN: no candidates of this row
     float* score = reinterpret_cast<float*>(lse + beams);                    // [beams]
     unsigned char* state = reinterpret_cast<unsigned char*>(score + beams);  // [beams] 1: the sum is formed again, 2: exactly known, 3: none
@@ -362,8 +370,23 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
     auto value = [&](int row, float x) {
         return x == -INFINITY ? __longlong_as_double(0x7ff8000000000000ll) : double(score[row]) + (double(x) - lse[row]);
     };
-    // Whether two beams' candidates lie too close to each other in best[0 .. n - 1]; then their sums are formed again.
-    auto settle = [&](int n) {
+    // Whether two beams' candidates lie too close to each other, in best[0 .. n - 1] or around the k-th best; then their sums are formed
+    // again.  (Of kept candidates within kNear of one that is not, all have their neighbours' beams marked, or are of the k-th one's.)
+    auto settle = [&](int n, auto&& each) {
+        if (n > k) {
+            const Found last = sh.best[k - 1];
+            auto near = [&](double v, unsigned, int row) {
+                if (row == last.row || !(last.score - v < kNear) || v > last.score) return;
+                if (state[row] == 0) state[row] = 1, sh.redo = 1;
+                if (state[last.row] == 0) state[last.row] = 1, sh.redo = 1;
+            };
+            const int pushed = sh.count;
+            if (pushed <= kCap) {
+                for (int i = tid; i < pushed; i += threads) near(sh.found[i].score, sh.found[i].at, sh.found[i].row);
+            } else {
+                each(near);
+            }
+        }
         for (int i = tid; i + 1 < n; i += threads) {
             const Found &a = sh.best[i], &b = sh.best[i + 1];
             if (a.row != b.row && a.score - b.score < kNear) {
@@ -398,6 +421,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
     };
     // the best tiles, by their largest candidates; an ended beam counts as a tile of one candidate
     int n;
+    bool again;
     do {
         double held[kHeld];
         unsigned top = 0;
@@ -417,24 +441,26 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
                     if (state[b] == 2 && lse[b] != lse[b]) f(double(score[b]), unsigned(b) * unsigned(row_tiles), b);
         };
         others([&](double v, unsigned, int) { top = max(top, order_hi(v)); });
-        const unsigned least = threshold_of(sh, k, top);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-            if (held[u] == held[u] && order_hi(held[u]) >= least) push(sh, held[u], unsigned(tid + u * threads), held_row[u]);
-        others([&](double v, unsigned at, int row) {
-            if (order_hi(v) >= least) push(sh, v, at, row);
-        });
-        n = rank_found(sh, k, [&](auto&& f) {
+        const double least = threshold_of(sh, k, top);
+        auto all = [&](auto&& f) {
 #pragma unroll
             for (int u = 0; u < kHeld; ++u)
                 if (held[u] == held[u]) f(held[u], unsigned(tid + u * threads), held_row[u]);
             others(f);
+        };
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (held[u] >= least) push(sh, held[u], unsigned(tid + u * threads), held_row[u]);
+        others([&](double v, unsigned at, int row) {
+            if (v >= least) push(sh, v, at, row);
         });
-    } while (settle(n));
+        n = rank_found(sh, k, all);
+        again = settle(n, all);
+    } while (again);
     // the candidates of the k best tiles that reach the last one's largest
     const int open = min(n, k);
     bool bounded = n >= k;
-    const double floor = bounded ? sh.best[k - 1].score : 0.;
+    const double floor = bounded ? sh.best[k - 1].score - kNear : 0.;
     for (int i = tid; i < open; i += threads) tile_of[i] = sh.best[i];
     __syncthreads();
     auto each_token = [&](auto&& f) {
@@ -469,13 +495,13 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
         } else {
             unsigned top = 0;
             each_token([&](double v, unsigned, int) { top = max(top, order_hi(v)); });
-            const unsigned least = threshold_of(sh, k, top);
+            const double least = threshold_of(sh, k, top);
             each_token([&](double v, unsigned at, int row) {
-                if (order_hi(v) >= least) push(sh, v, at, row);
+                if (v >= least) push(sh, v, at, row);
             });
         }
         n = rank_found(sh, k, each_token);
-        if (!settle(n)) break;
+        if (!settle(n, each_token)) break;
     }
     const int have = min(n, k);
     out_scores += size_t(group) * k;

@@ -108,6 +108,29 @@ def test_candidates_next_to_each_other(qb, name, step, v):
 
 
 @pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 7, 8])
+@pytest.mark.parametrize("copies, beams", [(1, 3), (3, 2), (3, 4), (40, 3)])
+@pytest.mark.parametrize("v, apart", [(700, True), (6000, True), (6000, False)])
+def test_equal_logits_next_to_another_beam(qb, name, k, copies, beams, v, apart):
+    """The last kept candidates have equals in their own beam, and another beam's lie closer than the sums' roundings: whichever beam
+    is ahead in truth is kept.  Equals across tiles, or next to each other."""
+    r = torch.Generator(device="cuda").manual_seed(100 * copies + k)
+    x = torch.randn(64, 1, v, generator=r, device="cuda") * 2
+    top = torch.randperm(v, generator=r, device="cuda")[:copies] if apart else torch.arange(copies, device="cuda") + 901
+    x[..., top] = 9.5
+    x = x.to(TYPES[name])
+    order = torch.rand(64, beams, v, generator=r, device="cuda")  # a beam's own order of the other tokens, so its own roundings
+    rest = torch.ones(v, dtype=torch.bool, device="cuda")
+    rest[top] = False
+    both = x.expand(64, beams, v).clone()
+    both[..., rest] = both[..., rest].gather(2, order[..., rest].argsort(-1))
+    s = torch.full((64, beams), -(2.0 ** -6), device="cuda")
+    s += torch.arange(beams, device="cuda") * 2.0 ** -26 * torch.where(torch.rand(64, 1, generator=r, device="cuda") < 0.5, -1.0, 1.0)
+    assert all(bool((s[:, i] != s[:, i + 1]).all()) for i in range(beams - 1))
+    check(qb, both, s, k)
+
+
+@pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("share", [0.5, 0.999, 1.0])
 @pytest.mark.parametrize("k", [1, 20, 64])
 def test_forbidden_tokens(qb, name, share, k):
