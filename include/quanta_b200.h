@@ -87,7 +87,7 @@ int qnt_matmul_host(const qnt_dtensor* W, const int8_t* qx, const float* dx, int
  *   h = x + residual (f32; residual := h, rounded to its type; NULL: h = x),  y = h / sqrt(mean h^2 + eps) * weight,
  *   per 32 values: d = max |y| / 127,  q = y / d to the nearest integer, halves away from zero.
  * x [n_tok][n] at x_stride, of dtype QNT_F32, QNT_F16 or QNT_BF16; residual [n_tok][n] at residual_stride, of x's dtype or
- * QNT_F32, not x itself; weight f32 [n]; q [n_tok][n] and d [n_tok][n / 32], 16-byte aligned; n a multiple of 32, at most 32768.
+ * QNT_F32, which does not overlap x; weight f32 [n]; q [n_tok][n] and d [n_tok][n / 32], 16-byte aligned; n a multiple of 32, at most 32768.
  * Sums are in f32 (h below 10^18).  A value that is not finite makes its block read as NaN (its row, where h is not). */
 int qnt_rms_norm_q8(const void* x, int dtype, long long x_stride, void* residual, int residual_dtype, long long residual_stride,
                     const float* weight, float eps, int n_tok, int n, int8_t* q, float* d, void* stream);
@@ -113,7 +113,7 @@ int qnt_rope(const void* q, long long q_stride, void* q_out, long long q_out_str
  * [groups][beams]: such a beam has one candidate, its own score with token end_id.  Candidates that are -inf or no numbers (a
  * forbidden token, a row with NaN or +inf, a score that is not finite) come behind all others, with score -inf, in order of their
  * places.  Scores are formed and compared in f64.  k <= 64, beams <= 1024, vocab <= 2^30, beams * vocab < 2^31.
- * workspace: qnt_beam_workspace bytes, 16-byte aligned, contents irrelevant. */
+ * workspace: qnt_beam_workspace bytes, 16-byte aligned, contents irrelevant.  Results overlap neither the inputs nor each other. */
 size_t qnt_beam_workspace(int groups, int beams, int vocab, int k);
 int qnt_beam_select(const void* logits, int dtype, long long stride, const float* scores, const uint8_t* ended, int end_id,
                     int groups, int beams, int vocab, int k, float* out_scores, int* tokens, int* parents, void* workspace,

@@ -69,18 +69,6 @@ __device__ __forceinline__ Pack<__nv_bfloat16, N> from_floats(const float (&x)[N
 }
 
 template <class T, int N>
-__device__ __forceinline__ void load_row(const T* p, float (&x)[N], bool aligned) {
-    if (aligned) {
-        const Pack<T, N> w = *reinterpret_cast<const Pack<T, N>*>(p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = to_float(w.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = to_float(p[i]);
-    }
-}
-
-template <class T, int N>
 __device__ __forceinline__ void store_row(T* p, const float (&x)[N], bool aligned) {
     if (aligned) {
         *reinterpret_cast<Pack<T, N>*>(p) = from_floats(x, T());

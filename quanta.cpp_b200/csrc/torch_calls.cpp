@@ -71,7 +71,7 @@ bool to_long(PyObject* o, long long* v) {
     return !(*v == -1 && PyErr_Occurred());
 }
 
-int narrow(int64_t n) { return n > INT32_MAX ? INT32_MAX : int(n); }  // (what does not fit is refused further down)
+int narrow(int64_t n) { return n > INT32_MAX ? INT32_MAX : n < INT32_MIN ? INT32_MIN : int(n); }  // (what does not fit is refused further down)
 
 // x, weight, eps, residual or None -> (q, d)
 PyObject* rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -140,7 +140,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         // (of a single head the stride between heads says nothing)
         const int rc = qnt_rope(q->const_data_ptr(), q->stride(0), q_out.mutable_data_ptr(), q_out.stride(0), narrow(q->size(1)),
                                 k ? k->const_data_ptr() : nullptr, k ? k->stride(0) : 0, k ? k_out.mutable_data_ptr() : nullptr,
-                                k ? k_out.stride(0) : 0, k ? narrow(k->size(1)) : 0, dtype_of(*q), narrow(q->size(2)), int(rotary_dim),
+                                k ? k_out.stride(0) : 0, k ? narrow(k->size(1)) : 0, dtype_of(*q), narrow(q->size(2)), narrow(rotary_dim),
                                 int(interleaved), static_cast<const double*>(t->const_data_ptr()), float(scale),
                                 static_cast<const int*>(p->const_data_ptr()), narrow(p->size(0)), c10::cuda::getCurrentCUDAStream().stream());
         if (rc) return PyLong_FromLong(rc);
@@ -167,11 +167,12 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             refuse("ended must be a contiguous bool or uint8 CUDA tensor [groups, beams] on the logits' device");
         if (!ws || ws->device() != x->device() || !ws->is_contiguous()) refuse("workspace");
         const c10::cuda::CUDAGuard on(x->device());
-        at::Tensor out = empty({g, k}, at::kFloat, x->device()), tokens = empty({g, k}, at::kInt, x->device()),
-                   parents = empty({g, k}, at::kInt, x->device());
+        const int64_t width = k < 0 ? 0 : k > 64 ? 64 : k;  // (any other k is refused below)
+        at::Tensor out = empty({g, width}, at::kFloat, x->device()), tokens = empty({g, width}, at::kInt, x->device()),
+                   parents = empty({g, width}, at::kInt, x->device());
         const int rc = qnt_beam_select(x->const_data_ptr(), dtype_of(*x), row, static_cast<const float*>(s->const_data_ptr()),
-                                       e ? static_cast<const uint8_t*>(e->const_data_ptr()) : nullptr, int(end_id), narrow(g), narrow(b),
-                                       narrow(v), int(k), static_cast<float*>(out.mutable_data_ptr()), static_cast<int*>(tokens.mutable_data_ptr()),
+                                       e ? static_cast<const uint8_t*>(e->const_data_ptr()) : nullptr, narrow(end_id), narrow(g), narrow(b),
+                                       narrow(v), narrow(k), static_cast<float*>(out.mutable_data_ptr()), static_cast<int*>(tokens.mutable_data_ptr()),
                                        static_cast<int*>(parents.mutable_data_ptr()), ws->mutable_data_ptr(), size_t(ws->nbytes()),
                                        c10::cuda::getCurrentCUDAStream().stream());
         if (rc) return PyLong_FromLong(rc);

@@ -254,3 +254,28 @@ def test_what_is_refused(qb):
         qb.BeamSelector(65)(x, s)
     out = sel(x[:0], s[:0])
     assert all(t.shape == (0, 4) for t in out)
+
+
+@pytest.mark.parametrize("k, end_id, word", [(2 ** 32 + 4, -1, "at most 64"), (-(2 ** 32) + 4, -1, "positive"), (4, 2 ** 32 + 5, "end_id"),
+                                             (4, -(2 ** 32) + 5, "end_id")])
+def test_numbers_past_32_bits_are_refused(qb, k, end_id, word):
+    """Not taken for what their lower half says."""
+    x, s = make(2, 3, 100, "f32")
+    with pytest.raises(qb.QntError, match=word):
+        qb.BeamSelector(k, end_id=end_id)(x, s, torch.zeros(2, 3, dtype=torch.bool, device="cuda"))
+
+
+def test_two_streams_at_once(qb):
+    """One object on two streams, with sizes that make both calls overlap."""
+    sel, streams = qb.BeamSelector(8), [torch.cuda.Stream() for _ in range(2)]
+    sets = [make(64, 4, 50000, "bf16", seed=70 + i) for i in range(2)]
+    want = [sel(*a) for a in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            got[i].append(sel(*sets[i], stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
