@@ -14,15 +14,30 @@ bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>
 
 // With h = x + r (r: the residual row, h rounded once into it):
 //     y = h * (1 / sqrt(mean h^2 + eps)) * w;  per 32 values: d = max |y| / 127, q = y / d to the nearest, halves away from 0
-// A CTA per row, which stays in registers between the sum and the rounding: every byte crosses HBM once.  A thread holds R chunks
-// of 8 consecutive values, so that a block of 32 is 4 neighbouring lanes and its maximum two shuffles.  Sums in f32: per thread,
-// then per warp, then over warps (an error of a few 2^-24).  A block with a value that is not finite gets a NaN for its scale.  Next
-// to HBM instructions bound it, so values go in pairs (f32x2), and a code is the low byte of t + 1.5 * 2^23: with t = y * (1 / d, one
-// step up) that addition rounds to the nearest, halves away from 0 as far as t says where they are.
+// A row stays in registers between the sum and the rounding: every byte crosses HBM once.  A thread holds R chunks of 8 consecutive
+// values, so that a block of 32 is 4 neighbouring lanes and its maximum two shuffles.  Sums in f32: per thread, then per warp, then
+// over warps (an error of a few 2^-24).  A block with a value that is not finite gets a NaN for its scale.  Next to HBM, and without a
+// residual more than HBM (8192 rows of 4096 bf16: 23.7 us, 16.4 of them for the bytes), instructions bound it.  So values go in pairs
+// (f32x2), and a code is the low byte of y * u + 1.5 * 2^23, one operation whose rounding is that to the nearest integer; u is 1 / d
+// one step up, so that halves go away from 0.
 __device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
     unsigned long long r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+// max |.| that keeps a NaN
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 1 / d of a normal d below 2^126: an approximation and a step of Newton's method, within a unit in the last place.
+__device__ __forceinline__ float reciprocal(float d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return fmaf(r, fmaf(-d, r, 1.f), r);
 }
 
 // 8 elements as they are in memory, as 4 pairs of f32, and back with one rounding.
@@ -62,7 +77,7 @@ __device__ __forceinline__ void store_pairs(T* p, const unsigned long long (&x)[
 }
 
 // RES: there is a residual.  Rows blockIdx.x, blockIdx.x + gridDim.x, ...: the weights stay in registers, and the next row is on its
-// way while one is worked on.  8192 rows of 4096 bf16 with a bf16 residual: 38.7 us, 6.2 TB/s (a CTA per row reads its weights, twice
+// way while one is worked on.  8192 rows of 4096 bf16 with a bf16 residual: 38.2 us, 6.3 TB/s (a CTA per row reads its weights, twice
 // as many bytes as a 16-bit row, from L2 each time: 46 us).
 template <class T, class RT, int R, int THREADS, bool RES, bool VEC>
 __global__ void __launch_bounds__(THREADS)
@@ -98,6 +113,7 @@ __global__ void __launch_bounds__(THREADS)
     for (int r = 0; r < R; ++r) {
         const int c = r * threads + tid;
         if (c < chunks) to_pairs(load_raw<float, VEC>(weight + c * C), w[r]);
+        else w[r][0] = w[r][1] = w[r][2] = w[r][3] = 0;
     }
     for (int row = blockIdx.x, turn = 0; row < n_tok; row += gridDim.x, turn ^= 1) {
         unsigned long long h[R][4], squares = 0;
@@ -128,7 +144,10 @@ __global__ void __launch_bounds__(THREADS)
         if (threads > 32) {
             if (lane == 0) part[turn][warp] = sum;
             __syncthreads();  // (the other half is written again only after the next one)
-            sum = warp_sum(lane < threads >> 5 ? part[turn][lane] : 0.f);
+            constexpr int W = THREADS / 32;  // (every lane ends with the sum of all)
+            sum = (lane & (W - 1)) < threads >> 5 ? part[turn][lane & (W - 1)] : 0.f;
+#pragma unroll
+            for (int o = W / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
         const float inv = __frsqrt_rn(sum / float(n) + eps);
         const unsigned long long inv2 = f2_pack(inv, inv), magic = f2_pack(12582912.f, 12582912.f);
@@ -140,19 +159,19 @@ __global__ void __launch_bounds__(THREADS)
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                y[i] = in ? f2_mul(f2_mul(h[r][i], inv2), w[r][i]) : 0;
+                y[i] = f2_mul(f2_mul(h[r][i], inv2), w[r][i]);
                 const float2 v = f2_unpack(y[i]);
-                top = max_or_nan(top, max_or_nan(fabsf(v.x), fabsf(v.y)));
+                top = max3_or_nan(top, fabsf(v.x), fabsf(v.y));
             }
             top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float scale = div127(top), step = scale > 0.f ? __frcp_rn(scale) : 0.f;
-            const float up = step > 0.f && step <= 3.402823466e38f ? __uint_as_float(__float_as_uint(step) + 1) : 0.f;
+            const float scale = div127(top);
+            const float up = scale >= 1.17549435e-38f ? __uint_as_float(__float_as_uint(reciprocal(scale)) + 1) : 0.f;
             const unsigned long long up2 = f2_pack(up, up);
             unsigned b[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float2 t = f2_unpack(f2_add(f2_mul(y[i], up2), magic));
+                const float2 t = f2_unpack(f2_fma(y[i], up2, magic));
                 b[2 * i] = __float_as_uint(t.x);
                 b[2 * i + 1] = __float_as_uint(t.y);
             }
@@ -169,8 +188,12 @@ __global__ void __launch_bounds__(THREADS)
 
 template <class T, class RT, bool RES, bool VEC>
 cudaError_t norm_r(const NormQ8Args& a, cudaStream_t st) {
-    // a chunk a thread up to 2048 values, two up to 16384: rows of 4096 bf16 with their residual 38.7 us for 8192 (one chunk: 49, four: 59)
-    const int chunks = a.n / 8, r = chunks <= 256 ? 1 : chunks <= 2048 ? 2 : 4;
+    // Two chunks a thread halve a row's shuffles and its barrier: 8192 rows of 4096 bf16 with their residual 38.2 us (one chunk: 49,
+    // four: 59), 16384 of 2048 38.0 (one: 46.4).  One has the shorter chain where rows are few: 256 of 896 f32 1.9 us (two: 2.3), 1000
+    // of 1024 3.2 (3.3), 600 of 2048 bf16 3.0 (2.9).
+    const int chunks = a.n / 8;
+    const bool many = chunks > 32 && (long long)a.n_tok * chunks >= 148 * 1024;
+    const int r = chunks <= 256 && !many ? 1 : chunks <= 2048 ? 2 : 4;
     const int threads = ((chunks + r - 1) / r + 31) / 32 * 32;
     auto kern = r == 1           ? k_rms_norm_q8<T, RT, 1, 256, RES, VEC>
                 : r == 4         ? k_rms_norm_q8<T, RT, 4, 1024, RES, VEC>
