@@ -59,6 +59,28 @@ def test_norm(qb, name, residual, m, n):
 
 
 @pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("residual, pad, lead", [(None, 0, 0), ("same", 0, 0), ("f32", 0, 0), (None, 3, 1), ("same", 5, 3), ("f32", 1, 1)])
+@pytest.mark.parametrize("m, n", [(5000, 256), (4700, 288), (3900, 352), (2000, 896), (1201, 1024), (651, 2048)])
+def test_norm_of_many_short_rows(qb, name, residual, pad, lead, m, n):
+    x = rows(m, n, name, seed=n, pad=pad, lead=lead)
+    w = 1 + 0.3 * rows(1, n, "f32", seed=1, lead=lead)[0]
+    r = None if residual is None else rows(m, n, name if residual == "same" else "f32", seed=2, pad=pad, lead=lead, std=3.0)
+    check_norm(qb, x, w, 1e-6, r)
+
+
+def test_norm_of_the_smallest_numbers(qb):
+    """Scales below the normal numbers: a block reads as zeros, which is within 128 of 2^-126; above, as ever."""
+    x, w = rows(2, 160, "f32", seed=12), torch.full((160,), 1e-36, device="cuda")
+    w[32:64], w[64:96], w[96:128] = 1e-38, 3e-37, 1e-35
+    q, d = qb.rms_norm_q8(x, w)
+    v = qb.dequantize_q8(q, d, torch.float32).double().unflatten(1, (-1, 32))
+    y = (x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()).unflatten(1, (-1, 32))
+    top = y.abs().amax(-1, keepdim=True)
+    assert bool(((v - y).abs() <= torch.where(top > 127.5 * 2.0 ** -126, (0.5 + 3e-4) * top / 127, 128 * 2.0 ** -126)).all())
+    assert bool((q.unflatten(1, (-1, 32))[:, 3] != 0).any()) and not q.unflatten(1, (-1, 32))[:, 1].any()
+
+
+@pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("pad, lead", [(8, 0), (8, 8), (1, 0), (0, 1), (3, 5)])
 def test_norm_of_rows_in_wider_ones(qb, name, pad, lead):
     w = rows(1, 896, "f32", seed=3, lead=lead)[0]
