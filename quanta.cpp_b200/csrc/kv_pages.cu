@@ -356,9 +356,9 @@ __device__ __forceinline__ int cta_scan(int x, int* total) {
 }
 
 // words[g] = bit i set where page 32 g + i is free (pages past the pool are not).
-__device__ __forceinline__ void free_bitmap(const KvView& c, unsigned* words, int n_words) {
+template <int U>  // loads in flight
+__device__ __forceinline__ void free_bitmap_of(const KvView& c, unsigned* words, int n_words) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    constexpr int U = 16;  // loads in flight
     for (int g0 = warp * U; g0 < n_words; g0 += warps * U) {
         int r[U];
 #pragma unroll
@@ -374,18 +374,33 @@ __device__ __forceinline__ void free_bitmap(const KvView& c, unsigned* words, in
     }
 }
 
+__device__ __forceinline__ void free_bitmap(const KvView& c, unsigned* words, int n_words) {
+    if (n_words <= int(blockDim.x >> 5) * 4) free_bitmap_of<4>(c, words, n_words);  // (small pools: all warps take part)
+    else free_bitmap_of<16>(c, words, n_words);
+}
+
 // list[r] = the r-th free page for r < want; returns how many pages are free.  All threads of the CTA; ends synchronised.
 __device__ int lowest_free(const KvView& c, unsigned* words, int want, int* list) {
+    __shared__ int first[kPlanThreads];  // how many are free before a thread's words
     const int n_words = (c.n_pages + 31) / 32, per = (n_words + blockDim.x - 1) / int(blockDim.x);
+    const int lane = threadIdx.x & 31, warps = int(blockDim.x >> 5);
     free_bitmap(c, words, n_words);
     __syncthreads();
     const int w0 = min(int(threadIdx.x) * per, n_words), w1 = min(w0 + per, n_words);
     int mine = 0, total;
     for (int w = w0; w < w1; ++w) mine += __popc(words[w]);
-    int r = cta_scan(mine, &total);
-    if (total >= want)
-        for (int w = w0; w < w1 && r < want; ++w)
-            for (unsigned b = words[w]; b && r < want; b &= b - 1) list[r++] = w * 32 + __ffs(b) - 1;
+    first[threadIdx.x] = cta_scan(mine, &total);
+    __syncthreads();
+    if (total >= want)  // a warp writes a word's pages at once
+        for (int t = int(threadIdx.x >> 5); t * per < n_words; t += warps) {
+            int r = first[t];
+            for (int w = t * per; w < min(t * per + per, n_words) && r < want; ++w) {
+                const unsigned b = words[w];
+                const int at = r + __popc(b & ((1u << lane) - 1));
+                if ((b >> lane & 1) && at < want) list[at] = w * 32 + lane;
+                r += __popc(b);
+            }
+        }
     __syncthreads();
     return total;
 }
@@ -502,6 +517,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
 constexpr int kReorderAhead = 4;
 constexpr int kReorderCtas = 8;
 
+// A CTA's shared variable, as CTA `rank` of the cluster has it.
+__device__ __forceinline__ int shared_of(const int* x, unsigned rank) {
+    unsigned at;
+    int v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(unsigned(__cvta_generic_to_shared(x))), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -525,7 +549,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
     const int tid = threadIdx.x, lane = tid & 31;
     const int warps = gridDim.x * (blockDim.x >> 5), warp = blockIdx.x * (blockDim.x >> 5) + (tid >> 5);  // of the cluster
     if (tid == 0) bad = 0;
-    if (tid == 0 && blockIdx.x == 0) plan[0] = 0;
     for (int s = tid; s < kKvMaxSeqs / 32; s += blockDim.x) mark[s] = 0;
     for (int i = tid; i < n; i += blockDim.x) heir[i] = INT_MAX;
     __syncthreads();
@@ -561,8 +584,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
     const int before = cta_scan(mine, &want);
     for (int i = i0; i < i1; ++i) base[i] = uint16_t(base[i] + before);
     const bool alone = gridDim.x == 1;
-    if (alone) __syncthreads();
-    else cluster_sync();  // (every CTA has read the lengths, plan[0] is 0)
+    __syncthreads();
     // entry i: changed, gets a copy, pages before and after
     struct Entry {
         bool changed, copy;
@@ -579,15 +601,13 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         }
         return e;
     };
+    int held[kReorderAhead];  // entry (warp + u * warps)'s page `lane`, as `rows` has it
     // the pages that the rows lose and gain; sign -1 takes it back
     auto count = [&](int sign) {
         auto one = [&](const Entry& e, int i, int k, int a, int b) {
-            if (sign > 0) rows[size_t(i) * c.max_pages + k] = b;
+            if (sign > 0 && (k >= 32 || i >= warps * kReorderAhead)) rows[size_t(i) * c.max_pages + k] = b;
             if (e.copy && k == e.n_now - 1) {
-                if (sign > 0 && (b < 0 || b >= c.n_pages)) {
-                    if (alone) bad = 1;
-                    else atomicExch(plan, -1);
-                }
+                if (sign > 0 && (b < 0 || b >= c.n_pages)) bad = 1;
                 b = -1;  // a fresh page
             }
             if (a == b) return;
@@ -602,6 +622,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
                 const Entry e = entry(i);
                 a[u] = e.changed && lane < e.n_old ? c.table[size_t(seq[i]) * c.max_pages + lane] : -1;
                 b[u] = e.changed && lane < e.n_now ? c.table[size_t(seq[par[i]]) * c.max_pages + lane] : -1;
+                if (i0 == warp) held[u] = b[u];
             }
 #pragma unroll
             for (int u = 0; u < kReorderAhead; ++u) {
@@ -620,8 +641,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
     if (alone) __syncthreads();
     else cluster_sync();  // every row has been read, every page counted
     int* list = heir;  // fresh pages
-    int status = (alone ? bad : __ldcg(plan) < 0) ? int(ERR_BAD_POS) : 0;
-    if (!status && want > 0 && lowest_free(c, words, want, list) < want) status = int(ERR_CAPACITY);
+    const int wrong = alone ? bad : lane < int(gridDim.x) ? shared_of(&bad, unsigned(lane)) : 0;
+    const bool enough = want == 0 || lowest_free(c, words, want, list) >= want;
+    const int status = __any_sync(0xffffffffu, wrong) ? int(ERR_BAD_POS) : enough ? 0 : int(ERR_CAPACITY);
     if (!alone) cluster_sync();  // every CTA has found the free pages
     if (status) {  // (in every CTA alike)
         count(-1);
@@ -637,7 +659,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         for (int u = 0; u < kReorderAhead; ++u) {
             const int i = i0 + u * warps;
             const Entry e = entry(i);
-            p[u] = e.changed && lane < max(e.n_old, e.n_now) ? rows[size_t(i) * c.max_pages + lane] : -1;
+            p[u] = i0 == warp ? held[u] : e.changed && lane < max(e.n_old, e.n_now) ? rows[size_t(i) * c.max_pages + lane] : -1;
         }
 #pragma unroll
         for (int u = 0; u < kReorderAhead; ++u) {
