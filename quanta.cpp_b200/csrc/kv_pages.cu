@@ -350,7 +350,7 @@ __device__ __forceinline__ int cta_scan(int x, int* total) {
     __syncthreads();
     if (lane == 31) part[warp] = inc;
     __syncthreads();
-    const int p = lane < int(blockDim.x >> 5) ? part[lane] : 0;
+    const int p = part[lane];
     *total = __reduce_add_sync(0xffffffffu, p);
     return __reduce_add_sync(0xffffffffu, lane < warp ? p : 0) + inc - x;
 }
@@ -358,7 +358,8 @@ __device__ __forceinline__ int cta_scan(int x, int* total) {
 // words[g] = bit i set where page 32 g + i is free (pages past the pool are not).
 template <int U>  // loads in flight
 __device__ __forceinline__ void free_bitmap_of(const KvView& c, unsigned* words, int n_words) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    constexpr int warps = kPlanThreads / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int g0 = warp * U; g0 < n_words; g0 += warps * U) {
         int r[U];
 #pragma unroll
@@ -375,15 +376,15 @@ __device__ __forceinline__ void free_bitmap_of(const KvView& c, unsigned* words,
 }
 
 __device__ __forceinline__ void free_bitmap(const KvView& c, unsigned* words, int n_words) {
-    if (n_words <= int(blockDim.x >> 5) * 4) free_bitmap_of<4>(c, words, n_words);  // (small pools: all warps take part)
+    if (n_words <= kPlanThreads / 32 * 4) free_bitmap_of<4>(c, words, n_words);  // (small pools: all warps take part)
     else free_bitmap_of<16>(c, words, n_words);
 }
 
 // list[r] = the r-th free page for r < want; returns how many pages are free.  All threads of the CTA; ends synchronised.
 __device__ int lowest_free(const KvView& c, unsigned* words, int want, int* list) {
     __shared__ int first[kPlanThreads];  // how many are free before a thread's words
-    const int n_words = (c.n_pages + 31) / 32, per = (n_words + blockDim.x - 1) / int(blockDim.x);
-    const int lane = threadIdx.x & 31, warps = int(blockDim.x >> 5);
+    const int n_words = (c.n_pages + 31) / 32, per = (n_words + kPlanThreads - 1) / kPlanThreads;
+    const int lane = threadIdx.x & 31;
     free_bitmap(c, words, n_words);
     __syncthreads();
     const int w0 = min(int(threadIdx.x) * per, n_words), w1 = min(w0 + per, n_words);
@@ -392,7 +393,7 @@ __device__ int lowest_free(const KvView& c, unsigned* words, int want, int* list
     first[threadIdx.x] = cta_scan(mine, &total);
     __syncthreads();
     if (total >= want)  // a warp writes a word's pages at once
-        for (int t = int(threadIdx.x >> 5); t * per < n_words; t += warps) {
+        for (int t = int(threadIdx.x >> 5); t * per < n_words; t += kPlanThreads / 32) {
             int r = first[t];
             for (int w = t * per; w < min(t * per + per, n_words) && r < want; ++w) {
                 const unsigned b = words[w];
@@ -547,12 +548,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
     __shared__ unsigned mark[kKvMaxSeqs / 32];
     __shared__ int bad;
     const int tid = threadIdx.x, lane = tid & 31;
-    const int warps = gridDim.x * (blockDim.x >> 5), warp = blockIdx.x * (blockDim.x >> 5) + (tid >> 5);  // of the cluster
+    const int warps = gridDim.x * (kPlanThreads / 32), warp = blockIdx.x * (kPlanThreads / 32) + (tid >> 5);  // of the cluster
     if (tid == 0) bad = 0;
-    for (int s = tid; s < kKvMaxSeqs / 32; s += blockDim.x) mark[s] = 0;
-    for (int i = tid; i < n; i += blockDim.x) heir[i] = INT_MAX;
+    for (int s = tid; s < kKvMaxSeqs / 32; s += kPlanThreads) mark[s] = 0;
+    for (int i = tid; i < n; i += kPlanThreads) heir[i] = INT_MAX;
     __syncthreads();
-    for (int i = tid; i < n; i += blockDim.x) {
+    for (int i = tid; i < n; i += kPlanThreads) {
         const int s = seqs[i], p = parents[i];
         if (s < 0 || s >= c.max_seqs || p < 0 || p >= group || (atomicOr(mark + s / 32, 1u << s % 32) >> s % 32 & 1)) {
             bad = int(ERR_BAD_POS);
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
         }
         return;
     }
-    const int per = (n + int(blockDim.x) - 1) / int(blockDim.x);
+    const int per = (n + kPlanThreads - 1) / kPlanThreads;
     const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
     int mine = 0, want;
     for (int i = i0; i < i1; ++i) {
