@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas)
                  const uint8_t* __restrict__ ended, int row_tiles, int tiles, Tile* __restrict__ out) {
     constexpr int U = kTilePieces, V = 16 / sizeof(T);
     const int lane = threadIdx.x & 31, warps = gridDim.x * (kTileThreads / 32);
-    pdl_launch_dependents();
+    pdl_wait();
+    pdl_launch_dependents();  // (only now: the merge reads the scores before its own wait)
     for (int t = blockIdx.x * (kTileThreads / 32) + (threadIdx.x >> 5); t < tiles; t += warps) {
         const int r = t / row_tiles, j = t - r * row_tiles;
         const float score = __ldg(scores + r);
@@ -342,14 +343,15 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = blockDim.x, warps = threads >> 5;
     const int group = blockIdx.x, r0 = group * beams;
     for (int b = tid; b < beams; b += threads) {
-        const float sc = __ldg(scores + r0 + b);
-        const bool over = ended && __ldg(ended + r0 + b);
+        const float sc = __ldcg(scores + r0 + b);  // (from L2: an older call's line may be nearer)
+        const bool over = ended && __ldcg(ended + r0 + b);
         score[b] = sc;
         state[b] = fabsf(sc) <= kMaxF ? over ? 2 : 0 : 3;
     }
     if (tid == 0) sh.redo = 0;
     __syncthreads();
     pdl_wait();
+    pdl_launch_dependents();
     const int n_tiles = beams * row_tiles;
     const Tile* mine = tiles + size_t(r0) * row_tiles;
     auto row_of = [&](int c) { return row_magic ? int(__umulhi(unsigned(c), row_magic)) : c / row_tiles; };
@@ -541,7 +543,7 @@ template <class T>
 cudaError_t select_t(const BeamArgs& a, Tile* ws, cudaStream_t st) {
     const int row_tiles = row_tiles_of(a), tiles = a.groups * a.beams * row_tiles, warps = kTileThreads / 32;
     const int ctas = (tiles + warps - 1) / warps, most = 148 * kTileCtas;
-    cudaError_t e = launch_pdl(k_beam_tiles<T>, dim3(unsigned(ctas < most ? ctas : most)), dim3(kTileThreads), 0, st, false,
+    cudaError_t e = launch_pdl(k_beam_tiles<T>, dim3(unsigned(ctas < most ? ctas : most)), dim3(kTileThreads), 0, st, true,
                                static_cast<const T*>(a.logits), a.stride, a.vocab, a.scores, a.ended, row_tiles, tiles, ws);
     if (e != cudaSuccess) return e;
     // c / row_tiles = umulhi(c, ceil(2^32 / row_tiles)) for both below 2^16, row_tiles > 1

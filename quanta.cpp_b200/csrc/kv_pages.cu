@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(KvView c, const i
 // positions} of copy r.  rows, far_len: workspace for the list's new table rows, which are all read before one is written, and for its
 // lengths where shared memory does not hold them (LEN).  Pages that no sequence uses any more are free for the copies of the same
 // call.  Bound by latency, and by instructions where one SM has all entries: many
-// go to a cluster of kReorderCtas CTAs (256 sequences of up to 32 pages: the call 22 instead of 23 us).  Each looks up what the entries need and finds the free pages, alike; counting pages and
+// go to a cluster of kReorderCtas CTAs (256 sequences of up to 32 pages: 8.0 us, the call 16.2).  Each looks up what the entries need and finds the free pages, alike; counting pages and
 // writing rows is dealt out to their warps, which have the table rows of kReorderAhead entries in flight.
 constexpr int kReorderAhead = 4;
 constexpr int kReorderCtas = 8;
@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_reorder_plan(KvView c, cons
                                                                   int* __restrict__ plan, int* __restrict__ rows,
                                                                   int* __restrict__ far_len) {
     extern __shared__ __align__(16) unsigned smem[];
+    pdl_wait();
     pdl_launch_dependents();
     unsigned* words = smem;
     int* heir = reinterpret_cast<int*>(words + plan_words(c));  // of each place of the list: who gets its part-filled page
@@ -1037,11 +1038,13 @@ cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* paren
     cfg.blockDim = dim3(kPlanThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {cfg.gridDim.x, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kern, c, seqs, parents, n, group, plan, rows, len);
     if (e != cudaSuccess) return e;
     const size_t per = size_t(kReorderThreads) * kReorderPieces * 16, parts = (c.page_codes() + per - 1) / per, tasks = parts * size_t(n);

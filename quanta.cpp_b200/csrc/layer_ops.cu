@@ -85,6 +85,8 @@ __global__ void __launch_bounds__(THREADS)
                   const float* __restrict__ weight, float eps, int n_tok, int n, int8_t* __restrict__ q, float* __restrict__ d) {
     constexpr int C = 8;
     __shared__ float part[2][32];
+    pdl_wait();
+    pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = n / C, threads = blockDim.x;
     Raw8<T> rx[R];
     Raw8<RT> rr[R];
@@ -200,7 +202,7 @@ cudaError_t norm_r(const NormQ8Args& a, cudaStream_t st) {
                 : threads <= 512 ? k_rms_norm_q8<T, RT, 2, 512, RES, VEC>
                                  : k_rms_norm_q8<T, RT, 2, 1024, RES, VEC>;
     const int most = 148 * (2048 / threads > 16 ? 16 : 2048 / threads);
-    return launch_pdl(kern, dim3(unsigned(a.n_tok < most ? a.n_tok : most)), dim3(unsigned(threads)), 0, st, false,
+    return launch_pdl(kern, dim3(unsigned(a.n_tok < most ? a.n_tok : most)), dim3(unsigned(threads)), 0, st, true,
                       static_cast<const T*>(a.x), a.x_stride, static_cast<RT*>(a.residual), a.residual_stride, a.weight, a.eps, a.n_tok,
                       a.n, a.q, a.d);
 }
@@ -224,6 +226,8 @@ __global__ void __launch_bounds__(256) k_dequantize_q8(const int8_t* __restrict_
                                                        T* __restrict__ out) {
     constexpr int V = 16 / sizeof(T);
     using Codes = typename std::conditional<V == 8, uint2, unsigned>::type;
+    pdl_wait();
+    pdl_launch_dependents();
     const long long first = (long long)blockIdx.x * (256 * kDequantAhead) + threadIdx.x;
     Codes w[kDequantAhead];
     float s[kDequantAhead];
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(256) k_dequantize_q8(const int8_t* __restrict_
 template <class T>
 cudaError_t dequantize_t(const int8_t* q, const float* d, long long n, void* out, cudaStream_t st) {
     const long long pieces = n * sizeof(T) / 16, per = 256 * kDequantAhead;
-    return launch_pdl(k_dequantize_q8<T>, dim3(unsigned((pieces + per - 1) / per)), dim3(256), 0, st, false, q, d, pieces,
+    return launch_pdl(k_dequantize_q8<T>, dim3(unsigned((pieces + per - 1) / per)), dim3(256), 0, st, true, q, d, pieces,
                       static_cast<T*>(out));
 }
 
@@ -298,6 +302,8 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(RopeHeads qh, RopeHeads k
                                                        const int* __restrict__ positions, const double* __restrict__ turns, float scale,
                                                        int units) {
     constexpr int P = INTER ? V / 2 : V, AHEAD = INTER ? 4 : 2;  // pairs of a unit, heads in flight
+    pdl_wait();
+    pdl_launch_dependents();
     const int pairs = rotary_dim / 2, n_rot = INTER ? rotary_dim / V : pairs / V;
     // thread -> token, slot, unit; units: rotated ones first, then ones (half layout: two) of V dims that are only copied
     const long long id = (long long)blockIdx.x * kRopeThreads + threadIdx.x;
@@ -376,7 +382,7 @@ cudaError_t rope_v(const RopeArgs& a, cudaStream_t st) {
     if (slots > most) slots = most;
     const long long threads = (long long)a.n_tok * slots * units, ctas = (threads + kRopeThreads - 1) / kRopeThreads;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return launch_pdl(k_rope<T, V, INTER, VEC>, dim3(unsigned(ctas)), dim3(kRopeThreads), 0, st, false, a.q, a.k, a.head_dim, a.rotary_dim,
+    return launch_pdl(k_rope<T, V, INTER, VEC>, dim3(unsigned(ctas)), dim3(kRopeThreads), 0, st, true, a.q, a.k, a.head_dim, a.rotary_dim,
                       a.n_tok, slots, a.positions, a.turns, a.scale, units);
 }
 
