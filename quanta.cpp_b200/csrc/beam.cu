@@ -284,9 +284,10 @@ __device__ __forceinline__ void push(MergeShared& sh, double score, unsigned at,
 }
 
 // best[0 .. n - 1] = the n = min(k + 1, all) best of the items that have been pushed, in order; where they are too many, of all that
-// each(f) calls f(score, place, row) for.  A warp ranks an item by counting.  Ends synchronised.
-template <class Each>
-__device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each) {
+// each(f) calls f(score, place, row) for.  A warp ranks an item by counting, and calls close(row, other row) where an item among the k
+// best and one of another row lie within kNear of each other.  Ends synchronised.
+template <class Each, class Close>
+__device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each, Close&& close) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     __syncthreads();
     const int n = sh.count;
@@ -294,9 +295,17 @@ __device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each) {
         for (int c = warp; c < n; c += warps) {
             const Found mine = sh.found[c];
             int rank = 0;
-            for (int o = lane; o < n; o += 32) rank += before(sh.found[o], mine);
+            bool near = false;
+            for (int o = lane; o < n; o += 32) {
+                const Found f = sh.found[o];
+                rank += before(f, mine);
+                near |= f.row != mine.row && fabs(f.score - mine.score) < kNear;
+            }
             rank = __reduce_add_sync(0xffffffffu, rank);
             if (rank <= k && lane == 0) sh.best[rank] = mine;
+            if (near && rank < k)
+                for (int o = lane; o < n; o += 32)
+                    if (fabs(sh.found[o].score - mine.score) < kNear) close(sh.found[o].row, mine.row);
         }
     } else {  // very many that reach the threshold: the best one behind the last, k + 1 times
         Found last{INFINITY, 0, 0};
@@ -320,13 +329,20 @@ __device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each) {
                 if (before(sh.found[w], last)) last = sh.found[w];
             if (tid == 0) sh.best[i] = last;
         }
+        __syncthreads();
+        for (int i = 0; i < min(n, k); ++i) {
+            const Found kept = sh.best[i];
+            each([&](double score, unsigned, int row) {
+                if (row != kept.row && fabs(score - kept.score) < kNear) close(row, kept.row);
+            });
+        }
     }
     __syncthreads();
     return min(n, k + 1);
 }
 
-// A CTA per group; bound by the latency of its ten or so steps, one behind the other: 5.3 us for one group of 4 rows of 151665 f32
-// logits, 6.2 us for 64 (the k best tiles' ranking is a step of its own: opening every tile above a threshold instead took as long
+// A CTA per group; bound by the latency of its ten or so steps, one behind the other: 5.8 us for one group of 4 rows of 151936 bf16
+// logits, 6.5 us for 64 (close candidates looked for in steps of their own: 6.4 and 7.2; the k best tiles' ranking is a step of its own: opening every tile above a threshold instead took as long
 // on ordinary groups and 377 us where few beams live and their tiles lie together).
 template <class T>
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restrict__ logits, long long stride, int vocab, int beams,
@@ -372,31 +388,13 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
     auto value = [&](int row, float x) {
         return x == -INFINITY ? __longlong_as_double(0x7ff8000000000000ll) : double(score[row]) + (double(x) - lse[row]);
     };
-    // Whether two beams' candidates lie too close to each other, in best[0 .. n - 1] or around the k-th best; then their sums are formed
-    // again.  (Of kept candidates within kNear of one that is not, all have their neighbours' beams marked, or are of the k-th one's.)
-    auto settle = [&](int n, auto&& each) {
-        if (n > k) {
-            const Found last = sh.best[k - 1];
-            auto near = [&](double v, unsigned, int row) {
-                if (row == last.row || !(last.score - v < kNear) || v > last.score) return;
-                if (state[row] == 0) state[row] = 1, sh.redo = 1;
-                if (state[last.row] == 0) state[last.row] = 1, sh.redo = 1;
-            };
-            const int pushed = sh.count;
-            if (pushed <= kCap) {
-                for (int i = tid; i < pushed; i += threads) near(sh.found[i].score, sh.found[i].at, sh.found[i].row);
-            } else {
-                each(near);
-            }
-        }
-        for (int i = tid; i + 1 < n; i += threads) {
-            const Found &a = sh.best[i], &b = sh.best[i + 1];
-            if (a.row != b.row && a.score - b.score < kNear) {
-                if (state[a.row] == 0) state[a.row] = 1, sh.redo = 1;
-                if (state[b.row] == 0) state[b.row] = 1, sh.redo = 1;
-            }
-        }
-        __syncthreads();
+    // Two beams' candidates that lie too close to each other, one of them kept: their sums are formed again.
+    auto close = [&](int a, int b) {
+        if (a == b) return;
+        if (state[a] == 0) state[a] = 1, sh.redo = 1;
+        if (state[b] == 0) state[b] = 1, sh.redo = 1;
+    };
+    auto settle = [&] {  // (behind rank_found's barrier)
         if (!sh.redo) return false;
         for (int b = 0; b < beams; ++b) {
             if (state[b] != 1) continue;
@@ -456,8 +454,8 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
         others([&](double v, unsigned at, int row) {
             if (v >= least) push(sh, v, at, row);
         });
-        n = rank_found(sh, k, all);
-        again = settle(n, all);
+        n = rank_found(sh, k, all, close);
+        again = settle();
     } while (again);
     // the candidates of the k best tiles that reach the last one's largest
     const int open = min(n, k);
@@ -502,8 +500,8 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restric
                 if (v >= least) push(sh, v, at, row);
             });
         }
-        n = rank_found(sh, k, each_token);
-        if (!settle(n, each_token)) break;
+        n = rank_found(sh, k, each_token, close);
+        if (!settle()) break;
     }
     const int have = min(n, k);
     out_scores += size_t(group) * k;
