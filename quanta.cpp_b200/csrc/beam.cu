@@ -342,8 +342,9 @@ __device__ __forceinline__ int rank_found(MergeShared& sh, int k, Each&& each, C
 }
 
 // A CTA per group; bound by the latency of its ten or so steps, one behind the other: 5.8 us for one group of 4 rows of 151936 bf16
-// logits, 6.5 us for 64 (close candidates looked for in steps of their own: 6.4 and 7.2; the k best tiles' ranking is a step of its own: opening every tile above a threshold instead took as long
-// on ordinary groups and 377 us where few beams live and their tiles lie together).
+// logits, 6.5 us for 64 (close candidates looked for in steps of their own: 6.4 and 7.2).  The k best tiles' ranking is a step of its
+// own: opening every tile above a threshold instead took as long on ordinary groups and 377 us where few beams live and their tiles
+// lie together.
 template <class T>
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const T* __restrict__ logits, long long stride, int vocab, int beams,
                                                               const float* __restrict__ scores, const uint8_t* __restrict__ ended,
