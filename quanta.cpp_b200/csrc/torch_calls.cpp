@@ -1,7 +1,8 @@
 // The operators on torch tensors as a CPython extension: argument checks, output tensors and the call of the C ABI
 // (include/quanta_b200.h) in a microsecond or two of host time, which is what a call on a few rows costs next to its launch
 // (through ctypes and torch's Python calls 8 to 12 us).  quanta_b200.py has the functions' documentation.  Every function works on
-// torch's current stream and returns its result, or a negative QNT_ERR_* as an int; wrong types raise TypeError.
+// torch's current stream and returns its result, or a negative QNT_ERR_* as an int; wrong types raise TypeError, more tokens than an
+// int counts ValueError.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
@@ -13,10 +14,11 @@
 
 namespace {
 
-struct TypeError {
+struct Refused {
+    PyObject* type;
     const char* message;
 };
-[[noreturn]] void refuse(const char* message) { throw TypeError{message}; }
+[[noreturn]] void refuse(const char* message) { throw Refused{PyExc_TypeError, message}; }
 
 const at::Tensor* tensor_or_null(PyObject* o) { return o != Py_None && THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
@@ -46,8 +48,8 @@ template <class F>
 PyObject* guarded(F&& f) {
     try {
         return f();
-    } catch (const TypeError& e) {
-        PyErr_SetString(PyExc_TypeError, e.message);
+    } catch (const Refused& e) {
+        PyErr_SetString(e.type, e.message);
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {
@@ -71,7 +73,14 @@ bool to_long(PyObject* o, long long* v) {
     return !(*v == -1 && PyErr_Occurred());
 }
 
-int narrow(int64_t n) { return n > INT32_MAX ? INT32_MAX : n < INT32_MIN ? INT32_MIN : int(n); }  // (what does not fit is refused further down)
+// A size or a number as the C ABI takes it; what does not fit becomes one that the C ABI refuses.
+int narrow(int64_t n) { return n > INT32_MAX ? INT32_MAX : n < INT32_MIN ? INT32_MIN : int(n); }
+
+// A count of tokens: any that fits is as good as another.
+int token_count(int64_t n) {
+    if (n > INT32_MAX) throw Refused{PyExc_ValueError, "at most 2147483647 tokens in one call"};
+    return int(n);
+}
 
 // x, weight, eps, residual or None -> (q, d)
 PyObject* rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -81,7 +90,7 @@ PyObject* rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const at::Tensor *x = tensor_or_null(a[0]), *w = tensor_or_null(a[1]), *r = tensor_or_null(a[3]);
         if (!x || !x->is_cuda() || dtype_of(*x) < 0 || x->dim() != 2 || x->stride(1) != 1)
             refuse("x must be a float32, float16 or bfloat16 CUDA tensor [tokens, n] whose rows are contiguous");
-        const int64_t m = x->size(0), n = x->size(1);
+        const int64_t m = token_count(x->size(0)), n = x->size(1);
         if (!w || w->scalar_type() != at::kFloat || w->device() != x->device() || w->dim() != 1 || w->size(0) != n || !w->is_contiguous())
             refuse("weight must be a contiguous float32 CUDA tensor [n] on x's device");
         if (a[3] != Py_None && (!r || r->dim() != 2 || r->size(0) != m || r->size(1) != n || r->device() != x->device() || r->stride(1) != 1 ||
@@ -91,7 +100,7 @@ PyObject* rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         at::Tensor q = empty({m, n}, at::kChar, x->device()), d = empty({m, n / 32}, at::kFloat, x->device());
         const int rc = qnt_rms_norm_q8(x->const_data_ptr(), dtype_of(*x), x->stride(0), r ? r->mutable_data_ptr() : nullptr,
                                        r ? dtype_of(*r) : 0, r ? r->stride(0) : 0, static_cast<const float*>(w->const_data_ptr()), float(eps),
-                                       narrow(m), narrow(n), static_cast<int8_t*>(q.mutable_data_ptr()), static_cast<float*>(d.mutable_data_ptr()),
+                                       int(m), narrow(n), static_cast<int8_t*>(q.mutable_data_ptr()), static_cast<float*>(d.mutable_data_ptr()),
                                        c10::cuda::getCurrentCUDAStream().stream());
         return rc ? PyLong_FromLong(rc) : pair(wrap(std::move(q)), wrap(std::move(d)));
     });
@@ -107,10 +116,11 @@ PyObject* dequantize_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             d->scalar_type() != at::kFloat || d->device() != q->device() || !d->is_contiguous() || d->dim() != 2 || q->size(1) % 32 ||
             d->size(0) != q->size(0) || d->size(1) != q->size(1) / 32)
             refuse("q must be a contiguous int8 CUDA tensor [tokens, n], d a contiguous float32 one [tokens, n / 32] on its device");
+        const int n_tok = token_count(q->size(0));
         const c10::cuda::CUDAGuard on(q->device());
         at::Tensor out = empty(q->sizes(), dtype == QNT_F32 ? at::kFloat : dtype == QNT_F16 ? at::kHalf : at::kBFloat16, q->device());
         const int rc = qnt_dequantize_q8(static_cast<const int8_t*>(q->const_data_ptr()), static_cast<const float*>(d->const_data_ptr()),
-                                         narrow(q->size(0)), narrow(q->size(1)), out.mutable_data_ptr(), int(dtype),
+                                         n_tok, narrow(q->size(1)), out.mutable_data_ptr(), int(dtype),
                                          c10::cuda::getCurrentCUDAStream().stream());
         return rc ? PyLong_FromLong(rc) : wrap(std::move(out));
     });
@@ -134,6 +144,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (!fits(q) || dtype_of(*q) < 0 || (a[1] != Py_None && (!fits(k) || k->scalar_type() != q->scalar_type() || k->size(2) != q->size(2))))
             refuse("q and k must be CUDA tensors [tokens, heads, head_dim] of one type, float32, float16 or bfloat16, on the table's device, "
                    "whose heads are contiguous within a token");
+        const int n_tok = token_count(p->size(0));
         const c10::cuda::CUDAGuard on(q->device());
         at::Tensor q_out = inplace ? *q : empty(q->sizes(), q->scalar_type(), q->device()), k_out;
         if (k) k_out = inplace ? *k : empty(k->sizes(), k->scalar_type(), k->device());
@@ -142,7 +153,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                                 k ? k->const_data_ptr() : nullptr, k ? k->stride(0) : 0, k ? k_out.mutable_data_ptr() : nullptr,
                                 k ? k_out.stride(0) : 0, k ? narrow(k->size(1)) : 0, dtype_of(*q), narrow(q->size(2)), narrow(rotary_dim),
                                 int(interleaved), static_cast<const double*>(t->const_data_ptr()), float(scale),
-                                static_cast<const int*>(p->const_data_ptr()), narrow(p->size(0)), c10::cuda::getCurrentCUDAStream().stream());
+                                static_cast<const int*>(p->const_data_ptr()), n_tok, c10::cuda::getCurrentCUDAStream().stream());
         if (rc) return PyLong_FromLong(rc);
         if (!k) Py_INCREF(Py_None);
         return pair(wrap(std::move(q_out)), k ? wrap(std::move(k_out)) : Py_None);
