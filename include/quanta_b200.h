@@ -88,8 +88,9 @@ int qnt_matmul_host(const qnt_dtensor* W, const int8_t* qx, const float* dx, int
  *   per 32 values: d = max |y| / 127,  q = y / d to the nearest integer, halves away from zero.
  * x [n_tok][n] at x_stride, of dtype QNT_F32, QNT_F16 or QNT_BF16; residual [n_tok][n] at residual_stride, of x's dtype or
  * QNT_F32, which does not overlap x; weight f32 [n]; q [n_tok][n] and d [n_tok][n / 32], 16-byte aligned; n a multiple of 32, at most 32768.
- * Sums are in f32 (h below 10^18).  A value that is not finite makes its block read as NaN (its row, where h is not); a block whose
- * d is below 2^-126 reads as zeros. */
+ * Sums are in f32.  A row reads as NaN where a value of h, or its sum of squares, is not finite (the sum is, for a root mean square
+ * below 1.8e19 / sqrt(n), which is 10^17 or more), a block where a weight is not; a block whose d is below 2^-126 reads as zeros.
+ * Squares below 2^-126 lose bits: with eps = 0 the root mean square should be 10^-18 or more. */
 int qnt_rms_norm_q8(const void* x, int dtype, long long x_stride, void* residual, int residual_dtype, long long residual_stride,
                     const float* weight, float eps, int n_tok, int n, int8_t* q, float* d, void* stream);
 

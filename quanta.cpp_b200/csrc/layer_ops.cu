@@ -16,10 +16,10 @@ bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>
 //     y = h * (1 / sqrt(mean h^2 + eps)) * w;  per 32 values: d = max |y| / 127, q = y / d to the nearest, halves away from 0
 // A row stays in registers between the sum and the rounding: every byte crosses HBM once.  A thread holds R chunks of 8 consecutive
 // values, so that a block of 32 is 4 neighbouring lanes and its maximum two shuffles.  Sums in f32: per thread, then per warp, then
-// over warps (an error of a few 2^-24).  A block with a value that is not finite gets a NaN for its scale.  Next to HBM, and without a
-// residual more than HBM (8192 rows of 4096 bf16: 23.7 us, 16.4 of them for the bytes), instructions bound it.  So values go in pairs
-// (f32x2), and a code is the low byte of y * u + 1.5 * 2^23, one operation whose rounding is that to the nearest integer; u is 1 / d
-// one step up, so that halves go away from 0.
+// over warps (an error of a few 2^-24).  A block with a value that is not finite gets a NaN for its scale, every block of a row whose
+// sum is not finite does.  Next to HBM, and without a residual more than HBM (8192 rows of 4096 bf16: 23.7 us, 16.4 of them for the
+// bytes), instructions bound it.  So values go in pairs (f32x2), and a code is the low byte of y * u + 1.5 * 2^23, one operation whose
+// rounding is that to the nearest integer; u is 1 / d one step up, so that halves go away from 0.
 __device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
     unsigned long long r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
             for (int o = W / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        const float inv = __frsqrt_rn(sum / float(n) + eps);
+        // (an infinite sum is an infinite value's or an overflow: NaN, where 1 / sqrt would make the row's other blocks zeros)
+        const float inv = sum <= 3.402823466e38f ? __frsqrt_rn(sum / float(n) + eps) : __int_as_float(0x7fc00000);
         const unsigned long long inv2 = f2_pack(inv, inv), magic = f2_pack(12582912.f, 12582912.f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
