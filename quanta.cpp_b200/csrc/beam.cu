@@ -208,14 +208,17 @@ __device__ __forceinline__ double least_of(unsigned key) {
 }
 
 // Twice the error of a log sum: of a term 2^-22 (the exponential), ln 2 2^-20 (y above -32), 21 * 1.4e-8 (log2 e as f32); 12 roundings
-// of a tile's sum; 2^-22 of its weight and 8 roundings in the row's.  In all below 2.7e-6.
+// of a tile's sum; 2^-22 of its weight, at its exact distance from the row's largest, and 8 roundings in the row's.  In all below 2.7e-6.
 constexpr double kNear = 6e-6;
 
-// e^t for t <= 0 as f32: the rounding of t log2 e made good.
-__device__ __forceinline__ float exp_neg(float t) {
-    t = fmaxf(t, -150.f);
-    const float y = fmul(t, kLog2e), e = ex2(y);
-    return fmaf(fmul(e, fmaf(t, kLog2e, -y)), 0.6931471805599453f, e);
+// e^(x - top) for x <= top as f32: what the difference loses (up to 2^-20 where it counts, all of it in one direction in a row whose
+// tiles are alike) and the rounding of its product with log2 e are made good.
+__device__ __forceinline__ float exp_below(float x, float top) {
+    const float d = fsub(x, top), back = fsub(d, x);
+    const float lost = fsub(fsub(x, fsub(d, back)), fadd(top, back));  // x - top = d + lost
+    const float t = fmaxf(d, -150.f), y = fmul(t, kLog2e), e = ex2(y);
+    const float more = fmaf(t, kLog2e, -y) + (d > -150.f ? fmul(lost, kLog2e) : 0.f);
+    return fmaf(fmul(e, more), 0.6931471805599453f, e);
 }
 
 // log of the sum of exponentials of a row, by a warp, from its tiles; NaN where the row has no candidates.
@@ -233,11 +236,11 @@ __device__ __forceinline__ double join_sums(const Tile* tiles, int n) {
     top = unorder(__reduce_max_sync(0xffffffffu, order(top)));
     float part = 0.f;  // (a tile of forbidden tokens has the sum 0)
 #pragma unroll
-    for (int u = 0; u < N; ++u) part = fmaf(t[u].y, exp_neg(t[u].x - top), part);
+    for (int u = 0; u < N; ++u) part = fmaf(t[u].y, exp_below(t[u].x, top), part);
     double sum = double(part);
     for (int i = lane + 32 * N; i < n; i += 32) {
         const float2 v = __ldcg(in + i);
-        sum += double(v.y) * double(exp_neg(v.x - top));
+        sum += double(v.y) * double(exp_below(v.x, top));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
