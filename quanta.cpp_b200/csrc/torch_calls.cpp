@@ -2,12 +2,13 @@
 // (include/quanta_b200.h) in a microsecond or two of host time, which is what a call on a few rows costs next to its launch
 // (through ctypes and torch's Python calls 8 to 12 us).  quanta_b200.py has the functions' documentation.  Every function works on
 // torch's current stream and returns its result, or a negative QNT_ERR_* as an int; wrong types raise TypeError, more tokens than an
-// int counts ValueError.
+// int counts ValueError, tensors that would be written in place although a gradient is recorded through them RuntimeError.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "quanta_b200.h"
@@ -33,6 +34,16 @@ int dtype_of(const at::Tensor& t) {  // -1: none of ours
 
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, at::Device device) {
     return at::Tensor(at::detail::empty_cuda(size, type, device, std::nullopt));
+}
+
+// A tensor that a call writes in place.  The operators have no gradients, so none may be recorded through it; and what autograd has
+// saved of it learns that it is stale (written()).
+void will_write(const at::Tensor& t) {
+    if ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())
+        throw Refused{PyExc_RuntimeError, "a tensor that requires a gradient cannot be written in place (no gradient is recorded)"};
+}
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }
@@ -96,13 +107,16 @@ PyObject* rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (a[3] != Py_None && (!r || r->dim() != 2 || r->size(0) != m || r->size(1) != n || r->device() != x->device() || r->stride(1) != 1 ||
                                 (r->scalar_type() != x->scalar_type() && r->scalar_type() != at::kFloat)))
             refuse("residual must be a CUDA tensor of x's shape, on its device, of its type or float32, whose rows are contiguous");
+        if (r) will_write(*r);
         const c10::cuda::CUDAGuard on(x->device());
         at::Tensor q = empty({m, n}, at::kChar, x->device()), d = empty({m, n / 32}, at::kFloat, x->device());
         const int rc = qnt_rms_norm_q8(x->const_data_ptr(), dtype_of(*x), x->stride(0), r ? r->mutable_data_ptr() : nullptr,
                                        r ? dtype_of(*r) : 0, r ? r->stride(0) : 0, static_cast<const float*>(w->const_data_ptr()), float(eps),
                                        int(m), narrow(n), static_cast<int8_t*>(q.mutable_data_ptr()), static_cast<float*>(d.mutable_data_ptr()),
                                        c10::cuda::getCurrentCUDAStream().stream());
-        return rc ? PyLong_FromLong(rc) : pair(wrap(std::move(q)), wrap(std::move(d)));
+        if (rc) return PyLong_FromLong(rc);
+        if (r) written(*r);
+        return pair(wrap(std::move(q)), wrap(std::move(d)));
     });
 }
 
@@ -145,6 +159,10 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             refuse("q and k must be CUDA tensors [tokens, heads, head_dim] of one type, float32, float16 or bfloat16, on the table's device, "
                    "whose heads are contiguous within a token");
         const int n_tok = token_count(p->size(0));
+        if (inplace) {
+            will_write(*q);
+            if (k) will_write(*k);
+        }
         const c10::cuda::CUDAGuard on(q->device());
         at::Tensor q_out = inplace ? *q : empty(q->sizes(), q->scalar_type(), q->device()), k_out;
         if (k) k_out = inplace ? *k : empty(k->sizes(), k->scalar_type(), k->device());
@@ -155,6 +173,10 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                                 int(interleaved), static_cast<const double*>(t->const_data_ptr()), float(scale),
                                 static_cast<const int*>(p->const_data_ptr()), n_tok, c10::cuda::getCurrentCUDAStream().stream());
         if (rc) return PyLong_FromLong(rc);
+        if (inplace) {
+            written(*q);
+            if (k) written(*k);
+        }
         if (!k) Py_INCREF(Py_None);
         return pair(wrap(std::move(q_out)), k ? wrap(std::move(k_out)) : Py_None);
     });

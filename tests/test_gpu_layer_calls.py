@@ -1,4 +1,5 @@
-"""Calls of the operators on torch tensors that are refused: counts past 32 bits."""
+"""Calls of the operators on torch tensors that are refused, or that others have to notice: counts past 32 bits, tensors
+that the call writes in place."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -20,3 +21,49 @@ def test_more_tokens_than_a_call_takes(qb):
     del pos
     with pytest.raises(ValueError, match="2147483647"):
         qb.rms_norm_q8(torch.ones(32, device="cuda").expand(MANY, 32), torch.ones(32, device="cuda"))
+
+
+class InPlace:
+    """The calls that write one of their arguments: (call, tensors that it writes)."""
+
+    def __init__(self, qb):
+        self.x, self.w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+        self.pos, rope = torch.arange(4, device="cuda", dtype=torch.int32), qb.Rope(16)
+        self.calls = {"residual": lambda t: qb.rms_norm_q8(self.x, self.w, residual=t),
+                      "q": lambda t: rope(t.view(4, 4, 16), None, self.pos, inplace=True),
+                      "k": lambda t: rope(self.x.view(4, 4, 16).clone(), t.view(4, 4, 16), self.pos, inplace=True)}
+
+
+@pytest.mark.parametrize("which", ["residual", "q", "k"])
+def test_writes_in_place_are_seen_by_autograd(qb, which):
+    call = InPlace(qb).calls[which]
+    leaf = torch.randn(4, 64, device="cuda", requires_grad=True)
+    kept = leaf.detach().clone()
+    with pytest.raises(RuntimeError, match="gradient"):
+        call(leaf)
+    with pytest.raises(RuntimeError, match="gradient"):
+        call(leaf * 1.0)
+    assert torch.equal(leaf, kept)
+    # where no gradients are recorded the call goes through, and what was saved before it is known to be stale
+    y = (leaf * 1.0).exp()
+    before = y._version
+    with torch.no_grad():
+        call(y)
+    assert y._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    plain = torch.randn(4, 64, device="cuda")
+    before = plain._version
+    call(plain)
+    assert plain._version > before
+    with torch.inference_mode():
+        call(torch.randn(4, 64, device="cuda"))
+
+
+def test_tangents_of_what_is_written_are_not_lost(qb):
+    calls, fw = InPlace(qb).calls, torch.autograd.forward_ad
+    with fw.dual_level():
+        t = fw.make_dual(torch.randn(4, 64, device="cuda"), torch.ones(4, 64, device="cuda"))
+        for call in calls.values():
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(t)
