@@ -101,9 +101,9 @@ int qnt_dequantize_q8(const int8_t* q, const float* d, int n_tok, int n, void* o
 /* Rotary positions of query and key heads (either may be NULL with 0 heads): pair i of a head's first rotary_dim dims, (i, i +
  * rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), turns by positions[t] * turns[i] revolutions and is multiplied by `scale`; the
  * dims behind are copied.  Token t, head h, dim i at t * stride + h * head_dim + i (elements) of dtype QNT_F32, QNT_F16 or QNT_BF16; an
- * output may be its input (with one stride), and must not overlap it otherwise.  turns: f64 [rotary_dim / 2] = frequency / (2 pi),
- * with whatever scaling for long contexts; the revolution count is formed in f64, so that far positions keep their angles.
- * positions int32 [n_tok], of any sign.  head_dim even, at most 1024. */
+ * output may be its input (with one stride), and must not overlap it otherwise, nor the other output or input.  turns: f64
+ * [rotary_dim / 2] = frequency / (2 pi), with whatever scaling for long contexts; the revolution count is formed in f64, so that far
+ * positions keep their angles.  positions int32 [n_tok], of any sign.  head_dim even, at most 1024. */
 int qnt_rope(const void* q, long long q_stride, void* q_out, long long q_out_stride, int n_heads, const void* k, long long k_stride,
              void* k_out, long long k_out_stride, int n_kv_heads, int dtype, int head_dim, int rotary_dim, int interleaved,
              const double* turns, float scale, const int* positions, int n_tok, void* stream);

@@ -28,6 +28,26 @@ int make_type(int dtype, qb::KvType* t) {
 
 uintptr_t size_of(qb::KvType t) { return t == qb::KV_F32 ? 4 : 2; }
 
+// n rows of `row` bytes, `stride` bytes from each other.
+using Wide = __int128;  // (strides are the caller's)
+struct Rows {
+    const void* at;
+    Wide stride, row;
+};
+
+// Whether rows of a and of b share a byte.  Where the strides differ and there are several rows, only the first ones are compared.
+bool overlap(const Rows& a, const Rows& b, int n) {
+    const Wide d = Wide(reinterpret_cast<uintptr_t>(b.at)) - Wide(reinterpret_cast<uintptr_t>(a.at));
+    if (d < a.row && d > -b.row) return true;
+    if (n <= 1 || a.stride != b.stride) return false;
+    if (d >= (n - 1) * a.stride + a.row || -d >= (n - 1) * b.stride + b.row) return false;
+    // row j of b lies d + (j - i) stride behind row i of a: the largest such distance below a.row, with |j - i| < n
+    const Wide room = a.row - 1 - d;
+    Wide k = room / a.stride - (room < 0 && room % a.stride ? 1 : 0);
+    if (k > n - 1) k = n - 1;
+    return k > -Wide(n) && d + k * a.stride > -b.row;
+}
+
 int done(cudaError_t e, const char* what) { return e == cudaSuccess ? QNT_OK : cuda_err(e, what); }
 
 cudaStream_t stream_of(void* s) { return static_cast<cudaStream_t>(s); }
@@ -81,6 +101,9 @@ int qnt_rms_norm_q8(const void* x, int dtype, long long x_stride, void* residual
             return set_err(QNT_ERR_INVALID, "rms norm: the residual must be aligned to its elements");
         if (n_tok > 1 && residual_stride < n) return set_err(QNT_ERR_INVALID, "rms norm: residual_stride is smaller than a row");
         if (residual == x) return set_err(QNT_ERR_INVALID, "rms norm: the residual must not be x");
+        const Wide xb = size_of(a.type), rb = a.residual_f32 ? 4 : xb;
+        if (overlap({x, x_stride * xb, n * xb}, {residual, residual_stride * rb, n * rb}, n_tok))
+            return set_err(QNT_ERR_INVALID, "rms norm: the residual must not overlap x");
     }
     a.x = x;
     a.x_stride = x_stride;
@@ -120,6 +143,14 @@ int qnt_rope(const void* q, long long q_stride, void* q_out, long long q_out_str
     if (n_tok > 0) {
         if (int r = check_heads("q", a.q, head_dim, n_tok, size_of(a.type))) return r;
         if (int r = check_heads("k", a.k, head_dim, n_tok, size_of(a.type))) return r;
+        const Wide b = size_of(a.type);
+        const auto in = [&](const qb::RopeHeads& h) { return Rows{h.in, h.in_stride * b, h.heads * head_dim * b}; };
+        const auto out = [&](const qb::RopeHeads& h) { return Rows{h.out, h.out_stride * b, h.heads * head_dim * b}; };
+        const bool both = a.q.heads && a.k.heads;
+        if ((both && (overlap(out(a.q), out(a.k), n_tok) || overlap(out(a.q), in(a.k), n_tok) || overlap(in(a.q), out(a.k), n_tok))) ||
+            (a.q.heads && a.q.in != a.q.out && overlap(in(a.q), out(a.q), n_tok)) ||
+            (a.k.heads && a.k.in != a.k.out && overlap(in(a.k), out(a.k), n_tok)))
+            return set_err(QNT_ERR_INVALID, "rope: an output must not overlap the other or an input that it is not");
     }
     if (n_tok == 0 || a.q.heads + a.k.heads == 0) return QNT_OK;
     if (!turns || !positions || !aligned(turns, 8) || !aligned(positions, 4))

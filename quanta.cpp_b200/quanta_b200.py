@@ -563,9 +563,9 @@ def _on_stream(stream, device):
 def rms_norm_q8(x, weight, eps: float = 1e-6, residual=None, stream=None):
     """RMS norm of rows x [tokens, n] (float32, float16 or bfloat16 CUDA tensor; rows may lie in wider ones) with 8-bit rows out:
     (q int8 [tokens, n], d float32 [tokens, n / 32]), the operand of the quantized products.  weight float32 [n].  With residual
-    [tokens, n] (x's type or float32), residual += x first, in place, and the sum (before its rounding) is normed.
-    There are no gradients: results are outside autograd's graph, as within torch.no_grad(), and a tensor that a call writes in place
-    is refused while a gradient is recorded through it.
+    [tokens, n] (x's type or float32; the two must not overlap), residual += x first, in place, and the sum (before its rounding) is
+    normed.  There are no gradients: results are outside autograd's graph, as within torch.no_grad(), and a tensor that a call writes
+    in place is refused while a gradient is recorded through it.
     Work is queued on `stream` (a torch stream or a cudaStream_t's number; default: torch's current stream); with another one than
     the current one the call is as if made within torch.cuda.stream(stream).  So for the functions and objects below."""
     if stream is not None:
@@ -657,7 +657,7 @@ class Rope:
     def __call__(self, q, k, positions, inplace: bool = False, stream=None):
         """q [tokens, heads, head_dim] and k [tokens, kv heads, head_dim] (or None) of one type, float32, float16 or bfloat16; heads
         contiguous within a token, so that they may lie in the rows of one projection's output; positions int32 [tokens].
-        Returns rotated (q, k), new contiguous tensors, or with inplace=True the ones given."""
+        Returns rotated (q, k), new contiguous tensors, or with inplace=True the ones given, which must not overlap."""
         if stream is not None:
             with _on_stream(stream, q.device):
                 return self(q, k, positions, inplace)

@@ -67,3 +67,24 @@ def test_tangents_of_what_is_written_are_not_lost(qb):
         for call in calls.values():
             with pytest.raises(RuntimeError, match="gradient"):
                 call(t)
+
+
+@pytest.mark.parametrize("side", [0, 64])
+def test_operands_side_by_side_in_one_buffer(qb, side):
+    """Rows of x beside those of the residual, heads rotated in place beside each other: not the overlap that is refused."""
+    buf = torch.randn(50, 128, device="cuda")
+    x, r = buf[:, side: side + 64], buf[:, 64 - side: 128 - side]
+    want = x + r
+    qb.rms_norm_q8(x, torch.ones(64, device="cuda"), residual=r)
+    assert torch.equal(r, want)
+    rope, pos = qb.Rope(16), torch.arange(50, device="cuda", dtype=torch.int32)
+    q, k = x.unflatten(1, (4, 16)), r.unflatten(1, (4, 16))
+    want = rope(q, k, pos)
+    got = rope(q, k, pos, inplace=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[0].data_ptr() == x.data_ptr()
+    with pytest.raises(qb.QntError, match="overlap"):
+        rope(q, q, pos, inplace=True)
+    with pytest.raises(qb.QntError, match="overlap"):
+        rope(q[:49], q[1:], pos[:49], inplace=True)
+    with pytest.raises(qb.QntError, match="overlap"):
+        qb.rms_norm_q8(buf[:-1, :64], torch.ones(64, device="cuda"), residual=buf[1:, :64])
