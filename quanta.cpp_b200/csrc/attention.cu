@@ -630,7 +630,7 @@ cudaError_t launch_attn(const AttnArgs& a, const float* Q, const int* pos_dev, i
     auto kern = cs == 8 ? k_attn<8, 0, 0> : cs == 4 ? k_attn<4, 0, 0> : cs == 2 ? k_attn<2, 0, 0> : k_attn<1, 0, 0>;
     const size_t smem = attn_smem_bytes(ctx, cs);
     if (smem > 227 * 1024) return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaError_t e = allow_smem(kern, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(cs * a.n_heads), unsigned(n_tok));
@@ -679,7 +679,7 @@ cudaError_t launch_qkv_attn(const QkvArgs& qa, const AttnArgs& a, const float* X
     auto kern = uo == 0 ? (u6 ? k_attn<kMaxCluster, 6, 0> : k_attn<kMaxCluster, 12, 0>)
               : uo == 2 ? (u6 ? k_attn<kMaxCluster, 6, 2> : k_attn<kMaxCluster, 12, 2>)
                         : (u6 ? k_attn<kMaxCluster, 6, 4> : k_attn<kMaxCluster, 12, 4>);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaError_t e = allow_smem(kern, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(kMaxCluster * a.n_heads), 1u);

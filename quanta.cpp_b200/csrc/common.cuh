@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace qb {
 
 constexpr int QK = 32;  // quantization block (engine/src/model_file.h:17)
@@ -131,6 +133,29 @@ __device__ __forceinline__ int8_t quantize_lane(float x, float* d_out) {
     return (int8_t)round_away(fmul(x, inv));  // |x * inv| <= 127 (plus rounding)
 }
 
+// Allows launches of `kernel` on the current device `smem` bytes of dynamic shared memory.  The limit is the kernel's on the device,
+// not the launch's: another host thread may have set it and not launched yet, so that it is never lowered.
+inline cudaError_t allow_smem_of(const void* kernel, size_t smem) {
+    struct Most {
+        const void* kernel;
+        size_t smem;
+    };
+    static std::mutex lock;
+    static Most asked[512];  // the most asked for so far, on any device; many times the kernels that there are
+    std::lock_guard<std::mutex> hold(lock);
+    size_t i = reinterpret_cast<uintptr_t>(kernel) / 16 % 512;
+    for (size_t tries = 0; tries < 512 && asked[i].kernel && asked[i].kernel != kernel; ++tries) i = (i + 1) % 512;
+    if (asked[i].kernel && asked[i].kernel != kernel) return cudaErrorInvalidValue;
+    const size_t want = smem > asked[i].smem ? smem : asked[i].smem;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(want));
+    if (e == cudaSuccess) asked[i] = Most{kernel, want};
+    return e;
+}
+template <class... KArgs>
+inline cudaError_t allow_smem(void (*kernel)(KArgs...), size_t smem) {
+    return allow_smem_of(reinterpret_cast<const void*>(kernel), smem);
+}
+
 // Launches `kernel`, optionally as a programmatic dependent of the previous launch on the stream (the kernel then
 // calls griddepcontrol.launch_dependents / .wait); raises the dynamic shared memory limit when it needs more than 48 KB.
 template <class... KArgs, class... Args>
@@ -147,7 +172,7 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
     if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        cudaError_t e = allow_smem(kernel, smem);
         if (e != cudaSuccess) return e;
     }
     return cudaLaunchKernelEx(&cfg, kernel, args...);

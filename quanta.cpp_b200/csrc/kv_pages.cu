@@ -940,7 +940,7 @@ __global__ void __launch_bounds__(256) k_kv_copy(KvView c, const int* __restrict
 template <class... KArgs, class... Args>
 cudaError_t launch_plan(void (*kernel)(KArgs...), int ctas, int threads, size_t smem, cudaStream_t st, Args... args) {
     if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        const cudaError_t e = allow_smem(kernel, smem);
         if (e != cudaSuccess) return e;
     }
     return launch_pdl(kernel, dim3(unsigned(ctas)), dim3(unsigned(threads)), smem, st, false, args...);
@@ -1031,7 +1031,7 @@ cudaError_t launch_kv_reorder(const KvView& c, const int* seqs, const int* paren
     const bool with_len = all <= 200 * 1024, many = n > 32;
     auto kern = with_len ? k_kv_reorder_plan<true> : k_kv_reorder_plan<false>;
     const size_t smem = with_len ? all : less;
-    cudaError_t e = smem > 32 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) : cudaSuccess;
+    cudaError_t e = smem > 32 * 1024 ? allow_smem(kern, smem) : cudaSuccess;
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(many ? kReorderCtas : 1);

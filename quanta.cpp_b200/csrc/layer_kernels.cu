@@ -491,7 +491,7 @@ cudaError_t launch_gateup_dec(const DMat& W, const SlicePlan& p, const float* X,
         cfg.attrs = attr;
         cfg.numAttrs = pdl ? 2 : 1;
         auto go = [&](auto kern) {
-            cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+            cudaError_t r = allow_smem(kern, smem);
             if (r != cudaSuccess) return r;
             return cudaLaunchKernelEx(&cfg, kern, W, X, norm_w, eps, HQ, HD, bpc, p.magic, tab, T, nbo, X2, xo, Hf);
         };

@@ -86,11 +86,11 @@ cudaError_t launch_matvec(const DMat& W, const int8_t* qx, const float* dx, int 
     const unsigned magic = div_magic(unsigned(row_bytes_host(W.dtype, W.cols) / 16));
     if (W.dtype == DT_Q8_0) {
         auto k = k_matvec<DT_Q8_0, kMatvecU>;
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sm));
+        allow_smem(k, sm);
         k<<<grid, kThreads, sm, st>>>(W, qx, dx, r0, r1, rpc, magic, out);
     } else if (W.dtype == DT_Q4_0) {
         auto k = k_matvec<DT_Q4_0, kMatvecU>;
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sm));
+        allow_smem(k, sm);
         k<<<grid, kThreads, sm, st>>>(W, qx, dx, r0, r1, rpc, magic, out);
     } else {
         return cudaErrorInvalidValue;

@@ -1,6 +1,10 @@
 """Calls of the operators on torch tensors that are refused, or that others have to notice: counts past 32 bits, tensors
-that the call writes in place."""
+that the call writes in place, calls from several threads."""
+import threading
+
 import pytest
+
+from test_gpu_kv_cache import ints
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -88,3 +92,35 @@ def test_operands_side_by_side_in_one_buffer(qb, side):
         rope(q[:49], q[1:], pos[:49], inplace=True)
     with pytest.raises(qb.QntError, match="overlap"):
         qb.rms_norm_q8(buf[:-1, :64], torch.ones(64, device="cuda"), residual=buf[1:, :64])
+
+
+def test_reordering_and_reserving_from_threads(qb):
+    """Caches whose plans need different amounts of shared memory, each on a thread of its own (the C calls leave Python's lock)."""
+    wrong = []
+
+    def work(pages, calls):
+        try:
+            torch.cuda.set_device(0)
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                c = qb.PagedKV.empty(1, 1, 64, pages, 4, 4, 16)
+                seqs, parents, none = ints([0, 1]), ints([0, 1]), ints([0, 0])
+                ws = torch.empty(qb.lib().qnt_kv_reorder_workspace(c._p) + c._page_ws, dtype=torch.uint8, device="cuda")
+                for _ in range(calls):
+                    for rc in (qb.lib().qnt_kv_reorder(c._p, seqs.data_ptr(), parents.data_ptr(), 2, 2, ws.data_ptr(), ws.numel(),
+                                                       stream.cuda_stream),
+                               qb.lib().qnt_kv_reserve(c._p, seqs.data_ptr(), none.data_ptr(), 2, ws.data_ptr(), ws.numel(),
+                                                       stream.cuda_stream)):
+                        if rc:
+                            wrong.append((pages, rc, qb.lib().qnt_last_error()))
+                            return
+                c.check()
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(p, 6000)) for p in (280_000, 1_000_000, 400_000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
