@@ -5,15 +5,18 @@
 
 Outputs (git-ignored, shipped with the repository snapshot):
     quanta.cpp_b200/lib/libquanta_b200.so   CUDA kernels + engine + the C ABI of include/quanta_b200.h
-    quanta.cpp_b200/lib/quanta_b200_torch.so  the operators on torch tensors (csrc/torch_calls.cpp; needs torch's headers)
+    quanta.cpp_b200/lib/quanta_b200_torch.so  the operators on torch tensors (csrc/torch_calls.cpp; only where torch has CUDA)
     quanta.cpp_b200/lib/libqnt_synth.so     seeded random-init .qnt writer
     quanta.cpp_b200/lib/quanta_b200         command-line driver (selftest / gen / bench / checkbatch / checkhead / run)
 Objects go to quanta.cpp_b200/_build/.  Rebuilds only what changed (source or header mtimes).
 """
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -80,36 +83,51 @@ def build(verbose: bool = False, jobs: int = 0, stamps: bool = False) -> None:
     so = lib_dir / "libquanta_b200.so"
     if _newer(so, objs):
         _run([NVCC] + ARCH + ["-shared", "-o", str(so)] + [str(o) for o in objs] + ["-lpthread"])
-    if stamps:
-        return
-    synth = LIB / "libqnt_synth.so"
-    ssrc = CSRC / "synth" / "qnt_synth.cpp"
-    if _newer(synth, [ssrc, CSRC / "synth" / "qnt_synth.h"]):
-        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-march=x86-64-v3", "-o", str(synth), str(ssrc), "-pthread"])
-    build_torch_calls(so)
-    cli_src = CSRC / "cli" / "main.cpp"
-    cli = LIB / "quanta_b200"
-    if cli_src.exists() and _newer(cli, [cli_src, so] + hdrs):
-        _run(["g++", "-O2", "-std=c++17", f"-I{ROOT / 'include'}", "-o", str(cli), str(cli_src), f"-L{LIB}", "-lquanta_b200",
-              f"-Wl,-rpath,$ORIGIN", "-pthread"])
+    if not stamps:
+        synth = LIB / "libqnt_synth.so"
+        ssrc = CSRC / "synth" / "qnt_synth.cpp"
+        if _newer(synth, [ssrc, CSRC / "synth" / "qnt_synth.h"]):
+            _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-march=x86-64-v3", "-o", str(synth), str(ssrc), "-pthread"])
+        cli_src = CSRC / "cli" / "main.cpp"
+        cli = LIB / "quanta_b200"
+        if cli_src.exists() and _newer(cli, [cli_src, so] + hdrs):
+            _run(["g++", "-O2", "-std=c++17", f"-I{ROOT / 'include'}", "-o", str(cli), str(cli_src), f"-L{LIB}", "-lquanta_b200",
+                  f"-Wl,-rpath,$ORIGIN", "-pthread"])
+        build_torch_calls(so)
+
+
+def torch_build():
+    """(folder, a text that tells its binary interface) of the installed torch if it is one with CUDA, else None."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.origin:
+        return None
+    folder = Path(spec.origin).resolve().parent
+    if not (folder / "lib" / "libtorch_cuda.so").exists():
+        return None
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        version = str((folder / "version.py").stat().st_mtime_ns)
+    return folder, f"torch {version} in {folder}, Python {sysconfig.get_config_var('SOABI')}"
 
 
 def build_torch_calls(so: Path) -> None:
-    """The CPython extension over the C ABI for torch tensors; without torch there is nothing that could call it."""
-    src, out = CSRC / "torch_calls.cpp", LIB / "quanta_b200_torch.so"
-    if not _newer(out, [src, ROOT / "include" / "quanta_b200.h"]):
+    """The CPython extension over the C ABI for torch tensors, beside libquanta_b200.so; built again for another torch.  Without a torch
+    that has CUDA there is nothing that could call it."""
+    src, out = CSRC / "torch_calls.cpp", so.parent / "quanta_b200_torch.so"
+    found, built_for = torch_build(), so.parent / "quanta_b200_torch.txt"
+    if found is None:
         return
-    try:
-        import torch
-    except ImportError:
+    t, interface = found
+    if not _newer(out, [src, ROOT / "include" / "quanta_b200.h"]) and built_for.exists() and built_for.read_text() == interface:
         return
-    import sysconfig
-    t = Path(torch.__file__).resolve().parent
+    import torch
     inc = [t / "include", t / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
            Path(NVCC).resolve().parent.parent / "include"]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
          [x for i in inc for x in ("-isystem", str(i))] + [f"-I{ROOT / 'include'}", str(src), "-o", str(out), f"-L{t / 'lib'}", "-ltorch_python",
           "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{so.parent}", "-lquanta_b200", "-Wl,-rpath,$ORIGIN"])
+    built_for.write_text(interface)
 
 
 if __name__ == "__main__":
