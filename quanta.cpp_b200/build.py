@@ -93,7 +93,7 @@ def build(verbose: bool = False, jobs: int = 0, stamps: bool = False) -> None:
         if cli_src.exists() and _newer(cli, [cli_src, so] + hdrs):
             _run(["g++", "-O2", "-std=c++17", f"-I{ROOT / 'include'}", "-o", str(cli), str(cli_src), f"-L{LIB}", "-lquanta_b200",
                   f"-Wl,-rpath,$ORIGIN", "-pthread"])
-        build_torch_calls(so)
+    build_torch_calls(so)
 
 
 def torch_build():

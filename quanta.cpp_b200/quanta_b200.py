@@ -534,7 +534,7 @@ _torch_module = None
 
 
 def _torch_calls():
-    """quanta_b200_torch.so: the operators on torch tensors (csrc/torch_calls.cpp)."""
+    """quanta_b200_torch.so: the operators on torch tensors (csrc/torch_calls.cpp), of the folder that libquanta_b200.so is taken from."""
     global _torch_module
     if _torch_module is None:
         import importlib.machinery
@@ -542,9 +542,9 @@ def _torch_calls():
 
         import torch  # noqa: F401  (its libraries come first)
         lib()
-        p = PKG / "lib" / "quanta_b200_torch.so"
+        p = LIB_DIR / "quanta_b200_torch.so"
         if not p.exists():
-            raise RuntimeError(f"{p} is missing: run `python quanta.cpp_b200/build.py` where torch is installed")
+            raise RuntimeError(f"{p} is missing: run `python quanta.cpp_b200/build.py` where a torch with CUDA is installed")
         loader = importlib.machinery.ExtensionFileLoader("quanta_b200_torch", str(p))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("quanta_b200_torch", loader))
         loader.exec_module(module)

@@ -69,3 +69,9 @@ def test_built_again_for_another_torch(build, monkeypatch, tmp_path):
         use(m, folder_of_torch(tmp_path, "2", with_cuda=True))
         build.build()
         assert build.made == ["quanta_b200_torch.so"]
+
+
+def test_the_phase_timed_library_has_one_of_its_own(build, tmp_path):
+    build.PKG = tmp_path
+    build.build(stamps=True)
+    assert "quanta_b200_torch.so" in build.made and (tmp_path / "lib_stamps" / "quanta_b200_torch.so").exists()
