@@ -149,7 +149,9 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         return nullptr;
     return guarded([&]() -> PyObject* {
         const at::Tensor *q = tensor_or_null(a[0]), *k = tensor_or_null(a[1]), *p = tensor_or_null(a[2]), *t = tensor_or_null(a[3]);
-        if (!p || !t || p->scalar_type() != at::kInt || p->device() != t->device() || p->dim() != 1 || !p->is_contiguous())
+        if (!t || !t->is_cuda() || t->scalar_type() != at::kDouble || !t->is_contiguous() || rotary_dim < 0 || t->numel() != rotary_dim / 2)
+            refuse("the table of turns must be a contiguous float64 CUDA tensor [rotary_dim / 2]");
+        if (!p || p->scalar_type() != at::kInt || p->device() != t->device() || p->dim() != 1 || !p->is_contiguous())
             refuse("positions must be a contiguous int32 CUDA tensor [tokens] on the table's device");
         const auto fits = [&](const at::Tensor* x) {
             return x && x->dim() == 3 && x->stride(2) == 1 && (x->stride(1) == x->size(2) || x->size(1) == 1) && x->size(0) == p->size(0) &&

@@ -94,6 +94,18 @@ def test_operands_side_by_side_in_one_buffer(qb, side):
         qb.rms_norm_q8(buf[:-1, :64], torch.ones(64, device="cuda"), residual=buf[1:, :64])
 
 
+def test_a_table_that_is_not_the_rotations(qb):
+    """A Rope whose table or size a caller has replaced: refused, nothing is read past its end."""
+    x, pos = torch.randn(3, 2, 128, device="cuda"), torch.arange(3, device="cuda", dtype=torch.int32)
+    for change in (dict(rotary_dim=128), dict(rotary_dim=66), dict(rotary_dim=32), dict(rotary_dim=-64), dict(turns=qb.Rope(64).turns.float()),
+                   dict(turns=qb.Rope(64).turns.cpu()), dict(turns=qb.Rope(128).turns[::2]), dict(turns=None)):
+        rope = qb.Rope(64)
+        for name, value in change.items():
+            setattr(rope, name, value)
+        with pytest.raises(TypeError, match="turns"):
+            rope(x, None, pos)
+
+
 def test_reordering_and_reserving_from_threads(qb):
     """Caches whose plans need different amounts of shared memory, each on a thread of its own (the C calls leave Python's lock)."""
     wrong = []
