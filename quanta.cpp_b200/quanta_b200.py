@@ -902,7 +902,11 @@ class Model:
     def beam_search(self, prompt, beams: int, n_gen: int, end_id: int = -1):
         """Beam search from the paged cache (batch_init_paged first; sequences 0 .. beams - 1 must be empty and are so afterwards):
         (ids, score) of every beam, best first; ids end with end_id where the beam did."""
-        t = np.ascontiguousarray(prompt, np.int32)
+        t = np.asarray(prompt)
+        for v in (beams, n_gen, end_id, *((t.min(), t.max()) if t.size else ())):
+            if not -(2 ** 31) <= v < 2 ** 31:  # (a C int would take its lower half)
+                raise ValueError(f"beam_search: {v} is past 32 bits")
+        t = np.ascontiguousarray(t, np.int32)
         ids, lens, scores = np.zeros((max(beams, 1), max(n_gen, 1)), np.int32), np.zeros(max(beams, 1), np.int32), np.zeros(max(beams, 1), np.float32)
         _check(lib().qnt_beam_search(self.h, _ptr(t), t.size, beams, n_gen, end_id, _ptr(ids), _ptr(lens), _ptr(scores)))
         return [(ids[i, : lens[i]].copy(), float(scores[i])) for i in range(beams)]
