@@ -11,6 +11,8 @@
 #include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <mutex>
+
 #include "quanta_b200.h"
 
 namespace {
@@ -84,6 +86,19 @@ bool to_long(PyObject* o, long long* v) {
     return !(*v == -1 && PyErr_Occurred());
 }
 
+// A call of the C ABI without Python's lock: a launch waits while a thousand others are queued before it, and what those wait for may
+// be another of Python's threads.  Calls of several launches that share a workspace stay in one piece (between_calls).
+std::mutex between_calls;
+template <class... P, class... A>
+int unlocked(bool several, int (*call)(P...), A... args) {
+    PyThreadState* state = PyEval_SaveThread();
+    if (several) between_calls.lock();
+    const int rc = call(args...);
+    if (several) between_calls.unlock();
+    PyEval_RestoreThread(state);
+    return rc;
+}
+
 // A size or a number as the C ABI takes it; what does not fit becomes one that the C ABI refuses.
 int narrow(int64_t n) { return n > INT32_MAX ? INT32_MAX : n < INT32_MIN ? INT32_MIN : int(n); }
 
@@ -110,10 +125,10 @@ PyObject* rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (r) will_write(*r);
         const c10::cuda::CUDAGuard on(x->device());
         at::Tensor q = empty({m, n}, at::kChar, x->device()), d = empty({m, n / 32}, at::kFloat, x->device());
-        const int rc = qnt_rms_norm_q8(x->const_data_ptr(), dtype_of(*x), x->stride(0), r ? r->mutable_data_ptr() : nullptr,
-                                       r ? dtype_of(*r) : 0, r ? r->stride(0) : 0, static_cast<const float*>(w->const_data_ptr()), float(eps),
-                                       int(m), narrow(n), static_cast<int8_t*>(q.mutable_data_ptr()), static_cast<float*>(d.mutable_data_ptr()),
-                                       c10::cuda::getCurrentCUDAStream().stream());
+        const int rc = unlocked(false, qnt_rms_norm_q8, x->const_data_ptr(), dtype_of(*x), x->stride(0), r ? r->mutable_data_ptr() : nullptr,
+                                r ? dtype_of(*r) : 0, r ? r->stride(0) : 0, static_cast<const float*>(w->const_data_ptr()), float(eps), int(m),
+                                narrow(n), static_cast<int8_t*>(q.mutable_data_ptr()), static_cast<float*>(d.mutable_data_ptr()),
+                                c10::cuda::getCurrentCUDAStream(x->device().index()).stream());
         if (rc) return PyLong_FromLong(rc);
         if (r) written(*r);
         return pair(wrap(std::move(q)), wrap(std::move(d)));
@@ -133,9 +148,9 @@ PyObject* dequantize_q8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const int n_tok = token_count(q->size(0));
         const c10::cuda::CUDAGuard on(q->device());
         at::Tensor out = empty(q->sizes(), dtype == QNT_F32 ? at::kFloat : dtype == QNT_F16 ? at::kHalf : at::kBFloat16, q->device());
-        const int rc = qnt_dequantize_q8(static_cast<const int8_t*>(q->const_data_ptr()), static_cast<const float*>(d->const_data_ptr()),
-                                         n_tok, narrow(q->size(1)), out.mutable_data_ptr(), int(dtype),
-                                         c10::cuda::getCurrentCUDAStream().stream());
+        const int rc = unlocked(false, qnt_dequantize_q8, static_cast<const int8_t*>(q->const_data_ptr()),
+                                static_cast<const float*>(d->const_data_ptr()), n_tok, narrow(q->size(1)), out.mutable_data_ptr(), int(dtype),
+                                c10::cuda::getCurrentCUDAStream(q->device().index()).stream());
         return rc ? PyLong_FromLong(rc) : wrap(std::move(out));
     });
 }
@@ -169,11 +184,12 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         at::Tensor q_out = inplace ? *q : empty(q->sizes(), q->scalar_type(), q->device()), k_out;
         if (k) k_out = inplace ? *k : empty(k->sizes(), k->scalar_type(), k->device());
         // (of a single head the stride between heads says nothing)
-        const int rc = qnt_rope(q->const_data_ptr(), q->stride(0), q_out.mutable_data_ptr(), q_out.stride(0), narrow(q->size(1)),
-                                k ? k->const_data_ptr() : nullptr, k ? k->stride(0) : 0, k ? k_out.mutable_data_ptr() : nullptr,
-                                k ? k_out.stride(0) : 0, k ? narrow(k->size(1)) : 0, dtype_of(*q), narrow(q->size(2)), narrow(rotary_dim),
-                                int(interleaved), static_cast<const double*>(t->const_data_ptr()), float(scale),
-                                static_cast<const int*>(p->const_data_ptr()), n_tok, c10::cuda::getCurrentCUDAStream().stream());
+        const int rc = unlocked(false, qnt_rope, q->const_data_ptr(), q->stride(0), q_out.mutable_data_ptr(), q_out.stride(0),
+                                narrow(q->size(1)), k ? k->const_data_ptr() : nullptr, k ? k->stride(0) : 0,
+                                k ? k_out.mutable_data_ptr() : nullptr, k ? k_out.stride(0) : 0, k ? narrow(k->size(1)) : 0, dtype_of(*q),
+                                narrow(q->size(2)), narrow(rotary_dim), int(interleaved), static_cast<const double*>(t->const_data_ptr()),
+                                float(scale), static_cast<const int*>(p->const_data_ptr()), n_tok,
+                                c10::cuda::getCurrentCUDAStream(q->device().index()).stream());
         if (rc) return PyLong_FromLong(rc);
         if (inplace) {
             written(*q);
@@ -205,11 +221,11 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const int64_t width = k < 0 ? 0 : k > 64 ? 64 : k;  // (any other k is refused below)
         at::Tensor out = empty({g, width}, at::kFloat, x->device()), tokens = empty({g, width}, at::kInt, x->device()),
                    parents = empty({g, width}, at::kInt, x->device());
-        const int rc = qnt_beam_select(x->const_data_ptr(), dtype_of(*x), row, static_cast<const float*>(s->const_data_ptr()),
-                                       e ? static_cast<const uint8_t*>(e->const_data_ptr()) : nullptr, narrow(end_id), narrow(g), narrow(b),
-                                       narrow(v), narrow(k), static_cast<float*>(out.mutable_data_ptr()), static_cast<int*>(tokens.mutable_data_ptr()),
-                                       static_cast<int*>(parents.mutable_data_ptr()), ws->mutable_data_ptr(), size_t(ws->nbytes()),
-                                       c10::cuda::getCurrentCUDAStream().stream());
+        const int rc = unlocked(true, qnt_beam_select, x->const_data_ptr(), dtype_of(*x), row, static_cast<const float*>(s->const_data_ptr()),
+                                e ? static_cast<const uint8_t*>(e->const_data_ptr()) : nullptr, narrow(end_id), narrow(g), narrow(b),
+                                narrow(v), narrow(k), static_cast<float*>(out.mutable_data_ptr()), static_cast<int*>(tokens.mutable_data_ptr()),
+                                static_cast<int*>(parents.mutable_data_ptr()), ws->mutable_data_ptr(), size_t(ws->nbytes()),
+                                c10::cuda::getCurrentCUDAStream(x->device().index()).stream());
         if (rc) return PyLong_FromLong(rc);
         PyObject *o = wrap(std::move(out)), *t = wrap(std::move(tokens)), *p = wrap(std::move(parents));
         PyObject* all = o && t && p ? PyTuple_Pack(3, o, t, p) : nullptr;
@@ -236,10 +252,10 @@ PyObject* kv_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             return nullptr;
         }
         const c10::cuda::CUDAGuard on(ws->device());
-        return PyLong_FromLong(qnt_kv_reorder(reinterpret_cast<const qnt_kv_cache*>(intptr_t(cache)), static_cast<const int*>(s->const_data_ptr()),
-                                              static_cast<const int*>(p->const_data_ptr()), narrow(n),
-                                              a[3] == Py_None ? narrow(n) : narrow(group), ws->mutable_data_ptr(), size_t(ws->nbytes()),
-                                              c10::cuda::getCurrentCUDAStream().stream()));
+        return PyLong_FromLong(unlocked(true, qnt_kv_reorder, reinterpret_cast<const qnt_kv_cache*>(intptr_t(cache)),
+                                        static_cast<const int*>(s->const_data_ptr()), static_cast<const int*>(p->const_data_ptr()), narrow(n),
+                                        a[3] == Py_None ? narrow(n) : narrow(group), ws->mutable_data_ptr(), size_t(ws->nbytes()),
+                                        c10::cuda::getCurrentCUDAStream(ws->device().index()).stream()));
     });
 }
 

@@ -1,6 +1,7 @@
 """Calls of the operators on torch tensors that are refused, or that others have to notice: counts past 32 bits, tensors
 that the call writes in place, calls from several threads."""
 import threading
+import time
 
 import pytest
 
@@ -136,3 +137,61 @@ def test_reordering_and_reserving_from_threads(qb):
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("which", ["norm", "values", "rope", "beams", "reorder"])
+def test_a_full_queue_does_not_stop_other_threads(qb, which):
+    """A call that waits for room in the GPU's queue, behind half a second of other work, leaves Python's lock to others."""
+    x, w, pos = torch.randn(2, 64, device="cuda"), torch.ones(64, device="cuda"), ints([0, 1])
+    q8, rope, select = qb.rms_norm_q8(x, w), qb.Rope(16), qb.BeamSelector(2)
+    c = qb.PagedKV.empty(1, 1, 64, 4, 2, 2, 16)
+    call = {"norm": lambda: qb.rms_norm_q8(x, w), "values": lambda: qb.dequantize_q8(*q8),
+            "rope": lambda: rope(x.view(2, 4, 16), None, pos), "beams": lambda: select(x.view(1, 2, 64), x[:1, :2].contiguous()),
+            "reorder": lambda: c.reorder(pos, pos)}[which]
+    call()
+    torch.cuda.synchronize()
+    stop, longest = threading.Event(), [0.0]
+
+    def tick():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            longest[0], last = max(longest[0], now - last), now
+
+    t = threading.Thread(target=tick)
+    t.start()
+    began = time.perf_counter()
+    torch.cuda._sleep(10 ** 9)  # (cycles)
+    for _ in range(2500):
+        call()
+    waited = time.perf_counter() - began
+    stop.set()
+    t.join()
+    torch.cuda.synchronize()
+    assert waited > 0.3 and longest[0] < 0.5 * waited, (waited, longest)
+
+
+def test_one_selector_for_two_threads_on_one_stream(qb):
+    """Calls of several launches that share a workspace: those of two threads stay apart."""
+    select, stream, wrong = qb.BeamSelector(4), torch.cuda.Stream(), []
+    sets = [(torch.randn(8, 4, 3000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)),
+             torch.zeros(8, 4, device="cuda")) for i in range(2)]
+    want = [select(*s) for s in sets]
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(stream):
+                got = [select(*sets[i]) for _ in range(1500)]
+                stream.synchronize()
+            wrong.extend(i for out in got if not all(torch.equal(a, b) for a, b in zip(out, want[i])))
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:5]
