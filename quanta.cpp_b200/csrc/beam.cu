@@ -9,7 +9,9 @@
 // more than its largest logit and its sum of exponentials: no warp waits for another, nothing is selected on the way.
 // k_beam_merge, a CTA per group, joins the sums, ranks the tiles and opens the k best of them.  Scores are formed and compared in
 // 64 bits.  The sums carry an error of their f32 exponentials and roundings, below 2.7e-6; where two beams' candidates lie closer
-// than that could move them, the sums of these beams are formed again in 64 bits.
+// than that could move them, the sums of these beams are formed again in 64 bits, by their group's CTA, a row after the other: rare
+// between beams of their own, but with beams that are alike (copies of one prompt with equal scores) it is all of them, 50 to 80 us
+// for each row of 151936 (64 x 4 bf16 610 us, 1 x 16 800, where unlike ones take 21 and 10.5).
 #include <climits>
 #include <type_traits>
 

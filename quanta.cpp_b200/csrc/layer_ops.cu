@@ -14,7 +14,8 @@ bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>
 
 // With h = x + r (r: the residual row, h rounded once into it):
 //     y = h * (1 / sqrt(mean h^2 + eps)) * w;  per 32 values: d = max |y| / 127, q = y / d to the nearest, halves away from 0
-// A row stays in registers between the sum and the rounding: every byte crosses HBM once.  A thread holds R chunks of 8 consecutive
+// A row stays in registers between the sum and the rounding: every byte crosses HBM once (rows above 16384 values, and above 8192 with
+// a f32 residual, are spilled in part).  A thread holds R chunks of 8 consecutive
 // values, so that a block of 32 is 4 neighbouring lanes and its maximum two shuffles.  Sums in f32: per thread, then per warp, then
 // over warps (an error of a few 2^-24).  A block with a value that is not finite gets a NaN for its scale, every block of a row whose
 // sum is not finite does.  Next to HBM, and without a residual more than HBM (8192 rows of 4096 bf16: 23.7 us, 16.4 of them for the
@@ -76,9 +77,9 @@ __device__ __forceinline__ void store_pairs(T* p, const unsigned long long (&x)[
     store_row(p, v, aligned);
 }
 
-// RES: there is a residual.  Rows blockIdx.x, blockIdx.x + gridDim.x, ...: the weights stay in registers, and the next row is on its
-// way while one is worked on.  8192 rows of 4096 bf16 with a bf16 residual: 38.2 us, 6.3 TB/s (a CTA per row reads its weights, twice
-// as many bytes as a 16-bit row, from L2 each time: 46 us).
+// RES: there is a residual.  Rows blockIdx.x, blockIdx.x + gridDim.x, ...: a CTA keeps the weights in registers from row to row, and
+// its next row is on its way while one is worked on.  8192 rows of 4096 with their residual: bf16 38.2 us, 6.3 TB/s (a CTA per row
+// reads its weights, twice as many bytes as a 16-bit row, from L2 each time: 46 us), f32 68.0 us, 6.5 TB/s.
 template <class T, class RT, int R, int THREADS, bool RES, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     k_rms_norm_q8(const T* __restrict__ x, long long x_stride, RT* __restrict__ residual, long long residual_stride,
@@ -193,7 +194,9 @@ template <class T, class RT, bool RES, bool VEC>
 cudaError_t norm_r(const NormQ8Args& a, cudaStream_t st) {
     // Two chunks a thread halve a row's shuffles and its barrier: 8192 rows of 4096 bf16 with their residual 38.2 us (one chunk: 49,
     // four: 59), 16384 of 2048 38.0 (one: 46.4).  One has the shorter chain where rows are few: 256 of 896 f32 1.9 us (two: 2.3), 1000
-    // of 1024 3.2 (3.3), 600 of 2048 bf16 3.0 (2.9).
+    // of 1024 3.2 (3.3), 600 of 2048 bf16 3.0 (2.9).  Four are for rows above 16384, the longest that 1024 threads hold in two; their
+    // registers spill (128 to 1220 bytes a thread, two with 1024 threads and a f32 residual 8 to 40): 1024 rows of 32768 bf16 29.6 us,
+    // 67.6 with their residual, f32 with it 289, where 2048 of 16384 take 25.0, 39.5 and 74.5 for as many bytes.
     const int chunks = a.n / 8;
     const bool many = chunks > 32 && (long long)a.n_tok * chunks >= 148 * 1024;
     const int r = chunks <= 256 && !many ? 1 : chunks <= 2048 ? 2 : 4;
@@ -202,6 +205,8 @@ cudaError_t norm_r(const NormQ8Args& a, cudaStream_t st) {
                 : r == 4         ? k_rms_norm_q8<T, RT, 4, 1024, RES, VEC>
                 : threads <= 512 ? k_rms_norm_q8<T, RT, 2, 512, RES, VEC>
                                  : k_rms_norm_q8<T, RT, 2, 1024, RES, VEC>;
+    // CTAs for 2048 threads an SM.  Two chunks a thread take 58 to 80 registers, so that half of these run at a time, or less (of 256
+    // threads 4 of 8 an SM; f32 with its residual 3): the rows go in two or three waves, and each CTA reads the weights for its share.
     const int most = 148 * (2048 / threads > 16 ? 16 : 2048 / threads);
     return launch_pdl(kern, dim3(unsigned(a.n_tok < most ? a.n_tok : most)), dim3(unsigned(threads)), 0, st, true,
                       static_cast<const T*>(a.x), a.x_stride, static_cast<RT*>(a.residual), a.residual_stride, a.weight, a.eps, a.n_tok,
@@ -267,11 +272,12 @@ cudaError_t dequantize_t(const int8_t* q, const float* d, long long n, void* out
 
 // Pair (a, b) of a head's first rotary_dim dims at position p: (a cos - b sin, a sin + b cos) * scale at p * turns[i] revolutions;
 // pairs are (i, i + rotary_dim / 2) or (2 i, 2 i + 1).  The revolution count is formed in 64 bits and only its fraction becomes
-// f32, so that an angle is as exact at position 2^31 as at the start.  A thread has a token and a unit of its heads (interleaved:
-// V dims of 16 bytes; half layout: V dims and the V that they turn with), forms these pairs' cosines and sines once and takes one
-// head after another, 64 bytes of them in flight; `slots` threads share the heads of a token.  Bound by HBM: 8192 tokens of 32 + 8
-// bf16 heads of 128: 28.9 us, 5.8 TB/s (128 bytes in flight: 44, too many registers; without streaming stores 44; cosines and
-// sines of a CTA's tokens in shared memory and a task of any head: 57).
+// f32: an angle is off by 1e-7 at the start, and by 4e-7 more at position 2^31 (the 64-bit roundings of a turn and its product).  A
+// thread has a token and a unit of its heads (interleaved: V dims of 16 bytes; half layout: V dims and the V that they turn with),
+// forms these pairs' cosines and sines once and takes one head after another, 64 bytes of them in flight; `slots` threads share the
+// heads of a token.  Bound by HBM: 8192 tokens of 32 + 8 heads of 128: bf16 28.9 us, 5.8 TB/s, f32 56.8 us, 5.9 TB/s (128 bytes in
+// flight: 44, too many registers; without streaming stores 44; cosines and sines of a CTA's tokens in shared memory and a task of any
+// head: 57).
 constexpr int kRopeThreads = 128;
 
 // VEC: V elements are one access; else they are read one by one.
