@@ -28,8 +28,9 @@ int make_type(int dtype, qb::KvType* t) {
 
 uintptr_t size_of(qb::KvType t) { return t == qb::KV_F32 ? 4 : 2; }
 
-// n rows of `row` bytes, `stride` bytes from each other.
 using Wide = __int128;  // (strides are the caller's)
+
+// Rows of `row` bytes, `stride` bytes from each other.
 struct Rows {
     const void* at;
     Wide stride, row;
